@@ -415,6 +415,78 @@ int lsurge_l2norm_rows_bwd(const void* x, const void* dy, const float* rnorm, in
                            lsurge_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Causal softmax attention of packed or dense sequences, the sequence mixer of the hybrid model's full-attention layers
+ * (no reference counterpart here: MaxText's attention, third-party and not vendored).
+ * ------------------------------------------------------------------------------------------------ */
+
+/* nseq sequences with hq query heads over hk key heads (hq a multiple of hk; query head h reads key head h / (hq / hk)),
+ * head dim d in {64, 128, 256}, dtype LSURGE_BF16 or LSURGE_F16.  With cu_q and cu_k ([nseq + 1] i32 on the device,
+ * ascending from 0) sequence s holds the query rows [cu_q[s], cu_q[s + 1]) and the key rows [cu_k[s], cu_k[s + 1]);
+ * without them (both NULL) total_q / nseq and total_k / nseq rows each.  A sequence's queries are the last of its
+ * positions: query i of nq sees the keys j <= i + nk - nq of nk.  A query that sees none gets o = 0 and lse = -inf.
+ * Totals below 2^30. */
+typedef struct {
+  int64_t nseq, total_q, total_k, hq, hk, d;
+  int dtype;
+} lsurge_attn_shape;
+/* rows [total, heads, d] of the shape's dtype: row r of head h at data + r row_stride + h head_stride (elements;
+ * multiples of 8, d <= row_stride < 2^22), its d values consecutive and 16-byte aligned */
+typedef struct {
+  const void* data;
+  int64_t row_stride, head_stride;
+} lsurge_attn_rows;
+
+/* o [total_q, hq, d] (contiguous) = softmax(scale q k^T, masked) v, f32 scores and sums; lse [hq, total_q] f32, the natural
+ * logarithm of each row's sum of exponentials (NULL: not written).  Rows behind the last sequence: o = 0, lse = -inf;
+ * those rows of q, k and v are not read.  scale positive and finite.  16-byte aligned. */
+int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, float* lse,
+                    lsurge_stream_t stream);
+/* Backward of lsurge_attn_fwd for upstream dout [total_q, hq, d] (contiguous) and dlse [hq, total_q] f32 (NULL: 0), from
+ * the forward's o and lse: dq [total_q, hq, d], dk and dv [total_k, hk, d], summed over the heads of a group, all of the
+ * shape's dtype and contiguous; 0 in the rows behind the last sequence.  No atomics: results repeat bit for bit. */
+size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s);
+int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
+                    const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
+                    size_t workspace_bytes, lsurge_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Paged key-value cache: one token's attention over it, and writing new tokens to it.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* k, v: num_pages pages of page_size tokens (a power of two from 8 to 4096) and `heads` key heads; the d values of page p,
+ * slot t and head h at k + p k_page_stride + t k_slot_stride + h k_head_stride (elements, multiples of 8; v alike), 16-byte
+ * aligned.  page_table [nseq, max_pages] i32 on the device, rows table_stride apart: entry i of row b is the page of
+ * sequence b's tokens i page_size .. + page_size - 1.  An entry outside [0, num_pages) names no page: its tokens take no
+ * part in the attention and are not written.  seq_lens [nseq] i32 on the device: tokens of each sequence, held to
+ * [0, max_pages page_size]. */
+typedef struct {
+  void *k, *v;
+  int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  int64_t num_pages, page_size, max_pages, heads, d;
+  int dtype;
+} lsurge_kv_cache;
+
+/* One query token a sequence over all seq_lens[b] tokens of its cache: o [nseq, hq, d] (contiguous) and lse [nseq, hq] f32
+ * (NULL: not written) as lsurge_attn_fwd's; a sequence of length 0 gets o = 0, lse = -inf.  q: [nseq, hq, d] by strides
+ * (row_stride and head_stride any multiples of 8).  The sequences' tokens are dealt to the GPU in equal shares whatever
+ * their lengths; the parts of a sequence are joined in a fixed order, so results repeat bit for bit.  Calls that share a
+ * workspace have to be ordered on one stream. */
+size_t lsurge_paged_attn_workspace_bytes(int64_t d);
+int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64_t nseq, int64_t hq, float scale, void* o,
+                      float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
+/* Write new tokens' keys and values (rows [rows, heads, d] by strides) to their pages: rows [cu[b], cu[b + 1]) are the last
+ * tokens of sequence b's seq_lens[b] (which counts them already); without cu (NULL) one token a sequence, rows = nseq, and
+ * a sequence of length 0 has none.  Rows behind the last sequence are left out, and every other place of the cache stays
+ * as it was. */
+int lsurge_kv_append(const lsurge_kv_cache* c, const lsurge_attn_rows* k, const lsurge_attn_rows* v, int64_t rows,
+                     int64_t nseq, const int32_t* cu, lsurge_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Test hooks (no reference counterpart): failure injection for the error paths.
  * ------------------------------------------------------------------------------------------------ */
 /* Arm a host-side failure: the nth launch (counting from 1) of the kernel with profiler id kernel_id

@@ -41,6 +41,23 @@ class MoeSavedViews(ctypes.Structure):
                                   "h", "y_pad")]
 
 
+class AttnShape(ctypes.Structure):
+    _fields_ = [(n, _i64) for n in ("nseq", "total_q", "total_k", "hq", "hk", "d")] + [("dtype", _int)]
+
+
+class AttnRows(ctypes.Structure):
+    _fields_ = [("data", _p), ("row_stride", _i64), ("head_stride", _i64)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = ([("k", _p), ("v", _p)] +
+                [(f"{t}_{n}_stride", _i64) for t in "kv" for n in ("page", "slot", "head")] +
+                [("page_table", _p), ("table_stride", _i64), ("seq_lens", _p)] +
+                [(n, _i64) for n in ("num_pages", "page_size", "max_pages", "heads", "d")] + [("dtype", _int)])
+
+
+_rows = ctypes.POINTER(AttnRows)
+
 # name -> (restype, argtypes)
 _SIGS = {
     "lsurge_abi_version": (_int, []),
@@ -112,6 +129,13 @@ _SIGS = {
     "lsurge_gdn_chunked_bwd_saved_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "lsurge_gdn_chunked_bwd_saved": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
                                             _p, _sz, _p, _sz, _p]),
+    "lsurge_attn_fwd": (_int, [ctypes.POINTER(AttnShape), _rows, _rows, _rows, _p, _p, ctypes.c_float, _p, _p, _p]),
+    "lsurge_attn_bwd_workspace_bytes": (_sz, [ctypes.POINTER(AttnShape)]),
+    "lsurge_attn_bwd": (_int, [ctypes.POINTER(AttnShape), _rows, _rows, _rows, _p, _p, ctypes.c_float, _p, _p, _p, _p, _p,
+                               _p, _p, _p, _sz, _p]),
+    "lsurge_paged_attn_workspace_bytes": (_sz, [_i64]),
+    "lsurge_paged_attn": (_int, [ctypes.POINTER(KvCache), _rows, _i64, _i64, ctypes.c_float, _p, _p, _p, _sz, _p]),
+    "lsurge_kv_append": (_int, [ctypes.POINTER(KvCache), _rows, _rows, _i64, _i64, _p, _p]),
     "lsurge_mfma_rate_probe_out_floats": (_sz, []),
     "lsurge_mfma_rate_probe": (_int, [_int, _int, _p, _p]),
     "lsurge_prof_enable": (_int, [_int]),

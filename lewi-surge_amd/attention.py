@@ -1,0 +1,236 @@
+"""Softmax attention of the hybrid model's full-attention layers on the HIP library: whole prompts and training, and one
+new token per sequence over a paged key-value cache.
+
+The Gated DeltaNet block (fast_conv, gdn_fast) mixes a sequence in the model's linear layers; these operators do it in the
+others.  The reference leaves them to MaxText (third-party, not vendored), so the names are this package's own.
+
+  causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, return_lse=False)
+      differentiable; dense [B, T, H, D] or packed [T, H, D] with the sequences' ends in cu_seqlens
+  alloc_kv_cache(num_pages, page_size, kv_heads, head_dim, dtype, device)
+      an empty key and value cache [num_pages, page_size, kv_heads, head_dim]
+  append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None)
+      new tokens' keys and values written to their pages, in place
+  paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, return_lse=False)
+      one query token per sequence over its cached tokens (inference only)
+
+Query head h reads key head h // (H // Hkv).  Types: bf16 and f16, head dims 64, 128 and 256; scores and sums are f32, and
+every output is rounded once.  Sequence ends, lengths and page tables stay on the device: no call waits for the GPU, and
+all of them can be captured in a graph.  What the device holds is not checked on the host; entries outside their range are
+held to it, so that nothing outside the tensors is read or written.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+import _lib as L
+
+HEAD_DIMS = (64, 128, 256)
+
+
+def _check_heads(what, q_heads, kv_heads, d, *ts):
+    L.require_cuda(*ts)
+    if any(t is not None and t.device != ts[0].device for t in ts):
+        raise ValueError(f"{what}: all tensors must be on one device (got {sorted({str(t.device) for t in ts if t is not None})})")
+    if d not in HEAD_DIMS:
+        raise ValueError(f"{what}: head dim must be one of {HEAD_DIMS} (got {d})")
+    if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"{what}: {q_heads} query heads are no multiple of {kv_heads} key heads")
+
+
+def _check_dtype(what, *ts):
+    if ts[0].dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != ts[0].dtype for t in ts):
+        raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
+
+
+def _check_index(what, name, t, shape):
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be int32 of shape {tuple(shape)} (got {t.dtype}, {tuple(t.shape)})")
+    return L.contig(t)
+
+
+def _scale(what, scale, d):
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"{what}: scale must be positive and finite (got {scale})")
+    return scale
+
+
+def _rows(t, min_row=None):
+    """t [rows, heads, D] as the kernels read it, by strides: a copy only where its last axis is not contiguous, a row or
+    head does not start on 16 bytes, or (min_row) rows overlap or lie too far apart."""
+    if t.is_contiguous():
+        return _aligned(t)
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+    if min_row is not None:
+        ok = ok and min_row <= t.stride(0) < 1 << 22
+    return t if ok else t.contiguous()
+
+
+def _aligned(t):
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _rows_arg(t):
+    row, head = (t.shape[1] * t.shape[2], t.shape[2]) if t.is_contiguous() else t.stride()[:2]
+    return ctypes.byref(L.AttnRows(t.data_ptr(), row, head))
+
+
+class _AttnFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale):
+        tq, hq, d = q.shape
+        tk, hk, _ = k.shape
+        q, k, v = (_rows(t.detach(), d) for t in (q, k, v))
+        shape = L.AttnShape(nseq, tq, tk, hq, hk, d, L.dt(q))
+        o = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
+        lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device)
+        with torch.cuda.device(q.device):
+            L.check(L.lib().lsurge_attn_fwd(ctypes.byref(shape), _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
+                                            L.ptr(cu_k), scale, L.ptr(o), L.ptr(lse), L.stream(q.device)), "attn_fwd")
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, lse)
+        ctx.shape, ctx.scale = shape, scale
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dlse):
+        q, k, v, cu_q, cu_k, o, lse = ctx.saved_tensors
+        if do is None:
+            do = torch.zeros_like(o)
+        do = _aligned(L.contig(do.to(o.dtype)))
+        dlse = None if dlse is None else L.contig(dlse.to(torch.float32))
+        dq = torch.empty_like(o)
+        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+        lib = L.lib()
+        with torch.cuda.device(q.device):
+            ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(ctypes.byref(ctx.shape)), q.device)
+            L.check(lib.lsurge_attn_bwd(ctypes.byref(ctx.shape), _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
+                                        L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq),
+                                        L.ptr(dk), L.ptr(dv), L.ptr(ws), ws.numel(), L.stream(q.device)), "attn_bwd")
+        return dq, dk, dv, None, None, None, None
+
+
+def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, return_lse=False):
+    """Causal attention of grouped heads.  q [B, Tq, H, D] with k, v [B, Tk, Hkv, D], or packed: q [Tq, H, D] with k, v
+    [Tk, Hkv, D], sequence s holding the query rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] and the key rows given by
+    cu_seqlens_k alike (None: cu_seqlens_q; int32 [sequences + 1] on the device, ascending from 0).  A sequence's queries
+    are its last positions: query i of nq sees the keys j <= i + nk - nq, so that k and v may hold a cached prefix; a query
+    that sees no key gives zeros.  scale (default D ** -0.5) multiplies the scores.
+
+    Returns o in q's shape and dtype, and with return_lse also the natural logarithm of each row's sum of exponentials, f32
+    [B, Tq, H] or [Tq, H] (-inf for a row without keys).  Both are differentiable (once); rows of packed tensors behind the
+    last sequence give zeros and get zero gradients.  Strides are free as long as the last axis is contiguous: q, k and v
+    may be views of one projection's output."""
+    what = "causal_attention"
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape or k.shape[-1] != q.shape[-1]:
+        raise ValueError(f"{what}: q [B, Tq, H, D] or [Tq, H, D], k and v alike with their own rows and heads (got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
+    d = q.shape[-1]
+    _check_heads(what, q.shape[-2], k.shape[-2], d, q, k, v, cu_seqlens_q, cu_seqlens_k)
+    _check_dtype(what, q, k, v)
+    scale = _scale(what, scale, d)
+    if q.dim() == 4:
+        if cu_seqlens_q is not None or cu_seqlens_k is not None:
+            raise ValueError(f"{what}: cu_seqlens go with packed [T, H, D] tensors")
+        if k.shape[0] != q.shape[0]:
+            raise ValueError(f"{what}: {q.shape[0]} sequences of queries, {k.shape[0]} of keys")
+        nseq, cu_q, cu_k = q.shape[0], None, None
+    else:
+        if cu_seqlens_q is None:
+            raise ValueError(f"{what}: packed tensors need cu_seqlens_q")
+        nseq = max(cu_seqlens_q.numel() - 1, 0)
+        cu_q = _check_index(what, "cu_seqlens_q", cu_seqlens_q, (nseq + 1,))
+        if cu_seqlens_k is None and k.shape[0] != q.shape[0]:
+            raise ValueError(f"{what}: {q.shape[0]} query rows and {k.shape[0]} key rows need cu_seqlens_k")
+        cu_k = cu_q if cu_seqlens_k is None else _check_index(what, "cu_seqlens_k", cu_seqlens_k, (nseq + 1,))
+    rows = [t.flatten(0, 1) if t.dim() == 4 else t for t in (q, k, v)]
+    o, lse = _AttnFn.apply(*rows, cu_q, cu_k, nseq, scale)
+    o = o.view(q.shape)
+    return (o, lse.t().reshape(q.shape[:-1])) if return_lse else o
+
+
+def alloc_kv_cache(num_pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
+    """An empty key and value cache, each [num_pages, page_size, kv_heads, head_dim], with the tokens of one head and page
+    consecutive in memory."""
+    shape = (num_pages, kv_heads, page_size, head_dim)
+    return tuple(torch.empty(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
+
+
+def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{what}: caches must be [num_pages, page_size, kv_heads, head_dim] (got {tuple(k_cache.shape)}, "
+                         f"{tuple(v_cache.shape)})")
+    pages, size, heads, d = k_cache.shape
+    if pages < 1 or size < 8 or size > 4096 or size & (size - 1):
+        raise ValueError(f"{what}: at least one page, of a power of two from 8 to 4096 tokens (got {pages} of {size})")
+    strides = []
+    for t in (k_cache, v_cache):
+        st = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
+        if t.stride(3) != 1 or any(n % 8 for n in st) or t.data_ptr() % 16:
+            raise ValueError(f"{what}: a token's values in a cache must be contiguous and 16-byte aligned (strides {t.stride()})")
+        strides += st
+    if page_table.dim() != 2 or page_table.shape[1] < 1:
+        raise ValueError(f"{what}: page_table must be [sequences, pages] (got {tuple(page_table.shape)})")
+    nseq, most = page_table.shape
+    table = _check_index(what, "page_table", page_table, (nseq, most))
+    lens = _check_index(what, "seq_lens", seq_lens, (nseq,))
+    arg = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), *strides, table.data_ptr(), most,
+                     lens.data_ptr(), pages, size, most, heads, d, L.dt(k_cache))
+    return ctypes.byref(arg), (table, lens)
+
+
+def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
+    """Write new tokens into a paged cache, in place.  k, v [rows, Hkv, D]: one token for each sequence, or with cu_seqlens
+    (int32 [sequences + 1]) the rows cu_seqlens[b] .. cu_seqlens[b + 1] of sequence b.  They become the last of its
+    seq_lens[b] tokens (int32, the new ones counted); token t goes to page page_table[b, t // page_size], slot
+    t % page_size.  Nothing is written for a sequence of length 0 without cu_seqlens, for rows behind the last sequence, or
+    where the table names no page.  Two sequences that share a page must not write to the same place of it."""
+    what = "append_kv"
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError(f"{what}: k and v must be [rows, kv_heads, head_dim] of the caches (got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}, caches {tuple(k_cache.shape)})")
+    _check_heads(what, k.shape[1], k.shape[1], k.shape[2], k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    _check_dtype(what, k, v, k_cache, v_cache)
+    arg, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
+    nseq = page_table.shape[0]
+    if cu_seqlens is not None:
+        cu_seqlens = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
+    elif k.shape[0] != nseq:
+        raise ValueError(f"{what}: {k.shape[0]} tokens for {nseq} sequences need cu_seqlens")
+    k, v = _rows(k.detach()), _rows(v.detach())
+    with torch.cuda.device(k.device):
+        L.check(L.lib().lsurge_kv_append(arg, _rows_arg(k), _rows_arg(v), k.shape[0], nseq, L.ptr(cu_seqlens),
+                                         L.stream(k.device)), "kv_append")
+    del keep
+
+
+def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, return_lse=False):
+    """Attention of one new token per sequence, q [sequences, H, D], over its seq_lens[b] cached tokens (the new one among
+    them, see append_kv).  Returns o [sequences, H, D] in q's dtype, and with return_lse also f32 [sequences, H].  Length 0
+    gives zeros (lse -inf); tokens whose page_table entry names no page are left out.  No gradient."""
+    what = "paged_attention"
+    if q.dim() != 3 or k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3] or q.shape[0] != page_table.shape[0]:
+        raise ValueError(f"{what}: q must be [sequences, heads, head_dim] (got {tuple(q.shape)}, caches "
+                         f"{tuple(k_cache.shape)}, page_table {tuple(page_table.shape)})")
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
+    n, hq, d = q.shape
+    _check_heads(what, hq, k_cache.shape[2], d, q, k_cache, v_cache, page_table, seq_lens)
+    _check_dtype(what, q, k_cache, v_cache)
+    scale = _scale(what, scale, d)
+    arg, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
+    q = _rows(q)
+    o = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lib = L.lib()
+    with torch.cuda.device(q.device):
+        ws = L.workspace(lib.lsurge_paged_attn_workspace_bytes(d), q.device)
+        L.check(lib.lsurge_paged_attn(arg, _rows_arg(q), n, hq, scale, L.ptr(o), L.ptr(lse), L.ptr(ws), ws.numel(),
+                                      L.stream(q.device)), "paged_attn")
+    del keep
+    return (o, lse) if return_lse else o

@@ -51,7 +51,7 @@ const char* g_names[KID_COUNT] = {
     "shared_gu_fwd",    "shared_down_fwd",   "shared_down_dgrad", "shared_down_wgrad", "shared_gu_dgrad",
     "shared_gu_wgrad",  "splitk_reduce",     "misc",             "router_select",
     "fp8_quantize",     "gdn_chunk",         "gdn_scan",          "gdn_bscan",        "gdn_bgrad",
-    "gdn_bchunk"};
+    "gdn_bchunk",       "attention"};
 static_assert(KID_COUNT <= 31, "lsurge_prof_enable takes the kernel ids as bits of an int");
 constexpr size_t kPool = 8192;
 }  // namespace

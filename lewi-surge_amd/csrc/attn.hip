@@ -1,0 +1,676 @@
+// Causal softmax attention of packed or dense sequences with grouped heads, forward and backward, on the matrix cores.
+//
+// Query i of a sequence with nq queries and nk keys attends to the keys j <= i + nk - nq (the queries are the last ones):
+//   s_ij = scale q_i . k_j,  o_i = sum_j e^(s_ij - lse_i) v_j,  lse_i = log sum_j e^(s_ij)
+// and o_i = 0, lse_i = -inf for a query with no key.  Scores and sums are f32, in base 2 (the scale carries log2 e); the
+// weights are rounded to the operands' type for the second product, as its operands have to be (at most 1, relative error
+// 2^-9 in bf16, and what is rounded off is not summed into the denominator, so errors average out over the keys).
+//
+// Every product is formed transposed: S^T = K Q^T has a query per lane (column l % 32), so a row's maximum and sum are
+// sums over a lane's own registers and one exchange with lane ^ 32, the accumulators O^T = V^T P^T have the same query in
+// the same lane, and P^T is in place as the second product's operand (the keys of 8 consecutive registers are the ones
+// its fragment takes, in an order that V^T's fragment is read in as well).  No value crosses lanes on the way.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "launchers.h"
+
+namespace lsattn {
+namespace {
+
+struct AttnArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  const int32_t *cu_q, *cu_k;
+  int nseq, total_q, total_k, hq, hk, ntiles;
+  float scale2;  // scale log2(e)
+};
+
+// Workgroup -> (head, tile), long tiles first.  Workgroups are dealt to the 8 XCDs round-robin; with a multiple of 8
+// heads every XCD gets heads of its own, whose keys its L2 then serves.
+__device__ __forceinline__ void head_tile(int heads, int ntiles, int& head, int& tile) {
+  const int id = (int)blockIdx.x;
+  int rank;
+  if (heads % 8 == 0) {
+    const int per = heads / 8, i = id / 8;
+    head = id % 8 * per + i % per;
+    rank = i / per;
+  } else {
+    head = id % heads;
+    rank = id / heads;
+  }
+  tile = ntiles - 1 - rank;
+}
+
+// rows [first, first + n) of [rows, heads, D] at one head, zeroed (rows behind the last sequence)
+template <int D>
+__device__ __forceinline__ void zero_rows(uint16_t* p, int64_t first, int n, int heads, int head, int tid, int nthr) {
+  for (int i = tid; i < n * (D / 8); i += nthr)
+    *reinterpret_cast<u32x4*>(p + ((first + i / (D / 8)) * heads + head) * D + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+}
+
+// ------------------------------------------------------------------------------------ forward
+constexpr int BN = 64;  // keys per stage
+
+// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 64, double-buffered in LDS:
+// one barrier a stage, the next stage's copies in flight during the products of this one.
+template <int D, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ lse) {
+  constexpr int BM = NW * 32, TILE = BN * D * 2;  // bytes of one operand of one stage
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  int head, slot;
+  head_tile(a.hq, a.ntiles, head, slot);
+  if (a.cu_q) {
+    const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
+    const int n = (int)min((int64_t)BM, a.total_q - end);
+    if (n > 0) {
+      zero_rows<D>(o, end, n, a.hq, head, threadIdx.x, NW * 64);
+      if (lse && (int)threadIdx.x < n) lse[(int64_t)head * a.total_q + end + threadIdx.x] = -INFINITY;
+    }
+  }
+  int tile;
+  const int seq = seq_of_tile<BM>(a.cu_q, a.nseq, a.total_q, slot, lane, tile);
+  if (seq < 0) return;
+  int q0, nq, k0, nk;
+  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
+  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
+  if (tile * BM >= nq) return;
+  const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
+  const int kvh = head / (a.hq / a.hk);
+
+  u32x4 qf[D / 16];
+  {
+    const uint16_t* qp = a.q + (int64_t)(q0 + min(row, nq - 1)) * a.q_row + head * a.q_head + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+  }
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+  float m = -INFINITY, l = 0.f;  // m: running maximum of the raw scores; l: this half's share of the row's sum
+
+  const uint32_t lds = lds_addr((const bf16_t*)smem);
+  TileCopy<D, BN, NW> ck, cv;
+  ck.init(a.k_row, wave, lane);
+  cv.init(a.v_row, wave, lane);
+  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
+  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
+  const int kend = min(nq, (tile + 1) * BM) + off;  // keys the workgroup's last row sees
+  const int nst = (max(kend, 0) + BN - 1) / BN;
+  auto issue = [&](int st) {
+    const uint32_t at = lds + (st & 1) * 2 * TILE;
+    ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - st * BN, at, wave);
+    cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
+  };
+  const uint32_t ka = row_addr<D>(lane);
+  uint32_t va[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) va[t] = col_addr<D>(lane, t);
+
+  if (nst) issue(0);
+  for (int st = 0; st < nst; ++st) {
+    stage_barrier<0>();  // this stage's copies have landed, and nobody reads the other half any more
+    if (st + 1 < nst) issue(st + 1);
+    if (st * BN > w0 + 31 + off) continue;  // nothing of this stage is visible to the wave's rows
+    const uint32_t kt = lds + (st & 1) * 2 * TILE, vt = kt + TILE;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) s[t] = mma32<DT>(lds_read16(kt + t * 32 * D * 2 + (ka ^ (x * 32))), qf[x], s[t]);
+    }
+    if (st * BN + BN - 1 > w0 + off) {  // the diagonal or the end of the keys
+      const int lim = row + off - st * BN;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * t + 8 * (r / 4) + 4 * hf + r % 4 > lim) s[t][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+    mx = fmaxf(m, halves(mx, [](float x, float y) { return fmaxf(x, y); }));
+    const float mc = mx == -INFINITY ? 0.f : mx * a.scale2;
+    const float alpha = exp2_hw(m * a.scale2 - mc);
+    m = mx;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = exp2_hw(fmaf(s[t][r], a.scale2, -mc));
+        sum += s[t][r];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] *= alpha;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = pack2<DT>(s[t][8 * h + 2 * i], s[t][8 * h + 2 * i + 1]);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          acc[d] = mma32<DT>(lds_read_col<D>(vt + (32 * t + 16 * h) * D * 2 + va[d]), p, acc[d]);
+      }
+  }
+  l = halves(l, [](float x, float y) { return x + y; });
+  if (row >= nq) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* op = o + ((int64_t)(q0 + row) * a.hq + head) * D + 4 * hf;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<u32x2*>(op + 32 * d + 2 * r) = u32x2{pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv),
+                                                             pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv)};
+  if (lse && hf == 0)
+    lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (m * a.scale2 + __log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------ backward
+// What the two passes need of each query, laid out [hq][total_q]: lse2 = lse log2(e) (+inf for a row with no key, whose
+// weights 2^(s - lse2) are then 0), delta = do . o - dlse.  f16 values have few exponent bits: weights of long rows (2^-15
+// and less) and their products with small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times
+// too large (lse2 smaller by SHIFT) and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's
+// own, from the largest |do| of the row, in the pass over queries; the head's, from the largest of all rows, in the pass
+// over keys, which sums over the rows (amax [hq][blocks], a block's largest).
+constexpr int PB = 64;  // rows per block of the preparation
+template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
+struct RowPrep {
+  float *lse2, *delta, *rscale, *amax;
+  int nblk;
+};
+// 2^e with 2^e amax in [1, 2); 1 for 0, infinities and NaN
+__device__ __forceinline__ float grad_scale(float amax) {
+  if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
+  int e;
+  (void)frexpf(amax, &e);
+  return ldexpf(1.f, min(max(1 - e, -60), 60));
+}
+template <int D, int DT>
+__global__ __launch_bounds__(256) void attn_prep_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
+                                                        const float* __restrict__ lse, const float* __restrict__ dlse,
+                                                        int total_q, int hq, RowPrep w) {
+  constexpr int LPR = D / 8, RPP = 256 / LPR;  // lanes per row, rows per pass
+  __shared__ float red[4];
+  const int head = blockIdx.y, sub = threadIdx.x % LPR;
+  float big = 0.f;
+  for (int r = threadIdx.x / LPR; r < PB; r += RPP) {
+    const int row = (int)blockIdx.x * PB + r;
+    float dot = 0.f, mx = 0.f;
+    if (row < total_q) {
+      const int64_t at = ((int64_t)row * hq + head) * D + sub * 8;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(o + at), y = *reinterpret_cast<const u32x4*>(dout + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x0, x1, y0, y1;
+        unpack2<DT>(x[i], x0, x1);
+        unpack2<DT>(y[i], y0, y1);
+        dot = fmaf(x0, y0, fmaf(x1, y1, dot));
+        mx = fmaxf(mx, fmaxf(fabsf(y0), fabsf(y1)));
+      }
+    }
+#pragma unroll
+    for (int s = LPR / 2; s > 0; s >>= 1) {
+      dot += __shfl_xor(dot, s, 64);
+      mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+    }
+    big = fmaxf(big, mx);
+    if (sub == 0 && row < total_q) {
+      const int64_t i = (int64_t)head * total_q + row;
+      const float v = lse[i];
+      w.lse2[i] = v == -INFINITY ? INFINITY : v * LOG2E - SHIFT<DT>;
+      w.delta[i] = dot - (dlse ? dlse[i] : 0.f);
+      if (DT == LSURGE_F16) w.rscale[i] = grad_scale(mx);
+    }
+  }
+  if constexpr (DT == LSURGE_F16) {
+    big = wave_max(big);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = big;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      w.amax[(int64_t)head * w.nblk + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+}
+
+// dq_i = scale sum_j ds_ij k_j with ds_ij = p_ij (do_i . v_j - delta_i): the forward's walk, a query per lane, dS^T in
+// place as the operand of dQ^T = K^T dS^T.  The scores are formed again rather than handed over by the pass over keys:
+// two products more, but no sum over workgroups, whose order would change the results.
+template <int D, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dq) {
+  constexpr int BM = NW * 32, TILE = BN * D * 2;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  int head, slot;
+  head_tile(a.hq, a.ntiles, head, slot);
+  if (a.cu_q) {
+    const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
+    const int n = (int)min((int64_t)BM, a.total_q - end);
+    if (n > 0) zero_rows<D>(dq, end, n, a.hq, head, threadIdx.x, NW * 64);
+  }
+  int tile;
+  const int seq = seq_of_tile<BM>(a.cu_q, a.nseq, a.total_q, slot, lane, tile);
+  if (seq < 0) return;
+  int q0, nq, k0, nk;
+  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
+  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
+  if (tile * BM >= nq) return;
+  const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
+  const int kvh = head / (a.hq / a.hk);
+
+  u32x4 qf[D / 16], df[D / 16];
+  const int crow = q0 + min(row, nq - 1);
+  {
+    const uint16_t* qp = a.q + (int64_t)crow * a.q_row + head * a.q_head + 8 * hf;
+    const uint16_t* dp = dout + ((int64_t)crow * a.hq + head) * D + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+      df[s] = *reinterpret_cast<const u32x4*>(dp + 16 * s);
+    }
+  }
+  const int64_t pi = (int64_t)head * a.total_q + crow;
+  const float lse2 = w.lse2[pi], delta = w.delta[pi];
+  const float gs = DT == LSURGE_F16 ? w.rscale[pi] : 1.f;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+
+  const uint32_t lds = lds_addr((const bf16_t*)smem);
+  TileCopy<D, BN, NW> ck, cv;
+  ck.init(a.k_row, wave, lane);
+  cv.init(a.v_row, wave, lane);
+  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
+  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
+  const int kend = min(nq, (tile + 1) * BM) + off;
+  const int nst = (max(kend, 0) + BN - 1) / BN;
+  auto issue = [&](int st) {
+    const uint32_t at = lds + (st & 1) * 2 * TILE;
+    ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - st * BN, at, wave);
+    cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
+  };
+  const uint32_t ra = row_addr<D>(lane);
+  uint32_t ca[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) ca[t] = col_addr<D>(lane, t);
+
+  if (nst) issue(0);
+  for (int st = 0; st < nst; ++st) {
+    stage_barrier<0>();
+    if (st + 1 < nst) issue(st + 1);
+    if (st * BN > w0 + 31 + off) continue;
+    const uint32_t kt = lds + (st & 1) * 2 * TILE, vt = kt + TILE;
+    const int lim = row + off - st * BN;
+    const bool edge = st * BN + BN - 1 > w0 + off;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 s, g;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        s = mma32<DT>(lds_read16(kt + t * 32 * D * 2 + (ra ^ (x * 32))), qf[x], s);
+        g = mma32<DT>(lds_read16(vt + t * 32 * D * 2 + (ra ^ (x * 32))), df[x], g);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = exp2_hw(fmaf(s[r], a.scale2, -lse2));
+        s[r] = p * ((g[r] - delta) * gs);
+      }
+      if (edge)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * t + 8 * (r / 4) + 4 * hf + r % 4 > lim) s[r] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = pack2<DT>(s[8 * h + 2 * i], s[8 * h + 2 * i + 1]);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          acc[d] = mma32<DT>(lds_read_col<D>(kt + (32 * t + 16 * h) * D * 2 + ca[d]), p, acc[d]);
+      }
+    }
+  }
+  if (row >= nq) return;
+  const float f = scale / gs * exp2_hw(-SHIFT<DT>);
+  uint16_t* op = dq + ((int64_t)(q0 + row) * a.hq + head) * D + 4 * hf;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<u32x2*>(op + 32 * d + 2 * r) = u32x2{pack2<DT>(acc[d][r] * f, acc[d][r + 1] * f),
+                                                             pack2<DT>(acc[d][r + 2] * f, acc[d][r + 3] * f)};
+}
+
+// dv_j = sum_i p_ij do_i, dk_j = scale sum_i ds_ij q_i over the queries of every head of the group.  A workgroup takes
+// NW x 32 keys of one key head, 32 a wave, a key per lane (S = Q K^T), and walks the group's queries in stages of QT rows
+// of q and do; dV^T = dO^T P and dK^T = Q^T dS take P and dS from the lanes they were formed in.
+template <int D, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dk,
+                     uint16_t* __restrict__ dv) {
+  constexpr int BK = NW * 32, QT = 64, TILE = QT * D * 2;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float rows[2][2][QT];  // lse2 and delta of a stage's rows
+  __shared__ float red[NW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, hf = lane >> 5;
+  int kvh, slot;
+  head_tile(a.hk, a.ntiles, kvh, slot);
+  slot = a.ntiles - 1 - slot;  // the first keys are seen by the most queries
+  if (a.cu_k) {
+    const int64_t end = cu_at(a.cu_k, a.nseq, a.total_k) + (int64_t)slot * BK;
+    const int n = (int)min((int64_t)BK, a.total_k - end);
+    if (n > 0) {
+      zero_rows<D>(dk, end, n, a.hk, kvh, threadIdx.x, NW * 64);
+      zero_rows<D>(dv, end, n, a.hk, kvh, threadIdx.x, NW * 64);
+    }
+  }
+  int tile;
+  const int seq = seq_of_tile<BK>(a.cu_k, a.nseq, a.total_k, slot, lane, tile);
+  if (seq < 0) return;
+  int q0, nq, k0, nk;
+  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
+  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
+  if (tile * BK >= nk) return;
+  const int off = nk - nq, w0 = tile * BK + wave * 32, col = w0 + ln, group = a.hq / a.hk;
+
+  u32x4 kf[D / 16], vf[D / 16];
+  {
+    const int64_t r = k0 + min(col, nk - 1);
+    const uint16_t *kp = a.k + r * a.k_row + kvh * a.k_head + 8 * hf, *vp = a.v + r * a.v_row + kvh * a.v_head + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      kf[s] = *reinterpret_cast<const u32x4*>(kp + 16 * s);
+      vf[s] = *reinterpret_cast<const u32x4*>(vp + 16 * s);
+    }
+  }
+  float gs = 1.f;
+  if constexpr (DT == LSURGE_F16) {  // one scale for the head's group: its largest |do|
+    float mx = 0.f;
+    const float* am = w.amax + (int64_t)kvh * group * w.nblk;
+    for (int i = threadIdx.x; i < group * w.nblk; i += NW * 64) mx = fmaxf(mx, am[i]);
+    mx = wave_max(mx);
+    if (lane == 0) red[wave] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) mx = fmaxf(mx, red[i]);
+    gs = grad_scale(mx);
+  }
+  f32x16 ak[D / 32], av[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ak[t][r] = av[t][r] = 0.f;
+
+  const uint32_t lds = lds_addr((const bf16_t*)smem), rows_lds = lds_addr((const bf16_t*)rows);
+  TileCopy<D, QT, NW> cq, cd;
+  const int64_t d_row = (int64_t)a.hq * D;
+  cq.init(a.q_row, wave, lane);
+  cd.init(d_row, wave, lane);
+  const int first = max(0, tile * BK - off) / QT;  // the stage of the first query that sees the tile's first key
+  const int per = max(0, (nq + QT - 1) / QT - first), nst = per * group;
+  auto issue = [&](int st) {
+    const int head = kvh * group + st / per, r0 = (first + st % per) * QT, n = nq - r0;
+    const uint32_t at = lds + (st & 1) * 2 * TILE;
+    cq.issue(a.q + (int64_t)(q0 + r0) * a.q_row + head * a.q_head, a.q_row, n, at, wave);
+    cd.issue(dout + (int64_t)(q0 + r0) * d_row + head * D, d_row, n, at + TILE, wave);
+    if (wave < 2) {  // rows past the end get zeros: q and do are zeros there, so any finite values do
+      const float* p = (wave ? w.delta : w.lse2) + (int64_t)head * a.total_q + q0 + r0;
+      copy4(make_rsrc(p, 4 * (int64_t)min(n, QT)), lane * 4, rows_lds + ((st & 1) * 2 + wave) * QT * 4);
+    }
+  };
+  const uint32_t ra = row_addr<D>(lane);
+  uint32_t ca[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) ca[t] = col_addr<D>(lane, t);
+
+  if (nst) issue(0);
+  for (int st = 0; st < nst; ++st) {
+    stage_barrier<0>();
+    if (st + 1 < nst) issue(st + 1);
+    const int r0 = (first + st % per) * QT;
+    if (r0 + QT - 1 + off < w0) continue;  // no row of this stage sees the wave's keys
+    const uint32_t qt = lds + (st & 1) * 2 * TILE, dt = qt + TILE;
+    const int lim = col - off - r0;  // rows from lim on see the lane's key
+    const bool edge = r0 + off < w0 + 31;
+#pragma unroll
+    for (int t = 0; t < QT / 32; ++t) {
+      f32x16 s, g;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        s = mma32<DT>(lds_read16(qt + t * 32 * D * 2 + (ra ^ (x * 32))), kf[x], s);
+        g = mma32<DT>(lds_read16(dt + t * 32 * D * 2 + (ra ^ (x * 32))), vf[x], g);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(&rows[st & 1][0][32 * t + 8 * b + 4 * hf]);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(&rows[st & 1][1][32 * t + 8 * b + 4 * hf]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * b + i;
+          float p = exp2_hw(fmaf(s[r], a.scale2, -ls[i]));
+          float x = p * ((g[r] - de[i]) * gs);
+          if (edge && 32 * t + 8 * b + 4 * hf + i < lim) p = x = 0.f;
+          s[r] = p;
+          g[r] = x;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 p, x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = pack2<DT>(s[8 * h + 2 * i], s[8 * h + 2 * i + 1]);
+          x[i] = pack2<DT>(g[8 * h + 2 * i], g[8 * h + 2 * i + 1]);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          av[d] = mma32<DT>(lds_read_col<D>(dt + (32 * t + 16 * h) * D * 2 + ca[d]), p, av[d]);
+          ak[d] = mma32<DT>(lds_read_col<D>(qt + (32 * t + 16 * h) * D * 2 + ca[d]), x, ak[d]);
+        }
+      }
+    }
+  }
+  if (col >= nk) return;
+  const float fv = exp2_hw(-SHIFT<DT>), fk = scale / gs * fv;
+  const int64_t at = ((int64_t)(k0 + col) * a.hk + kvh) * D + 4 * hf;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      *reinterpret_cast<u32x2*>(dk + at + 32 * d + 2 * r) = u32x2{
+          pack2<DT>(ak[d][r] * fk, ak[d][r + 1] * fk), pack2<DT>(ak[d][r + 2] * fk, ak[d][r + 3] * fk)};
+      *reinterpret_cast<u32x2*>(dv + at + 32 * d + 2 * r) = u32x2{
+          pack2<DT>(av[d][r] * fv, av[d][r + 1] * fv), pack2<DT>(av[d][r + 2] * fv, av[d][r + 3] * fv)};
+    }
+}
+
+// ------------------------------------------------------------------------------------ host
+int check_rows(const char* what, const lsurge_attn_rows& r, int64_t d) {
+  LSURGE_REQUIRE(r.data, "%s: null pointer", what);
+  LSURGE_REQUIRE((uintptr_t)r.data % 16 == 0 && r.row_stride % 8 == 0 && r.head_stride % 8 == 0,
+                 "%s: rows must be 16-byte aligned (strides %lld, %lld in elements)", what, (long long)r.row_stride,
+                 (long long)r.head_stride);
+  LSURGE_REQUIRE(r.row_stride >= d && r.row_stride < (1 << 22) && r.head_stride >= 0 && r.head_stride < (1ll << 40),
+                 "%s: row stride %lld outside [head_dim, 2^22), or head stride %lld outside [0, 2^40)", what,
+                 (long long)r.row_stride, (long long)r.head_stride);
+  return LSURGE_OK;
+}
+
+int check_shape(const char* what, const lsurge_attn_shape* s, const int32_t* cu_q, const int32_t* cu_k, float scale) {
+  LSURGE_REQUIRE(s, "%s: null shape", what);
+  LSURGE_REQUIRE(s->d == 64 || s->d == 128 || s->d == 256, "%s: head_dim %lld (64, 128 or 256)", what, (long long)s->d);
+  LSURGE_REQUIRE(s->hk >= 1 && s->hq >= s->hk && s->hq % s->hk == 0 && s->hq <= 65535,
+                 "%s: %lld query heads over %lld key heads", what, (long long)s->hq, (long long)s->hk);
+  LSURGE_REQUIRE(s->nseq >= 0 && s->nseq < (1 << 24) && s->total_q >= 0 && s->total_q < (1ll << 30) && s->total_k >= 0 &&
+                     s->total_k < (1ll << 30),
+                 "%s: nseq=%lld total_q=%lld total_k=%lld", what, (long long)s->nseq, (long long)s->total_q,
+                 (long long)s->total_k);
+  LSURGE_REQUIRE((cu_q != nullptr) == (cu_k != nullptr), "%s: cu_q and cu_k go together", what);
+  if (!cu_q)
+    LSURGE_REQUIRE(s->nseq == 0 ? s->total_q == 0 && s->total_k == 0 : s->total_q % s->nseq == 0 && s->total_k % s->nseq == 0,
+                   "%s: %lld and %lld rows are no whole number for each of %lld sequences", what, (long long)s->total_q,
+                   (long long)s->total_k, (long long)s->nseq);
+  LSURGE_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", what);
+  if (s->dtype != LSURGE_BF16 && s->dtype != LSURGE_F16) return lsurge::set_error(LSURGE_ERR_DTYPE, "%s: bf16 or f16", what);
+  return LSURGE_OK;
+}
+
+int64_t num_tiles(const lsurge_attn_shape& s, bool packed, int64_t total, int64_t rows) {
+  if (packed) return total / rows + std::max<int64_t>(s.nseq, 1);  // at least 1: rows behind the last sequence
+  return s.nseq * ((total / s.nseq + rows - 1) / rows);
+}
+
+AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const lsurge_attn_rows& k,
+                   const lsurge_attn_rows& v, const int32_t* cu_q, const int32_t* cu_k, float scale) {
+  AttnArgs a;
+  a.q = (const uint16_t*)q.data, a.k = (const uint16_t*)k.data, a.v = (const uint16_t*)v.data;
+  a.q_row = q.row_stride, a.k_row = k.row_stride, a.v_row = v.row_stride;
+  a.q_head = q.head_stride, a.k_head = k.head_stride, a.v_head = v.head_stride;
+  a.cu_q = cu_q, a.cu_k = cu_k;
+  a.nseq = (int)s.nseq, a.total_q = (int)s.total_q, a.total_k = (int)s.total_k, a.hq = (int)s.hq, a.hk = (int)s.hk;
+  a.ntiles = 0;
+  a.scale2 = scale * LOG2E;
+  return a;
+}
+
+// waves of a workgroup: 8 where 256 registers a lane hold a wave's operands and sums, 4 (512 registers) at D = 256
+template <int D> constexpr int WAVES = D == 256 ? 4 : 8;
+
+#define ATTN_DISPATCH(CALL)                                                     \
+  do {                                                                          \
+    if (s->dtype == LSURGE_BF16) {                                              \
+      if (s->d == 64) { CALL(64, LSURGE_BF16); }                                \
+      else if (s->d == 128) { CALL(128, LSURGE_BF16); }                         \
+      else { CALL(256, LSURGE_BF16); }                                          \
+    } else {                                                                    \
+      if (s->d == 64) { CALL(64, LSURGE_F16); }                                 \
+      else if (s->d == 128) { CALL(128, LSURGE_F16); }                          \
+      else { CALL(256, LSURGE_F16); }                                           \
+    }                                                                           \
+  } while (0)
+
+int tile_grid(const char* what, int64_t tiles, int64_t heads, unsigned* grid) {
+  LSURGE_REQUIRE(tiles * heads < (1ll << 31), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)heads);
+  *grid = (unsigned)(tiles * heads);
+  return LSURGE_OK;
+}
+
+}  // namespace
+}  // namespace lsattn
+
+using namespace lsattn;
+
+extern "C" {
+
+int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, float* lse,
+                    lsurge_stream_t stream) {
+  if (int rc = check_shape("attn_fwd", s, cu_q, cu_k, scale)) return rc;
+  if (s->total_q == 0) return LSURGE_OK;
+  LSURGE_REQUIRE(q && k && v && o && (uintptr_t)o % 16 == 0, "attn_fwd: null or misaligned pointer");
+  if (int rc = check_rows("attn_fwd q", *q, s->d)) return rc;
+  if (s->total_k) {
+    if (int rc = check_rows("attn_fwd k", *k, s->d)) return rc;
+    if (int rc = check_rows("attn_fwd v", *v, s->d)) return rc;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
+#define ATTN_FWD(D, DT)                                                                                             \
+  constexpr int NW = WAVES<D>;                                                                                      \
+  a.ntiles = (int)num_tiles(*s, cu_q, s->total_q, NW * 32);                                                         \
+  unsigned grid;                                                                                                    \
+  if (int rc = tile_grid("attn_fwd", a.ntiles, s->hq, &grid)) return rc;                                            \
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a, \
+                                                 (uint16_t*)o, lse))
+  ATTN_DISPATCH(ATTN_FWD);
+#undef ATTN_FWD
+  return LSURGE_OK;
+}
+
+static size_t prep_floats(const lsurge_attn_shape* s) {
+  const int64_t rows = s->hq * s->total_q, blk = (s->total_q + PB - 1) / PB;
+  return (size_t)(s->dtype == LSURGE_F16 ? 3 * rows + s->hq * blk : 2 * rows);
+}
+size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
+  if (!s || s->hq < 1 || s->total_q < 0) return 0;
+  return sizeof(float) * prep_floats(s) + 64;
+}
+
+int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
+                    const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
+                    size_t workspace_bytes, lsurge_stream_t stream) {
+  if (int rc = check_shape("attn_bwd", s, cu_q, cu_k, scale)) return rc;
+  LSURGE_REQUIRE(q && k && v && workspace, "attn_bwd: null pointer");
+  const size_t need = lsurge_attn_bwd_workspace_bytes(s);
+  if (workspace_bytes < need)
+    return lsurge::set_error(LSURGE_ERR_WORKSPACE, "attn_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
+  LSURGE_REQUIRE(((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) %
+                         16 == 0,
+                 "attn_bwd: buffers must be 16-byte aligned");
+  if (s->total_q) {
+    LSURGE_REQUIRE(o && lse && dout && dq, "attn_bwd: null pointer");
+    if (int rc = check_rows("attn_bwd q", *q, s->d)) return rc;
+  }
+  if (s->total_k) {
+    LSURGE_REQUIRE(dk && dv, "attn_bwd: null pointer");
+    if (int rc = check_rows("attn_bwd k", *k, s->d)) return rc;
+    if (int rc = check_rows("attn_bwd v", *v, s->d)) return rc;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
+  const int64_t nrow = s->hq * s->total_q;
+  RowPrep w;
+  w.lse2 = (float*)workspace, w.delta = w.lse2 + nrow, w.rscale = w.delta + nrow, w.amax = w.rscale + nrow;
+  w.nblk = (int)((s->total_q + PB - 1) / PB);
+  const uint16_t* g = (const uint16_t*)dout;
+#define ATTN_BWD(D, DT)                                                                                                  \
+  constexpr int NW = WAVES<D>;                                                                                           \
+  unsigned gq = 0, gk = 0;                                                                                               \
+  const int64_t tq = s->total_q ? num_tiles(*s, cu_q, s->total_q, NW * 32) : 0;                                          \
+  const int64_t tk = s->total_k ? num_tiles(*s, cu_k, s->total_k, NW * 32) : 0;                                          \
+  if (int rc = tile_grid("attn_bwd", tq, s->hq, &gq)) return rc;                                                         \
+  if (int rc = tile_grid("attn_bwd", tk, s->hk, &gk)) return rc;                                                         \
+  if (gq)                                                                                                                \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_prep_kernel<D, DT>), dim3(w.nblk, (unsigned)s->hq), dim3(256),  \
+                                                   0, st, (const uint16_t*)o, g, lse, dlse, a.total_q, a.hq, w));        \
+  if (gk) {                                                                                                              \
+    a.ntiles = (int)tk;                                                                                                  \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, a, g, w, \
+                                                   scale, (uint16_t*)dk, (uint16_t*)dv));                                \
+  }                                                                                                                      \
+  if (gq) {                                                                                                              \
+    a.ntiles = (int)tq;                                                                                                  \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a, g, w,  \
+                                                   scale, (uint16_t*)dq));                                               \
+  }
+  ATTN_DISPATCH(ATTN_BWD);
+#undef ATTN_BWD
+  return LSURGE_OK;
+}
+
+}  // extern "C"

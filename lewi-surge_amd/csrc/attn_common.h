@@ -1,0 +1,177 @@
+// Device helpers of the softmax attention kernels (attn.hip, attn_decode.hip): 16-bit matrix-core products, the LDS tile
+// layout and its copies, and the lookup of a packed sequence's tiles.
+#pragma once
+#include "gemm_kernels.h"
+
+namespace lsattn {
+
+using lsgemm::copy16;
+using lsgemm::lds_addr;
+using lsgemm::make_rsrc;
+using lsgemm::stage_barrier;
+using lsgemm::u32x2;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Products of the 16-bit type DT (LSURGE_BF16 or LSURGE_F16) with f32 sums.  mma32: D[32 x 32] += P[32 x 16] Q[16 x 32];
+// lane l supplies row l % 32 of P and column l % 32 of Q at k = 8 (l / 32) .. + 7 and holds
+// D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32] in register r.  mma16: D[16 x 16] += P[16 x 32] Q[32 x 16]; lane l supplies
+// row / column l % 16 at k = 8 (l / 16) .. + 7 and holds D[4 (l / 16) + r][l % 16].
+template <int DT>
+__device__ __forceinline__ f32x16 mma32(u32x4 p, u32x4 q, f32x16 c) {
+  if constexpr (DT == LSURGE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ f32x4 mma16(u32x4 p, u32x4 q, f32x4 c) {
+  if constexpr (DT == LSURGE_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+// two f32 -> two values of DT in one register, rounded to nearest even
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == LSURGE_F16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, f16x2_t));
+  else
+    return pack_bf16x2(lo, hi);
+}
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t v, float& lo, float& hi) {
+  if constexpr (DT == LSURGE_F16) {
+    lo = f16_to_f32((uint16_t)v);
+    hi = f16_to_f32((uint16_t)(v >> 16));
+  } else {
+    lo = __uint_as_float(v << 16);
+    hi = __uint_as_float(v & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// a value's partner in the other half of the wave (lane ^ 32), combined with op; both halves get the result
+template <class Op>
+__device__ __forceinline__ float halves(float x, Op&& op) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// ------------------------------------------------------------------------------------ LDS tiles
+// A tile holds rows of D 16-bit values, row-major, its 16-byte chunks permuted within a row: logical chunk c of row r
+// lies at chunk c ^ swz(r).  Both kinds of read are then free of bank conflicts.  A row read (ds_read_b128: 16 rows at
+// one chunk) needs 16 different places among the 16 chunks that fill the banks once: swz is one-to-one on 16 rows (for
+// D = 64, whose row fills half of the banks, on 8 row pairs).  A transpose read (ds_read_b64_tr_b16: 4 consecutive rows,
+// 4 aligned chunks of each) needs the rows in different groups of 4 chunks: the low row bits go to the upper bits.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 64) return ((r >> 1 & 1) << 2) | (r >> 2 & 3);
+  else return ((r & 3) << 2) | (r >> 2 & 3);
+}
+
+// Copies of a ROWS x D tile by NW waves straight into LDS, 1 KiB each: copy c fills chunks 64 c .. + 63.
+template <int D, int ROWS, int NW>
+struct TileCopy {
+  static constexpr int CPR = D / 8;                       // chunks per row
+  static constexpr int N = ROWS * CPR / 64 / NW;          // copies per wave
+  static_assert(N * 64 * NW == ROWS * CPR, "whole copies");
+  uint32_t off[N];  // this lane's byte offset in the source for each copy
+  __device__ __forceinline__ void init(int64_t row_stride, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = (wave * N + i) * 64 + lane, row = id / CPR, pc = id % CPR;
+      off[i] = (uint32_t)(row * (int)row_stride * 2 + ((pc ^ swz<D>(row)) * 16));
+    }
+  }
+  // rows [0, rows) of the tile that starts at `base`; the others are filled with zeros
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t row_stride, int rows, uint32_t lds, int wave) const {
+    const int n = min(rows, ROWS);
+    const u32x4 rs = make_rsrc(base, n > 0 ? (int64_t)(n - 1) * row_stride * 2 + D * 2 : 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) copy16(rs, off[i], lds + (wave * N + i) * 1024);
+  }
+};
+
+// 64 consecutive 4-byte values, lane p's at LDS byte address m0 + 4 p
+__device__ __forceinline__ void copy4(u32x4 rsrc, uint32_t byte_off, uint32_t m0) {
+  const uint32_t m0s = (uint32_t)__builtin_amdgcn_readfirstlane(m0);
+  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(byte_off), "s"(rsrc), "s"(m0s)
+               : "memory");
+}
+
+// Fragment addresses of a tile at LDS byte address `base` (a multiple of 1024).
+// rows: lane l holds row r0 + l % 32 at k = 16 s + 8 (l / 32) .. + 7, read from row_addr ^ (s * 32), r0 a multiple of 32
+template <int D>
+__device__ __forceinline__ uint32_t row_addr(int lane) {
+  const int r = lane & 31;
+  return (uint32_t)(r * D * 2 + (((lane >> 5) ^ swz<D>(r)) << 4));
+}
+typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ u32x4 lds_read16(uint32_t a) { return *(lds_u32x4*)(uintptr_t)a; }
+// columns: lane l holds column m0 + l % 32 (m0 = 32 dt) at the 8 rows k0 + 4 (l / 32) + {0..3, 8..11}, k0 a multiple of
+// 16: the rows whose scores lane l holds in 8 consecutive registers of a 32 x 32 product, so a product's result is
+// the next product's operand without leaving its lane
+template <int D>
+__device__ __forceinline__ uint32_t col_addr(int lane, int dt) {
+  const int g = lane >> 4, s = lane & 15;
+  const int r = 4 * (g >> 1) + (s >> 2), c = 32 * dt + 16 * (g & 1) + 4 * (s & 3);
+  return (uint32_t)(r * D * 2 + (((c >> 3) ^ swz<D>(r)) << 4) + (c & 7) * 2);
+}
+// r + 8 has another swizzle than r: bit 1 of row / 4 flips, so chunk bit 1 does
+template <int D>
+__device__ __forceinline__ u32x4 lds_read_col(uint32_t a) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)a);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((a ^ 32u) + 8 * D * 2));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(u32x4, v);
+}
+
+// ------------------------------------------------------------------------------------ packed sequences
+// Sequence s holds rows [cu[s], cu[s + 1]) (cu ascending from 0), or, without cu, total / nseq rows each.  Entries are
+// held to [0, total], so that no table makes a kernel read or write outside its rows.
+__device__ __forceinline__ int cu_at(const int32_t* cu, int i, int total) { return min(max(cu[i], 0), total); }
+
+// Tile t of the rows: sequence s owns the tiles from cu[s] / B + s, which leaves it at least ceil(rows / B).  Returns the
+// sequence (wave-uniform, by a 64-way search), or -1.
+template <int B>
+__device__ __forceinline__ int seq_of_tile(const int32_t* cu, int nseq, int total, int t, int lane, int& tile) {
+  if (!cu) {
+    const int per = total / nseq, tiles = (per + B - 1) / B;
+    if (tiles == 0 || t / tiles >= nseq) return -1;
+    tile = t % tiles;
+    return t / tiles;
+  }
+  int lo = 0, n = nseq;
+  while (true) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const bool in = lane * step < n && cu_at(cu, i, total) / B + i <= t;
+    const int c = __popcll(__ballot(in));
+    if (c == 0) return -1;
+    n = min(step, n - (c - 1) * step);
+    lo += (c - 1) * step;
+    if (step == 1) break;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  tile = t - (cu_at(cu, lo, total) / B + lo);
+  return tile < 0 ? -1 : lo;
+}
+__device__ __forceinline__ void seq_rows(const int32_t* cu, int nseq, int total, int s, int& r0, int& n) {
+  if (cu) {
+    r0 = cu_at(cu, s, total);
+    n = max(0, cu_at(cu, s + 1, total) - r0);
+  } else {
+    n = total / nseq;
+    r0 = s * n;
+  }
+  r0 = __builtin_amdgcn_readfirstlane(r0);
+  n = __builtin_amdgcn_readfirstlane(n);
+}
+
+}  // namespace lsattn

@@ -1,0 +1,462 @@
+// Attention of one new token per sequence over a paged key-value cache, and the write of new tokens into its pages.
+//
+// Cache: pages of `page_size` tokens; page p's key of head h at slot t starts at k + p page_stride + h head_stride + t
+// slot_stride (elements; v alike).  page_table[b][i] is the page of sequence b's tokens [i page_size, (i + 1) page_size).
+// An entry outside [0, num_pages) names no page: its tokens are left out (read) or not written.
+//
+// Bound by the cache's bytes: 4 D bytes a token and key head are read once for all query heads that share it, and the
+// 4 D flops a query head needs for them are a few percent of the matrix cores' rate even with one head a group.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "launchers.h"
+
+namespace lsattn {
+namespace {
+
+struct CacheArgs {
+  const uint16_t *k, *v;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+  const int32_t* table;
+  int64_t table_stride;
+  int num_pages, max_pages, page_log2;
+};
+
+// ------------------------------------------------------------------------------------ one token per sequence
+// Work is dealt by the keys that are there, not by sequence: the units of UK keys of every (sequence, key head) in a row
+// are cut into equal shares, one a workgroup, so a batch of uneven lengths keeps every CU equally busy and the host needs
+// no lengths.  A workgroup's share is a run of pieces, each of one (sequence, head); a piece that is the whole of it is
+// written out, another goes to the workspace (slot 0: the share began inside it; slot 1: it ends past the share) and the
+// join kernel adds the pieces of a (sequence, head) up in order.
+constexpr int DW = 4;             // waves of a workgroup; each takes 32 keys at a time
+constexpr int UK = DW * 32;       // keys of a unit
+constexpr int DT_THREADS = DW * 64;
+
+struct DecodeArgs {
+  CacheArgs c;
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  const int32_t* lens;
+  int nseq, hq, hk, group, hblocks;  // hblocks: blocks of 16 query heads a group
+  float scale2;
+  uint16_t* o;
+  float* lse;  // [nseq, hq] or null
+  float *po, *pm;  // [grid][2][16][D], [grid][2][2][16] (maximum in base 2, sum)
+  int grid;
+};
+
+__device__ __forceinline__ int seq_len(const DecodeArgs& a, int b) {
+  const int64_t cap = (int64_t)a.c.max_pages << a.c.page_log2;
+  return (int)min((int64_t)max(a.lens[b], 0), cap);
+}
+__device__ __forceinline__ int seq_units(const DecodeArgs& a, int b) { return (seq_len(a, b) + UK - 1) / UK; }
+
+// Sums of the units per head of sequences [slab i, slab i + 1) into pre[i] (exclusive), by all threads; pre[threads] is
+// the total.  int64: 2^24 sequences of 2^31 keys stay in range.
+__device__ __forceinline__ int slab_size(const DecodeArgs& a) { return (a.nseq + DT_THREADS - 1) / DT_THREADS; }
+__device__ void unit_prefix(const DecodeArgs& a, int64_t* pre) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slab = slab_size(a);
+  __shared__ int64_t wsum[DW];
+  int64_t mine = 0;
+  for (int i = 0; i < slab; ++i) {
+    const int b = tid * slab + i;
+    if (b < a.nseq) mine += seq_units(a, b);
+  }
+  int64_t x = mine;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int64_t y = __shfl_up(x, s, 64);
+    if (lane >= s) x += y;
+  }
+  if (lane == 63) wsum[wave] = x;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) x += wsum[w];
+  pre[tid] = x - mine;
+  if (tid == DT_THREADS - 1) pre[DT_THREADS] = x;
+  __syncthreads();
+}
+// units of a share when `total` units are dealt to the grid
+__device__ __forceinline__ int64_t share(const DecodeArgs& a, int64_t total) { return max((total + a.grid - 1) / a.grid, (int64_t)1); }
+
+template <int D, int DT>
+__global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
+  constexpr int KC = D / 32, VE = D / 16, VW = VE / 2;  // VW: registers of a value row's piece
+  __shared__ int64_t pre[DT_THREADS + 1];
+  __shared__ __attribute__((aligned(16))) float so[DW][16][D];
+  __shared__ float sm[DW][16], sl[DW][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 15, g = lane >> 4;
+  unit_prefix(a, pre);
+  const int heads = a.hk * a.hblocks;
+  const int64_t total = pre[DT_THREADS] * heads, per = share(a, total);
+  int64_t u = blockIdx.x * per;
+  const int64_t uend = min(total, u + per);
+  if (u >= uend) return;
+  // the sequence of the first unit: the last slab that starts at or before it, then one by one
+  int b;
+  int64_t base;  // units before sequence b (all heads)
+  {
+    int lo = 0, hi = DT_THREADS;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (pre[mid] * heads <= u) lo = mid;
+      else hi = mid;
+    }
+    b = lo * slab_size(a);
+    base = pre[lo] * heads;
+  }
+  const int pmask = (1 << a.c.page_log2) - 1;
+  while (u < uend) {
+    int len = seq_len(a, b);
+    int64_t nu = (len + UK - 1) / UK;
+    while (base + nu * heads <= u) {
+      base += nu * heads;
+      ++b;
+      len = seq_len(a, b);
+      nu = (len + UK - 1) / UK;
+    }
+    const int hb = (int)((u - base) / nu);
+    const int64_t item = base + hb * nu;  // first unit of this (sequence, head block)
+    const int u0 = (int)(u - item), u1 = (int)min(nu, uend - item);
+    const int kvh = hb / a.hblocks, h0 = kvh * a.group + hb % a.hblocks * 16;
+    const int nh = min(16, (kvh + 1) * a.group - h0);
+    const int32_t* tab = a.c.table + b * a.c.table_stride;
+    const uint16_t* kb = a.c.k + kvh * a.c.k_head + 8 * g;
+    const uint16_t* vb = a.c.v + kvh * a.c.v_head + VE * ln;
+
+    u32x4 qf[KC];
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+      qf[j] = ln < nh ? *reinterpret_cast<const u32x4*>(a.q + b * a.q_row + (h0 + ln) * a.q_head + 32 * j + 8 * g)
+                      : u32x4{0, 0, 0, 0};
+    f32x4 acc[VE];
+#pragma unroll
+    for (int t = 0; t < VE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    for (int uu = u0; uu < u1; ++uu) {
+      const int key0 = uu * UK + wave * 32;
+      if (key0 >= len) break;
+      // pages of this lane's keys (rows 16 t + l % 16) and of its values (rows 16 t + 4 (l / 16) .. + 3)
+      int64_t ko[2], vo[2];
+      bool vok[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int kk = key0 + 16 * t + ln, kv = key0 + 16 * t + 4 * g;
+        const int kp = kk < len ? tab[kk >> a.c.page_log2] : -1, vp = kv < len ? tab[kv >> a.c.page_log2] : -1;
+        const bool kok = (unsigned)kp < (unsigned)a.c.num_pages;
+        vok[t] = (unsigned)vp < (unsigned)a.c.num_pages;
+        ko[t] = kok ? kp * a.c.k_page + (kk & pmask) * a.c.k_slot : 0;
+        vo[t] = vok[t] ? vp * a.c.v_page + (kv & pmask) * a.c.v_slot : 0;
+      }
+      u32x4 kr[2][KC];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < KC; ++j) kr[t][j] = *reinterpret_cast<const u32x4*>(kb + ko[t] + 32 * j);
+      uint32_t vr[8][VW];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // a page's slots are followed by 3 more here (pages hold multiples of 8 tokens); without a page, token 0 of page 0
+        const uint16_t* p = vb + vo[i / 4] + (vok[i / 4] ? i % 4 * a.c.v_slot : 0);
+        if constexpr (VW == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          vr[i][0] = x[0], vr[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int c = 0; c < VW / 4; ++c) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p + 8 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[i][4 * c + e] = x[e];
+          }
+        }
+      }
+      f32x4 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KC; ++j) s[t] = mma16<DT>(kr[t][j], qf[j], s[t]);
+      }
+      if (!__all(vok[0] && vok[1] && key0 + 32 <= len)) {  // keys past the end or without a page: weight 0, value 0
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!vok[i / 4] || key0 + 16 * (i / 4) + 4 * g + i % 4 >= len) {
+            s[i / 4][i % 4] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < VW; ++c) vr[i][c] = 0;
+          }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+      const float mc = mx == -INFINITY ? 0.f : mx * a.scale2;
+      const float alpha = exp2_hw(m * a.scale2 - mc);
+      m = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[t][r] = exp2_hw(fmaf(s[t][r], a.scale2, -mc));
+          sum += s[t][r];
+        }
+      l = l * alpha + sum;
+      const u32x4 p = {pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]),
+                       pack2<DT>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int t = 0; t < VE; ++t) {
+        const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;  // the pair's high or low halves
+        u32x4 f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2], sel);
+        f32x4 c = acc[t];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] *= alpha;
+        acc[t] = mma16<DT>(f, p, c);
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // the waves' pieces, joined in wave order
+    if (g == 0) {
+      sm[wave][ln] = m;
+      sl[wave][ln] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < VE; t += 4)
+        *reinterpret_cast<f32x4*>(&so[wave][ln][VE * (4 * g + r) + t]) =
+            f32x4{acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]};
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == nu;
+    const int64_t slot = blockIdx.x * 2 + (u0 == 0);
+    for (int i = tid; i < nh * (D / 4); i += DT_THREADS) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float mm = sm[0][h];
+#pragma unroll
+      for (int w = 1; w < DW; ++w) mm = fmaxf(mm, sm[w][h]);
+      const float mc = mm == -INFINITY ? 0.f : mm * a.scale2;
+      float ll = 0.f;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < DW; ++w) {
+        const float f = exp2_hw(sm[w][h] * a.scale2 - mc);
+        ll += f * sl[w][h];
+        x += f * *reinterpret_cast<const f32x4*>(&so[w][h][d]);
+      }
+      if (whole) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        *reinterpret_cast<u32x2*>(a.o + ((int64_t)b * a.hq + h0 + h) * D + d) =
+            u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+        if (a.lse && d == 0) a.lse[(int64_t)b * a.hq + h0 + h] = ll == 0.f ? -INFINITY : (mc + __log2f(ll)) * LN2;
+      } else {
+        *reinterpret_cast<f32x4*>(a.po + (slot * 16 + h) * D + d) = x;
+        if (d == 0) {
+          a.pm[slot * 32 + h] = ll == 0.f ? -INFINITY : mc;
+          a.pm[slot * 32 + 16 + h] = ll;
+        }
+      }
+    }
+    __syncthreads();
+    u = item + u1;
+  }
+}
+
+// One workgroup per (sequence, head block): adds up the pieces that the shares cut it into, in order; writes zeros for a
+// sequence without keys.
+template <int D, int DT>
+__global__ __launch_bounds__(DT_THREADS) void attn_join_kernel(DecodeArgs a) {
+  __shared__ int64_t pre[DT_THREADS + 1];
+  const int heads = a.hk * a.hblocks, b = blockIdx.x / heads, hb = blockIdx.x % heads, tid = threadIdx.x;
+  const int kvh = hb / a.hblocks, h0 = kvh * a.group + hb % a.hblocks * 16, nh = min(16, (kvh + 1) * a.group - h0);
+  unit_prefix(a, pre);
+  const int slab = slab_size(a);
+  int64_t base = pre[b / slab];
+  for (int i = b / slab * slab; i < b; ++i) base += seq_units(a, i);
+  const int64_t per = share(a, pre[DT_THREADS] * heads), nu = seq_units(a, b);
+  const int64_t first = base * heads + hb * nu;
+  const int64_t w0 = first / per, w1 = nu ? (first + nu - 1) / per : w0;
+  if (nu && w0 == w1) return;
+  for (int i = tid; i < nh * (D / 4); i += DT_THREADS) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (nu) {
+      for (int64_t w = w0; w <= w1; ++w) m = fmaxf(m, a.pm[(w * 2 + (w == w0)) * 32 + h]);
+      for (int64_t w = w0; w <= w1; ++w) {
+        const int64_t slot = w * 2 + (w == w0);
+        const float pm = a.pm[slot * 32 + h], f = pm == -INFINITY ? 0.f : exp2_hw(pm - m);
+        l += f * a.pm[slot * 32 + 16 + h];
+        x += f * *reinterpret_cast<const f32x4*>(a.po + (slot * 16 + h) * D + d);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<u32x2*>(a.o + ((int64_t)b * a.hq + h0 + h) * D + d) =
+        u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+    if (a.lse && d == 0) a.lse[(int64_t)b * a.hq + h0 + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+  }
+}
+
+// ------------------------------------------------------------------------------------ writing to the cache
+// One 16-byte chunk a thread.  The new tokens of sequence b, rows [cu[b], cu[b + 1]) of k and v (without cu: row b), are
+// the last ones of its seq_lens[b].
+struct AppendArgs {
+  CacheArgs c;
+  const uint16_t *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  const int32_t *cu, *lens;
+  int nseq, rows, hk, dchunks;
+};
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
+  const int64_t n = (int64_t)a.rows * a.hk * a.dchunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int row = (int)(i / (a.hk * a.dchunks)), rest = (int)(i % (a.hk * a.dchunks));
+    const int h = rest / a.dchunks, c = rest % a.dchunks * 8;
+    int b = row, after = 1;  // tokens from this one to the sequence's end
+    if (a.cu) {
+      int lo = 0, hi = a.nseq;  // the last sequence that starts at or before the row
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu[mid] <= row) lo = mid;
+        else hi = mid;
+      }
+      b = lo;
+      if (a.nseq == 0 || a.cu[b] > row) continue;
+      after = a.cu[b + 1] - row;
+      if (after <= 0) continue;  // behind the last sequence
+    }
+    const int pos = max(a.lens[b], 0) - after;
+    if (pos < 0 || (pos >> a.c.page_log2) >= a.c.max_pages) continue;
+    const int page = a.c.table[b * a.c.table_stride + (pos >> a.c.page_log2)];
+    if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
+    const int slot = pos & ((1 << a.c.page_log2) - 1);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(a.k + row * a.k_row + h * a.k_head + c);
+    const u32x4 y = *reinterpret_cast<const u32x4*>(a.v + row * a.v_row + h * a.v_head + c);
+    *reinterpret_cast<u32x4*>(const_cast<uint16_t*>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot + h * a.c.k_head + c) = x;
+    *reinterpret_cast<u32x4*>(const_cast<uint16_t*>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot + h * a.c.v_head + c) = y;
+  }
+}
+
+// ------------------------------------------------------------------------------------ host
+int check_cache(const char* what, const lsurge_kv_cache* c, CacheArgs* a) {
+  LSURGE_REQUIRE(c, "%s: null cache", what);
+  LSURGE_REQUIRE(c->d == 64 || c->d == 128 || c->d == 256, "%s: head_dim %lld (64, 128 or 256)", what, (long long)c->d);
+  LSURGE_REQUIRE(c->heads >= 1 && c->heads <= 65535, "%s: %lld key heads", what, (long long)c->heads);
+  LSURGE_REQUIRE(c->num_pages >= 1 && c->num_pages < (1ll << 31) && c->max_pages >= 1 && c->max_pages < (1ll << 31) &&
+                     c->table_stride >= c->max_pages,
+                 "%s: num_pages=%lld max_pages=%lld table_stride=%lld", what, (long long)c->num_pages,
+                 (long long)c->max_pages, (long long)c->table_stride);
+  int lg = 3;
+  while (lg < 12 && (1ll << lg) < c->page_size) ++lg;
+  LSURGE_REQUIRE((1ll << lg) == c->page_size, "%s: page_size %lld (a power of two from 8 to 4096)", what,
+                 (long long)c->page_size);
+  LSURGE_REQUIRE(c->k && c->v && c->page_table && c->seq_lens, "%s: null pointer", what);
+  LSURGE_REQUIRE(((uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0, "%s: the caches must be 16-byte aligned", what);
+  for (const int64_t st : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride,
+                           c->v_head_stride})
+    LSURGE_REQUIRE(st >= 0 && st < (1ll << 40) && st % 8 == 0,
+                   "%s: cache stride %lld (elements; a multiple of 8 in [0, 2^40))", what, (long long)st);
+  if (c->dtype != LSURGE_BF16 && c->dtype != LSURGE_F16) return lsurge::set_error(LSURGE_ERR_DTYPE, "%s: bf16 or f16", what);
+  a->k = (const uint16_t*)c->k, a->v = (const uint16_t*)c->v;
+  a->k_page = c->k_page_stride, a->k_slot = c->k_slot_stride, a->k_head = c->k_head_stride;
+  a->v_page = c->v_page_stride, a->v_slot = c->v_slot_stride, a->v_head = c->v_head_stride;
+  a->table = c->page_table, a->table_stride = c->table_stride;
+  a->num_pages = (int)c->num_pages, a->max_pages = (int)c->max_pages, a->page_log2 = lg;
+  return LSURGE_OK;
+}
+int check_new_rows(const char* what, const lsurge_attn_rows* r) {
+  LSURGE_REQUIRE(r && r->data && (uintptr_t)r->data % 16 == 0, "%s: null or misaligned rows", what);
+  LSURGE_REQUIRE(r->row_stride >= 0 && r->row_stride < (1ll << 40) && r->head_stride >= 0 && r->head_stride < (1ll << 40) &&
+                     r->row_stride % 8 == 0 && r->head_stride % 8 == 0,
+                 "%s: row and head strides (%lld, %lld elements) must be multiples of 8 in [0, 2^40)", what,
+                 (long long)r->row_stride, (long long)r->head_stride);
+  return LSURGE_OK;
+}
+
+constexpr int DECODE_GRID = 512;
+int64_t decode_grid(int64_t nseq, int64_t hk, int64_t hblocks, int64_t max_pages, int64_t page_size) {
+  const double most = (double)nseq * hk * hblocks * (((double)max_pages * page_size + UK - 1) / UK);
+  return most < DECODE_GRID ? std::max<int64_t>(1, (int64_t)most) : DECODE_GRID;
+}
+
+}  // namespace
+}  // namespace lsattn
+
+using namespace lsattn;
+
+extern "C" {
+
+size_t lsurge_paged_attn_workspace_bytes(int64_t d) {
+  if (d < 1 || d > 256) return 0;
+  return sizeof(float) * (size_t)DECODE_GRID * 2 * 16 * (size_t)(d + 2);
+}
+
+int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64_t nseq, int64_t hq, float scale, void* o,
+                      float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
+  DecodeArgs a;
+  if (int rc = check_cache("paged_attn", c, &a.c)) return rc;
+  LSURGE_REQUIRE(nseq >= 0 && nseq < (1 << 24) && hq >= c->heads && hq % c->heads == 0 && hq <= 65535,
+                 "paged_attn: nseq=%lld, %lld query heads over %lld key heads", (long long)nseq, (long long)hq,
+                 (long long)c->heads);
+  LSURGE_REQUIRE(scale > 0.f && scale < INFINITY, "paged_attn: scale must be positive and finite");
+  if (nseq == 0) return LSURGE_OK;
+  if (int rc = check_new_rows("paged_attn q", q)) return rc;
+  LSURGE_REQUIRE(o && workspace && ((uintptr_t)o | (uintptr_t)workspace) % 16 == 0, "paged_attn: null or misaligned pointer");
+  const size_t need = lsurge_paged_attn_workspace_bytes(c->d);
+  if (workspace_bytes < need)
+    return lsurge::set_error(LSURGE_ERR_WORKSPACE, "paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
+  LSURGE_REQUIRE((int64_t)c->max_pages * c->page_size < (1ll << 31), "paged_attn: %lld pages of %lld tokens a sequence",
+                 (long long)c->max_pages, (long long)c->page_size);
+  a.q = (const uint16_t*)q->data, a.q_row = q->row_stride, a.q_head = q->head_stride;
+  a.lens = c->seq_lens;
+  a.nseq = (int)nseq, a.hq = (int)hq, a.hk = (int)c->heads, a.group = (int)(hq / c->heads);
+  a.hblocks = (a.group + 15) / 16;
+  a.scale2 = scale * LOG2E;
+  a.o = (uint16_t*)o, a.lse = lse;
+  a.grid = (int)decode_grid(nseq, a.hk, a.hblocks, c->max_pages, c->page_size);
+  a.po = (float*)workspace;
+  a.pm = a.po + (size_t)DECODE_GRID * 2 * 16 * c->d;
+  const int64_t items = nseq * a.hk * a.hblocks;
+  LSURGE_REQUIRE(items < (1ll << 31), "paged_attn: %lld sequences of %lld heads", (long long)nseq, (long long)hq);
+  hipStream_t st = (hipStream_t)stream;
+#define DECODE(D, DT)                                                                                              \
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_decode_kernel<D, DT>), dim3(a.grid), dim3(DT_THREADS), 0, st, a)); \
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_join_kernel<D, DT>), dim3((unsigned)items), dim3(DT_THREADS), 0, st, a))
+  if (c->dtype == LSURGE_BF16) {
+    if (c->d == 64) { DECODE(64, LSURGE_BF16); }
+    else if (c->d == 128) { DECODE(128, LSURGE_BF16); }
+    else { DECODE(256, LSURGE_BF16); }
+  } else {
+    if (c->d == 64) { DECODE(64, LSURGE_F16); }
+    else if (c->d == 128) { DECODE(128, LSURGE_F16); }
+    else { DECODE(256, LSURGE_F16); }
+  }
+#undef DECODE
+  return LSURGE_OK;
+}
+
+int lsurge_kv_append(const lsurge_kv_cache* c, const lsurge_attn_rows* k, const lsurge_attn_rows* v, int64_t rows,
+                     int64_t nseq, const int32_t* cu, lsurge_stream_t stream) {
+  AppendArgs a;
+  if (int rc = check_cache("kv_append", c, &a.c)) return rc;
+  LSURGE_REQUIRE(rows >= 0 && rows < (1ll << 31) && nseq >= 0 && nseq < (1 << 24) && (cu || rows == nseq),
+                 "kv_append: %lld rows for %lld sequences", (long long)rows, (long long)nseq);
+  if (rows == 0 || nseq == 0) return LSURGE_OK;
+  if (int rc = check_new_rows("kv_append k", k)) return rc;
+  if (int rc = check_new_rows("kv_append v", v)) return rc;
+  a.k = (const uint16_t*)k->data, a.k_row = k->row_stride, a.k_head = k->head_stride;
+  a.v = (const uint16_t*)v->data, a.v_row = v->row_stride, a.v_head = v->head_stride;
+  a.cu = cu, a.lens = c->seq_lens;
+  a.nseq = (int)nseq, a.rows = (int)rows, a.hk = (int)c->heads, a.dchunks = (int)c->d / 8;
+  const int64_t chunks = rows * a.hk * a.dchunks;
+  const unsigned grid = (unsigned)std::min<int64_t>((chunks + 255) / 256, 16384);
+  hipStream_t st = (hipStream_t)stream;
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL(kv_append_kernel, dim3(grid), dim3(256), 0, st, a));
+  return LSURGE_OK;
+}
+
+}  // extern "C"

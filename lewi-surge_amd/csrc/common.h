@@ -153,6 +153,7 @@ enum {
   KID_GDN_BSCAN,
   KID_GDN_BGRAD,
   KID_GDN_BCHUNK,
+  KID_ATTN,
   KID_COUNT
 };
 
