@@ -3,8 +3,8 @@
 // Query i of a sequence with nq queries and nk keys attends to the keys j <= i + nk - nq (the queries are the last ones):
 //   s_ij = scale q_i . k_j,  o_i = sum_j e^(s_ij - lse_i) v_j,  lse_i = log sum_j e^(s_ij)
 // and o_i = 0, lse_i = -inf for a query with no key.  Scores and sums are f32, in base 2 (the scale carries log2 e); the
-// weights are rounded to the operands' type for the second product, as its operands have to be (at most 1, relative error
-// 2^-9 in bf16, and what is rounded off is not summed into the denominator, so errors average out over the keys).
+// weights are rounded to the operands' type for the second product, as its operands have to be (half a step of the type,
+// relative to each weight, so that errors average out over the keys; the denominator sums them unrounded).
 //
 // Every product is formed transposed: S^T = K Q^T has a query per lane (column l % 32), so a row's maximum and sum are
 // sums over a lane's own registers and one exchange with lane ^ 32, the accumulators O^T = V^T P^T have the same query in
@@ -49,16 +49,66 @@ __device__ __forceinline__ void zero_rows(uint16_t* p, int64_t first, int n, int
     *reinterpret_cast<u32x4*>(p + ((first + i / (D / 8)) * heads + head) * D + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
 }
 
-// ------------------------------------------------------------------------------------ forward
-constexpr int BN = 64;  // keys per stage
+// Issue orders for the compiler's scheduler.  feed: MFMAS products that take READS LDS reads each, AHEAD reads issued
+// before the first, the others spread between the products.
+enum { SG_VALU = 0x2, SG_MFMA = 0x8, SG_DS_R = 0x100, SG_TRANS = 0x400 };
+template <int MFMAS, int READS, int AHEAD>
+__device__ __forceinline__ void feed() {
+  __builtin_amdgcn_sched_group_barrier(SG_DS_R, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+    if (i < MFMAS - AHEAD / READS) __builtin_amdgcn_sched_group_barrier(SG_DS_R, READS, 0);
+  }
+}
+// interleave: MFMAS products of one LDS read each (AHEAD reads first) with a softmax's arithmetic between them
+template <int MFMAS, int AHEAD>
+__device__ __forceinline__ void interleave() {
+  __builtin_amdgcn_sched_group_barrier(SG_DS_R, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+    if (i < MFMAS - AHEAD) __builtin_amdgcn_sched_group_barrier(SG_DS_R, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(SG_VALU, (64 + MFMAS - 1) / MFMAS, 0);
+    if (i >= MFMAS / 4) __builtin_amdgcn_sched_group_barrier(SG_TRANS, (24 + MFMAS - 1) / MFMAS, 0);
+  }
+}
 
-// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 64, double-buffered in LDS:
-// one barrier a stage, the next stage's copies in flight during the products of this one.
+// ------------------------------------------------------------------------------------ forward
+constexpr int FN = 32;  // keys per stage of the forward
+constexpr int BN = 64;  // keys per stage of the pass over queries
+
+// acc *= f.  At D = 256 the accumulators fill half of the registers and have to stay in the accumulation file, which the
+// vector unit cannot work on: written as plain products, the compiler moves all of them to the other file and back in
+// every stage (256 moves for 32 matrix instructions).  They go through a temporary here, in the rare branch only; the
+// no-ops cover the distance that a matrix instruction's result needs before it is read, and a move's before the next.
+template <int D>
+__device__ __forceinline__ void rescale(f32x16& acc, float f) {
+  if constexpr (D == 256) {
+    asm volatile("s_nop 15\n\ts_nop 7" ::: );
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float x = acc[r], t;
+      asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                   : "+a"(x), "=&v"(t) : "v"(f));
+      acc[r] = x;
+    }
+    asm volatile("s_nop 7" ::: );
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] *= f;
+  }
+}
+
+// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a three-deep LDS
+// ring.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
+// work at the same time; one barrier a stage.
+template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
 template <int D, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(FWD_EU<D>)))
 void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ lse) {
-  constexpr int BM = NW * 32, TILE = BN * D * 2;  // bytes of one operand of one stage
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+  constexpr int BM = NW * 32, TILE = FN * D * 2;  // bytes of one operand of one stage
+  __shared__ __attribute__((aligned(1024))) char smem[6 * TILE];  // three stages of K, then three of V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   int head, slot;
@@ -81,6 +131,29 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
   const int kvh = head / (a.hq / a.hk);
 
+  const uint32_t lds = lds_addr((const bf16_t*)smem);
+  TileCopy<D, FN, NW> ck, cv;
+  ck.init(a.k_row, wave, lane);
+  cv.init(a.v_row, wave, lane);
+  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
+  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
+  const int kend = min(nq, (tile + 1) * BM) + off;  // keys the workgroup's last row sees
+  const int nst = (max(kend, 0) + FN - 1) / FN;
+  const int nsw = min(nst, (max(w0 + 32 + off, 0) + FN - 1) / FN);  // stages that the wave's rows see
+  auto issue_k = [&](int st, int slot) {  // stages past the end fill with zeros
+    ck.issue(kb + (int64_t)st * FN * a.k_row, a.k_row, nk - st * FN, lds + slot * TILE, wave);
+  };
+  auto issue_v = [&](int st, int slot) {
+    cv.issue(vb + (int64_t)st * FN * a.v_row, a.v_row, nk - st * FN, lds + (3 + slot) * TILE, wave);
+  };
+  constexpr int CP = 2 * TileCopy<D, FN, NW>::N;  // copies of a stage
+  if (nst) {
+    issue_k(0, 0);
+    issue_v(0, 0);
+    issue_k(1, 1);
+    issue_v(1, 1);
+    issue_k(2, 2);
+  }
   u32x4 qf[D / 16];
   {
     const uint16_t* qp = a.q + (int64_t)(q0 + min(row, nq - 1)) * a.q_row + head * a.q_head + 8 * hf;
@@ -92,81 +165,90 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-  float m = -INFINITY, l = 0.f;  // m: running maximum of the raw scores; l: this half's share of the row's sum
+  // m: base of the weights, in base 2 (mc: 0 before the first); l: this half's share of the row's sum
+  float m = -INFINITY, mc = 0.f, l = 0.f;
+  const uint32_t ka = lds + row_addr<D>(lane);
+  uint32_t va[COLS<D>];
+#pragma unroll
+  for (int t = 0; t < COLS<D>; ++t) va[t] = lds + 3 * TILE + col_addr<D>(lane, t);
 
-  const uint32_t lds = lds_addr((const bf16_t*)smem);
-  TileCopy<D, BN, NW> ck, cv;
-  ck.init(a.k_row, wave, lane);
-  cv.init(a.v_row, wave, lane);
-  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
-  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
-  const int kend = min(nq, (tile + 1) * BM) + off;  // keys the workgroup's last row sees
-  const int nst = (max(kend, 0) + BN - 1) / BN;
-  auto issue = [&](int st) {
-    const uint32_t at = lds + (st & 1) * 2 * TILE;
-    ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - st * BN, at, wave);
-    cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
+  auto scores = [&](int slot, f32x16& s) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) s = mma32<DT>(lds_read16(row_step<D>(ka, x) + slot * TILE), qf[x], s);
   };
-  const uint32_t ka = row_addr<D>(lane);
-  uint32_t va[D / 32];
+  // Stage st in slot u: the next stage's scores on the matrix cores beside this one's softmax, then the weights times V.
+  auto step = [&](int st, auto uc, f32x16& s, f32x16& next) {
+    constexpr int u = decltype(uc)::value;
+    if constexpr (D == 256) {
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) va[t] = col_addr<D>(lane, t);
-
-  if (nst) issue(0);
-  for (int st = 0; st < nst; ++st) {
-    stage_barrier<0>();  // this stage's copies have landed, and nobody reads the other half any more
-    if (st + 1 < nst) issue(st + 1);
-    if (st * BN > w0 + 31 + off) continue;  // nothing of this stage is visible to the wave's rows
-    const uint32_t kt = lds + (st & 1) * 2 * TILE, vt = kt + TILE;
-    f32x16 s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) s[t] = mma32<DT>(lds_read16(kt + t * 32 * D * 2 + (ka ^ (x * 32))), qf[x], s[t]);
+      for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(acc[d]));
     }
-    if (st * BN + BN - 1 > w0 + off) {  // the diagonal or the end of the keys
-      const int lim = row + off - st * BN;
+    stage_barrier<CP>();  // K of st + 1 and V of st have landed, and nobody reads K of st and V of st - 1 any more
+    issue_v(st + 2, (u + 2) % 3);
+    issue_k(st + 3, u);
+    if (st >= nsw) return;  // nothing of this stage is visible to the wave's rows
+    if (st * FN + FN - 1 > w0 + off) {  // the diagonal or the end of the keys
+      const int lim = row + off - st * FN;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * t + 8 * (r / 4) + 4 * hf + r % 4 > lim) s[t][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + 4 * hf + r % 4 > lim) s[r] = -INFINITY;
     }
-    float mx = s[0][0];
+    __builtin_amdgcn_sched_barrier(0);
+    scores((u + 1) % 3, next);
+    float mx = s[0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = halves(mx, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
+    // the weights' base follows the maximum only when it has grown by 2^8: any base does, and f32 sums and 16-bit
+    // weights have room for it (weights up to 2^8), so that the accumulators are rescaled in few stages
+    mx = mx > m + 8.f ? mx : m;
+    mc = mx == -INFINITY ? 0.f : mx;
+    const float alpha = exp2_hw(m - mc);
+    float sum[2] = {0.f, 0.f};
+    u32x4 p[2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-    mx = fmaxf(m, halves(mx, [](float x, float y) { return fmaxf(x, y); }));
-    const float mc = mx == -INFINITY ? 0.f : mx * a.scale2;
-    const float alpha = exp2_hw(m * a.scale2 - mc);
+    for (int r = 0; r < 16; r += 2) {
+      const float e0 = exp2_hw(fmaf(s[r], a.scale2, -mc)), e1 = exp2_hw(fmaf(s[r + 1], a.scale2, -mc));
+      sum[0] += e0;
+      sum[1] += e1;
+      p[r / 8][r % 8 / 2] = pack2<DT>(e0, e1);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(p[i]));  // formed here, not after the branch below
+    interleave<D / 16, 4>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(mx != m)) {
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) rescale<D>(acc[d], alpha);
+    }
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(acc[d]));
+    }
     m = mx;
-    float sum = 0.f;
+    l += sum[0] + sum[1];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[t][r] = exp2_hw(fmaf(s[t][r], a.scale2, -mc));
-        sum += s[t][r];
-      }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[t][r] *= alpha;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = pack2<DT>(s[t][8 * h + 2 * i], s[t][8 * h + 2 * i + 1]);
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          acc[d] = mma32<DT>(lds_read_col<D>(vt + (32 * t + 16 * h) * D * 2 + va[d]), p, acc[d]);
-      }
+      for (int d = 0; d < D / 32; ++d)
+        acc[d] = mma32<DT>(lds_read_col<D>(col_step<D>(va, d) + 16 * i * D * 2 + u * TILE), p[i], acc[d]);
+    feed<D / 16, 2, 8>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (nst) {
+    stage_barrier<CP + CP>();  // K of stage 0
+    f32x16 s0, s1, s2;
+    scores(0, s0);
+    for (int st = 0; st < nst; st += 3) {
+      step(st, std::integral_constant<int, 0>(), s0, s1);
+      if (st + 1 < nst) step(st + 1, std::integral_constant<int, 1>(), s1, s2);
+      if (st + 2 < nst) step(st + 2, std::integral_constant<int, 2>(), s2, s0);
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before the wave ends
   }
   l = halves(l, [](float x, float y) { return x + y; });
   if (row >= nq) return;
@@ -179,7 +261,7 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
       *reinterpret_cast<u32x2*>(op + 32 * d + 2 * r) = u32x2{pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv),
                                                              pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv)};
   if (lse && hf == 0)
-    lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (m * a.scale2 + __log2f(l)) * LN2;
+    lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * LN2;
 }
 
 // ------------------------------------------------------------------------------------ backward
@@ -252,7 +334,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const uint16_t* __restri
 // place as the operand of dQ^T = K^T dS^T.  The scores are formed again rather than handed over by the pass over keys:
 // two products more, but no sum over workgroups, whose order would change the results.
 template <int D, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dq) {
   constexpr int BM = NW * 32, TILE = BN * D * 2;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
@@ -309,9 +391,9 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
     cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
   };
   const uint32_t ra = row_addr<D>(lane);
-  uint32_t ca[D / 32];
+  uint32_t ca[COLS<D>];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) ca[t] = col_addr<D>(lane, t);
+  for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
 
   if (nst) issue(0);
   for (int st = 0; st < nst; ++st) {
@@ -328,8 +410,8 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
-        s = mma32<DT>(lds_read16(kt + t * 32 * D * 2 + (ra ^ (x * 32))), qf[x], s);
-        g = mma32<DT>(lds_read16(vt + t * 32 * D * 2 + (ra ^ (x * 32))), df[x], g);
+        s = mma32<DT>(lds_read16(row_step<D>(ra, x) + kt + t * 32 * D * 2), qf[x], s);
+        g = mma32<DT>(lds_read16(row_step<D>(ra, x) + vt + t * 32 * D * 2), df[x], g);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -347,7 +429,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
         for (int i = 0; i < 4; ++i) p[i] = pack2<DT>(s[8 * h + 2 * i], s[8 * h + 2 * i + 1]);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
-          acc[d] = mma32<DT>(lds_read_col<D>(kt + (32 * t + 16 * h) * D * 2 + ca[d]), p, acc[d]);
+          acc[d] = mma32<DT>(lds_read_col<D>(kt + (32 * t + 16 * h) * D * 2 + col_step<D>(ca, d)), p, acc[d]);
       }
     }
   }
@@ -366,7 +448,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
 // NW x 32 keys of one key head, 32 a wave, a key per lane (S = Q K^T), and walks the group's queries in stages of QT rows
 // of q and do; dV^T = dO^T P and dK^T = Q^T dS take P and dS from the lanes they were formed in.
 template <int D, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dk,
                      uint16_t* __restrict__ dv) {
   constexpr int BK = NW * 32, QT = 64, TILE = QT * D * 2;
@@ -441,9 +523,9 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     }
   };
   const uint32_t ra = row_addr<D>(lane);
-  uint32_t ca[D / 32];
+  uint32_t ca[COLS<D>];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) ca[t] = col_addr<D>(lane, t);
+  for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
 
   if (nst) issue(0);
   for (int st = 0; st < nst; ++st) {
@@ -454,15 +536,15 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     const uint32_t qt = lds + (st & 1) * 2 * TILE, dt = qt + TILE;
     const int lim = col - off - r0;  // rows from lim on see the lane's key
     const bool edge = r0 + off < w0 + 31;
-#pragma unroll
+#pragma unroll 1
     for (int t = 0; t < QT / 32; ++t) {
       f32x16 s, g;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
-        s = mma32<DT>(lds_read16(qt + t * 32 * D * 2 + (ra ^ (x * 32))), kf[x], s);
-        g = mma32<DT>(lds_read16(dt + t * 32 * D * 2 + (ra ^ (x * 32))), vf[x], g);
+        s = mma32<DT>(lds_read16(row_step<D>(ra, x) + qt + t * 32 * D * 2), kf[x], s);
+        g = mma32<DT>(lds_read16(row_step<D>(ra, x) + dt + t * 32 * D * 2), vf[x], g);
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -488,8 +570,8 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
-          av[d] = mma32<DT>(lds_read_col<D>(dt + (32 * t + 16 * h) * D * 2 + ca[d]), p, av[d]);
-          ak[d] = mma32<DT>(lds_read_col<D>(qt + (32 * t + 16 * h) * D * 2 + ca[d]), x, ak[d]);
+          av[d] = mma32<DT>(lds_read_col<D>(dt + (32 * t + 16 * h) * D * 2 + col_step<D>(ca, d)), p, av[d]);
+          ak[d] = mma32<DT>(lds_read_col<D>(qt + (32 * t + 16 * h) * D * 2 + col_step<D>(ca, d)), x, ak[d]);
         }
       }
     }
@@ -558,7 +640,7 @@ AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const 
 }
 
 // waves of a workgroup: 8 where 256 registers a lane hold a wave's operands and sums, 4 (512 registers) at D = 256
-template <int D> constexpr int WAVES = D == 256 ? 4 : 8;
+template <int D> constexpr int WAVES = 4;
 
 #define ATTN_DISPATCH(CALL)                                                     \
   do {                                                                          \

@@ -105,12 +105,15 @@ __device__ __forceinline__ void copy4(u32x4 rsrc, uint32_t byte_off, uint32_t m0
 }
 
 // Fragment addresses of a tile at LDS byte address `base` (a multiple of 1024).
-// rows: lane l holds row r0 + l % 32 at k = 16 s + 8 (l / 32) .. + 7, read from row_addr ^ (s * 32), r0 a multiple of 32
+// rows: lane l holds row r0 + l % 32 at k = 16 s + 8 (l / 32) .. + 7, read from row_step(row_addr, s), r0 a multiple of 32
+// (the swizzle reaches the low 4 bits of a chunk's number, so at D = 256 the upper half of a row is a constant away)
 template <int D>
 __device__ __forceinline__ uint32_t row_addr(int lane) {
   const int r = lane & 31;
   return (uint32_t)(r * D * 2 + (((lane >> 5) ^ swz<D>(r)) << 4));
 }
+template <int D>
+__device__ __forceinline__ uint32_t row_step(uint32_t a, int s) { return (a ^ ((s & 7) * 32)) + (s >> 3) * 256; }
 typedef const __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ u32x4 lds_read16(uint32_t a) { return *(lds_u32x4*)(uintptr_t)a; }
@@ -123,6 +126,10 @@ __device__ __forceinline__ uint32_t col_addr(int lane, int dt) {
   const int r = 4 * (g >> 1) + (s >> 2), c = 32 * dt + 16 * (g & 1) + 4 * (s & 3);
   return (uint32_t)(r * D * 2 + (((c >> 3) ^ swz<D>(r)) << 4) + (c & 7) * 2);
 }
+template <int D> constexpr int COLS = D / 32 < 4 ? D / 32 : 4;
+// col_addr of all dt from those of dt < min(D / 32, 4)
+template <int D>
+__device__ __forceinline__ uint32_t col_step(const uint32_t* a, int dt) { return a[dt & 3] + (dt >> 2) * 256; }
 // r + 8 has another swizzle than r: bit 1 of row / 4 flips, so chunk bit 1 does
 template <int D>
 __device__ __forceinline__ u32x4 lds_read_col(uint32_t a) {

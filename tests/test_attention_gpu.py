@@ -154,7 +154,7 @@ def test_strides(D, dev):
 def test_long_rows(dev):
     """Many key stages, peaked and flat rows: large score jumps between stages (both directions)."""
     gen = torch.Generator().manual_seed(8)
-    for dt, D in ((BF16, 128), (F16, 64)):
+    for dt, D in ((BF16, 128), (F16, 64), (BF16, 256)):
         q, k, v = (_randn(gen, (1, 1500, h, D), dt, dev) for h in (2, 1, 1))
         ramp = torch.linspace(-1, 1, 1500).view(1, -1, 1, 1).to(dev)
         do = _randn(gen, (1, 1500, 2, D), dt, dev)
