@@ -11,6 +11,7 @@
 // the same lane, and P^T is in place as the second product's operand (the keys of 8 consecutive registers are the ones
 // its fragment takes, in an order that V^T's fragment is read in as well).  No value crosses lanes on the way.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_common.h"
 #include "launchers.h"
@@ -274,7 +275,8 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
 constexpr int PB = 64;  // rows per block of the preparation
 template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
 struct RowPrep {
-  float *lse2, *delta, *rscale, *amax;
+  f32x2_t* rows;  // lse2, delta
+  float *rscale, *amax;
   int nblk;
 };
 // 2^e with 2^e amax in [1, 2); 1 for 0, infinities and NaN
@@ -316,8 +318,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const uint16_t* __restri
     if (sub == 0 && row < total_q) {
       const int64_t i = (int64_t)head * total_q + row;
       const float v = lse[i];
-      w.lse2[i] = v == -INFINITY ? INFINITY : v * LOG2E - SHIFT<DT>;
-      w.delta[i] = dot - (dlse ? dlse[i] : 0.f);
+      w.rows[i] = f32x2_t{v == -INFINITY ? INFINITY : v * LOG2E - SHIFT<DT>, dot - (dlse ? dlse[i] : 0.f)};
       if (DT == LSURGE_F16) w.rscale[i] = grad_scale(mx);
     }
   }
@@ -369,7 +370,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
     }
   }
   const int64_t pi = (int64_t)head * a.total_q + crow;
-  const float lse2 = w.lse2[pi], delta = w.delta[pi];
+  const float lse2 = w.rows[pi][0], delta = w.rows[pi][1];
   const float gs = DT == LSURGE_F16 ? w.rscale[pi] : 1.f;
   f32x16 acc[D / 32];
 #pragma unroll
@@ -445,22 +446,30 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
 }
 
 // dv_j = sum_i p_ij do_i, dk_j = scale sum_i ds_ij q_i over the queries of every head of the group.  A workgroup takes
-// NW x 32 keys of one key head, 32 a wave, a key per lane (S = Q K^T), and walks the group's queries in stages of QT rows
-// of q and do; dV^T = dO^T P and dK^T = Q^T dS take P and dS from the lanes they were formed in.
+// NW x 32 keys of one key head, 32 a wave, a key per lane (S = Q K^T), and walks the group's queries in stages of 32 rows
+// of q and do through a three-deep LDS ring; dV^T = dO^T P and dK^T = Q^T dS take P and dS from the lanes they were formed
+// in.  Both accumulators and the fragments of K and V would fill all 256 registers that two waves a SIMD leave at
+// D = 128, so V waits in LDS there.  The stages of a tile are cut into `parts` equal runs, a workgroup each, where there
+// are too few tiles (the first keys of a causal sequence have many more queries than the last); the parts' sums are then
+// f32 in `psum` and added up in order by attn_dkv_sum_kernel.
+constexpr int QN = 32;  // query rows per stage
+template <int D> constexpr bool V_IN_LDS = D >= 128;
+template <int D> constexpr int DKV_EU = D == 256 ? 1 : 2;  // waves per SIMD that the registers allow
 template <int D, int DT, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dk,
-                     uint16_t* __restrict__ dv) {
-  constexpr int BK = NW * 32, QT = 64, TILE = QT * D * 2;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
-  __shared__ __attribute__((aligned(16))) float rows[2][2][QT];  // lse2 and delta of a stage's rows
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DKV_EU<D>)))
+void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, int parts,
+                     float* __restrict__ psum, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
+  constexpr int BK = NW * 32, R = V_IN_LDS<D> ? 2 : 3, TILE = QN * D * 2, VBYTES = V_IN_LDS<D> ? BK * D * 2 : 0;
+  // R stages of q, R of do, R of the rows' lse2 and delta, then V
+  __shared__ __attribute__((aligned(1024))) char smem[2 * R * TILE + 1024 + VBYTES];
   __shared__ float red[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  int kvh, slot;
-  head_tile(a.hk, a.ntiles, kvh, slot);
+  int unit, slot;
+  head_tile(a.hk * parts, a.ntiles, unit, slot);
+  const int kvh = unit / parts, part = unit % parts;
   slot = a.ntiles - 1 - slot;  // the first keys are seen by the most queries
-  if (a.cu_k) {
+  if (a.cu_k && part == 0) {
     const int64_t end = cu_at(a.cu_k, a.nseq, a.total_k) + (int64_t)slot * BK;
     const int n = (int)min((int64_t)BK, a.total_k - end);
     if (n > 0) {
@@ -477,15 +486,46 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   if (tile * BK >= nk) return;
   const int off = nk - nq, w0 = tile * BK + wave * 32, col = w0 + ln, group = a.hq / a.hk;
 
-  u32x4 kf[D / 16], vf[D / 16];
-  {
-    const int64_t r = k0 + min(col, nk - 1);
-    const uint16_t *kp = a.k + r * a.k_row + kvh * a.k_head + 8 * hf, *vp = a.v + r * a.v_row + kvh * a.v_head + 8 * hf;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      kf[s] = *reinterpret_cast<const u32x4*>(kp + 16 * s);
-      vf[s] = *reinterpret_cast<const u32x4*>(vp + 16 * s);
+  const uint32_t lds = lds_addr((const bf16_t*)smem), lds_rows = lds + 2 * R * TILE, lds_v = lds_rows + 1024;
+  TileCopy<D, QN, NW> cq, cd;
+  const int64_t d_row = (int64_t)a.hq * D;
+  cq.init(a.q_row, wave, lane);
+  cd.init(d_row, wave, lane);
+  const int first = max(0, tile * BK - off) / QN;  // the stage of the first query that sees the tile's first key
+  const int per = max(0, (nq + QN - 1) / QN - first), all = per * group;
+  const int begin = (int)((int64_t)all * part / parts), nst = (int)((int64_t)all * (part + 1) / parts) - begin;
+  // the stage to issue next: its head and first row
+  int ih = per ? kvh * group + begin / per : 0, ir = per ? (first + begin % per) * QN : 0;
+  auto issue = [&](int slot) {  // stages past the end fill with other rows of the group, or zeros
+    const int n = ih < (kvh + 1) * group ? nq - ir : 0;
+    cq.issue(a.q + (int64_t)(q0 + ir) * a.q_row + ih * a.q_head, a.q_row, n, lds + slot * TILE, wave);
+    cd.issue(dout + (int64_t)(q0 + ir) * d_row + ih * D, d_row, n, lds + (R + slot) * TILE, wave);
+    // rows past the end get zeros: q and do are zeros there, so any finite values do
+    copy4(make_rsrc(w.rows + (int64_t)ih * a.total_q + q0 + ir, 8 * (int64_t)max(0, min(n, QN))),
+          lane % 32 * 8 + lane / 32 * 4, lds_rows + slot * 256);
+    ir += QN;
+    if (ir >= nq) {
+      ir = first * QN;
+      ++ih;
     }
+  };
+  constexpr int CP = 2 * TileCopy<D, QN, NW>::N + 1;
+  const uint16_t* kp = a.k + (int64_t)(k0 + min(col, nk - 1)) * a.k_row + kvh * a.k_head + 8 * hf;
+  u32x4 kf[D / 16], vf[V_IN_LDS<D> ? 1 : D / 16];
+  if (nst) {
+    if constexpr (V_IN_LDS<D>) {
+      TileCopy<D, BK, NW> cv;
+      cv.init(a.v_row, wave, lane);
+      cv.issue(a.v + (int64_t)(k0 + tile * BK) * a.v_row + kvh * a.v_head, a.v_row, nk - tile * BK, lds_v, wave);
+    } else {
+      const uint16_t* vp = a.v + (int64_t)(k0 + min(col, nk - 1)) * a.v_row + kvh * a.v_head + 8 * hf;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) vf[s] = *reinterpret_cast<const u32x4*>(vp + 16 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) kf[s] = *reinterpret_cast<const u32x4*>(kp + 16 * s);
+    issue(0);
+    if (R > 2) issue(1);
   }
   float gs = 1.f;
   if constexpr (DT == LSURGE_F16) {  // one scale for the head's group: its largest |do|
@@ -504,81 +544,99 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) ak[t][r] = av[t][r] = 0.f;
-
-  const uint32_t lds = lds_addr((const bf16_t*)smem), rows_lds = lds_addr((const bf16_t*)rows);
-  TileCopy<D, QT, NW> cq, cd;
-  const int64_t d_row = (int64_t)a.hq * D;
-  cq.init(a.q_row, wave, lane);
-  cd.init(d_row, wave, lane);
-  const int first = max(0, tile * BK - off) / QT;  // the stage of the first query that sees the tile's first key
-  const int per = max(0, (nq + QT - 1) / QT - first), nst = per * group;
-  auto issue = [&](int st) {
-    const int head = kvh * group + st / per, r0 = (first + st % per) * QT, n = nq - r0;
-    const uint32_t at = lds + (st & 1) * 2 * TILE;
-    cq.issue(a.q + (int64_t)(q0 + r0) * a.q_row + head * a.q_head, a.q_row, n, at, wave);
-    cd.issue(dout + (int64_t)(q0 + r0) * d_row + head * D, d_row, n, at + TILE, wave);
-    if (wave < 2) {  // rows past the end get zeros: q and do are zeros there, so any finite values do
-      const float* p = (wave ? w.delta : w.lse2) + (int64_t)head * a.total_q + q0 + r0;
-      copy4(make_rsrc(p, 4 * (int64_t)min(n, QT)), lane * 4, rows_lds + ((st & 1) * 2 + wave) * QT * 4);
-    }
-  };
-  const uint32_t ra = row_addr<D>(lane);
+  const uint32_t ra = lds + row_addr<D>(lane), rv = lds_v + wave * 32 * D * 2 + row_addr<D>(lane);
   uint32_t ca[COLS<D>];
 #pragma unroll
-  for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
+  for (int t = 0; t < COLS<D>; ++t) ca[t] = lds + col_addr<D>(lane, t);
 
-  if (nst) issue(0);
-  for (int st = 0; st < nst; ++st) {
-    stage_barrier<0>();
-    if (st + 1 < nst) issue(st + 1);
-    const int r0 = (first + st % per) * QT;
-    if (r0 + QT - 1 + off < w0) continue;  // no row of this stage sees the wave's keys
-    const uint32_t qt = lds + (st & 1) * 2 * TILE, dt = qt + TILE;
-    const int lim = col - off - r0;  // rows from lim on see the lane's key
-    const bool edge = r0 + off < w0 + 31;
-#pragma unroll 1
-    for (int t = 0; t < QT / 32; ++t) {
-      f32x16 s, g;
+  int cr = per ? (first + begin % per) * QN : 0;  // first row of the stage being computed
+  // weights and score gradients of the stage in `slot`, packed as the products' operands
+  auto weigh = [&](int slot, const f32x16& s, const f32x16& g, u32x4* p, u32x4* x) {
+    const uint32_t rw = lds_rows + slot * 256 + 16 * hf;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+    for (int b = 0; b < 4; ++b) {
+      const u32x4 ls = lds_read16(rw + 32 * b), de = lds_read16(rw + 128 + 32 * b);
+      float e[4], f[4];
 #pragma unroll
-      for (int x = 0; x < D / 16; ++x) {
-        s = mma32<DT>(lds_read16(row_step<D>(ra, x) + qt + t * 32 * D * 2), kf[x], s);
-        g = mma32<DT>(lds_read16(row_step<D>(ra, x) + dt + t * 32 * D * 2), vf[x], g);
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * b + i;
+        e[i] = exp2_hw(fmaf(s[r], a.scale2, -__uint_as_float(ls[i])));
+        f[i] = g[r] - __uint_as_float(de[i]);
+        if (DT == LSURGE_F16) f[i] *= gs;
+        f[i] *= e[i];
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(&rows[st & 1][0][32 * t + 8 * b + 4 * hf]);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(&rows[st & 1][1][32 * t + 8 * b + 4 * hf]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * b + i;
-          float p = exp2_hw(fmaf(s[r], a.scale2, -ls[i]));
-          float x = p * ((g[r] - de[i]) * gs);
-          if (edge && 32 * t + 8 * b + 4 * hf + i < lim) p = x = 0.f;
-          s[r] = p;
-          g[r] = x;
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 p, x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = pack2<DT>(s[8 * h + 2 * i], s[8 * h + 2 * i + 1]);
-          x[i] = pack2<DT>(g[8 * h + 2 * i], g[8 * h + 2 * i + 1]);
-        }
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          av[d] = mma32<DT>(lds_read_col<D>(dt + (32 * t + 16 * h) * D * 2 + col_step<D>(ca, d)), p, av[d]);
-          ak[d] = mma32<DT>(lds_read_col<D>(qt + (32 * t + 16 * h) * D * 2 + col_step<D>(ca, d)), x, ak[d]);
-        }
+      for (int i = 0; i < 4; i += 2) {
+        p[b / 2][b % 2 * 2 + i / 2] = pack2<DT>(e[i], e[i + 1]);
+        x[b / 2][b % 2 * 2 + i / 2] = pack2<DT>(f[i], f[i + 1]);
       }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(p[h]), "+v"(x[h]));
+  };
+  auto products = [&](int slot, const u32x4* p, const u32x4* x) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        av[d] = mma32<DT>(lds_read_col<D>(col_step<D>(ca, d) + 16 * h * D * 2 + (R + slot) * TILE), p[h], av[d]);
+        ak[d] = mma32<DT>(lds_read_col<D>(col_step<D>(ca, d) + 16 * h * D * 2 + slot * TILE), x[h], ak[d]);
+      }
+  };
+  auto step = [&](auto uc) {
+    constexpr int u = decltype(uc)::value;
+    if constexpr (DKV_EU<D> == 1) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(ak[d]), "+a"(av[d]));
+    }
+    stage_barrier<(R - 2) * CP>();  // this stage has landed, and nobody reads the one before it any more
+    issue((u + R - 1) % R);
+    const int r0 = cr;
+    cr = cr + QN >= nq ? first * QN : cr + QN;
+    if (r0 + QN - 1 + off < w0) return;  // no row of this stage sees the wave's keys
+    f32x16 s, g;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) s = mma32<DT>(lds_read16(row_step<D>(ra, x) + u * TILE), kf[x], s);
+    if (r0 + off < w0 + 31) {  // the diagonal: a key's lane sees the rows from lim on
+      const int lim = col - off - r0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + 4 * hf + r % 4 < lim) s[r] = -INFINITY;
+    }
+    u32x4 p[2], x[2];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+      g = mma32<DT>(lds_read16(row_step<D>(ra, x) + (R + u) * TILE), V_IN_LDS<D> ? lds_read16(row_step<D>(rv, x)) : vf[V_IN_LDS<D> ? 0 : x], g);
+    weigh(u, s, g, p, x);
+    __builtin_amdgcn_sched_barrier(0);
+    products(u, p, x);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int st = 0; st < nst; st += R) {
+    step(std::integral_constant<int, 0>());
+    if (st + 1 < nst) step(std::integral_constant<int, 1>());
+    if constexpr (R > 2)
+      if (st + 2 < nst) step(std::integral_constant<int, R - 1>());
   }
+  __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before the wave ends
   if (col >= nk) return;
   const float fv = exp2_hw(-SHIFT<DT>), fk = scale / gs * fv;
   const int64_t at = ((int64_t)(k0 + col) * a.hk + kvh) * D + 4 * hf;
+  if (parts > 1) {
+    const int64_t size = (int64_t)a.total_k * a.hk * D;
+    float* pk = psum + 2 * part * size + at;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        *reinterpret_cast<f32x4*>(pk + 32 * d + 2 * r) = f32x4{ak[d][r] * fk, ak[d][r + 1] * fk, ak[d][r + 2] * fk, ak[d][r + 3] * fk};
+        *reinterpret_cast<f32x4*>(pk + size + 32 * d + 2 * r) = f32x4{av[d][r] * fv, av[d][r + 1] * fv, av[d][r + 2] * fv, av[d][r + 3] * fv};
+      }
+    return;
+  }
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -588,6 +646,22 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
       *reinterpret_cast<u32x2*>(dv + at + 32 * d + 2 * r) = u32x2{
           pack2<DT>(av[d][r] * fv, av[d][r + 1] * fv), pack2<DT>(av[d][r + 2] * fv, av[d][r + 3] * fv)};
     }
+}
+
+// dk and dv = the parts' sums, added in order: n values each, 4 a thread; rows from cu[nseq] on were zeroed already
+template <int DT>
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* __restrict__ psum, int parts, int64_t size,
+                                                           int64_t row, const int32_t* __restrict__ cu, int nseq, int total,
+                                                           uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
+  const int64_t n = cu ? cu_at(cu, nseq, total) * row : size;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < 2 * n; i += (int64_t)gridDim.x * 1024) {
+    const bool second = i >= n;
+    const int64_t at = second ? i - n : i;
+    const float* p = psum + (second ? size : 0) + at;
+    f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    for (int j = 1; j < parts; ++j) s += *reinterpret_cast<const f32x4*>(p + 2 * j * size);
+    *reinterpret_cast<u32x2*>((second ? dv : dk) + at) = u32x2{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
+  }
 }
 
 // ------------------------------------------------------------------------------------ host
@@ -642,6 +716,20 @@ AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const 
 // waves of a workgroup: 8 where 256 registers a lane hold a wave's operands and sums, 4 (512 registers) at D = 256
 template <int D> constexpr int WAVES = 4;
 
+// Parts that the stages of a tile of keys are cut into in attn_dkv_kernel, by the sizes that the host knows (the
+// sequences' own lengths are on the device).  A part costs a write and a read of the tile's f32 sums, an unsplit grid idle
+// CUs behind the workgroups with the most queries: the sum of a term that falls with the workgroups and one that rises
+// with the parts is least where parts^2 is in proportion to stages / tiles.  8 x 4096 tokens of 8 heads over 2: one part
+// 1697 us a training step, two 1655, four 1516, eight 1680; one sequence of 512: 150, 104, 81, 68; of 4096, 8 heads of
+// their own keys: 425, 346, 328, 389; packed documents (31 of 1150 tokens, 16 heads): 813 unsplit, 1028 in two.
+int64_t dkv_parts(const lsurge_attn_shape& s) {
+  if (s.total_q == 0 || s.total_k == 0 || s.nseq == 0) return 1;
+  const double tiles = (double)s.nseq * (double)((s.total_k / s.nseq + 127) / 128) * s.hk;
+  const double stages = (double)(s.hq / s.hk) * (double)s.total_q / (double)s.nseq / QN / 2;
+  const double parts = std::min(std::min(sqrt(64.0 * stages / std::max(tiles, 1.0)), 4096.0 / std::max(tiles, 1.0)), 8.0);
+  return std::max<int64_t>(1, (int64_t)parts);
+}
+
 #define ATTN_DISPATCH(CALL)                                                     \
   do {                                                                          \
     if (s->dtype == LSURGE_BF16) {                                              \
@@ -693,13 +781,14 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   return LSURGE_OK;
 }
 
-static size_t prep_floats(const lsurge_attn_shape* s) {
+static size_t prep_bytes(const lsurge_attn_shape* s) {
   const int64_t rows = s->hq * s->total_q, blk = (s->total_q + PB - 1) / PB;
-  return (size_t)(s->dtype == LSURGE_F16 ? 3 * rows + s->hq * blk : 2 * rows);
+  return (sizeof(float) * (size_t)(s->dtype == LSURGE_F16 ? 3 * rows + s->hq * blk : 2 * rows) + 255) / 256 * 256;
 }
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
-  if (!s || s->hq < 1 || s->total_q < 0) return 0;
-  return sizeof(float) * prep_floats(s) + 64;
+  if (!s || s->hq < 1 || s->hk < 1 || s->d < 1 || s->nseq < 0 || s->total_q < 0 || s->total_k < 0) return 0;
+  const int64_t parts = dkv_parts(*s);
+  return prep_bytes(s) + (parts > 1 ? sizeof(float) * (size_t)(2 * parts * s->total_k * s->hk * s->d) : 0) + 256;
 }
 
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
@@ -727,8 +816,10 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
   const int64_t nrow = s->hq * s->total_q;
   RowPrep w;
-  w.lse2 = (float*)workspace, w.delta = w.lse2 + nrow, w.rscale = w.delta + nrow, w.amax = w.rscale + nrow;
+  w.rows = (f32x2_t*)workspace, w.rscale = (float*)(w.rows + nrow), w.amax = w.rscale + nrow;
   w.nblk = (int)((s->total_q + PB - 1) / PB);
+  float* psum = (float*)((char*)workspace + prep_bytes(s));
+  const int parts = (int)dkv_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
 #define ATTN_BWD(D, DT)                                                                                                  \
   constexpr int NW = WAVES<D>;                                                                                           \
@@ -736,14 +827,20 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const int64_t tq = s->total_q ? num_tiles(*s, cu_q, s->total_q, NW * 32) : 0;                                          \
   const int64_t tk = s->total_k ? num_tiles(*s, cu_k, s->total_k, NW * 32) : 0;                                          \
   if (int rc = tile_grid("attn_bwd", tq, s->hq, &gq)) return rc;                                                         \
-  if (int rc = tile_grid("attn_bwd", tk, s->hk, &gk)) return rc;                                                         \
+  if (int rc = tile_grid("attn_bwd", tk, s->hk * parts, &gk)) return rc;                                                         \
   if (gq)                                                                                                                \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_prep_kernel<D, DT>), dim3(w.nblk, (unsigned)s->hq), dim3(256),  \
                                                    0, st, (const uint16_t*)o, g, lse, dlse, a.total_q, a.hq, w));        \
   if (gk) {                                                                                                              \
     a.ntiles = (int)tk;                                                                                                  \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, a, g, w, \
-                                                   scale, (uint16_t*)dk, (uint16_t*)dv));                                \
+                                                   scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                   \
+    const int64_t size = s->total_k * s->hk * D;                                                                         \
+    if (parts > 1)                                                                                                       \
+      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_sum_kernel<DT>),                                          \
+                                                     dim3((unsigned)std::min<int64_t>((2 * size + 1023) / 1024, 4096)),  \
+                                                     dim3(256), 0, st, psum, parts, size, s->hk * D, cu_k, a.nseq,       \
+                                                     a.total_k, (uint16_t*)dk, (uint16_t*)dv));                          \
   }                                                                                                                      \
   if (gq) {                                                                                                              \
     a.ntiles = (int)tq;                                                                                                  \
