@@ -476,7 +476,7 @@ typedef struct {
  * (row_stride and head_stride any multiples of 8).  The sequences' tokens are dealt to the GPU in equal shares whatever
  * their lengths; the parts of a sequence are joined in a fixed order, so results repeat bit for bit.  Calls that share a
  * workspace have to be ordered on one stream. */
-size_t lsurge_paged_attn_workspace_bytes(int64_t d);
+size_t lsurge_paged_attn_workspace_bytes(int64_t nseq, int64_t hq, int64_t d);
 int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64_t nseq, int64_t hq, float scale, void* o,
                       float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
 /* Write new tokens' keys and values (rows [rows, heads, d] by strides) to their pages: rows [cu[b], cu[b + 1]) are the last

@@ -32,8 +32,10 @@ HEAD_DIMS = (64, 128, 256)
 
 def _check_heads(what, q_heads, kv_heads, d, *ts):
     L.require_cuda(*ts)
-    if any(t is not None and t.device != ts[0].device for t in ts):
-        raise ValueError(f"{what}: all tensors must be on one device (got {sorted({str(t.device) for t in ts if t is not None})})")
+    device = ts[0].device
+    for t in ts:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors must be on one device (got {device} and {t.device})")
     if d not in HEAD_DIMS:
         raise ValueError(f"{what}: head dim must be one of {HEAD_DIMS} (got {d})")
     if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
@@ -41,14 +43,25 @@ def _check_heads(what, q_heads, kv_heads, d, *ts):
 
 
 def _check_dtype(what, *ts):
-    if ts[0].dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != ts[0].dtype for t in ts):
+    dt = ts[0].dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16 or any(t.dtype is not dt for t in ts):
         raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
 
 
 def _check_index(what, name, t, shape):
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: {name} must be int32 of shape {tuple(shape)} (got {t.dtype}, {tuple(t.shape)})")
+    if t.dtype is not torch.int32 or t.shape != shape:
+        raise ValueError(f"{what}: {name} must be int32 of shape {shape} (got {t.dtype}, {tuple(t.shape)})")
     return L.contig(t)
+
+
+def _call(what, device, fn, *args):
+    """fn(*args, the current stream of `device`), with `device` current while its kernels are launched."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, L.stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, L.stream(device))
+    L.check(rc, what)
 
 
 def _scale(what, scale, d):
@@ -78,20 +91,25 @@ def _rows_arg(t):
     return ctypes.byref(L.AttnRows(t.data_ptr(), row, head))
 
 
+def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse):
+    """o, lse (or None) of packed rows, and what the backward needs: the rows as read and the shape."""
+    tq, hq, d = q.shape
+    tk, hk, _ = k.shape
+    q, k, v = _rows(q, d), _rows(k, d), _rows(v, d)
+    shape = L.AttnShape(nseq, tq, tk, hq, hk, d, L.dt(q))
+    o = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device) if want_lse else None
+    _call("attn_fwd", q.device, L.lib().lsurge_attn_fwd, ctypes.byref(shape), _rows_arg(q), _rows_arg(k), _rows_arg(v),
+          L.ptr(cu_q), L.ptr(cu_k), scale, L.ptr(o), L.ptr(lse))
+    return o, lse, (q, k, v), shape
+
+
 class _AttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale):
-        tq, hq, d = q.shape
-        tk, hk, _ = k.shape
-        q, k, v = (_rows(t.detach(), d) for t in (q, k, v))
-        shape = L.AttnShape(nseq, tq, tk, hq, hk, d, L.dt(q))
-        o = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
-        lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device)
-        with torch.cuda.device(q.device):
-            L.check(L.lib().lsurge_attn_fwd(ctypes.byref(shape), _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
-                                            L.ptr(cu_k), scale, L.ptr(o), L.ptr(lse), L.stream(q.device)), "attn_fwd")
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, lse)
+        o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, True)
+        ctx.save_for_backward(*rows, cu_q, cu_k, o, lse)
         ctx.shape, ctx.scale = shape, scale
         ctx.set_materialize_grads(False)
         return o, lse
@@ -107,11 +125,11 @@ class _AttnFn(torch.autograd.Function):
         dq = torch.empty_like(o)
         dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
         lib = L.lib()
-        with torch.cuda.device(q.device):
-            ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(ctypes.byref(ctx.shape)), q.device)
-            L.check(lib.lsurge_attn_bwd(ctypes.byref(ctx.shape), _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
-                                        L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq),
-                                        L.ptr(dk), L.ptr(dv), L.ptr(ws), ws.numel(), L.stream(q.device)), "attn_bwd")
+        shape = ctypes.byref(ctx.shape)
+        ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(shape), q.device)
+        _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
+              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk), L.ptr(dv),
+              L.ptr(ws), ws.numel())
         return dq, dk, dv, None, None, None, None
 
 
@@ -148,10 +166,15 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
         if cu_seqlens_k is None and k.shape[0] != q.shape[0]:
             raise ValueError(f"{what}: {q.shape[0]} query rows and {k.shape[0]} key rows need cu_seqlens_k")
         cu_k = cu_q if cu_seqlens_k is None else _check_index(what, "cu_seqlens_k", cu_seqlens_k, (nseq + 1,))
-    rows = [t.flatten(0, 1) if t.dim() == 4 else t for t in (q, k, v)]
-    o, lse = _AttnFn.apply(*rows, cu_q, cu_k, nseq, scale)
-    o = o.view(q.shape)
-    return (o, lse.t().reshape(q.shape[:-1])) if return_lse else o
+    shape = q.shape
+    if q.dim() == 4:
+        q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _AttnFn.apply(q, k, v, cu_q, cu_k, nseq, scale)
+    else:
+        o, lse = _forward(q, k, v, cu_q, cu_k, nseq, scale, return_lse)[:2]
+    o = o.view(shape)
+    return (o, lse.t().reshape(shape[:-1])) if return_lse else o
 
 
 def alloc_kv_cache(num_pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -161,6 +184,15 @@ def alloc_kv_cache(num_pages, page_size, kv_heads, head_dim, dtype=torch.bfloat1
     return tuple(torch.empty(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
 
 
+def _cache_strides(what, t):
+    st = t.stride()
+    if 1 in t.shape:  # the stride of an axis of one means nothing
+        st = [0 if n == 1 else s for n, s in zip(t.shape, st)]
+    if t.stride(3) != 1 or (st[0] | st[1] | st[2]) % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{what}: a token's values in a cache must be contiguous and 16-byte aligned (strides {t.stride()})")
+    return st[:3]
+
+
 def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"{what}: caches must be [num_pages, page_size, kv_heads, head_dim] (got {tuple(k_cache.shape)}, "
@@ -168,19 +200,13 @@ def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
     pages, size, heads, d = k_cache.shape
     if pages < 1 or size < 8 or size > 4096 or size & (size - 1):
         raise ValueError(f"{what}: at least one page, of a power of two from 8 to 4096 tokens (got {pages} of {size})")
-    strides = []
-    for t in (k_cache, v_cache):
-        st = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
-        if t.stride(3) != 1 or any(n % 8 for n in st) or t.data_ptr() % 16:
-            raise ValueError(f"{what}: a token's values in a cache must be contiguous and 16-byte aligned (strides {t.stride()})")
-        strides += st
     if page_table.dim() != 2 or page_table.shape[1] < 1:
         raise ValueError(f"{what}: page_table must be [sequences, pages] (got {tuple(page_table.shape)})")
     nseq, most = page_table.shape
     table = _check_index(what, "page_table", page_table, (nseq, most))
     lens = _check_index(what, "seq_lens", seq_lens, (nseq,))
-    arg = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), *strides, table.data_ptr(), most,
-                     lens.data_ptr(), pages, size, most, heads, d, L.dt(k_cache))
+    arg = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), *_cache_strides(what, k_cache), *_cache_strides(what, v_cache),
+                    table.data_ptr(), most, lens.data_ptr(), pages, size, most, heads, d, L.dt(k_cache))
     return ctypes.byref(arg), (table, lens)
 
 
@@ -202,10 +228,9 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
         cu_seqlens = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
     elif k.shape[0] != nseq:
         raise ValueError(f"{what}: {k.shape[0]} tokens for {nseq} sequences need cu_seqlens")
-    k, v = _rows(k.detach()), _rows(v.detach())
-    with torch.cuda.device(k.device):
-        L.check(L.lib().lsurge_kv_append(arg, _rows_arg(k), _rows_arg(v), k.shape[0], nseq, L.ptr(cu_seqlens),
-                                         L.stream(k.device)), "kv_append")
+    k, v = _rows(k), _rows(v)
+    _call("kv_append", k.device, L.lib().lsurge_kv_append, arg, _rows_arg(k), _rows_arg(v), k.shape[0], nseq,
+          L.ptr(cu_seqlens))
     del keep
 
 
@@ -228,9 +253,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, retur
     o = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib = L.lib()
-    with torch.cuda.device(q.device):
-        ws = L.workspace(lib.lsurge_paged_attn_workspace_bytes(d), q.device)
-        L.check(lib.lsurge_paged_attn(arg, _rows_arg(q), n, hq, scale, L.ptr(o), L.ptr(lse), L.ptr(ws), ws.numel(),
-                                      L.stream(q.device)), "paged_attn")
+    ws = L.workspace(lib.lsurge_paged_attn_workspace_bytes(n, hq, d), q.device)
+    _call("paged_attn", q.device, lib.lsurge_paged_attn, arg, _rows_arg(q), n, hq, scale, L.ptr(o), L.ptr(lse), L.ptr(ws),
+          ws.numel())
     del keep
     return (o, lse) if return_lse else o

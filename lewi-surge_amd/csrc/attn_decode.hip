@@ -31,6 +31,8 @@ struct CacheArgs {
 constexpr int DW = 4;             // waves of a workgroup; each takes 32 keys at a time
 constexpr int UK = DW * 32;       // keys of a unit
 constexpr int DT_THREADS = DW * 64;
+template <int D> constexpr int DECODE_EU = D == 64 ? 3 : D == 128 ? 2 : 1;  // waves per SIMD that the registers leave
+constexpr int DECODE_GRID = 1024;                             // at most 4 workgroups a CU
 
 struct DecodeArgs {
   CacheArgs c;
@@ -42,6 +44,7 @@ struct DecodeArgs {
   uint16_t* o;
   float* lse;  // [nseq, hq] or null
   float *po, *pm;  // [grid][2][16][D], [grid][2][2][16] (maximum in base 2, sum)
+  int32_t* shares;  // [nseq heads] first and last share of a (sequence, head block)
   int grid;
 };
 
@@ -49,81 +52,141 @@ __device__ __forceinline__ int seq_len(const DecodeArgs& a, int b) {
   const int64_t cap = (int64_t)a.c.max_pages << a.c.page_log2;
   return (int)min((int64_t)max(a.lens[b], 0), cap);
 }
-__device__ __forceinline__ int seq_units(const DecodeArgs& a, int b) { return (seq_len(a, b) + UK - 1) / UK; }
-
-// Sums of the units per head of sequences [slab i, slab i + 1) into pre[i] (exclusive), by all threads; pre[threads] is
-// the total.  int64: 2^24 sequences of 2^31 keys stay in range.
-__device__ __forceinline__ int slab_size(const DecodeArgs& a) { return (a.nseq + DT_THREADS - 1) / DT_THREADS; }
-__device__ void unit_prefix(const DecodeArgs& a, int64_t* pre) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slab = slab_size(a);
-  __shared__ int64_t wsum[DW];
-  int64_t mine = 0;
-  for (int i = 0; i < slab; ++i) {
-    const int b = tid * slab + i;
-    if (b < a.nseq) mine += seq_units(a, b);
-  }
-  int64_t x = mine;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t y = __shfl_up(x, s, 64);
-    if (lane >= s) x += y;
-  }
-  if (lane == 63) wsum[wave] = x;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) x += wsum[w];
-  pre[tid] = x - mine;
-  if (tid == DT_THREADS - 1) pre[DT_THREADS] = x;
-  __syncthreads();
+__device__ __forceinline__ int units_of(int len) { return (len + UK - 1) / UK; }
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) |
+         (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
 }
-// units of a share when `total` units are dealt to the grid
-__device__ __forceinline__ int64_t share(const DecodeArgs& a, int64_t total) { return max((total + a.grid - 1) / a.grid, (int64_t)1); }
+// n / d, in 32 bits where that will do (a 64-bit division is hundreds of instructions)
+__device__ __forceinline__ int64_t div64(int64_t n, int64_t d) {
+  return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
 
 template <int D, int DT>
-__global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
-  constexpr int KC = D / 32, VE = D / 16, VW = VE / 2;  // VW: registers of a value row's piece
-  __shared__ int64_t pre[DT_THREADS + 1];
+__global__ __launch_bounds__(DT_THREADS) __attribute__((amdgpu_waves_per_eu(DECODE_EU<D>)))
+void attn_decode_kernel(DecodeArgs a) {
+  constexpr int KC = D / 32, VE = D / 16, VW = VE / 2;  // a lane's 16-byte chunks of a key, columns and registers of a value
+  __shared__ int64_t wsum[DW], found;
+  __shared__ int found_b;
   __shared__ __attribute__((aligned(16))) float so[DW][16][D];
   __shared__ float sm[DW][16], sl[DW][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 15, g = lane >> 4;
-  unit_prefix(a, pre);
   const int heads = a.hk * a.hblocks;
-  const int64_t total = pre[DT_THREADS] * heads, per = share(a, total);
+  // units of all sequences: each thread sums a slab of them, then a scan over the threads
+  const int slab = (a.nseq + DT_THREADS - 1) / DT_THREADS;
+  int64_t mine = 0;
+  for (int i = 0; i < slab; ++i) {
+    const int b = tid * slab + i;
+    if (b < a.nseq) mine += units_of(seq_len(a, b));
+  }
+  int64_t pre = mine;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int64_t y = __shfl_up(pre, s, 64);
+    if (lane >= s) pre += y;
+  }
+  if (lane == 63) wsum[wave] = pre;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < DW; ++w) {
+    if (w < wave) pre += wsum[w];
+    total += wsum[w];
+  }
+  total = uni64(total * heads);
+  const int64_t per = max(div64(total + a.grid - 1, a.grid), (int64_t)1);
   int64_t u = blockIdx.x * per;
   const int64_t uend = min(total, u + per);
   if (u >= uend) return;
-  // the sequence of the first unit: the last slab that starts at or before it, then one by one
-  int b;
-  int64_t base;  // units before sequence b (all heads)
-  {
-    int lo = 0, hi = DT_THREADS;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (pre[mid] * heads <= u) lo = mid;
-      else hi = mid;
+  // the sequence of the share's first unit: in the slab that holds it, then one by one
+  if (mine && (pre - mine) * heads <= u && u < pre * heads) {
+    int b = tid * slab;
+    int64_t base = (pre - mine) * heads;
+    for (;; ++b) {
+      const int64_t n = (int64_t)units_of(seq_len(a, b)) * heads;
+      if (u < base + n) break;
+      base += n;
     }
-    b = lo * slab_size(a);
-    base = pre[lo] * heads;
+    found = base;
+    found_b = b;
   }
+  __syncthreads();
+  int64_t base = uni64(found);  // units before sequence b (all heads)
+  int b = __builtin_amdgcn_readfirstlane(found_b);
+  int len = __builtin_amdgcn_readfirstlane(seq_len(a, b)), nu = units_of(len);
+  int hb = (int)div64(u - base, nu);
   const int pmask = (1 << a.c.page_log2) - 1;
+
   while (u < uend) {
-    int len = seq_len(a, b);
-    int64_t nu = (len + UK - 1) / UK;
-    while (base + nu * heads <= u) {
-      base += nu * heads;
-      ++b;
-      len = seq_len(a, b);
-      nu = (len + UK - 1) / UK;
-    }
-    const int hb = (int)((u - base) / nu);
-    const int64_t item = base + hb * nu;  // first unit of this (sequence, head block)
-    const int u0 = (int)(u - item), u1 = (int)min(nu, uend - item);
+    const int64_t item = base + (int64_t)hb * nu;  // first unit of this (sequence, head block)
+    const int u0 = (int)(u - item), u1 = (int)min((int64_t)nu, uend - item);
     const int kvh = hb / a.hblocks, h0 = kvh * a.group + hb % a.hblocks * 16;
     const int nh = min(16, (kvh + 1) * a.group - h0);
     const int32_t* tab = a.c.table + b * a.c.table_stride;
     const uint16_t* kb = a.c.k + kvh * a.c.k_head + 8 * g;
     const uint16_t* vb = a.c.v + kvh * a.c.v_head + VE * ln;
+    // this wave's tiles of 32 keys: from key first on, UK apart
+    const int first = u0 * UK + wave * 32, end = min(len, u1 * UK);
+    const int n = first < end ? (end - first + UK - 1) / UK : 0;
 
+    struct Pages {
+      int k[2], v[2];
+    };
+    struct Tile {
+      u32x4 k[2][KC];
+      uint32_t v[8][VW];
+      bool ok[2];
+    };
+    // pages of the lane's keys (rows 16 t + l % 16) and of its values (rows 16 t + 4 (l / 16) .. + 3)
+    auto pages = [&](int key0, Pages& p) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int kk = key0 + 16 * t + ln, kv = key0 + 16 * t + 4 * g;
+        p.k[t] = kk < len ? tab[kk >> a.c.page_log2] : -1;
+        p.v[t] = kv < len ? tab[kv >> a.c.page_log2] : -1;
+      }
+    };
+    // a key or value without a page is read from token 0 of page 0 and gets weight 0
+    auto load_k = [&](int key0, const Pages& p, Tile& x) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const bool ok = (unsigned)p.k[t] < (unsigned)a.c.num_pages;
+        const uint16_t* kp = kb + (ok ? p.k[t] * a.c.k_page + ((key0 + 16 * t + ln) & pmask) * a.c.k_slot : 0);
+#pragma unroll
+        for (int j = 0; j < KC; ++j) x.k[t][j] = *reinterpret_cast<const u32x4*>(kp + 32 * j);
+      }
+    };
+    auto load_v = [&](int key0, const Pages& p, Tile& x) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        x.ok[t] = (unsigned)p.v[t] < (unsigned)a.c.num_pages;
+        const uint16_t* vp = vb + (x.ok[t] ? p.v[t] * a.c.v_page + ((key0 + 16 * t + 4 * g) & pmask) * a.c.v_slot : 0);
+        const int64_t step = x.ok[t] ? a.c.v_slot : 0;  // pages hold multiples of 4 tokens: the next 3 are in this one
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (VW == 2) {
+            const u32x2 y = *reinterpret_cast<const u32x2*>(vp + i * step);
+            x.v[4 * t + i][0] = y[0], x.v[4 * t + i][1] = y[1];
+          } else {
+#pragma unroll
+            for (int c = 0; c < VW / 4; ++c) {
+              const u32x4 y = *reinterpret_cast<const u32x4*>(vp + i * step + 8 * c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x.v[4 * t + i][4 * c + e] = y[e];
+            }
+          }
+        }
+      }
+    };
+    Pages pg;
+    Tile x0;
+    if (n) {
+      pages(first, pg);
+      load_k(first, pg, x0);
+      load_v(first, pg, x0);
+      if (n > 1) pages(first + UK, pg);
+    }
     u32x4 qf[KC];
 #pragma unroll
     for (int j = 0; j < KC; ++j)
@@ -134,63 +197,28 @@ __global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
     for (int t = 0; t < VE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    for (int uu = u0; uu < u1; ++uu) {
-      const int key0 = uu * UK + wave * 32;
-      if (key0 >= len) break;
-      // pages of this lane's keys (rows 16 t + l % 16) and of its values (rows 16 t + 4 (l / 16) .. + 3)
-      int64_t ko[2], vo[2];
-      bool vok[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int kk = key0 + 16 * t + ln, kv = key0 + 16 * t + 4 * g;
-        const int kp = kk < len ? tab[kk >> a.c.page_log2] : -1, vp = kv < len ? tab[kv >> a.c.page_log2] : -1;
-        const bool kok = (unsigned)kp < (unsigned)a.c.num_pages;
-        vok[t] = (unsigned)vp < (unsigned)a.c.num_pages;
-        ko[t] = kok ? kp * a.c.k_page + (kk & pmask) * a.c.k_slot : 0;
-        vo[t] = vok[t] ? vp * a.c.v_page + (kv & pmask) * a.c.v_slot : 0;
-      }
-      u32x4 kr[2][KC];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < KC; ++j) kr[t][j] = *reinterpret_cast<const u32x4*>(kb + ko[t] + 32 * j);
-      uint32_t vr[8][VW];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // a page's slots are followed by 3 more here (pages hold multiples of 8 tokens); without a page, token 0 of page 0
-        const uint16_t* p = vb + vo[i / 4] + (vok[i / 4] ? i % 4 * a.c.v_slot : 0);
-        if constexpr (VW == 2) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-          vr[i][0] = x[0], vr[i][1] = x[1];
-        } else {
-#pragma unroll
-          for (int c = 0; c < VW / 4; ++c) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(p + 8 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vr[i][4 * c + e] = x[e];
-          }
-        }
-      }
+    auto compute = [&](int key0, Tile& x, auto&& after_scores) {
       f32x4 s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < KC; ++j) s[t] = mma16<DT>(kr[t][j], qf[j], s[t]);
+        for (int j = 0; j < KC; ++j) s[t] = mma16<DT>(x.k[t][j], qf[j], s[t]);
       }
-      if (!__all(vok[0] && vok[1] && key0 + 32 <= len)) {  // keys past the end or without a page: weight 0, value 0
+      after_scores();
+      if (!__all(x.ok[0] && x.ok[1] && key0 + 32 <= len)) {  // keys past the end or without a page: weight 0, value 0
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (!vok[i / 4] || key0 + 16 * (i / 4) + 4 * g + i % 4 >= len) {
+          if (!x.ok[i / 4] || key0 + 16 * (i / 4) + 4 * g + i % 4 >= len) {
             s[i / 4][i % 4] = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < VW; ++c) vr[i][c] = 0;
+            for (int c = 0; c < VW; ++c) x.v[i][c] = 0;
           }
       }
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }));
       const float mc = mx == -INFINITY ? 0.f : mx * a.scale2;
       const float alpha = exp2_hw(m * a.scale2 - mc);
       m = mx;
@@ -210,15 +238,40 @@ __global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
         const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;  // the pair's high or low halves
         u32x4 f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2], sel);
+        for (int e = 0; e < 4; ++e) f[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][t / 2], x.v[2 * e][t / 2], sel);
         f32x4 c = acc[t];
 #pragma unroll
         for (int r = 0; r < 4; ++r) c[r] *= alpha;
         acc[t] = mma16<DT>(f, p, c);
       }
+    };
+    if constexpr (D == 256) {  // no registers for a second tile: the next keys and values as soon as these are used
+      for (int i = 0; i < n; ++i) {
+        const int next = first + (i + 1) * UK;
+        compute(first + i * UK, x0, [&] {
+          if (i + 1 < n) load_k(next, pg, x0);
+        });
+        if (i + 1 < n) load_v(next, pg, x0);
+        if (i + 2 < n) pages(next + UK, pg);
+      }
+    } else {
+      Tile x1;
+      auto turn = [&](int i, Tile& now, Tile& then) {  // the next tile's loads and the one after's pages before the products
+        const int next = first + (i + 1) * UK;
+        if (i + 1 < n) {
+          load_k(next, pg, then);
+          load_v(next, pg, then);
+        }
+        if (i + 2 < n) pages(next + UK, pg);
+        compute(first + i * UK, now, [] {});
+      };
+      for (int i = 0; i < n; i += 2) {
+        turn(i, x0, x1);
+        if (i + 1 < n) turn(i + 1, x1, x0);
+      }
     }
     l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = halves(l, [](float p, float q) { return p + q; });
 
     // the waves' pieces, joined in wave order
     if (g == 0) {
@@ -234,6 +287,11 @@ __global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
     __syncthreads();
     const bool whole = u0 == 0 && u1 == nu;
     const int64_t slot = blockIdx.x * 2 + (u0 == 0);
+    if (u0 == 0 && tid == 0) {
+      const int64_t at = ((int64_t)b * heads + hb) * 2;
+      a.shares[at] = blockIdx.x;
+      a.shares[at + 1] = (int)div64(item + nu - 1, per);
+    }
     for (int i = tid; i < nh * (D / 4); i += DT_THREADS) {
       const int h = i / (D / 4), d = i % (D / 4) * 4;
       float mm = sm[0][h];
@@ -263,42 +321,60 @@ __global__ __launch_bounds__(DT_THREADS) void attn_decode_kernel(DecodeArgs a) {
     }
     __syncthreads();
     u = item + u1;
+    if (++hb == heads && u < uend) {  // the next sequence that has keys
+      base += (int64_t)nu * heads;
+      hb = 0;
+      do len = __builtin_amdgcn_readfirstlane(seq_len(a, ++b));
+      while (len == 0);
+      nu = units_of(len);
+    }
   }
 }
 
-// One workgroup per (sequence, head block): adds up the pieces that the shares cut it into, in order; writes zeros for a
-// sequence without keys.
+// One workgroup per (sequence, query head): adds up the pieces that the shares cut the head's keys into, in order; zeros
+// for a sequence without keys.  Groups of D / 4 threads take every so many-th piece, then their sums are added.
 template <int D, int DT>
-__global__ __launch_bounds__(DT_THREADS) void attn_join_kernel(DecodeArgs a) {
-  __shared__ int64_t pre[DT_THREADS + 1];
-  const int heads = a.hk * a.hblocks, b = blockIdx.x / heads, hb = blockIdx.x % heads, tid = threadIdx.x;
-  const int kvh = hb / a.hblocks, h0 = kvh * a.group + hb % a.hblocks * 16, nh = min(16, (kvh + 1) * a.group - h0);
-  unit_prefix(a, pre);
-  const int slab = slab_size(a);
-  int64_t base = pre[b / slab];
-  for (int i = b / slab * slab; i < b; ++i) base += seq_units(a, i);
-  const int64_t per = share(a, pre[DT_THREADS] * heads), nu = seq_units(a, b);
-  const int64_t first = base * heads + hb * nu;
-  const int64_t w0 = first / per, w1 = nu ? (first + nu - 1) / per : w0;
-  if (nu && w0 == w1) return;
-  for (int i = tid; i < nh * (D / 4); i += DT_THREADS) {
-    const int h = i / (D / 4), d = i % (D / 4) * 4;
-    float m = -INFINITY, l = 0.f;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (nu) {
-      for (int64_t w = w0; w <= w1; ++w) m = fmaxf(m, a.pm[(w * 2 + (w == w0)) * 32 + h]);
-      for (int64_t w = w0; w <= w1; ++w) {
-        const int64_t slot = w * 2 + (w == w0);
-        const float pm = a.pm[slot * 32 + h], f = pm == -INFINITY ? 0.f : exp2_hw(pm - m);
-        l += f * a.pm[slot * 32 + 16 + h];
-        x += f * *reinterpret_cast<const f32x4*>(a.po + (slot * 16 + h) * D + d);
-      }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<u32x2*>(a.o + ((int64_t)b * a.hq + h0 + h) * D + d) =
-        u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
-    if (a.lse && d == 0) a.lse[(int64_t)b * a.hq + h0 + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+__global__ __launch_bounds__(256) void attn_join_kernel(DecodeArgs a) {
+  constexpr int LPR = D / 4, G = 256 / LPR;
+  __shared__ float red[4], wt[DECODE_GRID + 1];
+  __shared__ __attribute__((aligned(16))) f32x4 part[G][LPR];
+  __shared__ float psum[G];
+  const int b = blockIdx.x / a.hq, hq = blockIdx.x % a.hq, tid = threadIdx.x;
+  const int kvh = hq / a.group, h = hq % a.group % 16, hb = kvh * a.hblocks + hq % a.group / 16;
+  const int grp = tid / LPR, d = tid % LPR * 4;
+  const int64_t at = ((int64_t)b * a.hk * a.hblocks + hb) * 2;
+  const bool empty = seq_len(a, b) == 0;
+  const int w0 = empty ? 0 : a.shares[at], n = empty ? 0 : a.shares[at + 1] - w0 + 1;
+  if (n == 1) return;
+  auto slot = [&](int i) { return (int64_t)(w0 + i) * 2 + (i == 0); };
+  float m = -INFINITY;
+  for (int i = tid; i < n; i += 256) m = fmaxf(m, wt[i] = a.pm[slot(i) * 32 + h]);
+  m = wave_max(m);
+  if (tid % 64 == 0) red[tid / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float l = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int i = grp; i < n; i += G) {
+    const float f = wt[i] == -INFINITY ? 0.f : exp2_hw(wt[i] - m);
+    l += f * a.pm[slot(i) * 32 + 16 + h];
+    x += f * *reinterpret_cast<const f32x4*>(a.po + (slot(i) * 16 + h) * D + d);
   }
+  part[grp][tid % LPR] = x;
+  if (d == 0) psum[grp] = l;
+  __syncthreads();
+  if (grp) return;
+  l = 0.f;
+  x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    l += psum[i];
+    x += part[i][tid];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(a.o + ((int64_t)b * a.hq + hq) * D + d) =
+      u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+  if (a.lse && d == 0) a.lse[(int64_t)b * a.hq + hq] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
 }
 
 // ------------------------------------------------------------------------------------ writing to the cache
@@ -377,11 +453,14 @@ int check_new_rows(const char* what, const lsurge_attn_rows* r) {
   return LSURGE_OK;
 }
 
-constexpr int DECODE_GRID = 512;
-int64_t decode_grid(int64_t nseq, int64_t hk, int64_t hblocks, int64_t max_pages, int64_t page_size) {
-  const double most = (double)nseq * hk * hblocks * (((double)max_pages * page_size + UK - 1) / UK);
-  return most < DECODE_GRID ? std::max<int64_t>(1, (int64_t)most) : DECODE_GRID;
+// Workgroups that the units are dealt to: as many as the registers let a GPU of 256 CUs hold at a time, or one for every
+// unit that the page table's width allows where that is less.
+int64_t decode_grid(int64_t nseq, int64_t heads, int64_t d, int64_t max_pages, int64_t page_size) {
+  const double most = (double)nseq * heads * (((double)max_pages * page_size + UK - 1) / UK);
+  const int64_t full = d == 64 ? DECODE_GRID * 3 / 4 : DECODE_GRID / 2;
+  return most < full ? std::max<int64_t>(1, (int64_t)most) : full;
 }
+size_t decode_parts_bytes(int64_t d) { return sizeof(float) * (size_t)DECODE_GRID * 2 * 16 * (size_t)(d + 2); }
 
 }  // namespace
 }  // namespace lsattn
@@ -390,9 +469,9 @@ using namespace lsattn;
 
 extern "C" {
 
-size_t lsurge_paged_attn_workspace_bytes(int64_t d) {
-  if (d < 1 || d > 256) return 0;
-  return sizeof(float) * (size_t)DECODE_GRID * 2 * 16 * (size_t)(d + 2);
+size_t lsurge_paged_attn_workspace_bytes(int64_t nseq, int64_t hq, int64_t d) {
+  if (nseq < 0 || nseq >= (1 << 24) || hq < 1 || hq > 65535 || d < 1 || d > 256) return 0;
+  return decode_parts_bytes(d) + sizeof(int32_t) * 2 * (size_t)(nseq * hq);
 }
 
 int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64_t nseq, int64_t hq, float scale, void* o,
@@ -406,7 +485,7 @@ int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64
   if (nseq == 0) return LSURGE_OK;
   if (int rc = check_new_rows("paged_attn q", q)) return rc;
   LSURGE_REQUIRE(o && workspace && ((uintptr_t)o | (uintptr_t)workspace) % 16 == 0, "paged_attn: null or misaligned pointer");
-  const size_t need = lsurge_paged_attn_workspace_bytes(c->d);
+  const size_t need = lsurge_paged_attn_workspace_bytes(nseq, hq, c->d);
   if (workspace_bytes < need)
     return lsurge::set_error(LSURGE_ERR_WORKSPACE, "paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
   LSURGE_REQUIRE((int64_t)c->max_pages * c->page_size < (1ll << 31), "paged_attn: %lld pages of %lld tokens a sequence",
@@ -417,15 +496,16 @@ int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64
   a.hblocks = (a.group + 15) / 16;
   a.scale2 = scale * LOG2E;
   a.o = (uint16_t*)o, a.lse = lse;
-  a.grid = (int)decode_grid(nseq, a.hk, a.hblocks, c->max_pages, c->page_size);
+  a.grid = (int)decode_grid(nseq, (int64_t)a.hk * a.hblocks, c->d, c->max_pages, c->page_size);
   a.po = (float*)workspace;
   a.pm = a.po + (size_t)DECODE_GRID * 2 * 16 * c->d;
-  const int64_t items = nseq * a.hk * a.hblocks;
-  LSURGE_REQUIRE(items < (1ll << 31), "paged_attn: %lld sequences of %lld heads", (long long)nseq, (long long)hq);
+  a.shares = (int32_t*)((char*)workspace + decode_parts_bytes(c->d));
+  const int64_t rows = nseq * hq;
+  LSURGE_REQUIRE(rows < (1ll << 31), "paged_attn: %lld sequences of %lld heads", (long long)nseq, (long long)hq);
   hipStream_t st = (hipStream_t)stream;
 #define DECODE(D, DT)                                                                                              \
   LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_decode_kernel<D, DT>), dim3(a.grid), dim3(DT_THREADS), 0, st, a)); \
-  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_join_kernel<D, DT>), dim3((unsigned)items), dim3(DT_THREADS), 0, st, a))
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_join_kernel<D, DT>), dim3((unsigned)rows), dim3(256), 0, st, a))
   if (c->dtype == LSURGE_BF16) {
     if (c->d == 64) { DECODE(64, LSURGE_BF16); }
     else if (c->d == 128) { DECODE(128, LSURGE_BF16); }

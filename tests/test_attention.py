@@ -221,7 +221,7 @@ def _kv(**kw):
 def test_c_abi_cache_refusals():
     lib = L.lib()
     r = ctypes.byref(L.AttnRows(256, 512, 64))
-    ws = lib.lsurge_paged_attn_workspace_bytes(64)
+    ws = lib.lsurge_paged_attn_workspace_bytes(2, 4, 64)
     attn = lambda c, n=2, hq=4, scale=1.0, o=FAKE, nb=ws: lib.lsurge_paged_attn(  # noqa: E731
         ctypes.byref(c), r, n, hq, scale, o, None, FAKE, nb, None)
     put = lambda c, rows=2, n=2, cu=None, k=r: lib.lsurge_kv_append(ctypes.byref(c), k, r, rows, n, cu, None)  # noqa: E731
