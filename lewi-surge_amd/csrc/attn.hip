@@ -27,20 +27,26 @@ struct AttnArgs {
   float scale2;  // scale log2(e)
 };
 
-// Workgroup -> (head, tile), long tiles first.  Workgroups are dealt to the 8 XCDs round-robin; with a multiple of 8
-// heads every XCD gets heads of its own, whose keys its L2 then serves.
-__device__ __forceinline__ void head_tile(int heads, int ntiles, int& head, int& tile) {
-  const int id = (int)blockIdx.x;
-  int rank;
-  if (heads % 8 == 0) {
-    const int per = heads / 8, i = id / 8;
-    head = id % 8 * per + i % per;
-    rank = i / per;
+// Workgroup -> (head, tile slot).  Workgroups are dealt to the 8 XCDs round-robin and each XCD has an L2 of its own, so the
+// (sequence, head) pairs are cut into 8 runs where their number allows, and within a run `share` heads that read the same
+// rows go tile by tile together: the workgroups that run on an XCD at a time then walk the same keys.  8 x 4096 tokens, 8
+// heads over 2: MEASURED_XCD.  Packed sequences have their borders on the device, so their tile slots are one sequence
+// here.  Tiles go from the last to the first (the long ones of a causal sequence first) or, with `up`, the other way.
+__device__ __forceinline__ void head_tile(int heads, int share, int nseq, int ntiles, bool up, int& head, int& slot) {
+  const int id = (int)blockIdx.x, tiles = ntiles / nseq, pairs = nseq * heads;  // tiles of one sequence
+  int pair, tile;
+  if (pairs % 8 == 0) {
+    const int run = pairs / 8, i = id / 8;
+    const int g = run * tiles <= 128 ? run : run % share == 0 ? share : share % run == 0 ? run : 1;
+    const int set = i / (g * tiles), r = i % (g * tiles);
+    pair = id % 8 * run + set * g + r % g;
+    tile = r / g;
   } else {
-    head = id % heads;
-    rank = id / heads;
+    pair = id % pairs;
+    tile = id / pairs;
   }
-  tile = ntiles - 1 - rank;
+  head = pair % heads;
+  slot = pair / heads * tiles + (up ? tile : tiles - 1 - tile);
 }
 
 // rows [first, first + n) of [rows, heads, D] at one head, zeroed (rows behind the last sequence)
@@ -113,7 +119,7 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   int head, slot;
-  head_tile(a.hq, a.ntiles, head, slot);
+  head_tile(a.hq, a.hq / a.hk, a.cu_q ? 1 : a.nseq, a.ntiles, false, head, slot);
   if (a.cu_q) {
     const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
     const int n = (int)min((int64_t)BM, a.total_q - end);
@@ -342,7 +348,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   int head, slot;
-  head_tile(a.hq, a.ntiles, head, slot);
+  head_tile(a.hq, a.hq / a.hk, a.cu_q ? 1 : a.nseq, a.ntiles, false, head, slot);
   if (a.cu_q) {
     const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
     const int n = (int)min((int64_t)BM, a.total_q - end);
@@ -466,9 +472,8 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   int unit, slot;
-  head_tile(a.hk * parts, a.ntiles, unit, slot);
+  head_tile(a.hk * parts, 1, a.cu_k ? 1 : a.nseq, a.ntiles, true, unit, slot);  // the first keys are seen by the most
   const int kvh = unit / parts, part = unit % parts;
-  slot = a.ntiles - 1 - slot;  // the first keys are seen by the most queries
   if (a.cu_k && part == 0) {
     const int64_t end = cu_at(a.cu_k, a.nseq, a.total_k) + (int64_t)slot * BK;
     const int n = (int)min((int64_t)BK, a.total_k - end);
@@ -727,7 +732,7 @@ int64_t dkv_parts(const lsurge_attn_shape& s) {
   const double tiles = (double)s.nseq * (double)((s.total_k / s.nseq + 127) / 128) * s.hk;
   const double stages = (double)(s.hq / s.hk) * (double)s.total_q / (double)s.nseq / QN / 2;
   const double parts = std::min(std::min(sqrt(64.0 * stages / std::max(tiles, 1.0)), 4096.0 / std::max(tiles, 1.0)), 8.0);
-  return std::max<int64_t>(1, (int64_t)parts);
+  return parts >= 8 ? 8 : parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
 }
 
 #define ATTN_DISPATCH(CALL)                                                     \
