@@ -99,8 +99,11 @@ def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse):
     shape = L.AttnShape(nseq, tq, tk, hq, hk, d, L.dt(q))
     o = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device) if want_lse else None
-    _call("attn_fwd", q.device, L.lib().lsurge_attn_fwd, ctypes.byref(shape), _rows_arg(q), _rows_arg(k), _rows_arg(v),
-          L.ptr(cu_q), L.ptr(cu_k), scale, L.ptr(o), L.ptr(lse))
+    lib, arg = L.lib(), ctypes.byref(shape)
+    nbytes = lib.lsurge_attn_fwd_workspace_bytes(arg)
+    ws = L.workspace(nbytes, q.device) if nbytes else None
+    _call("attn_fwd", q.device, lib.lsurge_attn_fwd, arg, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q), L.ptr(cu_k),
+          scale, L.ptr(o), L.ptr(lse), L.ptr(ws), nbytes)
     return o, lse, (q, k, v), shape
 
 

@@ -11,7 +11,6 @@
 // the same lane, and P^T is in place as the second product's operand (the keys of 8 consecutive registers are the ones
 // its fragment takes, in an order that V^T's fragment is read in as well).  No value crosses lanes on the way.
 #include <algorithm>
-#include <cmath>
 
 #include "attn_common.h"
 #include "launchers.h"
@@ -30,8 +29,9 @@ struct AttnArgs {
 // Workgroup -> (head, tile slot).  Workgroups are dealt to the 8 XCDs round-robin and each XCD has an L2 of its own, so the
 // (sequence, head) pairs are cut into 8 runs where their number allows, and within a run `share` heads that read the same
 // rows go tile by tile together: the workgroups that run on an XCD at a time then walk the same keys.  8 x 4096 tokens, 8
-// heads over 2: MEASURED_XCD.  Packed sequences have their borders on the device, so their tile slots are one sequence
-// here.  Tiles go from the last to the first (the long ones of a causal sequence first) or, with `up`, the other way.
+// heads over 2: 1530 us a training step with heads dealt to XCDs, 1441 so; 8 x 2048 prompts, 16 heads: 172 and 161.  Where an XCD has
+// few workgroups (two rounds) all its heads go together, so that the longest start first (one sequence of 4096: 356 and
+// 328 us).  Packed sequences have their borders on the device, so their tile slots are one sequence here.  Tiles go from the last to the first (the long ones of a causal sequence first) or, with `up`, the other way.
 __device__ __forceinline__ void head_tile(int heads, int share, int nseq, int ntiles, bool up, int& head, int& slot) {
   const int id = (int)blockIdx.x, tiles = ntiles / nseq, pairs = nseq * heads;  // tiles of one sequence
   int pair, tile;
@@ -113,45 +113,43 @@ __device__ __forceinline__ void rescale(f32x16& acc, float f) {
 template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(FWD_EU<D>)))
-void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ lse) {
+void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
+                     float* __restrict__ lse) {
   constexpr int BM = NW * 32, TILE = FN * D * 2;  // bytes of one operand of one stage
   __shared__ __attribute__((aligned(1024))) char smem[6 * TILE];  // three stages of K, then three of V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  int head, slot;
-  head_tile(a.hq, a.hq / a.hk, a.cu_q ? 1 : a.nseq, a.ntiles, false, head, slot);
-  if (a.cu_q) {
-    const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
-    const int n = (int)min((int64_t)BM, a.total_q - end);
-    if (n > 0) {
-      zero_rows<D>(o, end, n, a.hq, head, threadIdx.x, NW * 64);
-      if (lse && (int)threadIdx.x < n) lse[(int64_t)head * a.total_q + end + threadIdx.x] = -INFINITY;
-    }
+  const int group = a.hq / a.hk;
+  int unit, slot;  // unit: key head, part, head of the group, so that the heads that share keys stay together
+  head_tile(a.hq * parts, group, a.cu_q ? 1 : a.nseq, a.ntiles, false, unit, slot);
+  const int kvh = unit / (parts * group), part = unit / group % parts, head = kvh * group + unit % group;
+  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  if (pl.end + (int64_t)slot * BM < a.total_q && part == 0) {  // the slots cover the rows behind the last sequence too
+    const int64_t first = pl.end + (int64_t)slot * BM;
+    const int n = (int)min((int64_t)BM, a.total_q - first);
+    zero_rows<D>(o, first, n, a.hq, head, threadIdx.x, NW * 64);
+    if (lse && (int)threadIdx.x < n) lse[(int64_t)head * a.total_q + first + threadIdx.x] = -INFINITY;
   }
-  int tile;
-  const int seq = seq_of_tile<BM>(a.cu_q, a.nseq, a.total_q, slot, lane, tile);
-  if (seq < 0) return;
-  int q0, nq, k0, nk;
-  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
-  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
-  if (tile * BM >= nq) return;
+  const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
+  if (pl.seq < 0 || tile * BM >= nq) return;
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
-  const int kvh = head / (a.hq / a.hk);
 
   const uint32_t lds = lds_addr((const bf16_t*)smem);
   TileCopy<D, FN, NW> ck, cv;
   ck.init(a.k_row, wave, lane);
   cv.init(a.v_row, wave, lane);
-  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
-  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
   const int kend = min(nq, (tile + 1) * BM) + off;  // keys the workgroup's last row sees
-  const int nst = (max(kend, 0) + FN - 1) / FN;
-  const int nsw = min(nst, (max(w0 + 32 + off, 0) + FN - 1) / FN);  // stages that the wave's rows see
+  const int all = (max(kend, 0) + FN - 1) / FN;
+  const int begin = (int)((int64_t)all * part / parts), nst = (int)((int64_t)all * (part + 1) / parts) - begin;
+  const int nsw = (max(w0 + 32 + off, 0) + FN - 1) / FN - begin;  // stages that the wave's rows see
+  const int kfirst = begin * FN, left = nk - kfirst;  // the part's first key, and the keys from there on
+  const uint16_t* kb = a.k + (int64_t)(k0 + kfirst) * a.k_row + kvh * a.k_head;
+  const uint16_t* vb = a.v + (int64_t)(k0 + kfirst) * a.v_row + kvh * a.v_head;
   auto issue_k = [&](int st, int slot) {  // stages past the end fill with zeros
-    ck.issue(kb + (int64_t)st * FN * a.k_row, a.k_row, nk - st * FN, lds + slot * TILE, wave);
+    ck.issue(kb + (int64_t)st * FN * a.k_row, a.k_row, left - st * FN, lds + slot * TILE, wave);
   };
   auto issue_v = [&](int st, int slot) {
-    cv.issue(vb + (int64_t)st * FN * a.v_row, a.v_row, nk - st * FN, lds + (3 + slot) * TILE, wave);
+    cv.issue(vb + (int64_t)st * FN * a.v_row, a.v_row, left - st * FN, lds + (3 + slot) * TILE, wave);
   };
   constexpr int CP = 2 * TileCopy<D, FN, NW>::N;  // copies of a stage
   if (nst) {
@@ -196,8 +194,8 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
     issue_v(st + 2, (u + 2) % 3);
     issue_k(st + 3, u);
     if (st >= nsw) return;  // nothing of this stage is visible to the wave's rows
-    if (st * FN + FN - 1 > w0 + off) {  // the diagonal or the end of the keys
-      const int lim = row + off - st * FN;
+    if (st * FN + FN - 1 > w0 + off - kfirst) {  // the diagonal or the end of the keys
+      const int lim = row + off - kfirst - st * FN;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (8 * (r / 4) + 4 * hf + r % 4 > lim) s[r] = -INFINITY;
@@ -259,6 +257,17 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
   }
   l = halves(l, [](float x, float y) { return x + y; });
   if (row >= nq) return;
+  if (parts > 1) {  // the sums as they are, and what they are relative to
+    const int64_t at = (int64_t)part * a.total_q + q0 + row;
+    float* pp = po + (at * a.hq + head) * D + 4 * hf;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(pp + 32 * d + 2 * r) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+    if (hf == 0) pm[at * a.hq + head] = f32x2_t{mc, l};
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* op = o + ((int64_t)(q0 + row) * a.hq + head) * D + 4 * hf;
 #pragma unroll
@@ -269,6 +278,31 @@ void attn_fwd_kernel(AttnArgs a, uint16_t* __restrict__ o, float* __restrict__ l
                                                              pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv)};
   if (lse && hf == 0)
     lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * LN2;
+}
+
+// o and lse from the parts' sums, added in order: D / 4 threads a row and head
+template <int D, int DT>
+__global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int parts, const float* __restrict__ po,
+                                                            const f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
+                                                            float* __restrict__ lse) {
+  constexpr int LPR = D / 4;
+  const int64_t n = (a.cu_q ? cu_at(a.cu_q, a.nseq, a.total_q) : a.total_q) * (int64_t)a.hq, step = (int64_t)a.total_q * a.hq;
+  const int d = threadIdx.x % LPR * 4;
+  for (int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i < n; i += (int64_t)gridDim.x * (256 / LPR)) {
+    float m = -INFINITY, l = 0.f;
+    for (int p = 0; p < parts; ++p)
+      if (pm[p * step + i][1] != 0.f) m = fmaxf(m, pm[p * step + i][0]);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p) {
+      const f32x2_t s = pm[p * step + i];
+      const float f = s[1] == 0.f ? 0.f : exp2_hw(s[0] - m);
+      l += f * s[1];
+      if (f != 0.f) x += f * *reinterpret_cast<const f32x4*>(po + (p * step + i) * D + d);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<u32x2*>(o + i * D + d) = u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+    if (lse && d == 0) lse[i % a.hq * a.total_q + i / a.hq] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+  }
 }
 
 // ------------------------------------------------------------------------------------ backward
@@ -349,18 +383,13 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
   const int ln = lane & 31, hf = lane >> 5;
   int head, slot;
   head_tile(a.hq, a.hq / a.hk, a.cu_q ? 1 : a.nseq, a.ntiles, false, head, slot);
-  if (a.cu_q) {
-    const int64_t end = cu_at(a.cu_q, a.nseq, a.total_q) + (int64_t)slot * BM;
-    const int n = (int)min((int64_t)BM, a.total_q - end);
-    if (n > 0) zero_rows<D>(dq, end, n, a.hq, head, threadIdx.x, NW * 64);
+  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  if (pl.end + (int64_t)slot * BM < a.total_q) {
+    const int64_t first = pl.end + (int64_t)slot * BM;
+    zero_rows<D>(dq, first, (int)min((int64_t)BM, a.total_q - first), a.hq, head, threadIdx.x, NW * 64);
   }
-  int tile;
-  const int seq = seq_of_tile<BM>(a.cu_q, a.nseq, a.total_q, slot, lane, tile);
-  if (seq < 0) return;
-  int q0, nq, k0, nk;
-  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
-  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
-  if (tile * BM >= nq) return;
+  const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
+  if (pl.seq < 0 || tile * BM >= nq) return;
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
   const int kvh = head / (a.hq / a.hk);
 
@@ -474,21 +503,15 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   int unit, slot;
   head_tile(a.hk * parts, 1, a.cu_k ? 1 : a.nseq, a.ntiles, true, unit, slot);  // the first keys are seen by the most
   const int kvh = unit / parts, part = unit % parts;
-  if (a.cu_k && part == 0) {
-    const int64_t end = cu_at(a.cu_k, a.nseq, a.total_k) + (int64_t)slot * BK;
-    const int n = (int)min((int64_t)BK, a.total_k - end);
-    if (n > 0) {
-      zero_rows<D>(dk, end, n, a.hk, kvh, threadIdx.x, NW * 64);
-      zero_rows<D>(dv, end, n, a.hk, kvh, threadIdx.x, NW * 64);
-    }
+  const Place pl = find_tile<BK, true>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  if (pl.end + (int64_t)slot * BK < a.total_k && part == 0) {
+    const int64_t first = pl.end + (int64_t)slot * BK;
+    const int n = (int)min((int64_t)BK, a.total_k - first);
+    zero_rows<D>(dk, first, n, a.hk, kvh, threadIdx.x, NW * 64);
+    zero_rows<D>(dv, first, n, a.hk, kvh, threadIdx.x, NW * 64);
   }
-  int tile;
-  const int seq = seq_of_tile<BK>(a.cu_k, a.nseq, a.total_k, slot, lane, tile);
-  if (seq < 0) return;
-  int q0, nq, k0, nk;
-  seq_rows(a.cu_q, a.nseq, a.total_q, seq, q0, nq);
-  seq_rows(a.cu_k, a.nseq, a.total_k, seq, k0, nk);
-  if (tile * BK >= nk) return;
+  const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
+  if (pl.seq < 0 || tile * BK >= nk) return;
   const int off = nk - nq, w0 = tile * BK + wave * 32, col = w0 + ln, group = a.hq / a.hk;
 
   const uint32_t lds = lds_addr((const bf16_t*)smem), lds_rows = lds + 2 * R * TILE, lds_v = lds_rows + 1024;
@@ -722,17 +745,32 @@ AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const 
 template <int D> constexpr int WAVES = 4;
 
 // Parts that the stages of a tile of keys are cut into in attn_dkv_kernel, by the sizes that the host knows (the
-// sequences' own lengths are on the device).  A part costs a write and a read of the tile's f32 sums, an unsplit grid idle
-// CUs behind the workgroups with the most queries: the sum of a term that falls with the workgroups and one that rises
-// with the parts is least where parts^2 is in proportion to stages / tiles.  8 x 4096 tokens of 8 heads over 2: one part
-// 1697 us a training step, two 1655, four 1516, eight 1680; one sequence of 512: 150, 104, 81, 68; of 4096, 8 heads of
-// their own keys: 425, 346, 328, 389; packed documents (31 of 1150 tokens, 16 heads): 813 unsplit, 1028 in two.
+// sequences' own lengths are on the device): as many as give every place for a workgroup two of them, so that the ones
+// with few queries fill up behind the ones with many, but no part under 4 stages; one part for every 1024 stages where
+// they are that many.  A part costs a write and a read of the tile's f32 sums.  Measured, us a training step at 1, 2, 4
+// and 8 parts: 8 x 4096 tokens, 8 heads over 2 (512 tiles, 256 stages): 1568, 1346, 1435, 1485; one of 32768, 16 heads
+// over 4 (1024, 2048): 19532, 19021, 18961, 18864; one of 4096, 8 heads of their own keys (256, 64): 433, 351, 330, 391;
+// one of 512, 8 over 2 (8, 32): 154, 106, 82, 72; 2 x 4096, 16 over 2, 256-wide (128, 512): 3552, 2357, 1721, 1756.
 int64_t dkv_parts(const lsurge_attn_shape& s) {
   if (s.total_q == 0 || s.total_k == 0 || s.nseq == 0) return 1;
-  const double tiles = (double)s.nseq * (double)((s.total_k / s.nseq + 127) / 128) * s.hk;
-  const double stages = (double)(s.hq / s.hk) * (double)s.total_q / (double)s.nseq / QN / 2;
-  const double parts = std::min(std::min(sqrt(64.0 * stages / std::max(tiles, 1.0)), 4096.0 / std::max(tiles, 1.0)), 8.0);
+  const int64_t tiles = s.nseq * ((s.total_k / s.nseq + 127) / 128) * s.hk, places = s.d == 256 ? 256 : 512;
+  const int64_t stages = s.hq / s.hk * (s.total_q / s.nseq) / QN / 2;  // half of the queries, on average, see a key
+  const int64_t parts = std::min(std::max(2 * places / std::max<int64_t>(tiles, 1), stages / 1024), stages / 4);
   return parts >= 8 ? 8 : parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
+}
+
+// Parts that the keys of a tile of queries are cut into in attn_fwd_kernel: as many as fill the places for a workgroup,
+// where there are few tiles, and none under 16 stages (a part costs a write and a read of the tile's f32 sums).  Measured,
+// us at 1, 2, 3, 4, 8 parts: 3 chunks of 350 rows over 10000 keys, 32 heads (288 tiles, 300 stages): 369, 247, 260, 254,
+// 259; 64 rows over 6000 keys, 16 heads (16, 190): 118, 68, 51, 42, 33; one prompt of 2048 (256, 32): 48, 47, 52, 57, 83;
+// of 4096, 8 heads, 64-wide (256, 64): 71, 51, 44, 45, 57; of 512 (64, 8): 20, 23, 24, 26, 33.
+int64_t fwd_parts(const lsurge_attn_shape& s) {
+  if (s.total_q == 0 || s.total_k == 0 || s.nseq == 0) return 1;
+  const int64_t rows = s.total_q / s.nseq, keys = s.total_k / s.nseq;
+  const int64_t tiles = std::max<int64_t>(s.nseq * ((rows + 127) / 128) * s.hq, 1);
+  const int64_t places = s.d == 256 ? 256 : s.d == 128 ? 512 : 768;
+  const int64_t stages = std::max<int64_t>(keys - rows / 2, 0) / FN;  // of an average tile
+  return std::max<int64_t>(1, std::min((places + tiles / 2) / tiles, stages / 16));
 }
 
 #define ATTN_DISPATCH(CALL)                                                     \
@@ -761,9 +799,15 @@ using namespace lsattn;
 
 extern "C" {
 
+size_t lsurge_attn_fwd_workspace_bytes(const lsurge_attn_shape* s) {
+  if (!s || s->hq < 1 || s->hk < 1 || s->d < 1 || s->nseq < 0 || s->total_q < 0 || s->total_k < 0) return 0;
+  const int64_t parts = fwd_parts(*s);
+  return parts > 1 ? sizeof(float) * (size_t)(parts * s->total_q * s->hq * (s->d + 2)) : 0;
+}
+
 int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, float* lse,
-                    lsurge_stream_t stream) {
+                    void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
   if (int rc = check_shape("attn_fwd", s, cu_q, cu_k, scale)) return rc;
   if (s->total_q == 0) return LSURGE_OK;
   LSURGE_REQUIRE(q && k && v && o && (uintptr_t)o % 16 == 0, "attn_fwd: null or misaligned pointer");
@@ -772,15 +816,27 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
     if (int rc = check_rows("attn_fwd k", *k, s->d)) return rc;
     if (int rc = check_rows("attn_fwd v", *v, s->d)) return rc;
   }
+  const size_t need = lsurge_attn_fwd_workspace_bytes(s);
+  if (workspace_bytes < need)
+    return lsurge::set_error(LSURGE_ERR_WORKSPACE, "attn_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
+  LSURGE_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0), "attn_fwd: null or misaligned workspace");
   hipStream_t st = (hipStream_t)stream;
   AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
-#define ATTN_FWD(D, DT)                                                                                             \
-  constexpr int NW = WAVES<D>;                                                                                      \
-  a.ntiles = (int)num_tiles(*s, cu_q, s->total_q, NW * 32);                                                         \
-  unsigned grid;                                                                                                    \
-  if (int rc = tile_grid("attn_fwd", a.ntiles, s->hq, &grid)) return rc;                                            \
-  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a, \
-                                                 (uint16_t*)o, lse))
+  const int parts = (int)fwd_parts(*s);
+  float* po = (float*)workspace;
+  f32x2_t* pm = (f32x2_t*)(po + (size_t)parts * s->total_q * s->hq * s->d);
+#define ATTN_FWD(D, DT)                                                                                               \
+  constexpr int NW = WAVES<D>;                                                                                        \
+  a.ntiles = (int)num_tiles(*s, cu_q, s->total_q, NW * 32);                                                           \
+  unsigned grid;                                                                                                      \
+  if (int rc = tile_grid("attn_fwd", a.ntiles, s->hq * parts, &grid)) return rc;                                      \
+  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a,   \
+                                                 parts, po, pm, (uint16_t*)o, lse));                                  \
+  const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                              \
+  if (parts > 1)                                                                                                      \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_join_kernel<D, DT>),                                     \
+                                                   dim3((unsigned)std::min<int64_t>(rows, 8192)), dim3(256), 0, st, a, \
+                                                   parts, po, pm, (uint16_t*)o, lse))
   ATTN_DISPATCH(ATTN_FWD);
 #undef ATTN_FWD
   return LSURGE_OK;

@@ -145,40 +145,63 @@ __device__ __forceinline__ u32x4 lds_read_col(uint32_t a) {
 // held to [0, total], so that no table makes a kernel read or write outside its rows.
 __device__ __forceinline__ int cu_at(const int32_t* cu, int i, int total) { return min(max(cu[i], 0), total); }
 
-// Tile t of the rows: sequence s owns the tiles from cu[s] / B + s, which leaves it at least ceil(rows / B).  Returns the
-// sequence (wave-uniform, by a 64-way search), or -1.
-template <int B>
-__device__ __forceinline__ int seq_of_tile(const int32_t* cu, int nseq, int total, int t, int lane, int& tile) {
-  if (!cu) {
-    const int per = total / nseq, tiles = (per + B - 1) / B;
-    if (tiles == 0 || t / tiles >= nseq) return -1;
-    tile = t % tiles;
-    return t / tiles;
+// Tile t of the rows: sequence s owns the tiles from cu[s] / B + s, which leaves it at least ceil(rows / B).  A packed
+// sequence is found by a 64-way search; up to 63 sequences all ends are read at once, and one trip to memory is all that a
+// workgroup waits for before its first rows.
+struct Place {
+  int seq, tile;          // sequence (-1: none) and its tile
+  int q0, nq, k0, nk;     // its rows
+  int64_t end;            // the first row behind the last sequence
+};
+template <int B, bool KEYS>  // tiles of the keys, or of the queries
+__device__ __forceinline__ Place find_tile(const int32_t* cu_q, const int32_t* cu_k, int nseq, int total_q, int total_k,
+                                           int t, int lane) {
+  Place p;
+  p.seq = -1;
+  p.tile = p.q0 = p.nq = p.k0 = p.nk = 0;
+  if (!cu_q) {
+    p.nq = total_q / nseq, p.nk = total_k / nseq;
+    p.end = KEYS ? total_k : total_q;
+    const int tiles = ((KEYS ? p.nk : p.nq) + B - 1) / B;
+    if (tiles == 0 || t / tiles >= nseq) return p;
+    p.seq = t / tiles, p.tile = t % tiles;
+    p.q0 = p.seq * p.nq, p.k0 = p.seq * p.nk;
+    return p;
   }
-  int lo = 0, n = nseq;
-  while (true) {
-    const int step = (n + 63) / 64, i = lo + lane * step;
-    const bool in = lane * step < n && cu_at(cu, i, total) / B + i <= t;
-    const int c = __popcll(__ballot(in));
-    if (c == 0) return -1;
-    n = min(step, n - (c - 1) * step);
-    lo += (c - 1) * step;
-    if (step == 1) break;
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  tile = t - (cu_at(cu, lo, total) / B + lo);
-  return tile < 0 ? -1 : lo;
-}
-__device__ __forceinline__ void seq_rows(const int32_t* cu, int nseq, int total, int s, int& r0, int& n) {
-  if (cu) {
-    r0 = cu_at(cu, s, total);
-    n = max(0, cu_at(cu, s + 1, total) - r0);
+  const int32_t* cu = KEYS ? cu_k : cu_q;
+  const int total = KEYS ? total_k : total_q;
+  int q1, k1;
+  if (nseq < 64) {
+    const int i = min(lane, nseq), eq = cu_at(cu_q, i, total_q), ek = cu_at(cu_k, i, total_k), e = KEYS ? ek : eq;
+    p.end = __builtin_amdgcn_readlane(e, nseq);
+    const int c = __popcll(__ballot(lane < nseq && e / B + lane <= t));
+    if (c == 0) return p;
+    p.seq = c - 1;
+    p.tile = t - (__builtin_amdgcn_readlane(e, p.seq) / B + p.seq);
+    p.q0 = __builtin_amdgcn_readlane(eq, p.seq), q1 = __builtin_amdgcn_readlane(eq, c);
+    p.k0 = __builtin_amdgcn_readlane(ek, p.seq), k1 = __builtin_amdgcn_readlane(ek, c);
   } else {
-    n = total / nseq;
-    r0 = s * n;
+    p.end = cu_at(cu, nseq, total);
+    int lo = 0, n = nseq;
+    while (true) {
+      const int step = (n + 63) / 64, i = lo + lane * step;
+      const int c = __popcll(__ballot(lane * step < n && cu_at(cu, i, total) / B + i <= t));
+      if (c == 0) return p;
+      n = min(step, n - (c - 1) * step);
+      lo += (c - 1) * step;
+      if (step == 1) break;
+    }
+    p.seq = lo = __builtin_amdgcn_readfirstlane(lo);
+    p.tile = t - (cu_at(cu, lo, total) / B + lo);
+    p.q0 = cu_at(cu_q, lo, total_q), q1 = cu_at(cu_q, lo + 1, total_q);
+    p.k0 = cu_at(cu_k, lo, total_k), k1 = cu_at(cu_k, lo + 1, total_k);
+    p.tile = __builtin_amdgcn_readfirstlane(p.tile);
+    p.q0 = __builtin_amdgcn_readfirstlane(p.q0), p.k0 = __builtin_amdgcn_readfirstlane(p.k0);
+    q1 = __builtin_amdgcn_readfirstlane(q1), k1 = __builtin_amdgcn_readfirstlane(k1);
   }
-  r0 = __builtin_amdgcn_readfirstlane(r0);
-  n = __builtin_amdgcn_readfirstlane(n);
+  p.nq = max(0, q1 - p.q0), p.nk = max(0, k1 - p.k0);
+  if (p.tile < 0) p.seq = -1;  // ends out of order
+  return p;
 }
 
 }  // namespace lsattn

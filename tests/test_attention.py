@@ -173,9 +173,9 @@ def _shape(**kw):
     return L.AttnShape(*(d[n] for n in ("nseq", "total_q", "total_k", "hq", "hk", "d", "dtype")))
 
 
-def _fwd(shape, rows=None, cu=(None, None), scale=1.0, o=FAKE):
+def _fwd(shape, rows=None, cu=(None, None), scale=1.0, o=FAKE, ws=FAKE, nbytes=1 << 40):
     r = [ctypes.byref(x) for x in (rows or [L.AttnRows(256, 512, 64)] * 3)]
-    return L.lib().lsurge_attn_fwd(ctypes.byref(shape), *r, *cu, scale, o, None, None)
+    return L.lib().lsurge_attn_fwd(ctypes.byref(shape), *r, *cu, scale, o, None, ws, nbytes, None)
 
 
 def test_c_abi_forward_refusals():
@@ -195,6 +195,11 @@ def test_c_abi_forward_refusals():
             rows[i] = bad
             assert _fwd(_shape(), rows) == -1 and msg in lib.lsurge_last_error()
     assert _fwd(_shape(nseq=0, total_q=0, total_k=0)) == 0  # nothing to do
+    few = _shape(total_q=16, total_k=16384)  # few rows over many keys: split, and the parts need room
+    need = lib.lsurge_attn_fwd_workspace_bytes(ctypes.byref(few))
+    assert need > 2 * 16 * 4 * 66 * 4 and lib.lsurge_attn_fwd_workspace_bytes(ctypes.byref(_shape())) == 0
+    assert _fwd(few, nbytes=need - 1) == -4 and b"workspace" in lib.lsurge_last_error()
+    assert _fwd(few, ws=None, nbytes=need) == -1 and _fwd(few, ws=ctypes.c_void_p(264), nbytes=need) == -1
 
 
 def test_c_abi_backward_refusals():
