@@ -141,7 +141,8 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
   const int kend = min(nq, (tile + 1) * BM) + off;  // keys the workgroup's last row sees
   const int all = (max(kend, 0) + FN - 1) / FN;
   const int begin = (int)((int64_t)all * part / parts), nst = (int)((int64_t)all * (part + 1) / parts) - begin;
-  const int nsw = (max(w0 + 32 + off, 0) + FN - 1) / FN - begin;  // stages that the wave's rows see
+  // stages that the wave's rows see
+  const int nsw = w0 < nq ? (max(w0 + 32 + off, 0) + FN - 1) / FN - begin : 0;
   const int kfirst = begin * FN, left = nk - kfirst;  // the part's first key, and the keys from there on
   const uint16_t* kb = a.k + (int64_t)(k0 + kfirst) * a.k_row + kvh * a.k_head;
   const uint16_t* vb = a.v + (int64_t)(k0 + kfirst) * a.v_row + kvh * a.v_head;
@@ -306,17 +307,17 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
 }
 
 // ------------------------------------------------------------------------------------ backward
-// What the two passes need of each query, laid out [hq][total_q]: lse2 = lse log2(e) (+inf for a row with no key, whose
-// weights 2^(s - lse2) are then 0), delta = do . o - dlse.  f16 values have few exponent bits: weights of long rows (2^-15
-// and less) and their products with small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times
-// too large (lse2 smaller by SHIFT) and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's
-// own, from the largest |do| of the row, in the pass over queries; the head's, from the largest of all rows, in the pass
-// over keys, which sums over the rows (amax [hq][blocks], a block's largest).
-constexpr int PB = 64;  // rows per block of the preparation
+// What the passes need of each query, laid out [hq][total_q]: lse2 = lse log2(e) (+inf for a row with no key, whose weights
+// 2^(s - lse2) are then 0) and delta = do . o - dlse, found by the pass over queries, whose lanes hold do already, and kept
+// for the pass over keys.  f16 values have few exponent bits: weights of long rows (2^-15 and less) and their products with
+// small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times too large (lse2 smaller by SHIFT)
+// and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's own, from the largest |do| of the
+// row, in the pass over queries; the group's, from the largest of all rows, in the pass over keys, which sums over the rows
+// (amax [hq][nblk]: a tile's largest).
 template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
 struct RowPrep {
   f32x2_t* rows;  // lse2, delta
-  float *rscale, *amax;
+  float* amax;
   int nblk;
 };
 // 2^e with 2^e amax in [1, 2); 1 for 0, infinities and NaN
@@ -326,59 +327,18 @@ __device__ __forceinline__ float grad_scale(float amax) {
   (void)frexpf(amax, &e);
   return ldexpf(1.f, min(max(1 - e, -60), 60));
 }
-template <int D, int DT>
-__global__ __launch_bounds__(256) void attn_prep_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
-                                                        const float* __restrict__ lse, const float* __restrict__ dlse,
-                                                        int total_q, int hq, RowPrep w) {
-  constexpr int LPR = D / 8, RPP = 256 / LPR;  // lanes per row, rows per pass
-  __shared__ float red[4];
-  const int head = blockIdx.y, sub = threadIdx.x % LPR;
-  float big = 0.f;
-  for (int r = threadIdx.x / LPR; r < PB; r += RPP) {
-    const int row = (int)blockIdx.x * PB + r;
-    float dot = 0.f, mx = 0.f;
-    if (row < total_q) {
-      const int64_t at = ((int64_t)row * hq + head) * D + sub * 8;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(o + at), y = *reinterpret_cast<const u32x4*>(dout + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x0, x1, y0, y1;
-        unpack2<DT>(x[i], x0, x1);
-        unpack2<DT>(y[i], y0, y1);
-        dot = fmaf(x0, y0, fmaf(x1, y1, dot));
-        mx = fmaxf(mx, fmaxf(fabsf(y0), fabsf(y1)));
-      }
-    }
-#pragma unroll
-    for (int s = LPR / 2; s > 0; s >>= 1) {
-      dot += __shfl_xor(dot, s, 64);
-      mx = fmaxf(mx, __shfl_xor(mx, s, 64));
-    }
-    big = fmaxf(big, mx);
-    if (sub == 0 && row < total_q) {
-      const int64_t i = (int64_t)head * total_q + row;
-      const float v = lse[i];
-      w.rows[i] = f32x2_t{v == -INFINITY ? INFINITY : v * LOG2E - SHIFT<DT>, dot - (dlse ? dlse[i] : 0.f)};
-      if (DT == LSURGE_F16) w.rscale[i] = grad_scale(mx);
-    }
-  }
-  if constexpr (DT == LSURGE_F16) {
-    big = wave_max(big);
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = big;
-    __syncthreads();
-    if (threadIdx.x == 0)
-      w.amax[(int64_t)head * w.nblk + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  }
-}
 
 // dq_i = scale sum_j ds_ij k_j with ds_ij = p_ij (do_i . v_j - delta_i): the forward's walk, a query per lane, dS^T in
 // place as the operand of dQ^T = K^T dS^T.  The scores are formed again rather than handed over by the pass over keys:
 // two products more, but no sum over workgroups, whose order would change the results.
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, float scale, uint16_t* __restrict__ dq) {
+void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
+                    const float* __restrict__ lse, const float* __restrict__ dlse, RowPrep w, float scale,
+                    uint16_t* __restrict__ dq) {
   constexpr int BM = NW * 32, TILE = BN * D * 2;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+  __shared__ float red[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   int head, slot;
@@ -389,29 +349,12 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
     zero_rows<D>(dq, first, (int)min((int64_t)BM, a.total_q - first), a.hq, head, threadIdx.x, NW * 64);
   }
   const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
-  if (pl.seq < 0 || tile * BM >= nq) return;
+  if (pl.seq < 0 || tile * BM >= nq) {
+    if (DT == LSURGE_F16 && threadIdx.x == 0) w.amax[(int64_t)head * w.nblk + slot] = 0.f;
+    return;
+  }
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
   const int kvh = head / (a.hq / a.hk);
-
-  u32x4 qf[D / 16], df[D / 16];
-  const int crow = q0 + min(row, nq - 1);
-  {
-    const uint16_t* qp = a.q + (int64_t)crow * a.q_row + head * a.q_head + 8 * hf;
-    const uint16_t* dp = dout + ((int64_t)crow * a.hq + head) * D + 8 * hf;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
-      df[s] = *reinterpret_cast<const u32x4*>(dp + 16 * s);
-    }
-  }
-  const int64_t pi = (int64_t)head * a.total_q + crow;
-  const float lse2 = w.rows[pi][0], delta = w.rows[pi][1];
-  const float gs = DT == LSURGE_F16 ? w.rscale[pi] : 1.f;
-  f32x16 acc[D / 32];
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
 
   const uint32_t lds = lds_addr((const bf16_t*)smem);
   TileCopy<D, BN, NW> ck, cv;
@@ -426,16 +369,66 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, fl
     ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - st * BN, at, wave);
     cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
   };
+  if (nst) issue(0);
+  // delta and the row's scale from the fragments of do (the two halves of the wave hold the two halves of a row)
+  u32x4 qf[D / 16], df[D / 16];
+  const int crow = q0 + min(row, nq - 1);
+  const int64_t pi = (int64_t)head * a.total_q + crow;
+  const float row_lse = lse[pi];
+  float delta = 0.f, big = 0.f;
+  {
+    const uint16_t* qp = a.q + (int64_t)crow * a.q_row + head * a.q_head + 8 * hf;
+    const int64_t at = ((int64_t)crow * a.hq + head) * D + 8 * hf;
+    u32x4 of[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      df[s] = *reinterpret_cast<const u32x4*>(dout + at + 16 * s);
+      of[s] = *reinterpret_cast<const u32x4*>(o + at + 16 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x0, x1, y0, y1;
+        unpack2<DT>(of[s][i], x0, x1);
+        unpack2<DT>(df[s][i], y0, y1);
+        delta = fmaf(x0, y0, fmaf(x1, y1, delta));
+        if (DT == LSURGE_F16) big = fmaxf(big, fmaxf(fabsf(y0), fabsf(y1)));
+      }
+  }
+  delta = halves(delta, [](float x, float y) { return x + y; }) - (dlse ? dlse[pi] : 0.f);
+  const float lse2 = row_lse == -INFINITY ? INFINITY : row_lse * LOG2E - SHIFT<DT>;
+  if (hf == 0 && row < nq) w.rows[pi] = f32x2_t{lse2, delta};
+  float gs = 1.f;
+  if constexpr (DT == LSURGE_F16) {
+    big = halves(big, [](float x, float y) { return fmaxf(x, y); });
+    gs = grad_scale(big);
+    big = wave_max(big);  // rows past the end repeat the last one
+    if (lane == 0) red[wave] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int i = 1; i < NW; ++i) big = fmaxf(big, red[i]);
+      w.amax[(int64_t)head * w.nblk + slot] = big;
+    }
+  }
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+
   const uint32_t ra = row_addr<D>(lane);
   uint32_t ca[COLS<D>];
 #pragma unroll
   for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
 
-  if (nst) issue(0);
   for (int st = 0; st < nst; ++st) {
     stage_barrier<0>();
     if (st + 1 < nst) issue(st + 1);
-    if (st * BN > w0 + 31 + off) continue;
+    if (st * BN > w0 + 31 + off || w0 >= nq) continue;
     const uint32_t kt = lds + (st & 1) * 2 * TILE, vt = kt + TILE;
     const int lim = row + off - st * BN;
     const bool edge = st * BN + BN - 1 > w0 + off;
@@ -621,7 +614,7 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     issue((u + R - 1) % R);
     const int r0 = cr;
     cr = cr + QN >= nq ? first * QN : cr + QN;
-    if (r0 + QN - 1 + off < w0) return;  // no row of this stage sees the wave's keys
+    if (r0 + QN - 1 + off < w0 || w0 >= nk) return;  // no row of this stage sees the wave's keys
     f32x16 s, g;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
@@ -842,9 +835,12 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   return LSURGE_OK;
 }
 
+// tile slots of the queries, packed or not
+static int64_t most_query_tiles(const lsurge_attn_shape* s) { return s->total_q / 128 + std::max<int64_t>(s->nseq, 1); }
 static size_t prep_bytes(const lsurge_attn_shape* s) {
-  const int64_t rows = s->hq * s->total_q, blk = (s->total_q + PB - 1) / PB;
-  return (sizeof(float) * (size_t)(s->dtype == LSURGE_F16 ? 3 * rows + s->hq * blk : 2 * rows) + 255) / 256 * 256;
+  const int64_t rows = s->hq * s->total_q;
+  const int64_t floats = 2 * rows + (s->dtype == LSURGE_F16 ? s->hq * most_query_tiles(s) : 0);
+  return (sizeof(float) * (size_t)floats + 255) / 256 * 256;
 }
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
   if (!s || s->hq < 1 || s->hk < 1 || s->d < 1 || s->nseq < 0 || s->total_q < 0 || s->total_k < 0) return 0;
@@ -877,8 +873,7 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
   const int64_t nrow = s->hq * s->total_q;
   RowPrep w;
-  w.rows = (f32x2_t*)workspace, w.rscale = (float*)(w.rows + nrow), w.amax = w.rscale + nrow;
-  w.nblk = (int)((s->total_q + PB - 1) / PB);
+  w.rows = (f32x2_t*)workspace, w.amax = (float*)(w.rows + nrow);
   float* psum = (float*)((char*)workspace + prep_bytes(s));
   const int parts = (int)dkv_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
@@ -889,9 +884,12 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const int64_t tk = s->total_k ? num_tiles(*s, cu_k, s->total_k, NW * 32) : 0;                                          \
   if (int rc = tile_grid("attn_bwd", tq, s->hq, &gq)) return rc;                                                         \
   if (int rc = tile_grid("attn_bwd", tk, s->hk * parts, &gk)) return rc;                                                         \
-  if (gq)                                                                                                                \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_prep_kernel<D, DT>), dim3(w.nblk, (unsigned)s->hq), dim3(256),  \
-                                                   0, st, (const uint16_t*)o, g, lse, dlse, a.total_q, a.hq, w));        \
+  w.nblk = (int)tq;                                                                                                      \
+  if (gq) {                                                                                                              \
+    a.ntiles = (int)tq;                                                                                                  \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,       \
+                                                   (const uint16_t*)o, g, lse, dlse, w, scale, (uint16_t*)dq));          \
+  }                                                                                                                      \
   if (gk) {                                                                                                              \
     a.ntiles = (int)tk;                                                                                                  \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, a, g, w, \
@@ -902,11 +900,6 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
                                                      dim3((unsigned)std::min<int64_t>((2 * size + 1023) / 1024, 4096)),  \
                                                      dim3(256), 0, st, psum, parts, size, s->hk * D, cu_k, a.nseq,       \
                                                      a.total_k, (uint16_t*)dk, (uint16_t*)dv));                          \
-  }                                                                                                                      \
-  if (gq) {                                                                                                              \
-    a.ntiles = (int)tq;                                                                                                  \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a, g, w,  \
-                                                   scale, (uint16_t*)dq));                                               \
   }
   ATTN_DISPATCH(ATTN_BWD);
 #undef ATTN_BWD
