@@ -426,6 +426,10 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
   for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
 
   for (int st = 0; st < nst; ++st) {
+    if constexpr (D == 256) {  // as in the forward
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(acc[d]));
+    }
     stage_barrier<0>();
     if (st + 1 < nst) issue(st + 1);
     if (st * BN > w0 + 31 + off || w0 >= nq) continue;
