@@ -22,31 +22,34 @@ struct AttnArgs {
   const uint16_t *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
   const int32_t *cu_q, *cu_k;
-  int nseq, total_q, total_k, hq, hk, ntiles;
+  int nseq, total_q, total_k, hq, hk;
   float scale2;  // scale log2(e)
+  // the launch (see head_tile): heads of a sequence, their pairs with the sequences, pairs of an XCD (0: not cut into
+  // runs), heads that go together, tiles of a sequence
+  int heads, pairs, run, together, tiles;
 };
 
-// Workgroup -> (head, tile slot).  Workgroups are dealt to the 8 XCDs round-robin and each XCD has an L2 of its own, so the
-// (sequence, head) pairs are cut into 8 runs where their number allows, and within a run `share` heads that read the same
-// rows go tile by tile together: the workgroups that run on an XCD at a time then walk the same keys.  8 x 4096 tokens, 8
-// heads over 2: 1530 us a training step with heads dealt to XCDs, 1441 so; 8 x 2048 prompts, 16 heads: 172 and 161.  Where an XCD has
-// few workgroups (two rounds) all its heads go together, so that the longest start first (one sequence of 4096: 356 and
-// 328 us).  Packed sequences have their borders on the device, so their tile slots are one sequence here.  Tiles go from the last to the first (the long ones of a causal sequence first) or, with `up`, the other way.
-__device__ __forceinline__ void head_tile(int heads, int share, int nseq, int ntiles, bool up, int& head, int& slot) {
-  const int id = (int)blockIdx.x, tiles = ntiles / nseq, pairs = nseq * heads;  // tiles of one sequence
-  int pair, tile;
-  if (pairs % 8 == 0) {
-    const int run = pairs / 8, i = id / 8;
-    const int g = run * tiles <= 128 ? run : run % share == 0 ? share : share % run == 0 ? run : 1;
-    const int set = i / (g * tiles), r = i % (g * tiles);
-    pair = id % 8 * run + set * g + r % g;
-    tile = r / g;
+// Workgroup -> (sequence, head, tile).  Workgroups are dealt to the 8 XCDs round-robin and each XCD has an L2 of its own, so
+// the (sequence, head) pairs are cut into 8 runs where their number allows, and within a run `together` heads that read the
+// same rows go tile by tile: the workgroups that run on an XCD at a time then walk the same keys.  8 x 4096 tokens, 8 heads
+// over 2: 1530 us a training step with heads dealt to XCDs, 1441 so; 8 x 2048 prompts, 16 heads: 172 and 161.  Where an XCD
+// has few workgroups (two rounds) all its heads go together, so that the longest start first (one sequence of 4096: 356 and
+// 328 us).  Packed sequences have their borders on the device: their tile slots are one sequence here.  Tiles go from the
+// last to the first (the long ones of a causal sequence first) or, with `up`, the other way.
+__device__ __forceinline__ void head_tile(const AttnArgs& a, bool up, int& seq, int& head, int& tile) {
+  const int id = (int)blockIdx.x;
+  int pair;
+  if (a.run) {
+    const int i = id / 8, set = i / (a.together * a.tiles), r = i - set * a.together * a.tiles;
+    tile = r / a.together;
+    pair = id % 8 * a.run + set * a.together + r - tile * a.together;
   } else {
-    pair = id % pairs;
-    tile = id / pairs;
+    tile = id / a.pairs;
+    pair = id - tile * a.pairs;
   }
-  head = pair % heads;
-  slot = pair / heads * tiles + (up ? tile : tiles - 1 - tile);
+  seq = pair / a.heads;
+  head = pair - seq * a.heads;
+  if (!up) tile = a.tiles - 1 - tile;
 }
 
 // rows [first, first + n) of [rows, heads, D] at one head, zeroed (rows behind the last sequence)
@@ -83,6 +86,8 @@ __device__ __forceinline__ void interleave() {
 
 // ------------------------------------------------------------------------------------ forward
 constexpr int FN = 32;  // keys per stage of the forward
+// its stages in LDS; at D = 256 a fourth made prompts of 16384 slower (2385 -> 2779 us: the unrolled loop's code grows)
+template <int D> constexpr int STAGES = D == 256 ? 3 : 4;
 constexpr int BN = 64;  // keys per stage of the pass over queries
 
 // acc *= f.  At D = 256 the accumulators fill half of the registers and have to stay in the accumulation file, which the
@@ -107,23 +112,44 @@ __device__ __forceinline__ void rescale(f32x16& acc, float f) {
   }
 }
 
-// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a three-deep LDS
-// ring.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
+// f acc (a product's transposed result: lane l holds column l % 32) as 16-bit rows p[row][d], n of them, through the wave's
+// piece of LDS: stores straight from the lanes would be 8 bytes in each of 32 rows.
+template <int D, int DT>
+__device__ __forceinline__ void store_rows(char* lds, const f32x16* acc, float f, uint16_t* p, int64_t row_stride, int n,
+                                           int lane) {
+  constexpr int PITCH = D * 2 + 16, CPR = D / 8;  // bytes of a row in LDS; 16-byte chunks of a row
+  char* w = lds + (lane & 31) * PITCH + 8 * (lane >> 5);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<u32x2*>(w + 64 * d + 4 * r) = u32x2{pack2<DT>(acc[d][r] * f, acc[d][r + 1] * f),
+                                                            pack2<DT>(acc[d][r + 2] * f, acc[d][r + 3] * f)};
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave reads its own piece only
+#pragma unroll
+  for (int i = 0; i < CPR / 2; ++i) {
+    const int id = i * 64 + lane, row = id / CPR, c = id % CPR;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(lds + row * PITCH + c * 16);
+    if (row < n) *reinterpret_cast<u32x4*>(p + row * row_stride + c * 8) = x;
+  }
+}
+
+// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a ring in LDS.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
 // work at the same time; one barrier a stage.
 template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(FWD_EU<D>)))
 void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
                      float* __restrict__ lse) {
-  constexpr int BM = NW * 32, TILE = FN * D * 2;  // bytes of one operand of one stage
-  __shared__ __attribute__((aligned(1024))) char smem[6 * TILE];  // three stages of K, then three of V
+  constexpr int BM = NW * 32, FR = STAGES<D>, TILE = FN * D * 2;  // bytes of one operand of one stage
+  __shared__ __attribute__((aligned(1024))) char smem[2 * FR * TILE];  // FR stages of K, then FR of V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
   const int group = a.hq / a.hk;
-  int unit, slot;  // unit: key head, part, head of the group, so that the heads that share keys stay together
-  head_tile(a.hq * parts, group, a.cu_q ? 1 : a.nseq, a.ntiles, false, unit, slot);
-  const int kvh = unit / (parts * group), part = unit / group % parts, head = kvh * group + unit % group;
-  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  int sq, unit, slot;  // unit: key head, part, head of the group, so that the heads that share keys stay together
+  head_tile(a, false, sq, unit, slot);
+  const int kvh = unit / (parts * group), part = parts == 1 ? 0 : unit / group % parts, head = kvh * group + unit % group;
+  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
   if (pl.end + (int64_t)slot * BM < a.total_q && part == 0) {  // the slots cover the rows behind the last sequence too
     const int64_t first = pl.end + (int64_t)slot * BM;
     const int n = (int)min((int64_t)BM, a.total_q - first);
@@ -150,15 +176,16 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     ck.issue(kb + (int64_t)st * FN * a.k_row, a.k_row, left - st * FN, lds + slot * TILE, wave);
   };
   auto issue_v = [&](int st, int slot) {
-    cv.issue(vb + (int64_t)st * FN * a.v_row, a.v_row, left - st * FN, lds + (3 + slot) * TILE, wave);
+    cv.issue(vb + (int64_t)st * FN * a.v_row, a.v_row, left - st * FN, lds + (FR + slot) * TILE, wave);
   };
   constexpr int CP = 2 * TileCopy<D, FN, NW>::N;  // copies of a stage
   if (nst) {
     issue_k(0, 0);
-    issue_v(0, 0);
-    issue_k(1, 1);
-    issue_v(1, 1);
-    issue_k(2, 2);
+#pragma unroll
+    for (int s = 1; s < FR; ++s) {
+      issue_v(s - 1, s - 1);
+      issue_k(s, s);
+    }
   }
   u32x4 qf[D / 16];
   {
@@ -176,7 +203,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
   const uint32_t ka = lds + row_addr<D>(lane);
   uint32_t va[COLS<D>];
 #pragma unroll
-  for (int t = 0; t < COLS<D>; ++t) va[t] = lds + 3 * TILE + col_addr<D>(lane, t);
+  for (int t = 0; t < COLS<D>; ++t) va[t] = lds + FR * TILE + col_addr<D>(lane, t);
 
   auto scores = [&](int slot, f32x16& s) {
 #pragma unroll
@@ -191,9 +218,9 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(acc[d]));
     }
-    stage_barrier<CP>();  // K of st + 1 and V of st have landed, and nobody reads K of st and V of st - 1 any more
-    issue_v(st + 2, (u + 2) % 3);
-    issue_k(st + 3, u);
+    stage_barrier<(FR - 2) * CP>();  // K of st + 1 and V of st have landed; nobody reads K of st and V of st - 1 any more
+    issue_v(st + FR - 1, (u + FR - 1) % FR);
+    issue_k(st + FR, u);
     if (st >= nsw) return;  // nothing of this stage is visible to the wave's rows
     if (st * FN + FN - 1 > w0 + off - kfirst) {  // the diagonal or the end of the keys
       const int lim = row + off - kfirst - st * FN;
@@ -202,7 +229,8 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
         if (8 * (r / 4) + 4 * hf + r % 4 > lim) s[r] = -INFINITY;
     }
     __builtin_amdgcn_sched_barrier(0);
-    scores((u + 1) % 3, next);
+    __builtin_amdgcn_s_setprio(1);  // of the two waves of a SIMD the one with a softmax to do goes first (up to 4%)
+    scores((u + 1) % FR, next);
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -236,6 +264,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     }
     m = mx;
     l += sum[0] + sum[1];
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -246,19 +275,25 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     __builtin_amdgcn_sched_barrier(0);
   };
   if (nst) {
-    stage_barrier<CP + CP>();  // K of stage 0
+    stage_barrier<(FR - 1) * CP>();  // K of stage 0
     f32x16 s0, s1, s2;
     scores(0, s0);
-    for (int st = 0; st < nst; st += 3) {
+    for (int st = 0; st < nst; st += FR) {
       step(st, std::integral_constant<int, 0>(), s0, s1);
-      if (st + 1 < nst) step(st + 1, std::integral_constant<int, 1>(), s1, s2);
-      if (st + 2 < nst) step(st + 2, std::integral_constant<int, 2>(), s2, s0);
+      if constexpr (FR == 4) {
+        if (st + 1 < nst) step(st + 1, std::integral_constant<int, 1>(), s1, s0);
+        if (st + 2 < nst) step(st + 2, std::integral_constant<int, 2>(), s0, s1);
+        if (st + 3 < nst) step(st + 3, std::integral_constant<int, FR - 1>(), s1, s0);
+      } else {
+        if (st + 1 < nst) step(st + 1, std::integral_constant<int, 1>(), s1, s2);
+        if (st + 2 < nst) step(st + 2, std::integral_constant<int, 2>(), s2, s0);
+      }
     }
-    __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before the wave ends
+    __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before LDS is used again, or the wave ends
   }
   l = halves(l, [](float x, float y) { return x + y; });
-  if (row >= nq) return;
-  if (parts > 1) {  // the sums as they are, and what they are relative to
+  if (parts > 1) {
+    if (row >= nq) return;  // the sums as they are, and what they are relative to
     const int64_t at = (int64_t)part * a.total_q + q0 + row;
     float* pp = po + (at * a.hq + head) * D + 4 * hf;
 #pragma unroll
@@ -270,14 +305,10 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* op = o + ((int64_t)(q0 + row) * a.hq + head) * D + 4 * hf;
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *reinterpret_cast<u32x2*>(op + 32 * d + 2 * r) = u32x2{pack2<DT>(acc[d][r] * inv, acc[d][r + 1] * inv),
-                                                             pack2<DT>(acc[d][r + 2] * inv, acc[d][r + 3] * inv)};
-  if (lse && hf == 0)
+  __syncthreads();
+  store_rows<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, inv, o + ((int64_t)(q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D,
+                    min(32, nq - w0), lane);
+  if (lse && hf == 0 && row < nq)
     lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * LN2;
 }
 
@@ -341,16 +372,16 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
   __shared__ float red[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  int head, slot;
-  head_tile(a.hq, a.hq / a.hk, a.cu_q ? 1 : a.nseq, a.ntiles, false, head, slot);
-  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  int sq, head, slot;
+  head_tile(a, false, sq, head, slot);
+  const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
   if (pl.end + (int64_t)slot * BM < a.total_q) {
     const int64_t first = pl.end + (int64_t)slot * BM;
     zero_rows<D>(dq, first, (int)min((int64_t)BM, a.total_q - first), a.hq, head, threadIdx.x, NW * 64);
   }
   const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
   if (pl.seq < 0 || tile * BM >= nq) {
-    if (DT == LSURGE_F16 && threadIdx.x == 0) w.amax[(int64_t)head * w.nblk + slot] = 0.f;
+    if (DT == LSURGE_F16 && threadIdx.x == 0) w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = 0.f;
     return;
   }
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
@@ -411,7 +442,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
     if (threadIdx.x == 0) {
 #pragma unroll
       for (int i = 1; i < NW; ++i) big = fmaxf(big, red[i]);
-      w.amax[(int64_t)head * w.nblk + slot] = big;
+      w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = big;
     }
   }
   f32x16 acc[D / 32];
@@ -466,15 +497,10 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
       }
     }
   }
-  if (row >= nq) return;
   const float f = scale / gs * exp2_hw(-SHIFT<DT>);
-  uint16_t* op = dq + ((int64_t)(q0 + row) * a.hq + head) * D + 4 * hf;
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *reinterpret_cast<u32x2*>(op + 32 * d + 2 * r) = u32x2{pack2<DT>(acc[d][r] * f, acc[d][r + 1] * f),
-                                                             pack2<DT>(acc[d][r + 2] * f, acc[d][r + 3] * f)};
+  __syncthreads();
+  store_rows<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, f, dq + ((int64_t)(q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D,
+                    min(32, nq - w0), lane);
 }
 
 // dv_j = sum_i p_ij do_i, dk_j = scale sum_i ds_ij q_i over the queries of every head of the group.  A workgroup takes
@@ -497,10 +523,10 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   __shared__ float red[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  int unit, slot;
-  head_tile(a.hk * parts, 1, a.cu_k ? 1 : a.nseq, a.ntiles, true, unit, slot);  // the first keys are seen by the most
+  int sq, unit, slot;
+  head_tile(a, true, sq, unit, slot);  // the first keys are seen by the most queries
   const int kvh = unit / parts, part = unit % parts;
-  const Place pl = find_tile<BK, true>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, slot, lane);
+  const Place pl = find_tile<BK, true>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
   if (pl.end + (int64_t)slot * BK < a.total_k && part == 0) {
     const int64_t first = pl.end + (int64_t)slot * BK;
     const int n = (int)min((int64_t)BK, a.total_k - first);
@@ -647,10 +673,10 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
       if (st + 2 < nst) step(std::integral_constant<int, R - 1>());
   }
   __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before the wave ends
-  if (col >= nk) return;
   const float fv = exp2_hw(-SHIFT<DT>), fk = scale / gs * fv;
   const int64_t at = ((int64_t)(k0 + col) * a.hk + kvh) * D + 4 * hf;
   if (parts > 1) {
+    if (col >= nk) return;
     const int64_t size = (int64_t)a.total_k * a.hk * D;
     float* pk = psum + 2 * part * size + at;
 #pragma unroll
@@ -662,15 +688,12 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
       }
     return;
   }
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      *reinterpret_cast<u32x2*>(dk + at + 32 * d + 2 * r) = u32x2{
-          pack2<DT>(ak[d][r] * fk, ak[d][r + 1] * fk), pack2<DT>(ak[d][r + 2] * fk, ak[d][r + 3] * fk)};
-      *reinterpret_cast<u32x2*>(dv + at + 32 * d + 2 * r) = u32x2{
-          pack2<DT>(av[d][r] * fv, av[d][r + 1] * fv), pack2<DT>(av[d][r + 2] * fv, av[d][r + 3] * fv)};
-    }
+  __syncthreads();
+  char* piece = smem + wave * 32 * (D * 2 + 16);
+  const int64_t first_at = ((int64_t)(k0 + w0) * a.hk + kvh) * D;
+  const int n = min(32, nk - w0);
+  store_rows<D, DT>(piece, ak, fk, dk + first_at, (int64_t)a.hk * D, n, lane);
+  store_rows<D, DT>(piece, av, fv, dv + first_at, (int64_t)a.hk * D, n, lane);
 }
 
 // dk and dv = the parts' sums, added in order: n values each, 4 a thread; rows from cu[nseq] on were zeroed already
@@ -720,9 +743,20 @@ int check_shape(const char* what, const lsurge_attn_shape* s, const int32_t* cu_
   return LSURGE_OK;
 }
 
-int64_t num_tiles(const lsurge_attn_shape& s, bool packed, int64_t total, int64_t rows) {
-  if (packed) return total / rows + std::max<int64_t>(s.nseq, 1);  // at least 1: rows behind the last sequence
-  return s.nseq * ((total / s.nseq + rows - 1) / rows);
+// tile slots of the rows: of one dense sequence, or of all packed ones (at least 1: rows behind the last sequence)
+int64_t tile_slots(const lsurge_attn_shape& s, bool packed, int64_t total, int64_t rows) {
+  return packed ? total / rows + std::max<int64_t>(s.nseq, 1) : (total / s.nseq + rows - 1) / rows;
+}
+// the launch of `tiles` tile slots for each of `heads` heads, `share` of which read the same rows; 0 workgroups: none
+int plan_grid(const char* what, const lsurge_attn_shape& s, bool packed, int64_t heads, int64_t share, int64_t tiles,
+              AttnArgs* a, unsigned* grid) {
+  const int64_t pairs = (packed ? 1 : s.nseq) * heads;
+  LSURGE_REQUIRE(pairs * tiles < (1ll << 31), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)pairs);
+  const int64_t run = pairs % 8 == 0 ? pairs / 8 : 0;
+  a->heads = (int)heads, a->pairs = (int)pairs, a->tiles = (int)tiles, a->run = (int)run;
+  a->together = (int)(run * tiles <= 128 ? std::max<int64_t>(run, 1) : run % share == 0 ? share : share % run == 0 ? run : 1);
+  *grid = (unsigned)(pairs * tiles);
+  return LSURGE_OK;
 }
 
 AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const lsurge_attn_rows& k,
@@ -733,7 +767,7 @@ AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const 
   a.q_head = q.head_stride, a.k_head = k.head_stride, a.v_head = v.head_stride;
   a.cu_q = cu_q, a.cu_k = cu_k;
   a.nseq = (int)s.nseq, a.total_q = (int)s.total_q, a.total_k = (int)s.total_k, a.hq = (int)s.hq, a.hk = (int)s.hk;
-  a.ntiles = 0;
+  a.heads = a.pairs = a.run = a.together = a.tiles = 0;
   a.scale2 = scale * LOG2E;
   return a;
 }
@@ -783,12 +817,6 @@ int64_t fwd_parts(const lsurge_attn_shape& s) {
     }                                                                           \
   } while (0)
 
-int tile_grid(const char* what, int64_t tiles, int64_t heads, unsigned* grid) {
-  LSURGE_REQUIRE(tiles * heads < (1ll << 31), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)heads);
-  *grid = (unsigned)(tiles * heads);
-  return LSURGE_OK;
-}
-
 }  // namespace
 }  // namespace lsattn
 
@@ -824,9 +852,10 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   f32x2_t* pm = (f32x2_t*)(po + (size_t)parts * s->total_q * s->hq * s->d);
 #define ATTN_FWD(D, DT)                                                                                               \
   constexpr int NW = WAVES<D>;                                                                                        \
-  a.ntiles = (int)num_tiles(*s, cu_q, s->total_q, NW * 32);                                                           \
   unsigned grid;                                                                                                      \
-  if (int rc = tile_grid("attn_fwd", a.ntiles, s->hq * parts, &grid)) return rc;                                      \
+  if (int rc = plan_grid("attn_fwd", *s, cu_q, s->hq * parts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), \
+                         &a, &grid))                                                                                  \
+    return rc;                                                                                                        \
   LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a,   \
                                                  parts, po, pm, (uint16_t*)o, lse));                                  \
   const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                              \
@@ -883,21 +912,22 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const uint16_t* g = (const uint16_t*)dout;
 #define ATTN_BWD(D, DT)                                                                                                  \
   constexpr int NW = WAVES<D>;                                                                                           \
+  AttnArgs ak = a;                                                                                                       \
   unsigned gq = 0, gk = 0;                                                                                               \
-  const int64_t tq = s->total_q ? num_tiles(*s, cu_q, s->total_q, NW * 32) : 0;                                          \
-  const int64_t tk = s->total_k ? num_tiles(*s, cu_k, s->total_k, NW * 32) : 0;                                          \
-  if (int rc = tile_grid("attn_bwd", tq, s->hq, &gq)) return rc;                                                         \
-  if (int rc = tile_grid("attn_bwd", tk, s->hk * parts, &gk)) return rc;                                                         \
-  w.nblk = (int)tq;                                                                                                      \
-  if (gq) {                                                                                                              \
-    a.ntiles = (int)tq;                                                                                                  \
+  if (s->total_q)                                                                                                        \
+    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hq, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), &a,    \
+                           &gq))                                                                                         \
+      return rc;                                                                                                         \
+  if (s->total_k)                                                                                                        \
+    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hk * parts, 1, tile_slots(*s, cu_q, s->total_k, NW * 32), &ak, &gk)) \
+      return rc;                                                                                                         \
+  w.nblk = (int)(gq / s->hq);                                                                                            \
+  if (gq)                                                                                                                \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,       \
                                                    (const uint16_t*)o, g, lse, dlse, w, scale, (uint16_t*)dq));          \
-  }                                                                                                                      \
   if (gk) {                                                                                                              \
-    a.ntiles = (int)tk;                                                                                                  \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, a, g, w, \
-                                                   scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                   \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, ak, g,  \
+                                                   w, scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                \
     const int64_t size = s->total_k * s->hk * D;                                                                         \
     if (parts > 1)                                                                                                       \
       LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_sum_kernel<DT>),                                          \

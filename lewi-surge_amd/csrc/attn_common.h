@@ -147,7 +147,7 @@ __device__ __forceinline__ int cu_at(const int32_t* cu, int i, int total) { retu
 
 // Tile t of the rows: sequence s owns the tiles from cu[s] / B + s, which leaves it at least ceil(rows / B).  A packed
 // sequence is found by a 64-way search; up to 63 sequences all ends are read at once, and one trip to memory is all that a
-// workgroup waits for before its first rows.
+// workgroup waits for before its first rows.  Dense: tile t of sequence `seq`.
 struct Place {
   int seq, tile;          // sequence (-1: none) and its tile
   int q0, nq, k0, nk;     // its rows
@@ -155,17 +155,15 @@ struct Place {
 };
 template <int B, bool KEYS>  // tiles of the keys, or of the queries
 __device__ __forceinline__ Place find_tile(const int32_t* cu_q, const int32_t* cu_k, int nseq, int total_q, int total_k,
-                                           int t, int lane) {
+                                           int seq, int t, int lane) {
   Place p;
   p.seq = -1;
   p.tile = p.q0 = p.nq = p.k0 = p.nk = 0;
   if (!cu_q) {
     p.nq = total_q / nseq, p.nk = total_k / nseq;
     p.end = KEYS ? total_k : total_q;
-    const int tiles = ((KEYS ? p.nk : p.nq) + B - 1) / B;
-    if (tiles == 0 || t / tiles >= nseq) return p;
-    p.seq = t / tiles, p.tile = t % tiles;
-    p.q0 = p.seq * p.nq, p.k0 = p.seq * p.nk;
+    p.seq = seq, p.tile = t;
+    p.q0 = seq * p.nq, p.k0 = seq * p.nk;
     return p;
   }
   const int32_t* cu = KEYS ? cu_k : cu_q;
