@@ -663,7 +663,9 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
       g = mma32<DT>(lds_read16(row_step<D>(ra, x) + (R + u) * TILE), V_IN_LDS<D> ? lds_read16(row_step<D>(rv, x)) : vf[V_IN_LDS<D> ? 0 : x], g);
     weigh(u, s, g, p, x);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);  // the wave with products to issue goes first (1 to 2%)
     products(u, p, x);
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   };
   for (int st = 0; st < nst; st += R) {
