@@ -365,40 +365,43 @@ __device__ __forceinline__ float grad_scale(float amax) {
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
-                    const float* __restrict__ lse, const float* __restrict__ dlse, RowPrep w, float scale,
-                    uint16_t* __restrict__ dq) {
+                    const float* __restrict__ lse, const float* __restrict__ dlse, RowPrep w, float scale, int parts,
+                    float* __restrict__ psum, uint16_t* __restrict__ dq) {
   constexpr int BM = NW * 32, TILE = BN * D * 2;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
   __shared__ float red[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hf = lane >> 5;
-  int sq, head, slot;
-  head_tile(a, false, sq, head, slot);
+  const int group = a.hq / a.hk;
+  int sq, unit, slot;
+  head_tile(a, false, sq, unit, slot);
+  const int kvh = unit / (parts * group), part = parts == 1 ? 0 : unit / group % parts, head = kvh * group + unit % group;
   const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
-  if (pl.end + (int64_t)slot * BM < a.total_q) {
+  if (pl.end + (int64_t)slot * BM < a.total_q && part == 0) {
     const int64_t first = pl.end + (int64_t)slot * BM;
     zero_rows<D>(dq, first, (int)min((int64_t)BM, a.total_q - first), a.hq, head, threadIdx.x, NW * 64);
   }
   const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
   if (pl.seq < 0 || tile * BM >= nq) {
-    if (DT == LSURGE_F16 && threadIdx.x == 0) w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = 0.f;
+    if (DT == LSURGE_F16 && threadIdx.x == 0 && part == 0) w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = 0.f;
     return;
   }
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
-  const int kvh = head / (a.hq / a.hk);
 
   const uint32_t lds = lds_addr((const bf16_t*)smem);
   TileCopy<D, BN, NW> ck, cv;
   ck.init(a.k_row, wave, lane);
   cv.init(a.v_row, wave, lane);
-  const uint16_t* kb = a.k + (int64_t)k0 * a.k_row + kvh * a.k_head;
-  const uint16_t* vb = a.v + (int64_t)k0 * a.v_row + kvh * a.v_head;
   const int kend = min(nq, (tile + 1) * BM) + off;
-  const int nst = (max(kend, 0) + BN - 1) / BN;
+  const int all = (max(kend, 0) + BN - 1) / BN;
+  const int begin = (int)((int64_t)all * part / parts), nst = (int)((int64_t)all * (part + 1) / parts) - begin;
+  const int kfirst = begin * BN;  // the part's first key
+  const uint16_t* kb = a.k + (int64_t)(k0 + kfirst) * a.k_row + kvh * a.k_head;
+  const uint16_t* vb = a.v + (int64_t)(k0 + kfirst) * a.v_row + kvh * a.v_head;
   auto issue = [&](int st) {
     const uint32_t at = lds + (st & 1) * 2 * TILE;
-    ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - st * BN, at, wave);
-    cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - st * BN, at + TILE, wave);
+    ck.issue(kb + (int64_t)st * BN * a.k_row, a.k_row, nk - kfirst - st * BN, at, wave);
+    cv.issue(vb + (int64_t)st * BN * a.v_row, a.v_row, nk - kfirst - st * BN, at + TILE, wave);
   };
   if (nst) issue(0);
   // delta and the row's scale from the fragments of do (the two halves of the wave hold the two halves of a row)
@@ -431,7 +434,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
   }
   delta = halves(delta, [](float x, float y) { return x + y; }) - (dlse ? dlse[pi] : 0.f);
   const float lse2 = row_lse == -INFINITY ? INFINITY : row_lse * LOG2E - SHIFT<DT>;
-  if (hf == 0 && row < nq) w.rows[pi] = f32x2_t{lse2, delta};
+  if (hf == 0 && row < nq && part == 0) w.rows[pi] = f32x2_t{lse2, delta};
   float gs = 1.f;
   if constexpr (DT == LSURGE_F16) {
     big = halves(big, [](float x, float y) { return fmaxf(x, y); });
@@ -439,7 +442,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
     big = wave_max(big);  // rows past the end repeat the last one
     if (lane == 0) red[wave] = big;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && part == 0) {
 #pragma unroll
       for (int i = 1; i < NW; ++i) big = fmaxf(big, red[i]);
       w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = big;
@@ -463,10 +466,10 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
     }
     stage_barrier<0>();
     if (st + 1 < nst) issue(st + 1);
-    if (st * BN > w0 + 31 + off || w0 >= nq) continue;
+    if (kfirst + st * BN > w0 + 31 + off || w0 >= nq) continue;
     const uint32_t kt = lds + (st & 1) * 2 * TILE, vt = kt + TILE;
-    const int lim = row + off - st * BN;
-    const bool edge = st * BN + BN - 1 > w0 + off;
+    const int lim = row + off - kfirst - st * BN;
+    const bool edge = kfirst + st * BN + BN - 1 > w0 + off;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x16 s, g;
@@ -498,6 +501,16 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
     }
   }
   const float f = scale / gs * exp2_hw(-SHIFT<DT>);
+  if (parts > 1) {
+    if (row >= nq) return;
+    float* pp = psum + (((int64_t)part * a.total_q + q0 + row) * a.hq + head) * D + 4 * hf;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(pp + 32 * d + 2 * r) = f32x4{acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f};
+    return;
+  }
   __syncthreads();
   store_rows<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, f, dq + ((int64_t)(q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D,
                     min(32, nq - w0), lane);
@@ -509,7 +522,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
 // in.  Both accumulators and the fragments of K and V would fill all 256 registers that two waves a SIMD leave at
 // D = 128, so V waits in LDS there.  The stages of a tile are cut into `parts` equal runs, a workgroup each, where there
 // are too few tiles (the first keys of a causal sequence have many more queries than the last); the parts' sums are then
-// f32 in `psum` and added up in order by attn_dkv_sum_kernel.
+// f32 in `psum` and added up in order by attn_sum_kernel.
 constexpr int QN = 32;  // query rows per stage
 template <int D> constexpr bool V_IN_LDS = D >= 128;
 template <int D> constexpr int DKV_EU = D == 256 ? 1 : 2;  // waves per SIMD that the registers allow
@@ -698,19 +711,20 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
   store_rows<D, DT>(piece, av, fv, dv + first_at, (int64_t)a.hk * D, n, lane);
 }
 
-// dk and dv = the parts' sums, added in order: n values each, 4 a thread; rows from cu[nseq] on were zeroed already
+// `tensors` gradients (x, then y) of `size` values each = the parts' sums, added in order, 4 values a thread; psum
+// [parts][tensors][size].  The rows (`row` values each) from cu[nseq] on were zeroed already.
 template <int DT>
-__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* __restrict__ psum, int parts, int64_t size,
-                                                           int64_t row, const int32_t* __restrict__ cu, int nseq, int total,
-                                                           uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
-  const int64_t n = cu ? cu_at(cu, nseq, total) * row : size;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < 2 * n; i += (int64_t)gridDim.x * 1024) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ psum, int parts, int tensors, int64_t size,
+                                                       int64_t row, const int32_t* __restrict__ cu, int nseq, int total,
+                                                       uint16_t* __restrict__ x, uint16_t* __restrict__ y) {
+  const int64_t n = cu ? cu_at(cu, nseq, total) * row : size, step = tensors * size;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < tensors * n; i += (int64_t)gridDim.x * 1024) {
     const bool second = i >= n;
     const int64_t at = second ? i - n : i;
     const float* p = psum + (second ? size : 0) + at;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
-    for (int j = 1; j < parts; ++j) s += *reinterpret_cast<const f32x4*>(p + 2 * j * size);
-    *reinterpret_cast<u32x2*>((second ? dv : dk) + at) = u32x2{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
+    for (int j = 1; j < parts; ++j) s += *reinterpret_cast<const f32x4*>(p + j * step);
+    *reinterpret_cast<u32x2*>((second ? y : x) + at) = u32x2{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
   }
 }
 
@@ -797,14 +811,17 @@ int64_t dkv_parts(const lsurge_attn_shape& s) {
 // us at 1, 2, 3, 4, 8 parts: 3 chunks of 350 rows over 10000 keys, 32 heads (288 tiles, 300 stages): 369, 247, 260, 254,
 // 259; 64 rows over 6000 keys, 16 heads (16, 190): 118, 68, 51, 42, 33; one prompt of 2048 (256, 32): 48, 47, 52, 57, 83;
 // of 4096, 8 heads, 64-wide (256, 64): 71, 51, 44, 45, 57; of 512 (64, 8): 20, 23, 24, 26, 33.
-int64_t fwd_parts(const lsurge_attn_shape& s) {
+int64_t key_parts(const lsurge_attn_shape& s, int64_t places) {
   if (s.total_q == 0 || s.total_k == 0 || s.nseq == 0) return 1;
   const int64_t rows = s.total_q / s.nseq, keys = s.total_k / s.nseq;
   const int64_t tiles = std::max<int64_t>(s.nseq * ((rows + 127) / 128) * s.hq, 1);
-  const int64_t places = s.d == 256 ? 256 : s.d == 128 ? 512 : 768;
   const int64_t stages = std::max<int64_t>(keys - rows / 2, 0) / FN;  // of an average tile
   return std::max<int64_t>(1, std::min((places + tiles / 2) / tiles, stages / 16));
 }
+int64_t fwd_parts(const lsurge_attn_shape& s) { return key_parts(s, s.d == 256 ? 256 : s.d == 128 ? 512 : 768); }
+// The same for attn_dq_kernel, us a training step at 1, 2, 3, 4, 8 parts of it: one sequence of 4096, 8 heads of their own
+// keys (256 tiles, 64 stages): 314, 269, 257, 261, 288; 8 x 4096, 8 heads over 2 (2048, 64): 1361, 1477, 1546, 1613, 1889.
+int64_t dq_parts(const lsurge_attn_shape& s) { return key_parts(s, s.d == 256 ? 256 : s.d == 128 ? 512 : 1024); }
 
 #define ATTN_DISPATCH(CALL)                                                     \
   do {                                                                          \
@@ -879,8 +896,9 @@ static size_t prep_bytes(const lsurge_attn_shape* s) {
 }
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
   if (!s || s->hq < 1 || s->hk < 1 || s->d < 1 || s->nseq < 0 || s->total_q < 0 || s->total_k < 0) return 0;
-  const int64_t parts = dkv_parts(*s);
-  return prep_bytes(s) + (parts > 1 ? sizeof(float) * (size_t)(2 * parts * s->total_k * s->hk * s->d) : 0) + 256;
+  const int64_t kp = dkv_parts(*s), qp = dq_parts(*s);  // the passes run one after the other: one room for both
+  const int64_t sums = std::max(kp > 1 ? 2 * kp * s->total_k * s->hk : 0, qp > 1 ? qp * s->total_q * s->hq : 0) * s->d;
+  return prep_bytes(s) + sizeof(float) * (size_t)sums + 256;
 }
 
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
@@ -910,32 +928,39 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   RowPrep w;
   w.rows = (f32x2_t*)workspace, w.amax = (float*)(w.rows + nrow);
   float* psum = (float*)((char*)workspace + prep_bytes(s));
-  const int parts = (int)dkv_parts(*s);
+  const int parts = (int)dkv_parts(*s), qparts = (int)dq_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
 #define ATTN_BWD(D, DT)                                                                                                  \
   constexpr int NW = WAVES<D>;                                                                                           \
   AttnArgs ak = a;                                                                                                       \
   unsigned gq = 0, gk = 0;                                                                                               \
   if (s->total_q)                                                                                                        \
-    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hq, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), &a,    \
+    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hq * qparts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), &a,    \
                            &gq))                                                                                         \
       return rc;                                                                                                         \
   if (s->total_k)                                                                                                        \
     if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hk * parts, 1, tile_slots(*s, cu_q, s->total_k, NW * 32), &ak, &gk)) \
       return rc;                                                                                                         \
-  w.nblk = (int)(gq / s->hq);                                                                                            \
-  if (gq)                                                                                                                \
+  w.nblk = (int)(gq / (s->hq * qparts));                                                                                            \
+  const auto sum_grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, 4096)); };             \
+  if (gq) {                                                                                                              \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,       \
-                                                   (const uint16_t*)o, g, lse, dlse, w, scale, (uint16_t*)dq));          \
+                                                   (const uint16_t*)o, g, lse, dlse, w, scale, qparts, psum,             \
+                                                   (uint16_t*)dq));                                                      \
+    const int64_t size = s->total_q * s->hq * D;                                                                         \
+    if (qparts > 1)                                                                                                      \
+      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(size), dim3(256), 0, st, psum,      \
+                                                     qparts, 1, size, s->hq * D, cu_q, a.nseq, a.total_q,                \
+                                                     (uint16_t*)dq, (uint16_t*)dq));                                     \
+  }                                                                                                                      \
   if (gk) {                                                                                                              \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, ak, g,  \
                                                    w, scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                \
     const int64_t size = s->total_k * s->hk * D;                                                                         \
     if (parts > 1)                                                                                                       \
-      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_sum_kernel<DT>),                                          \
-                                                     dim3((unsigned)std::min<int64_t>((2 * size + 1023) / 1024, 4096)),  \
-                                                     dim3(256), 0, st, psum, parts, size, s->hk * D, cu_k, a.nseq,       \
-                                                     a.total_k, (uint16_t*)dk, (uint16_t*)dv));                          \
+      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(2 * size), dim3(256), 0, st, psum,  \
+                                                     parts, 2, size, s->hk * D, cu_k, a.nseq, a.total_k,                 \
+                                                     (uint16_t*)dk, (uint16_t*)dv));                                     \
   }
   ATTN_DISPATCH(ATTN_BWD);
 #undef ATTN_BWD

@@ -162,6 +162,17 @@ def test_long_rows(dev):
             check(q, kk, v, [1500], [1500], D ** -0.5, do, cu=False)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_rows_over_many_keys(dt, D, dev):
+    """The keys cut into parts that are joined, forward and backward: chunks of new tokens over long prefixes, a sequence
+    without queries, rows that see no key, rows behind the last sequence; and one dense sequence."""
+    run(dt, D, 2, 1, [40, 0, 1, 130, 5], [2500, 700, 3000, 130 + 2200, 3], dev, seed=D, dlse=True, tail=70)
+    gen = torch.Generator().manual_seed(D)
+    q, k, v, do = (_randn(gen, (1, 2400, 1, D), dt, dev) for _ in range(4))
+    check(q, k, v, [2400], [2400], D ** -0.5, do, cu=False)
+
+
 def test_small_gradients_in_f16(dev):
     """Upstream gradients near the bottom of f16's normal range, rows of very different sizes, long flat rows."""
     gen = torch.Generator().manual_seed(9)
