@@ -437,19 +437,20 @@ typedef struct {
 } lsurge_attn_rows;
 
 /* o [total_q, hq, d] (contiguous) = softmax(scale q k^T, masked) v, f32 scores and sums; lse [hq, total_q] f32, the natural
- * logarithm of each row's sum of exponentials (NULL: not written).  Rows behind the last sequence: o = 0, lse = -inf;
+ * logarithm of each row's sum of exponentials (NULL: not written); o_lo [total_q, hq, d] bytes, what the rounding of o left
+ * over, for the backward of a training step (E5M2 of 2^12 times the difference; NULL: not written).  Rows behind the last sequence: o = 0, lse = -inf;
  * those rows of q, k and v are not read.  scale positive and finite.  16-byte aligned. */
 size_t lsurge_attn_fwd_workspace_bytes(const lsurge_attn_shape* s); /* 0 where the keys of a tile are not split */
 int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
-                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, float* lse,
-                    void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, void* o_lo,
+                    float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
 /* Backward of lsurge_attn_fwd for upstream dout [total_q, hq, d] (contiguous) and dlse [hq, total_q] f32 (NULL: 0), from
- * the forward's o and lse: dq [total_q, hq, d], dk and dv [total_k, hk, d], summed over the heads of a group, all of the
+ * the forward's o, o_lo (NULL: the backward takes o as it was rounded, a little less exact) and lse: dq [total_q, hq, d], dk and dv [total_k, hk, d], summed over the heads of a group, all of the
  * shape's dtype and contiguous; 0 in the rows behind the last sequence.  No atomics: results repeat bit for bit. */
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s);
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
-                    const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
+                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
                     size_t workspace_bytes, lsurge_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------

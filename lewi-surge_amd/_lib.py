@@ -130,10 +130,11 @@ _SIGS = {
     "lsurge_gdn_chunked_bwd_saved": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
                                             _p, _sz, _p, _sz, _p]),
     "lsurge_attn_fwd_workspace_bytes": (_sz, [ctypes.POINTER(AttnShape)]),
-    "lsurge_attn_fwd": (_int, [ctypes.POINTER(AttnShape), _rows, _rows, _rows, _p, _p, ctypes.c_float, _p, _p, _p, _sz, _p]),
+    "lsurge_attn_fwd": (_int, [ctypes.POINTER(AttnShape), _rows, _rows, _rows, _p, _p, ctypes.c_float, _p, _p, _p, _p, _sz,
+                               _p]),
     "lsurge_attn_bwd_workspace_bytes": (_sz, [ctypes.POINTER(AttnShape)]),
     "lsurge_attn_bwd": (_int, [ctypes.POINTER(AttnShape), _rows, _rows, _rows, _p, _p, ctypes.c_float, _p, _p, _p, _p, _p,
-                               _p, _p, _p, _sz, _p]),
+                               _p, _p, _p, _p, _sz, _p]),
     "lsurge_paged_attn_workspace_bytes": (_sz, [_i64] * 3),
     "lsurge_paged_attn": (_int, [ctypes.POINTER(KvCache), _rows, _i64, _i64, ctypes.c_float, _p, _p, _p, _sz, _p]),
     "lsurge_kv_append": (_int, [ctypes.POINTER(KvCache), _rows, _rows, _i64, _i64, _p, _p]),

@@ -91,27 +91,29 @@ def _rows_arg(t):
     return ctypes.byref(L.AttnRows(t.data_ptr(), row, head))
 
 
-def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse):
-    """o, lse (or None) of packed rows, and what the backward needs: the rows as read and the shape."""
+def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training=False):
+    """o, lse (or None) of packed rows, and what the backward needs: the rows as read, what o's rounding left over, the
+    shape."""
     tq, hq, d = q.shape
     tk, hk, _ = k.shape
     q, k, v = _rows(q, d), _rows(k, d), _rows(v, d)
     shape = L.AttnShape(nseq, tq, tk, hq, hk, d, L.dt(q))
     o = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device) if want_lse else None
+    o_lo = torch.empty((tq, hq, d), dtype=torch.uint8, device=q.device) if training else None
     lib, arg = L.lib(), ctypes.byref(shape)
     nbytes = lib.lsurge_attn_fwd_workspace_bytes(arg)
     ws = L.workspace(nbytes, q.device) if nbytes else None
     _call("attn_fwd", q.device, lib.lsurge_attn_fwd, arg, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q), L.ptr(cu_k),
-          scale, L.ptr(o), L.ptr(lse), L.ptr(ws), nbytes)
-    return o, lse, (q, k, v), shape
+          scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(ws), nbytes)
+    return o, lse, (q, k, v, o_lo), shape
 
 
 class _AttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale):
-        o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, True)
+        o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, True, training=True)
         ctx.save_for_backward(*rows, cu_q, cu_k, o, lse)
         ctx.shape, ctx.scale = shape, scale
         ctx.set_materialize_grads(False)
@@ -120,7 +122,7 @@ class _AttnFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, dlse):
-        q, k, v, cu_q, cu_k, o, lse = ctx.saved_tensors
+        q, k, v, o_lo, cu_q, cu_k, o, lse = ctx.saved_tensors
         if do is None:
             do = torch.zeros_like(o)
         do = _aligned(L.contig(do.to(o.dtype)))
@@ -131,7 +133,7 @@ class _AttnFn(torch.autograd.Function):
         shape = ctypes.byref(ctx.shape)
         ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(shape), q.device)
         _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
-              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk), L.ptr(dv),
+              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk), L.ptr(dv),
               L.ptr(ws), ws.numel())
         return dq, dk, dv, None, None, None, None
 

@@ -134,13 +134,45 @@ __device__ __forceinline__ void store_rows(char* lds, const f32x16* acc, float f
   }
 }
 
+// What a 16-bit output leaves of f32 values, kept for the backward (delta = do . o would otherwise carry the output's
+// rounding into every score gradient: dq and dk 0.0027 off in bf16 at 2000 keys instead of 0.0024, where their own
+// rounding alone makes 0.0017): the difference times 2^12 as E5M2, an eighth of it left over at most.
+constexpr float LO_SCALE = 4096.f;
+template <int DT>
+__device__ __forceinline__ uint32_t left_over(float a, float b, float c, float d) {
+  float x[4];
+  unpack2<DT>(pack2<DT>(a, b), x[0], x[1]);
+  unpack2<DT>(pack2<DT>(c, d), x[2], x[3]);
+  return e5m2x4((a - x[0]) * LO_SCALE, (b - x[1]) * LO_SCALE, (c - x[2]) * LO_SCALE, (d - x[3]) * LO_SCALE);
+}
+// the left-overs of f acc as rows p[row][d] of bytes, as store_rows
+template <int D, int DT>
+__device__ __forceinline__ void store_left_over(char* lds, const f32x16* acc, float f, uint8_t* p, int64_t row_stride, int n,
+                                                int lane) {
+  constexpr int PITCH = D + 16, CPR = D / 16;
+  char* w = lds + (lane & 31) * PITCH + 4 * (lane >> 5);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<uint32_t*>(w + 32 * d + 2 * r) =
+          left_over<DT>(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < CPR / 2; ++i) {
+    const int id = i * 64 + lane, row = id / CPR, c = id % CPR;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(lds + row * PITCH + c * 16);
+    if (row < n) *reinterpret_cast<u32x4*>(p + row * row_stride + c * 16) = x;
+  }
+}
+
 // A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a ring in LDS.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
 // work at the same time; one barrier a stage.
 template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(FWD_EU<D>)))
 void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
-                     float* __restrict__ lse) {
+                     uint8_t* __restrict__ olo, float* __restrict__ lse) {
   constexpr int BM = NW * 32, FR = STAGES<D>, TILE = FN * D * 2;  // bytes of one operand of one stage
   __shared__ __attribute__((aligned(1024))) char smem[2 * FR * TILE];  // FR stages of K, then FR of V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -308,6 +340,9 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
   __syncthreads();
   store_rows<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, inv, o + ((int64_t)(q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D,
                     min(32, nq - w0), lane);
+  if (olo)
+    store_left_over<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, inv, olo + ((int64_t)(q0 + w0) * a.hq + head) * D,
+                           (int64_t)a.hq * D, min(32, nq - w0), lane);
   if (lse && hf == 0 && row < nq)
     lse[(int64_t)head * a.total_q + q0 + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * LN2;
 }
@@ -316,7 +351,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
 template <int D, int DT>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int parts, const float* __restrict__ po,
                                                             const f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
-                                                            float* __restrict__ lse) {
+                                                            uint8_t* __restrict__ olo, float* __restrict__ lse) {
   constexpr int LPR = D / 4;
   const int64_t n = (a.cu_q ? cu_at(a.cu_q, a.nseq, a.total_q) : a.total_q) * (int64_t)a.hq, step = (int64_t)a.total_q * a.hq;
   const int d = threadIdx.x % LPR * 4;
@@ -332,7 +367,9 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
       if (f != 0.f) x += f * *reinterpret_cast<const f32x4*>(po + (p * step + i) * D + d);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<u32x2*>(o + i * D + d) = u32x2{pack2<DT>(x[0] * inv, x[1] * inv), pack2<DT>(x[2] * inv, x[3] * inv)};
+    x *= inv;
+    *reinterpret_cast<u32x2*>(o + i * D + d) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+    if (olo) *reinterpret_cast<uint32_t*>(olo + i * D + d) = left_over<DT>(x[0], x[1], x[2], x[3]);
     if (lse && d == 0) lse[i % a.hq * a.total_q + i / a.hq] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
   }
 }
@@ -364,7 +401,7 @@ __device__ __forceinline__ float grad_scale(float amax) {
 // two products more, but no sum over workgroups, whose order would change the results.
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
+void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* __restrict__ olo, const uint16_t* __restrict__ dout,
                     const float* __restrict__ lse, const float* __restrict__ dlse, RowPrep w, float scale, int parts,
                     float* __restrict__ psum, uint16_t* __restrict__ dq) {
   constexpr int BM = NW * 32, TILE = BN * D * 2;
@@ -421,12 +458,19 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint16_t* 
     }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+    u32x2 lo[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      lo[s] = olo ? *reinterpret_cast<const u32x2*>(olo + at + 16 * s) : u32x2{0, 0};
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x0, x1, y0, y1;
         unpack2<DT>(of[s][i], x0, x1);
+        const f32x2_t e = i % 2 ? __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], true) : __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], false);
+        x0 = fmaf(e[0], 1.f / LO_SCALE, x0);
+        x1 = fmaf(e[1], 1.f / LO_SCALE, x1);
         unpack2<DT>(df[s][i], y0, y1);
         delta = fmaf(x0, y0, fmaf(x1, y1, delta));
         if (DT == LSURGE_F16) big = fmaxf(big, fmaxf(fabsf(y0), fabsf(y1)));
@@ -850,11 +894,11 @@ size_t lsurge_attn_fwd_workspace_bytes(const lsurge_attn_shape* s) {
 }
 
 int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
-                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, float* lse,
-                    void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
+                    const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, void* o_lo,
+                    float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
   if (int rc = check_shape("attn_fwd", s, cu_q, cu_k, scale)) return rc;
   if (s->total_q == 0) return LSURGE_OK;
-  LSURGE_REQUIRE(q && k && v && o && (uintptr_t)o % 16 == 0, "attn_fwd: null or misaligned pointer");
+  LSURGE_REQUIRE(q && k && v && o && ((uintptr_t)o | (uintptr_t)o_lo) % 16 == 0, "attn_fwd: null or misaligned pointer");
   if (int rc = check_rows("attn_fwd q", *q, s->d)) return rc;
   if (s->total_k) {
     if (int rc = check_rows("attn_fwd k", *k, s->d)) return rc;
@@ -876,12 +920,12 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
                          &a, &grid))                                                                                  \
     return rc;                                                                                                        \
   LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a,   \
-                                                 parts, po, pm, (uint16_t*)o, lse));                                  \
+                                                 parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse));                                  \
   const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                              \
   if (parts > 1)                                                                                                      \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_join_kernel<D, DT>),                                     \
                                                    dim3((unsigned)std::min<int64_t>(rows, 8192)), dim3(256), 0, st, a, \
-                                                   parts, po, pm, (uint16_t*)o, lse))
+                                                   parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse))
   ATTN_DISPATCH(ATTN_FWD);
 #undef ATTN_FWD
   return LSURGE_OK;
@@ -903,14 +947,14 @@ size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
 
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
-                    const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
+                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
                     size_t workspace_bytes, lsurge_stream_t stream) {
   if (int rc = check_shape("attn_bwd", s, cu_q, cu_k, scale)) return rc;
   LSURGE_REQUIRE(q && k && v && workspace, "attn_bwd: null pointer");
   const size_t need = lsurge_attn_bwd_workspace_bytes(s);
   if (workspace_bytes < need)
     return lsurge::set_error(LSURGE_ERR_WORKSPACE, "attn_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
-  LSURGE_REQUIRE(((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) %
+  LSURGE_REQUIRE(((uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) %
                          16 == 0,
                  "attn_bwd: buffers must be 16-byte aligned");
   if (s->total_q) {
@@ -945,7 +989,8 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const auto sum_grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, 4096)); };             \
   if (gq) {                                                                                                              \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,       \
-                                                   (const uint16_t*)o, g, lse, dlse, w, scale, qparts, psum,             \
+                                                   (const uint16_t*)o, (const uint8_t*)o_lo, g, lse, dlse, w, scale,     \
+                                                   qparts, psum,                                                         \
                                                    (uint16_t*)dq));                                                      \
     const int64_t size = s->total_q * s->hq * D;                                                                         \
     if (qparts > 1)                                                                                                      \

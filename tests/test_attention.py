@@ -175,7 +175,7 @@ def _shape(**kw):
 
 def _fwd(shape, rows=None, cu=(None, None), scale=1.0, o=FAKE, ws=FAKE, nbytes=1 << 40):
     r = [ctypes.byref(x) for x in (rows or [L.AttnRows(256, 512, 64)] * 3)]
-    return L.lib().lsurge_attn_fwd(ctypes.byref(shape), *r, *cu, scale, o, None, ws, nbytes, None)
+    return L.lib().lsurge_attn_fwd(ctypes.byref(shape), *r, *cu, scale, o, None, None, ws, nbytes, None)
 
 
 def test_c_abi_forward_refusals():
@@ -209,7 +209,7 @@ def test_c_abi_backward_refusals():
     assert need >= 2 * 4 * 8 * 4
     assert lib.lsurge_attn_bwd_workspace_bytes(ctypes.byref(_shape(dtype=L.F16))) > need
     call = lambda o=FAKE, g=FAKE, dk=FAKE, ws=FAKE, n=need: lib.lsurge_attn_bwd(  # noqa: E731
-        ctypes.byref(s), r, r, r, None, None, 1.0, o, FAKE, g, None, FAKE, dk, FAKE, ws, n, None)
+        ctypes.byref(s), r, r, r, None, None, 1.0, o, None, FAKE, g, None, FAKE, dk, FAKE, ws, n, None)
     assert call(n=need - 1) == -4 and b"workspace" in lib.lsurge_last_error()
     assert call(ws=None) == -1 and call(o=None) == -1 and call(dk=None) == -1
     assert call(g=ctypes.c_void_p(264)) == -1 and b"aligned" in lib.lsurge_last_error()
