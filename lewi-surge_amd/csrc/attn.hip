@@ -4,7 +4,7 @@
 //   s_ij = scale q_i . k_j,  o_i = sum_j e^(s_ij - lse_i) v_j,  lse_i = log sum_j e^(s_ij)
 // and o_i = 0, lse_i = -inf for a query with no key.  Scores and sums are f32, in base 2 (the scale carries log2 e); the
 // weights are rounded to the operands' type for the second product, as its operands have to be (half a step of the type,
-// relative to each weight, so that errors average out over the keys; the denominator sums them unrounded).
+// relative to each weight, so that errors average out over the keys).
 //
 // Every product is formed transposed: S^T = K Q^T has a query per lane (column l % 32), so a row's maximum and sum are
 // sums over a lane's own registers and one exchange with lane ^ 32, the accumulators O^T = V^T P^T have the same query in
@@ -169,9 +169,12 @@ __device__ __forceinline__ void store_left_over(char* lds, const f32x16* acc, fl
 // A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a ring in LDS.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
 // work at the same time; one barrier a stage.
 template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
-template <int D, int DT, int NW>
+// TRAIN: for a backward, with what o's rounding leaves over, and o divided by the sum of the weights as they were rounded:
+// a rounding then moves o by (v - o) of it and not by v, and a weight that makes up most of a row by nothing (o 0.0022 off
+// in bf16 without, 0.0020 with; dq, which takes delta from it, 0.0025 and 0.0024).  8% of the forward's time, 1% of a step.
+template <int D, int DT, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(FWD_EU<D>)))
-void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
+void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x4* __restrict__ pm, uint16_t* __restrict__ o,
                      uint8_t* __restrict__ olo, float* __restrict__ lse) {
   constexpr int BM = NW * 32, FR = STAGES<D>, TILE = FN * D * 2;  // bytes of one operand of one stage
   __shared__ __attribute__((aligned(1024))) char smem[2 * FR * TILE];  // FR stages of K, then FR of V
@@ -230,8 +233,9 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-  // m: base of the weights, in base 2 (mc: 0 before the first); l: this half's share of the row's sum
-  float m = -INFINITY, mc = 0.f, l = 0.f;
+  // m: base of the weights, in base 2 (mc: 0 before the first); this half's share of the row's sum of the weights (l: lse
+  // is from it) and of the weights as rounded (lr)
+  float m = -INFINITY, mc = 0.f, l = 0.f, lr = 0.f;
   const uint32_t ka = lds + row_addr<D>(lane);
   uint32_t va[COLS<D>];
 #pragma unroll
@@ -281,12 +285,18 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
       sum[1] += e1;
       p[r / 8][r % 8 / 2] = pack2<DT>(e0, e1);
     }
+    float rsum = 0.f;
+    if constexpr (TRAIN) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rsum = add2<DT>(p[i / 4][i % 4], rsum);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(p[i]));  // formed here, not after the branch below
     interleave<D / 16, 4>();
     __builtin_amdgcn_sched_barrier(0);
     if (__any(mx != m)) {
       l *= alpha;
+      if (TRAIN) lr *= alpha;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) rescale<D>(acc[d], alpha);
     }
@@ -296,6 +306,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     }
     m = mx;
     l += sum[0] + sum[1];
+    if (TRAIN) lr += rsum;
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -324,6 +335,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
     __builtin_amdgcn_s_waitcnt(0);  // the copies past the end land before LDS is used again, or the wave ends
   }
   l = halves(l, [](float x, float y) { return x + y; });
+  lr = TRAIN ? halves(lr, [](float x, float y) { return x + y; }) : l;
   if (parts > 1) {
     if (row >= nq) return;  // the sums as they are, and what they are relative to
     const int64_t at = (int64_t)part * a.total_q + q0 + row;
@@ -333,14 +345,14 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         *reinterpret_cast<f32x4*>(pp + 32 * d + 2 * r) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
-    if (hf == 0) pm[at * a.hq + head] = f32x2_t{mc, l};
+    if (hf == 0) pm[at * a.hq + head] = f32x4{mc, l, lr, 0.f};
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = lr == 0.f ? 0.f : 1.f / lr;
   __syncthreads();
   store_rows<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, inv, o + ((int64_t)(q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D,
                     min(32, nq - w0), lane);
-  if (olo)
+  if (TRAIN)
     store_left_over<D, DT>(smem + wave * 32 * (D * 2 + 16), acc, inv, olo + ((int64_t)(q0 + w0) * a.hq + head) * D,
                            (int64_t)a.hq * D, min(32, nq - w0), lane);
   if (lse && hf == 0 && row < nq)
@@ -350,23 +362,24 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x2_t* __r
 // o and lse from the parts' sums, added in order: D / 4 threads a row and head
 template <int D, int DT>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int parts, const float* __restrict__ po,
-                                                            const f32x2_t* __restrict__ pm, uint16_t* __restrict__ o,
+                                                            const f32x4* __restrict__ pm, uint16_t* __restrict__ o,
                                                             uint8_t* __restrict__ olo, float* __restrict__ lse) {
   constexpr int LPR = D / 4;
   const int64_t n = (a.cu_q ? cu_at(a.cu_q, a.nseq, a.total_q) : a.total_q) * (int64_t)a.hq, step = (int64_t)a.total_q * a.hq;
   const int d = threadIdx.x % LPR * 4;
   for (int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i < n; i += (int64_t)gridDim.x * (256 / LPR)) {
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, lr = 0.f;
     for (int p = 0; p < parts; ++p)
       if (pm[p * step + i][1] != 0.f) m = fmaxf(m, pm[p * step + i][0]);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     for (int p = 0; p < parts; ++p) {
-      const f32x2_t s = pm[p * step + i];
+      const f32x4 s = pm[p * step + i];
       const float f = s[1] == 0.f ? 0.f : exp2_hw(s[0] - m);
       l += f * s[1];
+      lr += f * s[2];
       if (f != 0.f) x += f * *reinterpret_cast<const f32x4*>(po + (p * step + i) * D + d);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
     x *= inv;
     *reinterpret_cast<u32x2*>(o + i * D + d) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
     if (olo) *reinterpret_cast<uint32_t*>(olo + i * D + d) = left_over<DT>(x[0], x[1], x[2], x[3]);
@@ -890,7 +903,7 @@ extern "C" {
 size_t lsurge_attn_fwd_workspace_bytes(const lsurge_attn_shape* s) {
   if (!s || s->hq < 1 || s->hk < 1 || s->d < 1 || s->nseq < 0 || s->total_q < 0 || s->total_k < 0) return 0;
   const int64_t parts = fwd_parts(*s);
-  return parts > 1 ? sizeof(float) * (size_t)(parts * s->total_q * s->hq * (s->d + 2)) : 0;
+  return parts > 1 ? sizeof(float) * (size_t)(parts * s->total_q * s->hq * (s->d + 4)) : 0;
 }
 
 int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
@@ -912,15 +925,19 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   AttnArgs a = make_args(*s, *q, *k, *v, cu_q, cu_k, scale);
   const int parts = (int)fwd_parts(*s);
   float* po = (float*)workspace;
-  f32x2_t* pm = (f32x2_t*)(po + (size_t)parts * s->total_q * s->hq * s->d);
+  f32x4* pm = (f32x4*)(po + (size_t)parts * s->total_q * s->hq * s->d);
 #define ATTN_FWD(D, DT)                                                                                               \
   constexpr int NW = WAVES<D>;                                                                                        \
   unsigned grid;                                                                                                      \
   if (int rc = plan_grid("attn_fwd", *s, cu_q, s->hq * parts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), \
                          &a, &grid))                                                                                  \
     return rc;                                                                                                        \
-  LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW>), dim3(grid), dim3(NW * 64), 0, st, a,   \
-                                                 parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse));                                  \
+  if (o_lo)                                                                                                           \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, true>), dim3(grid), dim3(NW * 64), 0,  \
+                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse));         \
+  else                                                                                                                \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, false>), dim3(grid), dim3(NW * 64), 0, \
+                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)nullptr, lse));      \
   const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                              \
   if (parts > 1)                                                                                                      \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_join_kernel<D, DT>),                                     \

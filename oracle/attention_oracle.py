@@ -12,7 +12,9 @@ sums and accumulators in f32 and rounds the weights and score gradients to the t
 once, is within (to first order, each term a count of roundings)
   score           es = (D + 4) x scale |q| . |k|           (D products summed, the scale, the base change)
   weight          ew = u + 2 max_j es + (nk + 8) x          (relative; its rounding, its exponent, the row's sum, exp2)
-  o               ew A + u |o| + tiny,   A = w |v|
+  o               ew (A + |o|) + u |o| + tiny,   A = w |v|   (divided by the sum of the weights as rounded, w (1 + e), |e| <= ew:
+                  sum w (1 + e) v / sum w (1 + e) - o = sum w e (v - o) / (1 + sum w e), at most ew (A + |o|) to first order; by
+                  the sum of the unrounded ones: ew A)
   do . v          ep = (D + 2) x |do| . |v|
   delta           ed = |do| . (error of o) + (D + 2) x |do| . |o|
   ds              eds = ew |ds| + w (ep + ed)               (one more u inside ew stands for its own rounding)
@@ -89,7 +91,7 @@ def bounds(q, k, v, scale, u, do=None, dlse=None, mask=None):
     tiny = 2.0 ** -25 if u == 2.0 ** -11 else 0.0
     vsum = av.sum(1, keepdims=True)
     o = w @ _heads(v, group)
-    eo = 1.05 * (ew * (w @ av) + u * np.abs(o) + tiny * (vsum + 1))
+    eo = 1.05 * (ew * (w @ av + np.abs(o)) + u * np.abs(o) + tiny * (vsum + 1))
     el = np.where(np.isfinite(lse), es[..., 0] + (nk + 8) * X + 4 * X * np.abs(np.where(np.isfinite(lse), lse, 0)), 0.0)
     out = [eo.transpose(1, 0, 2), el.T]
     if do is None:
