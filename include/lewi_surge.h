@@ -474,7 +474,7 @@ typedef struct {
 } lsurge_kv_cache;
 
 /* One query token a sequence over all seq_lens[b] tokens of its cache: o [nseq, hq, d] (contiguous) and lse [nseq, hq] f32
- * (NULL: not written) as lsurge_attn_fwd's; a sequence of length 0 gets o = 0, lse = -inf.  q: [nseq, hq, d] by strides
+ * (NULL: not written) as lsurge_attn_fwd's; a sequence of length 0 gets o = 0, lse = -inf.  max_pages page_size <= 2^30.  q: [nseq, hq, d] by strides
  * (row_stride and head_stride any multiples of 8).  The sequences' tokens are dealt to the GPU in equal shares whatever
  * their lengths; the parts of a sequence are joined in a fixed order, so results repeat bit for bit.  Calls that share a
  * workspace have to be ordered on one stream. */

@@ -394,7 +394,8 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
 // small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times too large (lse2 smaller by SHIFT)
 // and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's own, from the largest |do| of the
 // row, in the pass over queries; the group's, from the largest of all rows, in the pass over keys, which sums over the rows
-// (amax [hq][nblk]: a tile's largest).
+// (amax [hq][nblk]: a tile's largest).  With the weights' 2^SHIFT taken back to 2^4 a score gradient is 16 p (do . v - delta)
+// at |do| scaled to 1: normal down to 4e-6, and finite up to |do . v| of thousands.
 template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
 struct RowPrep {
   f32x2_t* rows;  // lse2, delta
@@ -407,6 +408,11 @@ __device__ __forceinline__ float grad_scale(float amax) {
   int e;
   (void)frexpf(amax, &e);
   return ldexpf(1.f, min(max(1 - e, -60), 60));
+}
+// the factor of (do . v - delta) beside a weight 2^SHIFT too large
+template <int DT>
+__device__ __forceinline__ float ds_scale(float amax) {
+  return DT == LSURGE_F16 ? grad_scale(amax) * exp2_hw(4.f - SHIFT<DT>) : 1.f;
 }
 
 // dq_i = scale sum_j ds_ij k_j with ds_ij = p_ij (do_i . v_j - delta_i): the forward's walk, a query per lane, dS^T in
@@ -495,7 +501,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
   float gs = 1.f;
   if constexpr (DT == LSURGE_F16) {
     big = halves(big, [](float x, float y) { return fmaxf(x, y); });
-    gs = grad_scale(big);
+    gs = ds_scale<DT>(big);
     big = wave_max(big);  // rows past the end repeat the last one
     if (lane == 0) red[wave] = big;
     __syncthreads();
@@ -658,7 +664,7 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NW; ++i) mx = fmaxf(mx, red[i]);
-    gs = grad_scale(mx);
+    gs = ds_scale<DT>(mx);
   }
   f32x16 ak[D / 32], av[D / 32];
 #pragma unroll

@@ -344,7 +344,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(DecodeArgs a) {
   const int grp = tid / LPR, d = tid % LPR * 4;
   const int64_t at = ((int64_t)b * a.hk * a.hblocks + hb) * 2;
   const bool empty = seq_len(a, b) == 0;
-  const int w0 = empty ? 0 : a.shares[at], n = empty ? 0 : a.shares[at + 1] - w0 + 1;
+  // held to the grid, so that lengths changed between the two kernels make no read outside the workspace
+  const int w0 = empty ? 0 : min(max(a.shares[at], 0), a.grid - 1);
+  const int n = empty ? 0 : min(max(a.shares[at + 1] - w0 + 1, 1), a.grid - w0);
   if (n == 1) return;
   auto slot = [&](int i) { return (int64_t)(w0 + i) * 2 + (i == 0); };
   float m = -INFINITY;
@@ -488,7 +490,7 @@ int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64
   const size_t need = lsurge_paged_attn_workspace_bytes(nseq, hq, c->d);
   if (workspace_bytes < need)
     return lsurge::set_error(LSURGE_ERR_WORKSPACE, "paged_attn: workspace %zu < %zu bytes", workspace_bytes, need);
-  LSURGE_REQUIRE((int64_t)c->max_pages * c->page_size < (1ll << 31), "paged_attn: %lld pages of %lld tokens a sequence",
+  LSURGE_REQUIRE((int64_t)c->max_pages * c->page_size <= (1ll << 30), "paged_attn: %lld pages of %lld tokens a sequence",
                  (long long)c->max_pages, (long long)c->page_size);
   a.q = (const uint16_t*)q->data, a.q_row = q->row_stride, a.q_head = q->head_stride;
   a.lens = c->seq_lens;

@@ -105,8 +105,8 @@ def bounds(q, k, v, scale, u, do=None, dlse=None, mask=None):
     ed = (ag * eo).sum(-1, keepdims=True) + (D + 2) * X * (ag * np.abs(o)).sum(-1, keepdims=True)
     ep = (D + 2) * X * (ag @ av.transpose(0, 2, 1))
     eds = (ew + u) * ds + w * (ep + ed)
-    if tiny:  # subnormal steps of the scaled gradients: 2^-25 of the largest |do|, of the scaled weights: 2^-35
-        eds = eds + 2.0 ** -35 * ag.max(initial=0)
+    if tiny:  # half a subnormal step of the score gradients, scaled by 2^4 / |do|; of the weights, scaled by 2^10: 2^-35
+        eds = eds + 2.0 ** -29 * ag.max(initial=0)
     ewt = ew * w + tiny * 2.0 ** -10 * (w > 0)
     dq, dk, dv = attention_bwd(q, k, v, do, scale, dlse)
     fold = lambda t: t.reshape(hk, group, *t.shape[1:]).sum(1).transpose(1, 0, 2)  # noqa: E731

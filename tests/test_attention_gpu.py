@@ -180,6 +180,7 @@ def test_small_gradients_in_f16(dev):
     do = _randn(gen, (1, 2000, 1, 64), F16, dev) * 2.0 ** -8
     do[:, ::3] *= 2.0 ** -4
     check(q, k, v * 10, [2000], [2000], 0.125, do, cu=False)
+    check(q * 20, k, v * 1000, [2000], [2000], 0.125, do * 256, cu=False)  # and values in the hundreds, peaked rows
 
 
 def test_extreme_scores(dev):
