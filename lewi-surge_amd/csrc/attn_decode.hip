@@ -67,7 +67,7 @@ __global__ __launch_bounds__(DT_THREADS) __attribute__((amdgpu_waves_per_eu(DECO
 void attn_decode_kernel(DecodeArgs a) {
   constexpr int KC = D / 32, VE = D / 16, VW = VE / 2;  // a lane's 16-byte chunks of a key, columns and registers of a value
   __shared__ int64_t wsum[DW], found;
-  __shared__ int found_b;
+  __shared__ int found_b, found_len;
   __shared__ __attribute__((aligned(16))) float so[DW][16][D];
   __shared__ float sm[DW][16], sl[DW][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,9 +76,11 @@ void attn_decode_kernel(DecodeArgs a) {
   // units of all sequences: each thread sums a slab of them, then a scan over the threads
   const int slab = (a.nseq + DT_THREADS - 1) / DT_THREADS;
   int64_t mine = 0;
+  int first_len = 0;
   for (int i = 0; i < slab; ++i) {
-    const int b = tid * slab + i;
-    if (b < a.nseq) mine += units_of(seq_len(a, b));
+    const int b = tid * slab + i, n = b < a.nseq ? seq_len(a, b) : 0;
+    if (i == 0) first_len = n;
+    mine += units_of(n);
   }
   int64_t pre = mine;
 #pragma unroll
@@ -101,20 +103,22 @@ void attn_decode_kernel(DecodeArgs a) {
   if (u >= uend) return;
   // the sequence of the share's first unit: in the slab that holds it, then one by one
   if (mine && (pre - mine) * heads <= u && u < pre * heads) {
-    int b = tid * slab;
+    int b = tid * slab, len = first_len;
     int64_t base = (pre - mine) * heads;
-    for (;; ++b) {
-      const int64_t n = (int64_t)units_of(seq_len(a, b)) * heads;
+    while (true) {
+      const int64_t n = (int64_t)units_of(len) * heads;
       if (u < base + n) break;
       base += n;
+      len = seq_len(a, ++b);
     }
     found = base;
     found_b = b;
+    found_len = len;
   }
   __syncthreads();
   int64_t base = uni64(found);  // units before sequence b (all heads)
   int b = __builtin_amdgcn_readfirstlane(found_b);
-  int len = __builtin_amdgcn_readfirstlane(seq_len(a, b)), nu = units_of(len);
+  int len = __builtin_amdgcn_readfirstlane(found_len), nu = units_of(len);
   int hb = (int)div64(u - base, nu);
   const int pmask = (1 << a.c.page_log2) - 1;
 
