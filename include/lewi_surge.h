@@ -438,20 +438,24 @@ typedef struct {
 
 /* o [total_q, hq, d] (contiguous) = softmax(scale q k^T, masked) v, f32 scores and sums; lse [hq, total_q] f32, the natural
  * logarithm of each row's sum of exponentials (NULL: not written); o_lo [total_q, hq, d] bytes, what the rounding of o left
- * over, for the backward of a training step (E5M2 of 2^12 times the difference; NULL: not written).  Rows behind the last sequence: o = 0, lse = -inf;
- * those rows of q, k and v are not read.  scale positive and finite.  16-byte aligned. */
+ * over, for the backward of a training step (E5M2 of 2^12 times the difference; NULL: not written, and o is a little less
+ * exact).  Rows behind the last sequence: o = 0, lse = -inf; those rows of q, k and v are not read.  A masked key's score
+ * never counts, whatever k holds there; a value of v that is not finite may reach, besides the queries that see it, ones of
+ * its sequence up to 62 before them (its weight there is 0, and 0 x inf is NaN).  scale positive and finite; buffers
+ * 16-byte aligned. */
 size_t lsurge_attn_fwd_workspace_bytes(const lsurge_attn_shape* s); /* 0 where the keys of a tile are not split */
 int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, void* o, void* o_lo,
                     float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
 /* Backward of lsurge_attn_fwd for upstream dout [total_q, hq, d] (contiguous) and dlse [hq, total_q] f32 (NULL: 0), from
- * the forward's o, o_lo (NULL: the backward takes o as it was rounded, a little less exact) and lse: dq [total_q, hq, d], dk and dv [total_k, hk, d], summed over the heads of a group, all of the
- * shape's dtype and contiguous; 0 in the rows behind the last sequence.  No atomics: results repeat bit for bit. */
+ * the forward's o, o_lo (NULL: the backward takes o as it was rounded, a little less exact) and lse: dq [total_q, hq, d],
+ * dk and dv [total_k, hk, d], summed over the heads of a group, all of the shape's dtype and contiguous; 0 in the rows
+ * behind the last sequence.  No atomics: results repeat bit for bit. */
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s);
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
-                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
-                    size_t workspace_bytes, lsurge_stream_t stream);
+                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv,
+                    void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Paged key-value cache: one token's attention over it, and writing new tokens to it.
@@ -474,10 +478,11 @@ typedef struct {
 } lsurge_kv_cache;
 
 /* One query token a sequence over all seq_lens[b] tokens of its cache: o [nseq, hq, d] (contiguous) and lse [nseq, hq] f32
- * (NULL: not written) as lsurge_attn_fwd's; a sequence of length 0 gets o = 0, lse = -inf.  max_pages page_size <= 2^30.  q: [nseq, hq, d] by strides
- * (row_stride and head_stride any multiples of 8).  The sequences' tokens are dealt to the GPU in equal shares whatever
- * their lengths; the parts of a sequence are joined in a fixed order, so results repeat bit for bit.  Calls that share a
- * workspace have to be ordered on one stream. */
+ * (NULL: not written) as lsurge_attn_fwd's; a sequence of length 0 gets o = 0, lse = -inf.  q: [nseq, hq, d] by strides
+ * (row_stride and head_stride any multiples of 8).  max_pages page_size <= 2^30.  The sequences' tokens are dealt to the GPU
+ * in equal shares whatever their lengths, and the parts of a sequence are joined in a fixed order: results repeat bit for
+ * bit for the same lengths, and a sequence's last bits depend on where the shares cut it.  Calls that share a workspace have
+ * to be ordered on one stream. */
 size_t lsurge_paged_attn_workspace_bytes(int64_t nseq, int64_t hq, int64_t d);
 int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64_t nseq, int64_t hq, float scale, void* o,
                       float* lse, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);

@@ -133,8 +133,8 @@ class _AttnFn(torch.autograd.Function):
         shape = ctypes.byref(ctx.shape)
         ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(shape), q.device)
         _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
-              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk), L.ptr(dv),
-              L.ptr(ws), ws.numel())
+              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk),
+              L.ptr(dv), L.ptr(ws), ws.numel())
         return dq, dk, dv, None, None, None, None
 
 
@@ -147,8 +147,10 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
 
     Returns o in q's shape and dtype, and with return_lse also the natural logarithm of each row's sum of exponentials, f32
     [B, Tq, H] or [Tq, H] (-inf for a row without keys).  Both are differentiable (once); rows of packed tensors behind the
-    last sequence give zeros and get zero gradients.  Strides are free as long as the last axis is contiguous: q, k and v
-    may be views of one projection's output."""
+    last sequence give zeros and get zero gradients.  A masked key never counts, whatever k holds there; a value of v that is
+    not finite may also reach queries up to 62 before the first that sees it (its weight there is 0, and 0 x inf is NaN), and
+    in the backward any input that is not finite gradients of rows up to 95 away.  Strides are free as long as the last axis
+    is contiguous: q, k and v may be views of one projection's output."""
     what = "causal_attention"
     if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape or k.shape[-1] != q.shape[-1]:
         raise ValueError(f"{what}: q [B, Tq, H, D] or [Tq, H, D], k and v alike with their own rows and heads (got "
@@ -242,7 +244,9 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
 def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, return_lse=False):
     """Attention of one new token per sequence, q [sequences, H, D], over its seq_lens[b] cached tokens (the new one among
     them, see append_kv).  Returns o [sequences, H, D] in q's dtype, and with return_lse also f32 [sequences, H].  Length 0
-    gives zeros (lse -inf); tokens whose page_table entry names no page are left out.  No gradient."""
+    gives zeros (lse -inf); tokens whose page_table entry names no page are left out.  Slots behind a sequence's last token are
+    never used, whatever they hold.  Results repeat bit for bit for the same lengths; a sequence's last bits depend on the
+    lengths of the others, which decide where its tokens are cut into parts.  No gradient."""
     what = "paged_attention"
     if q.dim() != 3 or k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3] or q.shape[0] != page_table.shape[0]:
         raise ValueError(f"{what}: q must be [sequences, heads, head_dim] (got {tuple(q.shape)}, caches "

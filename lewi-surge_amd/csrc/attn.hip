@@ -134,6 +134,17 @@ __device__ __forceinline__ void store_rows(char* lds, const f32x16* acc, float f
   }
 }
 
+// a part's f32 sums f acc, the lane's row from p on
+template <int D>
+__device__ __forceinline__ void store_sums(float* p, const f32x16* acc, float f) {
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<f32x4*>(p + 32 * d + 2 * r) =
+          f32x4{acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f};
+}
+
 // What a 16-bit output leaves of f32 values, kept for the backward (delta = do . o would otherwise carry the output's
 // rounding into every score gradient: dq and dk 0.0027 off in bf16 at 2000 keys instead of 0.0024, where their own
 // rounding alone makes 0.0017): the difference times 2^12 as E5M2, an eighth of it left over at most.
@@ -166,8 +177,14 @@ __device__ __forceinline__ void store_left_over(char* lds, const f32x16* acc, fl
   }
 }
 
-// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a ring in LDS.  The scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit
-// work at the same time; one barrier a stage.
+// A workgroup takes NW x 32 queries of one head, 32 a wave, and walks the keys in stages of 32 through a ring in LDS.  The
+// scores of stage j + 1 are formed beside the softmax of stage j, so that the matrix cores and the vector unit work at the
+// same time; one barrier a stage.
+// 32 queries a wave, not 64: the accumulators, Q's fragments and two stages of scores leave two waves a SIMD at D = 128.  K
+// and V then cost 1 KiB of LDS reads a matrix instruction, which its 128 bytes a clock just carry.
+// Measured, one sequence of 16384, 16 heads over 4 (2): 1.02 ms, 1080 TFLOP/s at D = 128 (a library product of 8192^3
+// reaches 1190 to 1240 on these cards); D = 64 0.60 ms, 910 (as many exponentials for half the products); D = 256 2.30 ms,
+// 955 (one wave a SIMD).  24 prompts of 1024: 136 us, 755; start and end are 9000 of a workgroup's 45000 cycles there.
 template <int D> constexpr int FWD_EU = D == 256 ? 1 : D == 128 ? 2 : 3;  // waves per SIMD that the registers allow
 // TRAIN: for a backward, with what o's rounding leaves over, and o divided by the sum of the weights as they were rounded:
 // a rounding then moves o by (v - o) of it and not by v, and a weight that makes up most of a row by nothing (o 0.0022 off
@@ -340,11 +357,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x4* __res
     if (row >= nq) return;  // the sums as they are, and what they are relative to
     const int64_t at = (int64_t)part * a.total_q + q0 + row;
     float* pp = po + (at * a.hq + head) * D + 4 * hf;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *reinterpret_cast<f32x4*>(pp + 32 * d + 2 * r) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+    store_sums<D>(pp, acc, 1.f);
     if (hf == 0) pm[at * a.hq + head] = f32x4{mc, l, lr, 0.f};
     return;
   }
@@ -365,7 +378,8 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
                                                             const f32x4* __restrict__ pm, uint16_t* __restrict__ o,
                                                             uint8_t* __restrict__ olo, float* __restrict__ lse) {
   constexpr int LPR = D / 4;
-  const int64_t n = (a.cu_q ? cu_at(a.cu_q, a.nseq, a.total_q) : a.total_q) * (int64_t)a.hq, step = (int64_t)a.total_q * a.hq;
+  const int64_t n = (int64_t)(a.cu_q ? cu_at(a.cu_q, a.nseq, a.total_q) : a.total_q) * a.hq;
+  const int64_t step = (int64_t)a.total_q * a.hq;
   const int d = threadIdx.x % LPR * 4;
   for (int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i < n; i += (int64_t)gridDim.x * (256 / LPR)) {
     float m = -INFINITY, l = 0.f, lr = 0.f;
@@ -394,8 +408,8 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
 // small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times too large (lse2 smaller by SHIFT)
 // and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's own, from the largest |do| of the
 // row, in the pass over queries; the group's, from the largest of all rows, in the pass over keys, which sums over the rows
-// (amax [hq][nblk]: a tile's largest).  With the weights' 2^SHIFT taken back to 2^4 a score gradient is 16 p (do . v - delta)
-// at |do| scaled to 1: normal down to 4e-6, and finite up to |do . v| of thousands.
+// (amax [hq][nblk]: a tile's largest).  With the weights' 2^SHIFT taken back to 2^4 a score gradient is
+// 16 p (do . v - delta) at |do| scaled to 1: normal down to 4e-6, and finite up to |do . v| of thousands.
 template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
 struct RowPrep {
   f32x2_t* rows;  // lse2, delta
@@ -417,12 +431,13 @@ __device__ __forceinline__ float ds_scale(float amax) {
 
 // dq_i = scale sum_j ds_ij k_j with ds_ij = p_ij (do_i . v_j - delta_i): the forward's walk, a query per lane, dS^T in
 // place as the operand of dQ^T = K^T dS^T.  The scores are formed again rather than handed over by the pass over keys:
-// two products more, but no sum over workgroups, whose order would change the results.
+// two products more, but no sum over workgroups, whose order would change the results.  Bound by the matrix cores: 6.0 ms
+// for one sequence of 32768, 16 heads over 4, 1110 TFLOP/s of its three products.
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* __restrict__ olo, const uint16_t* __restrict__ dout,
-                    const float* __restrict__ lse, const float* __restrict__ dlse, RowPrep w, float scale, int parts,
-                    float* __restrict__ psum, uint16_t* __restrict__ dq) {
+void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* __restrict__ olo,
+                    const uint16_t* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ dlse,
+                    RowPrep w, float scale, int parts, float* __restrict__ psum, uint16_t* __restrict__ dq) {
   constexpr int BM = NW * 32, TILE = BN * D * 2;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
   __shared__ float red[NW];
@@ -487,7 +502,8 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
       for (int i = 0; i < 4; ++i) {
         float x0, x1, y0, y1;
         unpack2<DT>(of[s][i], x0, x1);
-        const f32x2_t e = i % 2 ? __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], true) : __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], false);
+        const f32x2_t e = i % 2 ? __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], true)
+                                : __builtin_amdgcn_cvt_pk_f32_bf8(lo[s][i / 2], false);
         x0 = fmaf(e[0], 1.f / LO_SCALE, x0);
         x1 = fmaf(e[1], 1.f / LO_SCALE, x1);
         unpack2<DT>(df[s][i], y0, y1);
@@ -567,11 +583,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
   if (parts > 1) {
     if (row >= nq) return;
     float* pp = psum + (((int64_t)part * a.total_q + q0 + row) * a.hq + head) * D + 4 * hf;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *reinterpret_cast<f32x4*>(pp + 32 * d + 2 * r) = f32x4{acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f};
+    store_sums<D>(pp, acc, f);
     return;
   }
   __syncthreads();
@@ -585,7 +597,9 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
 // in.  Both accumulators and the fragments of K and V would fill all 256 registers that two waves a SIMD leave at
 // D = 128, so V waits in LDS there.  The stages of a tile are cut into `parts` equal runs, a workgroup each, where there
 // are too few tiles (the first keys of a causal sequence have many more queries than the last); the parts' sums are then
-// f32 in `psum` and added up in order by attn_sum_kernel.
+// f32 in `psum` and added up in order by attn_sum_kernel.  Bound by the matrix cores: 8.5 ms for one sequence of 32768, 16
+// heads over 4, 1030 TFLOP/s of its four products (10.5 with both fragments in registers, 75 of them spilled; 11 to 13.5
+// with one wave a SIMD, whose instructions alone outlast its products).
 constexpr int QN = 32;  // query rows per stage
 template <int D> constexpr bool V_IN_LDS = D >= 128;
 template <int D> constexpr int DKV_EU = D == 256 ? 1 : 2;  // waves per SIMD that the registers allow
@@ -736,7 +750,8 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int x = 0; x < D / 16; ++x)
-      g = mma32<DT>(lds_read16(row_step<D>(ra, x) + (R + u) * TILE), V_IN_LDS<D> ? lds_read16(row_step<D>(rv, x)) : vf[V_IN_LDS<D> ? 0 : x], g);
+      g = mma32<DT>(lds_read16(row_step<D>(ra, x) + (R + u) * TILE),
+                    V_IN_LDS<D> ? lds_read16(row_step<D>(rv, x)) : vf[V_IN_LDS<D> ? 0 : x], g);
     weigh(u, s, g, p, x);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);  // the wave with products to issue goes first (1 to 2%)
@@ -757,13 +772,8 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     if (col >= nk) return;
     const int64_t size = (int64_t)a.total_k * a.hk * D;
     float* pk = psum + 2 * part * size + at;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        *reinterpret_cast<f32x4*>(pk + 32 * d + 2 * r) = f32x4{ak[d][r] * fk, ak[d][r + 1] * fk, ak[d][r + 2] * fk, ak[d][r + 3] * fk};
-        *reinterpret_cast<f32x4*>(pk + size + 32 * d + 2 * r) = f32x4{av[d][r] * fv, av[d][r + 1] * fv, av[d][r + 2] * fv, av[d][r + 3] * fv};
-      }
+    store_sums<D>(pk, ak, fk);
+    store_sums<D>(pk + size, av, fv);
     return;
   }
   __syncthreads();
@@ -814,7 +824,8 @@ int check_shape(const char* what, const lsurge_attn_shape* s, const int32_t* cu_
                  (long long)s->total_k);
   LSURGE_REQUIRE((cu_q != nullptr) == (cu_k != nullptr), "%s: cu_q and cu_k go together", what);
   if (!cu_q)
-    LSURGE_REQUIRE(s->nseq == 0 ? s->total_q == 0 && s->total_k == 0 : s->total_q % s->nseq == 0 && s->total_k % s->nseq == 0,
+    LSURGE_REQUIRE(s->nseq == 0 ? s->total_q == 0 && s->total_k == 0
+                                : s->total_q % s->nseq == 0 && s->total_k % s->nseq == 0,
                    "%s: %lld and %lld rows are no whole number for each of %lld sequences", what, (long long)s->total_q,
                    (long long)s->total_k, (long long)s->nseq);
   LSURGE_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", what);
@@ -833,7 +844,8 @@ int plan_grid(const char* what, const lsurge_attn_shape& s, bool packed, int64_t
   LSURGE_REQUIRE(pairs * tiles < (1ll << 31), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)pairs);
   const int64_t run = pairs % 8 == 0 ? pairs / 8 : 0;
   a->heads = (int)heads, a->pairs = (int)pairs, a->tiles = (int)tiles, a->run = (int)run;
-  a->together = (int)(run * tiles <= 128 ? std::max<int64_t>(run, 1) : run % share == 0 ? share : share % run == 0 ? run : 1);
+  a->together = (int)(run * tiles <= 128 ? std::max<int64_t>(run, 1)
+                                         : run % share == 0 ? share : share % run == 0 ? run : 1);
   *grid = (unsigned)(pairs * tiles);
   return LSURGE_OK;
 }
@@ -886,17 +898,17 @@ int64_t fwd_parts(const lsurge_attn_shape& s) { return key_parts(s, s.d == 256 ?
 // keys (256 tiles, 64 stages): 314, 269, 257, 261, 288; 8 x 4096, 8 heads over 2 (2048, 64): 1361, 1477, 1546, 1613, 1889.
 int64_t dq_parts(const lsurge_attn_shape& s) { return key_parts(s, s.d == 256 ? 256 : s.d == 128 ? 512 : 1024); }
 
-#define ATTN_DISPATCH(CALL)                                                     \
-  do {                                                                          \
-    if (s->dtype == LSURGE_BF16) {                                              \
-      if (s->d == 64) { CALL(64, LSURGE_BF16); }                                \
-      else if (s->d == 128) { CALL(128, LSURGE_BF16); }                         \
-      else { CALL(256, LSURGE_BF16); }                                          \
-    } else {                                                                    \
-      if (s->d == 64) { CALL(64, LSURGE_F16); }                                 \
-      else if (s->d == 128) { CALL(128, LSURGE_F16); }                          \
-      else { CALL(256, LSURGE_F16); }                                           \
-    }                                                                           \
+#define ATTN_DISPATCH(CALL)                             \
+  do {                                                  \
+    if (s->dtype == LSURGE_BF16) {                      \
+      if (s->d == 64) { CALL(64, LSURGE_BF16); }        \
+      else if (s->d == 128) { CALL(128, LSURGE_BF16); } \
+      else { CALL(256, LSURGE_BF16); }                  \
+    } else {                                            \
+      if (s->d == 64) { CALL(64, LSURGE_F16); }         \
+      else if (s->d == 128) { CALL(128, LSURGE_F16); }  \
+      else { CALL(256, LSURGE_F16); }                   \
+    }                                                   \
   } while (0)
 
 }  // namespace
@@ -932,22 +944,22 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const int parts = (int)fwd_parts(*s);
   float* po = (float*)workspace;
   f32x4* pm = (f32x4*)(po + (size_t)parts * s->total_q * s->hq * s->d);
-#define ATTN_FWD(D, DT)                                                                                               \
-  constexpr int NW = WAVES<D>;                                                                                        \
-  unsigned grid;                                                                                                      \
+#define ATTN_FWD(D, DT)                                                                                                 \
+  constexpr int NW = WAVES<D>;                                                                                          \
+  unsigned grid;                                                                                                        \
   if (int rc = plan_grid("attn_fwd", *s, cu_q, s->hq * parts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), \
-                         &a, &grid))                                                                                  \
-    return rc;                                                                                                        \
-  if (o_lo)                                                                                                           \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, true>), dim3(grid), dim3(NW * 64), 0,  \
-                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse));         \
-  else                                                                                                                \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, false>), dim3(grid), dim3(NW * 64), 0, \
-                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)nullptr, lse));      \
-  const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                              \
-  if (parts > 1)                                                                                                      \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_join_kernel<D, DT>),                                     \
-                                                   dim3((unsigned)std::min<int64_t>(rows, 8192)), dim3(256), 0, st, a, \
+                         &a, &grid))                                                                                    \
+    return rc;                                                                                                          \
+  if (o_lo)                                                                                                             \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, true>), dim3(grid), dim3(NW * 64), 0,    \
+                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse));           \
+  else                                                                                                                  \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_kernel<D, DT, NW, false>), dim3(grid), dim3(NW * 64), 0,   \
+                                                   st, a, parts, po, pm, (uint16_t*)o, (uint8_t*)nullptr, lse));        \
+  const int64_t rows = (s->total_q * s->hq + 1024 / D - 1) / (1024 / D);                                                \
+  if (parts > 1)                                                                                                        \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_fwd_join_kernel<D, DT>),                                       \
+                                                   dim3((unsigned)std::min<int64_t>(rows, 8192)), dim3(256), 0, st, a,  \
                                                    parts, po, pm, (uint16_t*)o, (uint8_t*)o_lo, lse))
   ATTN_DISPATCH(ATTN_FWD);
 #undef ATTN_FWD
@@ -970,15 +982,15 @@ size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s) {
 
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
-                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv, void* workspace,
-                    size_t workspace_bytes, lsurge_stream_t stream) {
+                    const void* o_lo, const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv,
+                    void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
   if (int rc = check_shape("attn_bwd", s, cu_q, cu_k, scale)) return rc;
   LSURGE_REQUIRE(q && k && v && workspace, "attn_bwd: null pointer");
   const size_t need = lsurge_attn_bwd_workspace_bytes(s);
   if (workspace_bytes < need)
     return lsurge::set_error(LSURGE_ERR_WORKSPACE, "attn_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
-  LSURGE_REQUIRE(((uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) %
-                         16 == 0,
+  LSURGE_REQUIRE(((uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv |
+                  (uintptr_t)workspace) % 16 == 0,
                  "attn_bwd: buffers must be 16-byte aligned");
   if (s->total_q) {
     LSURGE_REQUIRE(o && lse && dout && dq, "attn_bwd: null pointer");
@@ -997,38 +1009,38 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   float* psum = (float*)((char*)workspace + prep_bytes(s));
   const int parts = (int)dkv_parts(*s), qparts = (int)dq_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
-#define ATTN_BWD(D, DT)                                                                                                  \
-  constexpr int NW = WAVES<D>;                                                                                           \
-  AttnArgs ak = a;                                                                                                       \
-  unsigned gq = 0, gk = 0;                                                                                               \
-  if (s->total_q)                                                                                                        \
-    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hq * qparts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), &a,    \
-                           &gq))                                                                                         \
-      return rc;                                                                                                         \
-  if (s->total_k)                                                                                                        \
-    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hk * parts, 1, tile_slots(*s, cu_q, s->total_k, NW * 32), &ak, &gk)) \
-      return rc;                                                                                                         \
-  w.nblk = (int)(gq / (s->hq * qparts));                                                                                            \
-  const auto sum_grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, 4096)); };             \
-  if (gq) {                                                                                                              \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,       \
-                                                   (const uint16_t*)o, (const uint8_t*)o_lo, g, lse, dlse, w, scale,     \
-                                                   qparts, psum,                                                         \
-                                                   (uint16_t*)dq));                                                      \
-    const int64_t size = s->total_q * s->hq * D;                                                                         \
-    if (qparts > 1)                                                                                                      \
-      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(size), dim3(256), 0, st, psum,      \
-                                                     qparts, 1, size, s->hq * D, cu_q, a.nseq, a.total_q,                \
-                                                     (uint16_t*)dq, (uint16_t*)dq));                                     \
-  }                                                                                                                      \
-  if (gk) {                                                                                                              \
-    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, ak, g,  \
-                                                   w, scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                \
-    const int64_t size = s->total_k * s->hk * D;                                                                         \
-    if (parts > 1)                                                                                                       \
-      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(2 * size), dim3(256), 0, st, psum,  \
-                                                     parts, 2, size, s->hk * D, cu_k, a.nseq, a.total_k,                 \
-                                                     (uint16_t*)dk, (uint16_t*)dv));                                     \
+#define ATTN_BWD(D, DT)                                                                                                    \
+  constexpr int NW = WAVES<D>;                                                                                             \
+  AttnArgs ak = a;                                                                                                         \
+  unsigned gq = 0, gk = 0;                                                                                                 \
+  if (s->total_q)                                                                                                          \
+    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hq * qparts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), \
+                           &a, &gq))                                                                                       \
+      return rc;                                                                                                           \
+  if (s->total_k)                                                                                                          \
+    if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hk * parts, 1, tile_slots(*s, cu_q, s->total_k, NW * 32), &ak, &gk))   \
+      return rc;                                                                                                           \
+  w.nblk = (int)(gq / (s->hq * qparts));                                                                                   \
+  const auto sum_grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, 4096)); };              \
+  if (gq) {                                                                                                                \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,         \
+                                                   (const uint16_t*)o, (const uint8_t*)o_lo, g, lse, dlse, w, scale,       \
+                                                   qparts, psum,                                                           \
+                                                   (uint16_t*)dq));                                                        \
+    const int64_t size = s->total_q * s->hq * D;                                                                           \
+    if (qparts > 1)                                                                                                        \
+      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(size), dim3(256), 0, st, psum,        \
+                                                     qparts, 1, size, s->hq * D, cu_q, a.nseq, a.total_q,                  \
+                                                     (uint16_t*)dq, (uint16_t*)dq));                                       \
+  }                                                                                                                        \
+  if (gk) {                                                                                                                \
+    LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dkv_kernel<D, DT, NW>), dim3(gk), dim3(NW * 64), 0, st, ak, g,    \
+                                                   w, scale, parts, psum, (uint16_t*)dk, (uint16_t*)dv));                  \
+    const int64_t size = s->total_k * s->hk * D;                                                                           \
+    if (parts > 1)                                                                                                         \
+      LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_sum_kernel<DT>), sum_grid(2 * size), dim3(256), 0, st, psum,    \
+                                                     parts, 2, size, s->hk * D, cu_k, a.nseq, a.total_k,                   \
+                                                     (uint16_t*)dk, (uint16_t*)dv));                                       \
   }
   ATTN_DISPATCH(ATTN_BWD);
 #undef ATTN_BWD

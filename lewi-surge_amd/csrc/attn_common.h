@@ -13,7 +13,6 @@ using lsgemm::u32x2;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-typedef __bf16 s16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -60,7 +59,8 @@ __device__ __forceinline__ float add2(uint32_t v, float c) {
   if constexpr (DT == LSURGE_F16)
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, v), f16x2_t{(_Float16)1, (_Float16)1}, c, false);
   else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2_t, v), __builtin_bit_cast(s16x2_t, 0x3f803f80u), c, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, v), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c,
+                                           false);
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
