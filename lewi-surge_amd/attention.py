@@ -44,8 +44,9 @@ def _check_heads(what, q_heads, kv_heads, d, *ts):
 
 def _check_dtype(what, *ts):
     dt = ts[0].dtype
-    if dt is not torch.bfloat16 and dt is not torch.float16 or any(t.dtype is not dt for t in ts):
-        raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
+    for t in ts:
+        if t.dtype is not dt or dt is not torch.bfloat16 and dt is not torch.float16:
+            raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
 
 
 def _check_index(what, name, t, shape):
@@ -55,13 +56,19 @@ def _check_index(what, name, t, shape):
 
 
 def _call(what, device, fn, *args):
-    """fn(*args, the current stream of `device`), with `device` current while its kernels are launched."""
+    """fn(*args, the current stream of `device`), with `device` current while its kernels are launched.  The stream's bare
+    handle: a Stream object around it costs 2 us, as much as a short call's launch."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        rc = fn(*args, L.stream(device))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, L.stream(device))
+            rc = fn(*args, stream)
     L.check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _scale(what, scale, d):
@@ -88,7 +95,7 @@ def _aligned(t):
 
 def _rows_arg(t):
     row, head = (t.shape[1] * t.shape[2], t.shape[2]) if t.is_contiguous() else t.stride()[:2]
-    return ctypes.byref(L.AttnRows(t.data_ptr(), row, head))
+    return L.AttnRows(t.data_ptr(), row, head)
 
 
 def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training=False):
@@ -104,8 +111,8 @@ def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training=False):
     lib, arg = L.lib(), ctypes.byref(shape)
     nbytes = lib.lsurge_attn_fwd_workspace_bytes(arg)
     ws = L.workspace(nbytes, q.device) if nbytes else None
-    _call("attn_fwd", q.device, lib.lsurge_attn_fwd, arg, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q), L.ptr(cu_k),
-          scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(ws), nbytes)
+    _call("attn_fwd", q.device, lib.lsurge_attn_fwd, arg, _rows_arg(q), _rows_arg(k), _rows_arg(v), _ptr(cu_q), _ptr(cu_k),
+          scale, _ptr(o), _ptr(o_lo), _ptr(lse), _ptr(ws), nbytes)
     return o, lse, (q, k, v, o_lo), shape
 
 
@@ -132,9 +139,9 @@ class _AttnFn(torch.autograd.Function):
         lib = L.lib()
         shape = ctypes.byref(ctx.shape)
         ws = L.workspace(lib.lsurge_attn_bwd_workspace_bytes(shape), q.device)
-        _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), L.ptr(cu_q),
-              L.ptr(cu_k), ctx.scale, L.ptr(o), L.ptr(o_lo), L.ptr(lse), L.ptr(do), L.ptr(dlse), L.ptr(dq), L.ptr(dk),
-              L.ptr(dv), L.ptr(ws), ws.numel())
+        _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), _ptr(cu_q),
+              _ptr(cu_k), ctx.scale, _ptr(o), _ptr(o_lo), _ptr(lse), _ptr(do), _ptr(dlse), _ptr(dq), _ptr(dk),
+              _ptr(dv), _ptr(ws), ws.numel())
         return dq, dk, dv, None, None, None, None
 
 
@@ -214,7 +221,7 @@ def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
     lens = _check_index(what, "seq_lens", seq_lens, (nseq,))
     arg = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), *_cache_strides(what, k_cache), *_cache_strides(what, v_cache),
                     table.data_ptr(), most, lens.data_ptr(), pages, size, most, heads, d, L.dt(k_cache))
-    return ctypes.byref(arg), (table, lens)
+    return arg, (table, lens)
 
 
 def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
@@ -237,7 +244,7 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
         raise ValueError(f"{what}: {k.shape[0]} tokens for {nseq} sequences need cu_seqlens")
     k, v = _rows(k), _rows(v)
     _call("kv_append", k.device, L.lib().lsurge_kv_append, arg, _rows_arg(k), _rows_arg(v), k.shape[0], nseq,
-          L.ptr(cu_seqlens))
+          _ptr(cu_seqlens))
     del keep
 
 
@@ -263,7 +270,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, retur
     lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib = L.lib()
     ws = L.workspace(lib.lsurge_paged_attn_workspace_bytes(n, hq, d), q.device)
-    _call("paged_attn", q.device, lib.lsurge_paged_attn, arg, _rows_arg(q), n, hq, scale, L.ptr(o), L.ptr(lse), L.ptr(ws),
+    _call("paged_attn", q.device, lib.lsurge_paged_attn, arg, _rows_arg(q), n, hq, scale, _ptr(o), _ptr(lse), _ptr(ws),
           ws.numel())
     del keep
     return (o, lse) if return_lse else o
