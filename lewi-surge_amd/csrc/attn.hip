@@ -841,7 +841,8 @@ int64_t tile_slots(const lsurge_attn_shape& s, bool packed, int64_t total, int64
 int plan_grid(const char* what, const lsurge_attn_shape& s, bool packed, int64_t heads, int64_t share, int64_t tiles,
               AttnArgs* a, unsigned* grid) {
   const int64_t pairs = (packed ? 1 : s.nseq) * heads;
-  LSURGE_REQUIRE(pairs * tiles < (1ll << 31), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)pairs);
+  // a launch holds less than 2^32 threads, 256 a workgroup
+  LSURGE_REQUIRE(pairs * tiles < (1ll << 24), "%s: %lld tiles of %lld heads", what, (long long)tiles, (long long)pairs);
   const int64_t run = pairs % 8 == 0 ? pairs / 8 : 0;
   a->heads = (int)heads, a->pairs = (int)pairs, a->tiles = (int)tiles, a->run = (int)run;
   a->together = (int)(run * tiles <= 128 ? std::max<int64_t>(run, 1)
@@ -863,8 +864,7 @@ AttnArgs make_args(const lsurge_attn_shape& s, const lsurge_attn_rows& q, const 
   return a;
 }
 
-// waves of a workgroup: 8 where 256 registers a lane hold a wave's operands and sums, 4 (512 registers) at D = 256
-template <int D> constexpr int WAVES = 4;
+constexpr int WAVES = 4;  // of a workgroup, 32 rows each (8 were as fast or slower at every head dim)
 
 // Parts that the stages of a tile of keys are cut into in attn_dkv_kernel, by the sizes that the host knows (the
 // sequences' own lengths are on the device): as many as give every place for a workgroup two of them, so that the ones
@@ -945,7 +945,7 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   float* po = (float*)workspace;
   f32x4* pm = (f32x4*)(po + (size_t)parts * s->total_q * s->hq * s->d);
 #define ATTN_FWD(D, DT)                                                                                                 \
-  constexpr int NW = WAVES<D>;                                                                                          \
+  constexpr int NW = WAVES;                                                                                             \
   unsigned grid;                                                                                                        \
   if (int rc = plan_grid("attn_fwd", *s, cu_q, s->hq * parts, s->hq / s->hk, tile_slots(*s, cu_q, s->total_q, NW * 32), \
                          &a, &grid))                                                                                    \
@@ -1010,7 +1010,7 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const int parts = (int)dkv_parts(*s), qparts = (int)dq_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
 #define ATTN_BWD(D, DT)                                                                                                    \
-  constexpr int NW = WAVES<D>;                                                                                             \
+  constexpr int NW = WAVES;                                                                                                \
   AttnArgs ak = a;                                                                                                         \
   unsigned gq = 0, gk = 0;                                                                                                 \
   if (s->total_q)                                                                                                          \

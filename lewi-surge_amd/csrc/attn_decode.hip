@@ -513,7 +513,8 @@ int lsurge_paged_attn(const lsurge_kv_cache* c, const lsurge_attn_rows* q, int64
   a.pm = a.po + (size_t)DECODE_GRID * 2 * 16 * c->d;
   a.shares = (int32_t*)((char*)workspace + decode_parts_bytes(c->d));
   const int64_t rows = nseq * hq;
-  LSURGE_REQUIRE(rows < (1ll << 31), "paged_attn: %lld sequences of %lld heads", (long long)nseq, (long long)hq);
+  // the join's launch holds less than 2^32 threads, 256 a row
+  LSURGE_REQUIRE(rows < (1ll << 24), "paged_attn: %lld sequences of %lld heads", (long long)nseq, (long long)hq);
   hipStream_t st = (hipStream_t)stream;
 #define DECODE(D, DT)                                                                                              \
   LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_decode_kernel<D, DT>), dim3(a.grid), dim3(DT_THREADS), 0, st, a)); \

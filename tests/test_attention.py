@@ -243,3 +243,17 @@ def test_c_abi_cache_refusals():
     assert attn(_kv(max_pages=1 << 28, table_stride=1 << 28)) == -1
     assert put(_kv(), rows=3) == -1 and put(_kv(), k=None) == -1
     assert attn(_kv(), n=0) == 0 and put(_kv(), rows=0, n=0) == 0
+
+
+def test_c_abi_refuses_grids_past_the_launch_limit():
+    """Workgroups of 256 threads, less than 2^32 threads a launch: 2^24 tiles times heads are refused before anything runs."""
+    lib = L.lib()
+    for kw in (dict(hq=64), dict(hq=4, nseq=1 << 22)):
+        s = _shape(total_q=1 << 29, total_k=1 << 29, **kw)
+        assert _fwd(s) == -1 and b"tiles" in lib.lsurge_last_error()
+        r = ctypes.byref(L.AttnRows(256, 512, 64))
+        assert lib.lsurge_attn_bwd(ctypes.byref(s), r, r, r, None, None, 1.0, FAKE, None, FAKE, FAKE, None, FAKE, FAKE, FAKE,
+                                   FAKE, 1 << 50, None) == -1 and b"tiles" in lib.lsurge_last_error()
+    c = _kv()
+    assert lib.lsurge_paged_attn(ctypes.byref(c), ctypes.byref(L.AttnRows(256, 512, 64)), 1 << 22, 4, 1.0, FAKE, None, FAKE,
+                                 1 << 50, None) == -1 and b"sequences" in lib.lsurge_last_error()

@@ -195,6 +195,51 @@ def test_extreme_scores(dev):
     assert torch.equal(o[:, :150], base[:, :150]) and o[:, 150:].isnan().all()
 
 
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 64), (F16, 128), (BF16, 256)])
+def test_other_sequences_never_reach(dt, D, dev):
+    """NaN and infinities everywhere in one sequence and behind the last leave the others' bits alone, gradients too."""
+    gen = torch.Generator().manual_seed(13)
+    lens, tail = [70, 150, 33, 1, 64], 50
+    a, b = sum(lens[:1]), sum(lens[:2])
+    t = [_randn(gen, (sum(lens) + tail, h, D), dt, dev) for h in (4, 2, 2, 4)]  # q, k, v, do
+    bad = [x.clone() for x in t]
+    for i, x in enumerate(bad):
+        x[a:b] = float("nan") if i % 2 else float("inf")
+        x[sum(lens):] = float("nan")
+    out = []
+    for q, k, v, do in (t, bad):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        o, lse = A.causal_attention(*leaves, _ends(lens, dev), return_lse=True)
+        out.append([o.detach(), lse.detach(), *torch.autograd.grad(o, leaves, do)])
+    for name, x, y in zip(("o", "lse", "dq", "dk", "dv"), *out):
+        assert torch.equal(x[:a], y[:a]) and torch.equal(x[b:], y[b:]), name
+        assert name == "lse" or not y[sum(lens):].any(), name
+
+
+def test_rows_past_32_bits(dev):
+    """Query rows, outputs and gradients of more than 2^31 elements: the last sequences are as if they were alone."""
+    lens = [512] * 2049 + [300, 77]
+    n, last, D = sum(lens), 377, 128
+    q, do = (torch.zeros((n, 16, D), dtype=BF16, device=dev) for _ in range(2))
+    k, v = (torch.zeros((n, 1, D), dtype=BF16, device=dev) for _ in range(2))
+    gen = torch.Generator().manual_seed(14)
+    part = [_randn(gen, (last, h, D), BF16, dev) for h in (16, 1, 1, 16)]
+    for big, small in zip((q, k, v, do), part):
+        big[-last:] = small
+    assert q.numel() > 2 ** 31
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    o = A.causal_attention(*leaves, _ends(lens, dev))
+    got = [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    a = 0
+    for m in lens[-2:]:
+        one = [_np(x[a:a + m]) for x in part]
+        want = [ao.attention(*one[:3], D ** -0.5)[0], *ao.attention_bwd(*one, D ** -0.5)]
+        bound = ao.bounds(*one[:3], D ** -0.5, HALF_STEP[BF16], do=one[3])
+        for name, x, y, e in zip(("o", "dq", "dk", "dv"), got, want, [bound[0], *bound[2:]]):
+            _within(x[x.shape[0] - last + a:][:m], y, e, name)
+        a += m
+
+
 def test_repeats_bitwise_on_another_stream(dev):
     gen = torch.Generator().manual_seed(11)
     lens = [513, 77, 1024]
@@ -362,6 +407,22 @@ def test_decode_values_behind_a_masked_key(dev):
     vc[table[0, 1].item(), 3] = float("inf")
     o = A.paged_attention(_randn(gen, (1, 1, 64), BF16, dev), kc, vc, table, sl)
     assert (o == float("inf")).all()
+
+
+def test_decode_shared_pages(dev):
+    """Sequences that share their first pages, and one that names a page twice, read what each of their entries names."""
+    gen = torch.Generator().manual_seed(15)
+    kc, vc = (_randn(gen, (6, 2, 32, 128), BF16, dev).transpose(1, 2) for _ in range(2))
+    table = torch.tensor([[0, 1, 2], [0, 1, 3], [4, 4, 4]], dtype=torch.int32, device=dev)
+    lens = [90, 70, 96]
+    q = _randn(gen, (3, 8, 128), BF16, dev)
+    o, lse = A.paged_attention(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=dev), return_lse=True)
+    for b, n in enumerate(lens):
+        k, v = (_np(torch.cat([c[i] for i in table[b].tolist()])[:n]) for c in (kc, vc))
+        one, m = (_np(q[b:b + 1]), k, v, 128 ** -0.5), np.ones((1, n), bool)
+        for name, x, y, e in zip(("o", "lse"), (o[b:b + 1], lse[b:b + 1]), ao.attention(*one, mask=m),
+                                 ao.bounds(*one, 2.0 ** -8, mask=m)):
+            _within(x, y, e, f"{name} {b}")
 
 
 def test_offsets_past_32_bits(dev):
