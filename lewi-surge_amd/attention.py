@@ -157,7 +157,8 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
     last sequence give zeros and get zero gradients.  A masked key never counts, whatever k holds there; a value of v that is
     not finite may also reach queries up to 62 before the first that sees it (its weight there is 0, and 0 x inf is NaN), and
     in the backward any input that is not finite gradients of rows up to 95 away.  Strides are free as long as the last axis
-    is contiguous: q, k and v may be views of one projection's output."""
+    is contiguous: q, k and v may be views of one projection's output.  While a training step is captured in a graph no eager
+    autograd graph of the same leaves may live (torch's accumulators of those leaves belong to the other stream)."""
     what = "causal_attention"
     if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape or k.shape[-1] != q.shape[-1]:
         raise ValueError(f"{what}: q [B, Tq, H, D] or [Tq, H, D], k and v alike with their own rows and heads (got "
