@@ -199,7 +199,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x4* __res
   const int ln = lane & 31, hf = lane >> 5;
   const int group = a.hq / a.hk;
   int sq, unit, slot;  // unit: key head, part, head of the group, so that the heads that share keys stay together
-  head_tile(a, false, sq, unit, slot);
+  head_tile(a, a.cu_q && a.nseq < IN_A_ROW, sq, unit, slot);
   const int kvh = unit / (parts * group), part = parts == 1 ? 0 : unit / group % parts, head = kvh * group + unit % group;
   const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
   if (pl.end + (int64_t)slot * BM < a.total_q && part == 0) {  // the slots cover the rows behind the last sequence too
@@ -445,7 +445,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
   const int ln = lane & 31, hf = lane >> 5;
   const int group = a.hq / a.hk;
   int sq, unit, slot;
-  head_tile(a, false, sq, unit, slot);
+  head_tile(a, a.cu_q && a.nseq < IN_A_ROW, sq, unit, slot);
   const int kvh = unit / (parts * group), part = parts == 1 ? 0 : unit / group % parts, head = kvh * group + unit % group;
   const Place pl = find_tile<BM, false>(a.cu_q, a.cu_k, a.nseq, a.total_q, a.total_k, sq, slot, lane);
   if (pl.end + (int64_t)slot * BM < a.total_q && part == 0) {

@@ -155,14 +155,28 @@ __device__ __forceinline__ u32x4 lds_read_col(uint32_t a) {
 // held to [0, total], so that no table makes a kernel read or write outside its rows.
 __device__ __forceinline__ int cu_at(const int32_t* cu, int i, int total) { return min(max(cu[i], 0), total); }
 
-// Tile t of the rows: sequence s owns the tiles from cu[s] / B + s, which leaves it at least ceil(rows / B).  A packed
-// sequence is found by a 64-way search; up to 63 sequences all ends are read at once, and one trip to memory is all that a
-// workgroup waits for before its first rows.  Dense: tile t of sequence `seq`.
+// Tile t of the rows.  Up to 63 sequences: the tiles in a row, the largest of a sequence first, and what a launch has more
+// of slots comes last; all ends are read at once, one trip to memory.  From 64 on sequence s owns the tiles from
+// cu[s] / B + s, which leaves it at least ceil(rows / B), and is found by a 64-way search (with few sequences too: 24 prompts
+// 182 us against 176 so, 3 prompts after 20000 keys 225 and 209, 24 prompts of 1024 146 and 149).  Tiles of all sequences by
+// size, in phases of an octave of keys or half one, were no faster: 179 to 188, 204, 151 to 159.  Dense: tile t of sequence
+// `seq`.
+constexpr int IN_A_ROW = 64;  // fewer sequences than this
 struct Place {
   int seq, tile;          // sequence (-1: none) and its tile
   int q0, nq, k0, nk;     // its rows
   int64_t end;            // the first row behind the last sequence
 };
+// sums over the lanes up to each
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // the lane 1, 2, 4, 8 before it in a row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last lane of row 0 to 1, of 2 to 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // of row 1 to 2 and 3
+  return v;
+}
 template <int B, bool KEYS>  // tiles of the keys, or of the queries
 __device__ __forceinline__ Place find_tile(const int32_t* cu_q, const int32_t* cu_k, int nseq, int total_q, int total_k,
                                            int seq, int t, int lane) {
@@ -179,15 +193,20 @@ __device__ __forceinline__ Place find_tile(const int32_t* cu_q, const int32_t* c
   const int32_t* cu = KEYS ? cu_k : cu_q;
   const int total = KEYS ? total_k : total_q;
   int q1, k1;
-  if (nseq < 64) {
-    const int i = min(lane, nseq), eq = cu_at(cu_q, i, total_q), ek = cu_at(cu_k, i, total_k), e = KEYS ? ek : eq;
-    p.end = __builtin_amdgcn_readlane(e, nseq);
-    const int c = __popcll(__ballot(lane < nseq && e / B + lane <= t));
-    if (c == 0) return p;
-    p.seq = c - 1;
-    p.tile = t - (__builtin_amdgcn_readlane(e, p.seq) / B + p.seq);
-    p.q0 = __builtin_amdgcn_readlane(eq, p.seq), q1 = __builtin_amdgcn_readlane(eq, c);
-    p.k0 = __builtin_amdgcn_readlane(ek, p.seq), k1 = __builtin_amdgcn_readlane(ek, c);
+  if (nseq < IN_A_ROW) {
+    const int i = min(lane, nseq), j = min(lane + 1, nseq);
+    const int eq = cu_at(cu_q, i, total_q), fq = cu_at(cu_q, j, total_q);
+    const int ek = cu_at(cu_k, i, total_k), fk = cu_at(cu_k, j, total_k);
+    p.end = __builtin_amdgcn_readlane(KEYS ? ek : eq, nseq);
+    const int nt = (max(0, KEYS ? fk - ek : fq - eq) + B - 1) / B;  // 0 from lane nseq on
+    const int upto = wave_scan(nt);
+    const int s = __popcll(__ballot(upto <= t));
+    if (s >= nseq) return p;
+    p.seq = s;
+    const int rest = __builtin_amdgcn_readlane(upto, s) - t;  // tiles from this one on
+    p.tile = KEYS ? __builtin_amdgcn_readlane(nt, s) - rest : rest - 1;
+    p.q0 = __builtin_amdgcn_readlane(eq, s), q1 = __builtin_amdgcn_readlane(fq, s);
+    p.k0 = __builtin_amdgcn_readlane(ek, s), k1 = __builtin_amdgcn_readlane(fk, s);
   } else {
     p.end = cu_at(cu, nseq, total);
     int lo = 0, n = nseq;
