@@ -87,12 +87,8 @@ void attn_decode_kernel(DecodeArgs a) {
     if (i == 0) first_len = n;
     mine += units_of(n);
   }
-  int64_t pre = mine;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t y = __shfl_up(pre, s, 64);
-    if (lane >= s) pre += y;
-  }
+  // below 2^39 (2^16 sequences a slab, 2^23 units each): scanned in two halves that cannot overflow
+  int64_t pre = ((int64_t)wave_scan((int)(mine >> 20)) << 20) + wave_scan((int)mine & 0xfffff);
   if (lane == 63) wsum[wave] = pre;
   __syncthreads();
   int64_t total = 0;
