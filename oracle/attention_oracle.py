@@ -1,6 +1,6 @@
 """CPU oracle of the softmax attention operators (numpy, float64), with first-order error bounds of 16-bit kernels.
 
-TEST INFRASTRUCTURE ONLY: only `tests/` may import this module, as the checker.  No product code calls it.
+TEST INFRASTRUCTURE ONLY: only `tests/` may import this module.  No product code calls it.
 
 One sequence: q [nq, Hq, D], k, v [nk, Hk, D]; query i sees the keys j <= i + nk - nq, head h reads key head
 h // (Hq // Hk).  s = scale q k^T, w = softmax(s) over the visible keys (all zero for a row that sees none), o = w v,
