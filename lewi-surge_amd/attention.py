@@ -49,6 +49,11 @@ def _check_dtype(what, *ts):
             raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
 
 
+def _check_no_grad(what, *ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
+
+
 def _check_index(what, name, t, shape):
     if t.dtype is not torch.int32 or t.shape != shape:
         raise ValueError(f"{what}: {name} must be int32 of shape {shape} (got {t.dtype}, {tuple(t.shape)})")
@@ -230,13 +235,15 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
     (int32 [sequences + 1]) the rows cu_seqlens[b] .. cu_seqlens[b + 1] of sequence b.  They become the last of its
     seq_lens[b] tokens (int32, the new ones counted); token t goes to page page_table[b, t // page_size], slot
     t % page_size.  Nothing is written for a sequence of length 0 without cu_seqlens, for rows behind the last sequence, or
-    where the table names no page.  Two sequences that share a page must not write to the same place of it."""
+    where the table names no page.  Two sequences that share a page must not write to the same place of it.  No gradient
+    passes through a cache; a backward that saved it before the call raises, as after any write in place."""
     what = "append_kv"
     if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or k.shape[1:] != k_cache.shape[2:]:
         raise ValueError(f"{what}: k and v must be [rows, kv_heads, head_dim] of the caches (got {tuple(k.shape)}, "
                          f"{tuple(v.shape)}, caches {tuple(k_cache.shape)})")
     _check_heads(what, k.shape[1], k.shape[1], k.shape[2], k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _check_dtype(what, k, v, k_cache, v_cache)
+    _check_no_grad(what, k, v, k_cache, v_cache)
     arg, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
     nseq = page_table.shape[0]
     if cu_seqlens is not None:
@@ -246,6 +253,7 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
     k, v = _rows(k), _rows(v)
     _call("kv_append", k.device, L.lib().lsurge_kv_append, arg, _rows_arg(k), _rows_arg(v), k.shape[0], nseq,
           _ptr(cu_seqlens))
+    torch.autograd.graph.increment_version((k_cache, v_cache))
     del keep
 
 
@@ -259,8 +267,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, retur
     if q.dim() != 3 or k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3] or q.shape[0] != page_table.shape[0]:
         raise ValueError(f"{what}: q must be [sequences, heads, head_dim] (got {tuple(q.shape)}, caches "
                          f"{tuple(k_cache.shape)}, page_table {tuple(page_table.shape)})")
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
+    _check_no_grad(what, q, k_cache, v_cache)
     n, hq, d = q.shape
     _check_heads(what, hq, k_cache.shape[2], d, q, k_cache, v_cache, page_table, seq_lens)
     _check_dtype(what, q, k_cache, v_cache)

@@ -257,3 +257,13 @@ def test_c_abi_refuses_grids_past_the_launch_limit():
     c = _kv()
     assert lib.lsurge_paged_attn(ctypes.byref(c), ctypes.byref(L.AttnRows(256, 512, 64)), 1 << 22, 4, 1.0, FAKE, None, FAKE,
                                  1 << 50, None) == -1 and b"sequences" in lib.lsurge_last_error()
+
+
+def test_gradients_are_refused_at_the_cache(monkeypatch):
+    _fake(monkeypatch)
+    kc, vc, table, lens = _cache()
+    k = _t(2, 2, 64)
+    for args in ((kc, vc, k.clone().requires_grad_(True), k), (kc, vc, k, k.clone().requires_grad_(True)),
+                 (kc.detach().requires_grad_(True), vc, k, k), (kc, vc.detach().requires_grad_(True), k, k)):
+        with pytest.raises(ValueError, match="no gradient"):
+            A.append_kv(args[0], args[1], table, lens, *args[2:])

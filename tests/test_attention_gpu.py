@@ -477,6 +477,18 @@ def test_append_one_token_each(dev):
     assert torch.equal(kc.nan_to_num(7), wk.nan_to_num(7)) and torch.equal(vc.nan_to_num(7), wv.nan_to_num(7))
 
 
+def test_append_is_a_write_in_place(dev):
+    """A backward that saved the cache before a token was appended raises instead of using the new values."""
+    gen = torch.Generator().manual_seed(16)
+    kc, vc, table, sl, _, _ = make_cache(gen, [20], 16, 1, 64, BF16, dev)
+    w = torch.ones(64, dtype=BF16, device=dev, requires_grad=True)
+    y = (kc * w).sum()
+    k = _randn(gen, (1, 1, 64), BF16, dev)
+    A.append_kv(kc, vc, table, sl, k, k)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_prompt_then_tokens(dev):
     """The operators as a serving program runs them: packed prompts through causal_attention and into the cache, then
     tokens one by one, each step captured once and replayed; every token's output equals whole-sequence attention."""
