@@ -200,6 +200,8 @@ void attn_decode_kernel(DecodeArgs a) {
     f32x4 acc[VE];
 #pragma unroll
     for (int t = 0; t < VE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // m: the largest score so far times the scale, as rounded.  Weights, sums and the join all take this one value as their
+    // base: the product formed anew inside an fma would be the unrounded one, a factor of 2^(its rounding) for every tile.
     float m = -INFINITY, l = 0.f;
 
     auto compute = [&](int key0, Tile& x, auto&& after_scores) {
@@ -223,9 +225,9 @@ void attn_decode_kernel(DecodeArgs a) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }));
-      const float mc = mx == -INFINITY ? 0.f : mx * a.scale2;
-      const float alpha = exp2_hw(m * a.scale2 - mc);
+      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }) * a.scale2);
+      const float mc = mx == -INFINITY ? 0.f : mx;
+      const float alpha = exp2_hw(m - mc);  // 1 where the largest score stays
       m = mx;
       float sum = 0.f;
 #pragma unroll
@@ -302,12 +304,12 @@ void attn_decode_kernel(DecodeArgs a) {
       float mm = sm[0][h];
 #pragma unroll
       for (int w = 1; w < DW; ++w) mm = fmaxf(mm, sm[w][h]);
-      const float mc = mm == -INFINITY ? 0.f : mm * a.scale2;
+      const float mc = mm == -INFINITY ? 0.f : mm;
       float ll = 0.f;
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < DW; ++w) {
-        const float f = exp2_hw(sm[w][h] * a.scale2 - mc);
+        const float f = exp2_hw(sm[w][h] - mc);
         ll += f * sl[w][h];
         x += f * *reinterpret_cast<const f32x4*>(&so[w][h][d]);
       }

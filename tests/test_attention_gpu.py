@@ -532,3 +532,37 @@ def test_prompt_then_tokens(dev):
     for b, t in enumerate(qkv):
         one = (_np(t[:, :hq]), _np(t[:, hq:hq + hk]), _np(t[:, hq + hk:]), D ** -0.5)
         _within(_np(torch.cat(got[b])), ao.attention(*one)[0], ao.bounds(*one, 2.0 ** -8)[0], f"sequence {b}")
+
+
+def shared_cache(k, v, size, rows, dt, dev):
+    """One sequence's tokens k, v [n, Hkv, D] in a cache whose table gives its pages to every one of `rows` sequences."""
+    n, hk, D = k.shape
+    pages = -(-n // size)
+    kc, vc = A.alloc_kv_cache(pages + 1, size, hk, D, dt, dev)
+    perm = torch.randperm(pages + 1, generator=torch.Generator().manual_seed(n))[:pages]
+    where = (perm.to(dev)[torch.arange(n, device=dev) // size], torch.arange(n, device=dev) % size)
+    kc[where], vc[where] = k.to(dev), v.to(dev)
+    return kc, vc, perm.to(torch.int32).to(dev).expand(rows, pages)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_equal_scores_over_many_units(dt, D, dev):
+    """Every weight of a row is the same, whatever part of the sequence it comes from: keys all alike, values 1 in the first
+    half and -1 in the second, hundreds of units of one sequence in a share.  Then o = 0 and lse = s + log n but for the f32
+    sums: a share adds up 512 units of 8 keys a lane and joins 16 lanes' and 4 waves' sums, 540 roundings of 2^-24 at most,
+    each relative to at most the whole; s = 3.4 (D = 64) to 6.8 times a power of two is exact, and its product with the
+    scale and log2 e, the sum of logarithms, its factor log 2 are rounded to half of 2^-23 |lse|, four times."""
+    n, rows = 65536, 768
+    k = torch.full((n, 1, D), 1.6875).to(dt)
+    v = torch.ones((n, 1, D)).to(dt)
+    v[n // 2:] = -1
+    kc, vc, table = shared_cache(k, v, 64, rows, dt, dev)
+    level = torch.tensor([0.34375, 2.203125, 5.40625, -3.3125])  # scores of some tens of nats, both signs
+    q = level.repeat(rows // 4).view(-1, 1, 1).expand(rows, 1, D).to(dt).to(dev)
+    o, lse = A.paged_attention(q, kc, vc, table, torch.full((rows,), n, dtype=torch.int32, device=dev), scale=0.125,
+                               return_lse=True)
+    s = 0.125 * D * 1.6875 * level.double().numpy()
+    want = np.tile(s + np.log(n), rows // 4)[:, None]
+    _within(lse, want, 540 * 2.0 ** -24 + 4 * 2.0 ** -24 * np.abs(want), "lse")
+    _within(o, np.zeros(o.shape), np.full(o.shape, 540 * 2.0 ** -24), "o")
