@@ -404,29 +404,50 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnArgs a, int part
 // ------------------------------------------------------------------------------------ backward
 // What the passes need of each query, laid out [hq][total_q]: lse2 = lse log2(e) (+inf for a row with no key, whose weights
 // 2^(s - lse2) are then 0) and delta = do . o - dlse, found by the pass over queries, whose lanes hold do already, and kept
-// for the pass over keys.  f16 values have few exponent bits: weights of long rows (2^-15 and less) and their products with
-// small gradients would be subnormal, so the f16 passes work on weights 2^SHIFT times too large (lse2 smaller by SHIFT)
-// and on gradients scaled by powers of two, exactly undone in f32 at the end: a row's own, from the largest |do| of the
-// row, in the pass over queries; the group's, from the largest of all rows, in the pass over keys, which sums over the rows
-// (amax [hq][nblk]: a tile's largest).  With the weights' 2^SHIFT taken back to 2^4 a score gradient is
-// 16 p (do . v - delta) at |do| scaled to 1: normal down to 4e-6, and finite up to |do . v| of thousands.
+// for the pass over keys.
+//
+// f16 values have few exponent bits: weights of long rows (2^-15 and less) and their products with small gradients would be
+// subnormal, so the f16 passes work on weights 2^SHIFT times too large (lse2 smaller by SHIFT) and on score gradients scaled
+// by a power of two, undone in f32 at the end.  The scale is a query's own in the pass over queries and a key's own in the
+// pass over keys: a lane's, both times.  It starts from the largest upstream gradient, the query's or that of all the
+// queries which see the workgroup's keys (amax: a tile's largest; other sequences have no part in it, nor do infinities),
+// which becomes 1 to 2, and is lowered whenever a score gradient would pass f16's largest (fit_f16).  What is lost is half of
+// f16's least subnormal, 2^-25, at that scale: 2^-35 of the largest upstream gradient, or 2^-25 of the largest score gradient
+// where the scale was lowered.  The check costs half an instruction a score gradient, 2% of a step (31 packed documents of
+// 64-wide heads: 776 -> 791 us).
 template <int DT> constexpr float SHIFT = DT == LSURGE_F16 ? 10.f : 0.f;
 struct RowPrep {
   f32x2_t* rows;  // lse2, delta
-  float* amax;
+  float* amax;    // f16: [hq][nblk], tile t of sequence s at entry (its first row) / rows of a tile + s + t
   int nblk;
 };
-// 2^e with 2^e amax in [1, 2); 1 for 0, infinities and NaN
+// 2^e with 2^e amax in [1, 2); 1 for 0
 __device__ __forceinline__ float grad_scale(float amax) {
-  if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
+  if (!(amax > 0.f)) return 1.f;
   int e;
   (void)frexpf(amax, &e);
   return ldexpf(1.f, min(max(1 - e, -60), 60));
 }
-// the factor of (do . v - delta) beside a weight 2^SHIFT too large
-template <int DT>
-__device__ __forceinline__ float ds_scale(float amax) {
-  return DT == LSURGE_F16 ? grad_scale(amax) * exp2_hw(4.f - SHIFT<DT>) : 1.f;
+__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+// Score gradients x of the lane's query or key, as scaled by gs, brought into f16's range, with what is summed up already.
+// A lane's partner in the other half of the wave has the same query or key.
+constexpr float F16_MAX = 65504.f;
+template <int D>
+__device__ __forceinline__ void fit_f16(f32x16& x, float& gs, f32x16* acc) {
+  float big = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(x[r]));
+  if (__any(big > F16_MAX)) {
+    big = halves(big, [](float p, float q) { return fmaxf(p, q); });
+    // a power of two that makes it 1 to 2; an infinite one is beyond help, and nobody else's business
+    const float c =
+        big > F16_MAX && big < INFINITY ? __uint_as_float(max(254 - (int)(__float_as_uint(big) >> 23), 1) << 23) : 1.f;
+    gs *= c;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= c;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) rescale<D>(acc[d], c);
+  }
 }
 
 // dq_i = scale sum_j ds_ij k_j with ds_ij = p_ij (do_i . v_j - delta_i): the forward's walk, a query per lane, dS^T in
@@ -453,10 +474,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
     zero_rows<D>(dq, first, (int)min((int64_t)BM, a.total_q - first), a.hq, head, threadIdx.x, NW * 64);
   }
   const int tile = pl.tile, q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk;
-  if (pl.seq < 0 || tile * BM >= nq) {
-    if (DT == LSURGE_F16 && threadIdx.x == 0 && part == 0) w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = 0.f;
-    return;
-  }
+  if (pl.seq < 0 || tile * BM >= nq) return;
   const int off = nk - nq, w0 = tile * BM + wave * 32, row = w0 + ln;
 
   const uint32_t lds = lds_addr((const bf16_t*)smem);
@@ -508,23 +526,24 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
         x1 = fmaf(e[1], 1.f / LO_SCALE, x1);
         unpack2<DT>(df[s][i], y0, y1);
         delta = fmaf(x0, y0, fmaf(x1, y1, delta));
-        if (DT == LSURGE_F16) big = fmaxf(big, fmaxf(fabsf(y0), fabsf(y1)));
+        if (DT == LSURGE_F16) big = fmaxf(big, fmaxf(finite_abs(y0), finite_abs(y1)));
       }
   }
-  delta = halves(delta, [](float x, float y) { return x + y; }) - (dlse ? dlse[pi] : 0.f);
+  const float row_dlse = dlse ? dlse[pi] : 0.f;
+  delta = halves(delta, [](float x, float y) { return x + y; }) - row_dlse;
   const float lse2 = row_lse == -INFINITY ? INFINITY : row_lse * LOG2E - SHIFT<DT>;
   if (hf == 0 && row < nq && part == 0) w.rows[pi] = f32x2_t{lse2, delta};
   float gs = 1.f;
   if constexpr (DT == LSURGE_F16) {
-    big = halves(big, [](float x, float y) { return fmaxf(x, y); });
-    gs = ds_scale<DT>(big);
+    big = fmaxf(halves(big, [](float x, float y) { return fmaxf(x, y); }), finite_abs(row_dlse));
+    gs = grad_scale(big);
     big = wave_max(big);  // rows past the end repeat the last one
     if (lane == 0) red[wave] = big;
     __syncthreads();
     if (threadIdx.x == 0 && part == 0) {
 #pragma unroll
       for (int i = 1; i < NW; ++i) big = fmaxf(big, red[i]);
-      w.amax[(int64_t)head * w.nblk + sq * a.tiles + slot] = big;
+      w.amax[(int64_t)head * w.nblk + q0 / BM + pl.seq + tile] = big;
     }
   }
   f32x16 acc[D / 32];
@@ -538,6 +557,10 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
 #pragma unroll
   for (int t = 0; t < COLS<D>; ++t) ca[t] = col_addr<D>(lane, t);
 
+  if constexpr (D == 256 && DT == LSURGE_F16) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) asm volatile("" : "+a"(acc[d]));
+  }
   for (int st = 0; st < nst; ++st) {
     if constexpr (D == 256) {  // as in the forward
 #pragma unroll
@@ -568,6 +591,7 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * t + 8 * (r / 4) + 4 * hf + r % 4 > lim) s[r] = 0.f;
+      if constexpr (DT == LSURGE_F16) fit_f16<D>(s, gs, acc);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4 p;
@@ -669,16 +693,17 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
     if (R > 2) issue(1);
   }
   float gs = 1.f;
-  if constexpr (DT == LSURGE_F16) {  // one scale for the head's group: its largest |do|
+  if constexpr (DT == LSURGE_F16) {  // the largest upstream gradient of the rows that see the tile's keys, all heads
     float mx = 0.f;
-    const float* am = w.amax + (int64_t)kvh * group * w.nblk;
-    for (int i = threadIdx.x; i < group * w.nblk; i += NW * 64) mx = fmaxf(mx, am[i]);
+    const int t0 = first * QN / BK, nt = (nq + BK - 1) / BK - t0;  // tiles of the pass over queries, as large as these
+    const float* am = w.amax + (int64_t)kvh * group * w.nblk + q0 / BK + pl.seq + t0;
+    for (int i = threadIdx.x; i < group * nt; i += NW * 64) mx = fmaxf(mx, am[(int64_t)(i / nt) * w.nblk + i % nt]);
     mx = wave_max(mx);
     if (lane == 0) red[wave] = mx;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NW; ++i) mx = fmaxf(mx, red[i]);
-    gs = ds_scale<DT>(mx);
+    gs = grad_scale(mx);
   }
   f32x16 ak[D / 32], av[D / 32];
 #pragma unroll
@@ -692,7 +717,7 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
 
   int cr = per ? (first + begin % per) * QN : 0;  // first row of the stage being computed
   // weights and score gradients of the stage in `slot`, packed as the products' operands
-  auto weigh = [&](int slot, const f32x16& s, const f32x16& g, u32x4* p, u32x4* x) {
+  auto weigh = [&](int slot, const f32x16& s, f32x16& g, u32x4* p, u32x4* x) {
     const uint32_t rw = lds_rows + slot * 256 + 16 * hf;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -705,12 +730,18 @@ void attn_dkv_kernel(AttnArgs a, const uint16_t* __restrict__ dout, RowPrep w, f
         f[i] = g[r] - __uint_as_float(de[i]);
         if (DT == LSURGE_F16) f[i] *= gs;
         f[i] *= e[i];
+        if (DT == LSURGE_F16) g[r] = f[i];
       }
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         p[b / 2][b % 2 * 2 + i / 2] = pack2<DT>(e[i], e[i + 1]);
-        x[b / 2][b % 2 * 2 + i / 2] = pack2<DT>(f[i], f[i + 1]);
+        if (DT != LSURGE_F16) x[b / 2][b % 2 * 2 + i / 2] = pack2<DT>(f[i], f[i + 1]);
       }
+    }
+    if constexpr (DT == LSURGE_F16) {
+      fit_f16<D>(g, gs, ak);
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) x[r / 8][r % 8 / 2] = pack2<DT>(g[r], g[r + 1]);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(p[h]), "+v"(x[h]));
@@ -966,7 +997,8 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   return LSURGE_OK;
 }
 
-// tile slots of the queries, packed or not
+// entries for the tiles of the queries of a head (see RowPrep): sequence s has at least as many as tiles between its first
+// and the next sequence's, packed or not
 static int64_t most_query_tiles(const lsurge_attn_shape* s) { return s->total_q / 128 + std::max<int64_t>(s->nseq, 1); }
 static size_t prep_bytes(const lsurge_attn_shape* s) {
   const int64_t rows = s->hq * s->total_q;
@@ -1006,6 +1038,7 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   const int64_t nrow = s->hq * s->total_q;
   RowPrep w;
   w.rows = (f32x2_t*)workspace, w.amax = (float*)(w.rows + nrow);
+  w.nblk = (int)most_query_tiles(s);
   float* psum = (float*)((char*)workspace + prep_bytes(s));
   const int parts = (int)dkv_parts(*s), qparts = (int)dq_parts(*s);
   const uint16_t* g = (const uint16_t*)dout;
@@ -1020,7 +1053,6 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
   if (s->total_k)                                                                                                          \
     if (int rc = plan_grid("attn_bwd", *s, cu_q, s->hk * parts, 1, tile_slots(*s, cu_q, s->total_k, NW * 32), &ak, &gk))   \
       return rc;                                                                                                           \
-  w.nblk = (int)(gq / (s->hq * qparts));                                                                                   \
   const auto sum_grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, 4096)); };              \
   if (gq) {                                                                                                                \
     LSURGE_LAUNCH(KID_ATTN, st, hipLaunchKernelGGL((attn_dq_kernel<D, DT, NW>), dim3(gq), dim3(NW * 64), 0, st, a,         \

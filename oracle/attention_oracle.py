@@ -105,7 +105,10 @@ def bounds(q, k, v, scale, u, do=None, dlse=None, mask=None):
     ed = (ag * eo).sum(-1, keepdims=True) + (D + 2) * X * (ag * np.abs(o)).sum(-1, keepdims=True)
     ep = (D + 2) * X * (ag @ av.transpose(0, 2, 1))
     eds = (ew + u) * ds + w * (ep + ed)
-    if tiny:  # half a subnormal step of the score gradients, scaled by 2^4 / |do|; of the weights, scaled by 2^10: 2^-35
+    # half a subnormal step of the score gradients at their scale: 2^-35 of the largest upstream gradient, or 2^-25 of the
+    # row's (key's) largest score gradient, which the second u of eds, unused since ds is formed of unrounded weights, covers
+    # for up to 2^14 keys (rows); of the weights, scaled by 2^10: 2^-35
+    if tiny:
         eds = eds + 2.0 ** -29 * ag.max(initial=0)
     ewt = ew * w + tiny * 2.0 ** -10 * (w > 0)
     dq, dk, dv = attention_bwd(q, k, v, do, scale, dlse)

@@ -566,3 +566,61 @@ def test_decode_equal_scores_over_many_units(dt, D, dev):
     want = np.tile(s + np.log(n), rows // 4)[:, None]
     _within(lse, want, 540 * 2.0 ** -24 + 4 * 2.0 ** -24 * np.abs(want), "lse")
     _within(o, np.zeros(o.shape), np.full(o.shape, 540 * 2.0 ** -24), "o")
+
+
+def grads(q, k, v, do, lens, dlse=None, scale=None):
+    """o, lse, dq, dk, dv of packed sequences, lens (queries, keys) of each."""
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    ends = [_ends([n[i] for n in lens], q.device) for i in (0, 1)]
+    o, lse = A.causal_attention(*leaves, *ends, scale=scale, return_lse=True)
+    up = [(a, b) for a, b in ((o, do), (lse, dlse)) if b is not None]
+    return [o.detach(), lse.detach(), *torch.autograd.grad([a for a, _ in up], leaves, [b for _, b in up])]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("others", [2.0 ** 14, float("inf")])
+def test_f16_gradients_do_not_depend_on_other_documents(D, others, dev):
+    """A document's gradients are the same bits beside a document whose upstream gradients are 2^20 times larger, or
+    infinite, and within the bounds that its own sizes give."""
+    gen = torch.Generator().manual_seed(D)
+    lens = [(300, 300), (257, 257), (500, 500)]
+    n, a, b = 1057, 300, 557
+    q, k, v, do = (_randn(gen, (n, h, D), F16, dev) for h in (4, 2, 2, 4))
+    do *= 2.0 ** -6
+    alone = grads(q, k, v, do, lens)
+    loud = do.clone()
+    loud[a:b] *= others
+    got = grads(q, k, v, loud, lens)
+    for name, x, y in zip(("o", "lse", "dq", "dk", "dv"), alone, got):
+        assert torch.equal(x[:a], y[:a]) and torch.equal(x[b:], y[b:]), name
+    check(*(t[b:] for t in (q, k, v)), [500], [500], D ** -0.5, do[b:])
+    if others < 65504:
+        check(*(t[:, :] for t in (q, k, v)), *([m for m, _ in lens],) * 2, D ** -0.5, loud)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** 5, 2.0 ** 11])
+def test_f16_values_of_every_size(D, size, dev):
+    """Score gradients p (do . v - delta) that are much larger or smaller than do: values of thousands and of thousandths,
+    peaked and flat rows, chunks whose keys are cut into parts."""
+    gen = torch.Generator().manual_seed(D)
+    for std, lens in ((2.0, [200, 77, 1]), (0.3, [700])):
+        n = sum(lens)
+        q, k, v, do = (_randn(gen, (n, h, D), F16, dev, s) for h, s in ((4, std), (2, std), (2, size), (4, 1 / size)))
+        check(q, k, v, lens, lens, D ** -0.5, do)
+    q, k, v, do = (_randn(gen, (m, 2, D), F16, dev, s) for m, s in ((40, 1.0), (2500, 1.0), (2500, size), (40, 0.25 / size)))
+    check(q, k, v, [40], [2500], D ** -0.5, do)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f16_gradients_of_lse(D, dev):
+    """Score gradients that come from lse alone, or that lse's upstream gradient makes larger than do by far."""
+    gen = torch.Generator().manual_seed(D)
+    q, k, v = (_randn(gen, (270, h, D), F16, dev, 1.5) for h in (4, 2, 2))
+    do = _randn(gen, (270, 4, D), F16, dev)
+    dl = torch.randn((270, 4), generator=gen).to(dev)
+    lens = [200, 70]
+    for a, b in ((0.0, 1.0), (0.0, 2000.0), (2.0 ** -7, 300.0)):
+        check(q, k, v, lens, lens, D ** -0.5, do * a, dl * b)
+    got = grads(q, k, v, None, [(200, 200), (70, 70)], dl)
+    assert all(torch.equal(x, y) for x, y in zip(got, grads(q, k, v, do * 0, [(200, 200), (70, 70)], dl)))
