@@ -529,13 +529,17 @@ void attn_dq_kernel(AttnArgs a, const uint16_t* __restrict__ o, const uint8_t* _
         if (DT == LSURGE_F16) big = fmaxf(big, fmaxf(finite_abs(y0), finite_abs(y1)));
       }
   }
-  const float row_dlse = dlse ? dlse[pi] : 0.f;
-  delta = halves(delta, [](float x, float y) { return x + y; }) - row_dlse;
-  const float lse2 = row_lse == -INFINITY ? INFINITY : row_lse * LOG2E - SHIFT<DT>;
+  // a row without a key: o and lse are constants there, whatever their upstream gradients (0 x NaN would reach dk)
+  const bool none = row_lse == -INFINITY;
+  const float row_dlse = dlse && !none ? dlse[pi] : 0.f;
+  delta = halves(delta, [](float x, float y) { return x + y; });
+  delta = none ? 0.f : delta - row_dlse;
+  const float lse2 = none ? INFINITY : row_lse * LOG2E - SHIFT<DT>;
   if (hf == 0 && row < nq && part == 0) w.rows[pi] = f32x2_t{lse2, delta};
   float gs = 1.f;
   if constexpr (DT == LSURGE_F16) {
-    big = fmaxf(halves(big, [](float x, float y) { return fmaxf(x, y); }), finite_abs(row_dlse));
+    big = halves(big, [](float x, float y) { return fmaxf(x, y); });
+    big = none ? 0.f : fmaxf(big, finite_abs(row_dlse));
     gs = grad_scale(big);
     big = wave_max(big);  // rows past the end repeat the last one
     if (lane == 0) red[wave] = big;

@@ -624,3 +624,21 @@ def test_f16_gradients_of_lse(D, dev):
         check(q, k, v, lens, lens, D ** -0.5, do * a, dl * b)
     got = grads(q, k, v, None, [(200, 200), (70, 70)], dl)
     assert all(torch.equal(x, y) for x, y in zip(got, grads(q, k, v, do * 0, [(200, 200), (70, 70)], dl)))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lse_gradient_of_rows_without_keys(dt, D, dev):
+    """lse is the constant -inf where a row sees no key, so its upstream gradient there counts for nothing, whatever it is:
+    one taken through a join of two such parts is NaN."""
+    gen = torch.Generator().manual_seed(D)
+    lens = [(45, 8), (70, 70), (9, 0)]  # 37 rows without a key: some share a stage of 32 with rows that have some
+    q, k, v, do = (_randn(gen, (m, h, D), dt, dev) for m, h in ((124, 4), (78, 2), (78, 2), (124, 4)))
+    dl = torch.randn((124, 4), generator=gen).to(dev)
+    dl[:37] = dl[115:] = 0
+    want = grads(q, k, v, do, lens, dl)
+    assert torch.isneginf(want[1][:37]).all() and torch.isneginf(want[1][115:]).all()
+    for bad in (float("nan"), float("inf"), 7.0):
+        dl[:37] = dl[115:] = bad
+        for name, x, y in zip(("o", "lse", "dq", "dk", "dv"), want, grads(q, k, v, do, lens, dl)):
+            assert torch.equal(x, y), (bad, name)
