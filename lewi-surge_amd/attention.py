@@ -24,6 +24,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 import _lib as L
 
@@ -52,6 +53,9 @@ def _check_dtype(what, *ts):
 def _check_no_grad(what, *ts):
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
         raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
+    # no level is open outside of forward-mode code (unpack_dual would say so too, 0.3 us a tensor)
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError(f"{what}: no gradient, of the forward mode neither; call it on detached tensors")
 
 
 def _check_index(what, name, t, shape):
@@ -77,7 +81,7 @@ def _ptr(t):
 
 
 def _scale(what, scale, d):
-    scale = d ** -0.5 if scale is None else float(scale)
+    scale = float(d) ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"{what}: scale must be positive and finite (got {scale})")
     return scale
@@ -103,7 +107,7 @@ def _rows_arg(t):
     return L.AttnRows(t.data_ptr(), row, head)
 
 
-def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training=False):
+def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training):
     """o, lse (or None) of packed rows, and what the backward needs: the rows as read, what o's rounding left over, the
     shape."""
     tq, hq, d = q.shape
@@ -122,13 +126,16 @@ def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training=False):
 
 
 class _AttnFn(torch.autograd.Function):
+    """Every call goes through here, with or without gradients, so that whatever records or differentiates functions sees
+    it: forward-mode tangents raise instead of being dropped, and a trace holds the call instead of an empty tensor."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale):
-        o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, True, training=True)
-        ctx.save_for_backward(*rows, cu_q, cu_k, o, lse)
-        ctx.shape, ctx.scale = shape, scale
-        ctx.set_materialize_grads(False)
+    def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale, want_lse, training):
+        o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse or training, training)
+        if training:
+            ctx.save_for_backward(*rows, cu_q, cu_k, o, lse)
+            ctx.shape, ctx.scale = shape, scale
+            ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
@@ -147,7 +154,7 @@ class _AttnFn(torch.autograd.Function):
         _call("attn_bwd", q.device, lib.lsurge_attn_bwd, shape, _rows_arg(q), _rows_arg(k), _rows_arg(v), _ptr(cu_q),
               _ptr(cu_k), ctx.scale, _ptr(o), _ptr(o_lo), _ptr(lse), _ptr(do), _ptr(dlse), _ptr(dq), _ptr(dk),
               _ptr(dv), _ptr(ws), ws.numel())
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, return_lse=False):
@@ -189,10 +196,8 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
     shape = q.shape
     if q.dim() == 4:
         q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _AttnFn.apply(q, k, v, cu_q, cu_k, nseq, scale)
-    else:
-        o, lse = _forward(q, k, v, cu_q, cu_k, nseq, scale, return_lse)[:2]
+    training = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    o, lse = _AttnFn.apply(q, k, v, cu_q, cu_k, nseq, scale, return_lse, training)
     o = o.view(shape)
     return (o, lse.t().reshape(shape[:-1])) if return_lse else o
 
@@ -230,6 +235,20 @@ def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
     return arg, (table, lens)
 
 
+class _Step(torch.autograd.Function):
+    """fn(*args) as one step of a trace."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        return fn(*args)
+
+
+def _step(fn, *args):
+    """fn(*args), which has no gradient: plainly, 3 us less than an autograd function takes, but as one where torch.jit
+    traces, which would otherwise record the empty output and not the call that fills it."""
+    return _Step.apply(fn, *args) if torch.jit.is_tracing() else fn(*args)
+
+
 def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
     """Write new tokens into a paged cache, in place.  k, v [rows, Hkv, D]: one token for each sequence, or with cu_seqlens
     (int32 [sequences + 1]) the rows cu_seqlens[b] .. cu_seqlens[b + 1] of sequence b.  They become the last of its
@@ -244,6 +263,11 @@ def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
     _check_heads(what, k.shape[1], k.shape[1], k.shape[2], k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _check_dtype(what, k, v, k_cache, v_cache)
     _check_no_grad(what, k, v, k_cache, v_cache)
+    _step(_append, k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens)
+
+
+def _append(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens):
+    what = "append_kv"
     arg, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
     nseq = page_table.shape[0]
     if cu_seqlens is not None:
@@ -271,8 +295,13 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, retur
     n, hq, d = q.shape
     _check_heads(what, hq, k_cache.shape[2], d, q, k_cache, v_cache, page_table, seq_lens)
     _check_dtype(what, q, k_cache, v_cache)
-    scale = _scale(what, scale, d)
-    arg, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
+    o, lse = _step(_paged, q, k_cache, v_cache, page_table, seq_lens, _scale(what, scale, d), return_lse)
+    return (o, lse) if return_lse else o
+
+
+def _paged(q, k_cache, v_cache, page_table, seq_lens, scale, return_lse):
+    n, hq, d = q.shape
+    arg, keep = _cache_arg("paged_attention", k_cache, v_cache, page_table, seq_lens)
     q = _rows(q)
     o = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
@@ -281,4 +310,4 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, retur
     _call("paged_attn", q.device, lib.lsurge_paged_attn, arg, _rows_arg(q), n, hq, scale, _ptr(o), _ptr(lse), _ptr(ws),
           ws.numel())
     del keep
-    return (o, lse) if return_lse else o
+    return o, lse

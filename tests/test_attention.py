@@ -267,3 +267,64 @@ def test_gradients_are_refused_at_the_cache(monkeypatch):
                  (kc.detach().requires_grad_(True), vc, k, k), (kc, vc.detach().requires_grad_(True), k, k)):
         with pytest.raises(ValueError, match="no gradient"):
             A.append_kv(args[0], args[1], table, lens, *args[2:])
+
+
+class _Stub:
+    """The library with calls that are noted instead of made."""
+
+    def __init__(self, monkeypatch):
+        self.calls = []
+        monkeypatch.setattr(A.L, "require_cuda", lambda *_: None)
+        monkeypatch.setattr(A.L, "lib", lambda: self)
+        monkeypatch.setattr(A, "_call", lambda what, device, fn, *args: fn(*args))
+
+    def __getattr__(self, name):
+        return (lambda *_: 0) if name.endswith("_bytes") else lambda *_: self.calls.append(name)
+
+
+def test_forward_mode_tangents_are_not_dropped(monkeypatch):
+    stub = _Stub(monkeypatch)
+    kc, vc, table, lens = _cache()
+    q, k = _t(4, 2, 64), _t(2, 2, 64)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for i in range(3):
+            args = [q, q, q]
+            args[i] = dual(q)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                A.causal_attention(*args, CU)
+        stub.calls.clear()
+        for i in range(3):
+            args = [k, kc, vc]
+            args[i] = dual(args[i])
+            with pytest.raises(ValueError, match="no gradient"):
+                A.paged_attention(*args, table, lens)
+        for i in range(4):
+            args = [kc, vc, table, lens, k, k]
+            args[(0, 1, 4, 5)[i]] = dual(args[(0, 1, 4, 5)[i]])
+            with pytest.raises(ValueError, match="no gradient"):
+                A.append_kv(*args)
+        assert not stub.calls  # nothing was written
+        A.append_kv(kc, vc, table, lens, k, k)
+        assert stub.calls == ["lsurge_kv_append"]
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_a_trace_holds_the_calls(monkeypatch):
+    """What torch.jit.trace records calls the kernels again, and returns their outputs instead of an empty tensor."""
+    stub = _Stub(monkeypatch)
+    kc, vc, table, lens = _cache()
+    q, k = _t(4, 2, 64), _t(2, 2, 64)
+
+    def step(k, v, q, table, lens):
+        A.append_kv(kc, vc, table, lens, k, v)
+        return A.paged_attention(q, kc, vc, table, lens)
+
+    for f, args, names in ((lambda q, k, v, cu: A.causal_attention(q, k, v, cu), (q, q, q, CU), ["lsurge_attn_fwd"]),
+                           (lambda q, k, v, cu: A.causal_attention(q, k, v, cu, return_lse=True), (q, q, q, CU), ["lsurge_attn_fwd"]),
+                           (step, (k, k, k, table, lens), ["lsurge_kv_append", "lsurge_paged_attn"])):
+        with torch.no_grad():
+            traced = torch.jit.trace(f, args, check_trace=False)
+        stub.calls.clear()
+        traced(*args)
+        assert stub.calls == names

@@ -642,3 +642,27 @@ def test_lse_gradient_of_rows_without_keys(dt, D, dev):
         dl[:37] = dl[115:] = bad
         for name, x, y in zip(("o", "lse", "dq", "dk", "dv"), want, grads(q, k, v, do, lens, dl)):
             assert torch.equal(x, y), (bad, name)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_traced_serving_step(dev):
+    """A prompt's attention and a token's, traced, compute on new inputs what the calls themselves do."""
+    gen = torch.Generator().manual_seed(23)
+    kc, vc, table, sl, _, _ = make_cache(gen, [20, 33], 16, 2, 64, BF16, dev)
+    cu = _ends([20, 33], dev)
+
+    def prompt(q, k, v):
+        return A.causal_attention(q, k, v, cu, return_lse=True)
+
+    def token(q, k, v):
+        A.append_kv(kc, vc, table, sl, k, v)
+        return A.paged_attention(q, kc, vc, table, sl)
+
+    draw = lambda n: [_randn(gen, (n, h, 64), BF16, dev) for h in (4, 2, 2)]  # noqa: E731
+    with torch.no_grad():
+        p, t = (torch.jit.trace(f, tuple(draw(n)), check_trace=False) for f, n in ((prompt, 53), (token, 2)))
+        for _ in range(2):
+            x, y = draw(53), draw(2)
+            assert all(torch.equal(a, b) for a, b in zip(p(*x), prompt(*x)))
+            got, rows = t(*y), kc.clone()
+            assert torch.equal(got, token(*y)) and torch.equal(rows.nan_to_num(7), kc.nan_to_num(7))
