@@ -90,6 +90,8 @@ constexpr int FN = 32;  // keys per stage of the forward
 template <int D> constexpr int STAGES = D == 256 ? 3 : 4;
 constexpr int BN = 64;  // keys per stage of the pass over queries
 
+constexpr float LAZY = 8.f;  // log2 of the growth of a row's largest weight that the base lets pass
+
 // acc *= f.  At D = 256 the accumulators fill half of the registers and have to stay in the accumulation file, which the
 // vector unit cannot work on: written as plain products, the compiler moves all of them to the other file and back in
 // every stage (256 moves for 32 matrix instructions).  They go through a temporary here, in the rare branch only; the
@@ -287,10 +289,10 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x4* __res
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = halves(mx, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
-    // the weights' base follows the maximum only when it has grown by 2^8: any base does, and f32 sums and 16-bit
-    // weights have room for it (weights up to 2^8), so that the accumulators are rescaled in few stages
-    mx = mx > m + 8.f ? mx : m;
+    mx = halves(mx, [](float x, float y) { return fmaxf(x, y); }) * a.scale2 - (DT == LSURGE_F16 ? ROOM<DT> - LAZY : 0.f);
+    // the weights' base follows the maximum only when it has grown by 2^8: any base does, and f32 sums and 16-bit weights
+    // have room for it, so that the accumulators are rescaled in few stages
+    mx = mx > m + LAZY ? mx : m;
     mc = mx == -INFINITY ? 0.f : mx;
     const float alpha = exp2_hw(m - mc);
     float sum[2] = {0.f, 0.f};

@@ -200,7 +200,7 @@ void attn_decode_kernel(DecodeArgs a) {
     f32x4 acc[VE];
 #pragma unroll
     for (int t = 0; t < VE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // m: the largest score so far times the scale, as rounded.  Weights, sums and the join all take this one value as their
+    // m: the largest score so far times the scale, less ROOM, as rounded.  Weights, sums and the join all take this one value as their
     // base: the product formed anew inside an fma would be the unrounded one, a factor of 2^(its rounding) for every tile.
     float m = -INFINITY, l = 0.f;
 
@@ -225,7 +225,7 @@ void attn_decode_kernel(DecodeArgs a) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }) * a.scale2);
+      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }) * a.scale2 - ROOM<DT>);
       const float mc = mx == -INFINITY ? 0.f : mx;
       const float alpha = exp2_hw(m - mc);  // 1 where the largest score stays
       m = mx;

@@ -666,3 +666,45 @@ def test_traced_serving_step(dev):
             assert all(torch.equal(a, b) for a, b in zip(p(*x), prompt(*x)))
             got, rows = t(*y), kc.clone()
             assert torch.equal(got, token(*y)) and torch.equal(rows.nan_to_num(7), kc.nan_to_num(7))
+
+
+# One key holds nearly all of a row's weight; 65535 others of value 1 hold 2^-25.5 of it each, less than half of f16's least
+# subnormal, and W = 1/720 of it together.
+FLAT_KEYS, FLAT = 65536, 65535 * 2.0 ** -25.5
+
+
+def flat_rows(D, value):
+    """Keys, values and the scale that with queries of ones makes the scores; `value` is that of the one."""
+    k, v = torch.zeros((FLAT_KEYS, 1, D), dtype=F16), torch.ones((FLAT_KEYS, 1, D), dtype=F16)
+    k[FLAT_KEYS // 3], v[FLAT_KEYS // 3] = 1.0, value
+    return k, v, 25.5 * np.log(2) / D
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f16_decode_weights_far_below_the_largest(D, dev):
+    """Value 0 for the one: o = W / (1 + W).  The others' weights are held as 2^-10.5, within 2^-11 of themselves, o is
+    rounded to 2^-11, and 2^-12 is for f32's sums and exponents."""
+    k, v, scale = flat_rows(D, 0.0)
+    rows = 768
+    kc, vc, table = shared_cache(k, v, 64, rows, F16, dev)
+    q = torch.ones((rows, 1, D), dtype=F16, device=dev)
+    o = A.paged_attention(q, kc, vc, table, torch.full((rows,), FLAT_KEYS, dtype=torch.int32, device=dev), scale=scale)
+    want = np.full(o.shape, FLAT / (1 + FLAT))
+    _within(o, want, want * (2 * 2.0 ** -11 + 2.0 ** -12), "o")
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f16_forward_weights_far_below_the_largest(D, grad, dev):
+    """Value -1 for the one: o = (W - 1) / (W + 1), -0.997.  The others' weights are held as 2^-18.5 at least (the base may
+    lag behind the largest score by 2^8), within half a subnormal step, 2^-25, or 2^-6.5 of themselves, which counts twice
+    in o; o's own rounding is 2^-12 of less than 1, but 2^-11 is allowed, and 2^-20 for f32.  128 rows of 768 heads leave the
+    keys in one part; the last rows see up to 127 keys more, of weight e^-1060."""
+    k, v, scale = (x.to(dev) if torch.is_tensor(x) else x for x in flat_rows(D, -1.0))
+    k = torch.cat([k, torch.full((127, 1, D), -60.0, dtype=F16, device=dev)])
+    v = torch.cat([v, torch.ones((127, 1, D), dtype=F16, device=dev)])
+    q = torch.ones((1, 128, 768, D), dtype=F16, device=dev)
+    o = A.causal_attention(q, *(x[None].detach().requires_grad_(grad) for x in (k, v)), scale=scale).detach()
+    assert o.shape == q.shape and (o == o[:, :, :1, :1]).all()
+    o = o[0, :, 0, :1]
+    _within(o, np.full(o.shape, (FLAT - 1) / (FLAT + 1)), np.full(o.shape, 2 * FLAT * 2.0 ** -6.5 + 2.0 ** -11 + 2.0 ** -20), "o")
