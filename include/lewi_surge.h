@@ -450,7 +450,9 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
 /* Backward of lsurge_attn_fwd for upstream dout [total_q, hq, d] (contiguous) and dlse [hq, total_q] f32 (NULL: 0), from
  * the forward's o, o_lo (NULL: the backward takes o as it was rounded, a little less exact) and lse: dq [total_q, hq, d],
  * dk and dv [total_k, hk, d], summed over the heads of a group, all of the shape's dtype and contiguous; 0 in the rows
- * behind the last sequence.  No atomics: results repeat bit for bit. */
+ * behind the last sequence.  No atomics: results repeat bit for bit.  The workspace holds 8 bytes a query and head, 4 a tile
+ * of 128 queries and head in f16, and, where the work is cut into parts, their f32 sums: up to 512 MiB, or 4 times dk and dv
+ * where that is more. */
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s);
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,

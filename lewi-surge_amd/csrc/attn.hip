@@ -911,15 +911,20 @@ constexpr int WAVES = 4;  // of a workgroup, 32 rows each (8 were as fast or slo
 // Parts that the stages of a tile of keys are cut into in attn_dkv_kernel, by the sizes that the host knows (the
 // sequences' own lengths are on the device): as many as give every place for a workgroup two of them, so that the ones
 // with few queries fill up behind the ones with many, but no part under 4 stages; one part for every 1024 stages where
-// they are that many.  A part costs a write and a read of the tile's f32 sums.  Measured, us a training step at 1, 2, 4
-// and 8 parts: 8 x 4096 tokens, 8 heads over 2 (512 tiles, 256 stages): 1568, 1346, 1435, 1485; one of 32768, 16 heads
-// over 4 (1024, 2048): 19532, 19021, 18961, 18864; one of 4096, 8 heads of their own keys (256, 64): 433, 351, 330, 391;
-// one of 512, 8 over 2 (8, 32): 154, 106, 82, 72; 2 x 4096, 16 over 2, 256-wide (128, 512): 3552, 2357, 1721, 1756.
+// they are that many, but no more than 2 of these where the sums would pass 512 MiB (two parts' are 4 times dk and dv).  A
+// part costs a write and a read of the tile's f32 sums.  Measured, us a training step at 1, 2, 4 and 8 parts: 8 x 4096 tokens,
+// 8 heads over 2 (512 tiles, 256 stages): 1568, 1346, 1435, 1485; one of 32768, 16 heads over 4 (1024, 2048): 19532, 19021,
+// 18961, 18864; one of 4096, 8 heads of their own keys (256, 64): 433, 351, 330, 391; one of 512, 8 over 2 (8, 32): 154, 106,
+// 82, 72; 2 x 4096, 16 over 2, 256-wide (128, 512): 3552, 2357, 1721, 1756.  What the limit costs: 65536 tokens, 16 heads over
+// 4, 2 parts instead of 4: 75.3 -> 75.9 ms; 131072, 8 over 2, instead of 8: 149.9 -> 152.9 ms.
 int64_t dkv_parts(const lsurge_attn_shape& s) {
   if (s.total_q == 0 || s.total_k == 0 || s.nseq == 0) return 1;
   const int64_t tiles = s.nseq * ((s.total_k / s.nseq + 127) / 128) * s.hk, places = s.d == 256 ? 256 : 512;
   const int64_t stages = s.hq / s.hk * (s.total_q / s.nseq) / QN / 2;  // half of the queries, on average, see a key
-  const int64_t parts = std::min(std::max(2 * places / std::max<int64_t>(tiles, 1), stages / 1024), stages / 4);
+  const int64_t bytes = 2 * sizeof(float) * s.total_k * s.hk * s.d;  // of a part's sums
+  const int64_t most = std::max<int64_t>((int64_t(512) << 20) / bytes, 2);
+  const int64_t parts =
+      std::min(std::max(2 * places / std::max<int64_t>(tiles, 1), std::min(stages / 1024, most)), stages / 4);
   return parts >= 8 ? 8 : parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
 }
 

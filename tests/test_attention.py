@@ -328,3 +328,17 @@ def test_a_trace_holds_the_calls(monkeypatch):
         stub.calls.clear()
         traced(*args)
         assert stub.calls == names
+
+
+def test_backward_workspace_is_bounded():
+    """lse2 and delta of every query and head, the tiles' maxima in f16, and f32 sums of parts: up to 512 MiB, or 4 times dk
+    and dv where that is more."""
+    lib = L.lib()
+    for nseq in (1, 4):
+        for n in (1, 300, 4096, 32768, 131072, 1 << 20):
+            for hq, hk in ((1, 1), (8, 8), (16, 2), (64, 8), (32, 32)):
+                for d in (64, 128, 256):
+                    s = _shape(nseq=nseq, total_q=nseq * n, total_k=nseq * n, hq=hq, hk=hk, d=d)
+                    prep = 8 * nseq * n * hq
+                    dkv = 2 * 2 * nseq * n * hk * d
+                    assert lib.lsurge_attn_bwd_workspace_bytes(ctypes.byref(s)) <= prep + 512 + max(512 << 20, 4 * dkv)
