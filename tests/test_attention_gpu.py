@@ -708,3 +708,86 @@ def test_f16_forward_weights_far_below_the_largest(D, grad, dev):
     assert o.shape == q.shape and (o == o[:, :, :1, :1]).all()
     o = o[0, :, 0, :1]
     _within(o, np.full(o.shape, (FLAT - 1) / (FLAT + 1)), np.full(o.shape, 2 * FLAT * 2.0 ** -6.5 + 2.0 ** -11 + 2.0 ** -20), "o")
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_many_units_of_a_sequence_in_a_share(dt, D, dev):
+    """Shares of 5 and more units of 128 keys of one sequence and head (odd and even numbers of them), borders of sequences
+    inside a share, lengths that end inside a tile: 300 sequences of 1 to 2300 tokens, 2 key heads."""
+    gen = torch.Generator().manual_seed(D)
+    n, rows = 2300, 300
+    k, v = _randn(gen, (n, 2, D), dt, "cpu", 1.5), _randn(gen, (n, 2, D), dt, "cpu")
+    kc, vc, table = shared_cache(k, v, 16, rows, dt, dev)
+    lens = [2300, 1, 0, 640, 641, 767, 768, 769, 1024] + [int(x) for x in np.random.default_rng(D).integers(900, n, rows - 9)]
+    q = _randn(gen, (rows, 4, D), dt, dev, 1.5)
+    o, lse = A.paged_attention(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=dev), return_lse=True)
+    o, lse = _np(o), _np(lse)
+    for b, m in enumerate(lens):
+        if b > 40 and b % 8:
+            continue
+        one = (_np(q[b:b + 1]), _np(k[:m]), _np(v[:m]), D ** -0.5)
+        mask = np.ones((1, m), bool)
+        for name, x, y, e in zip(("o", "lse"), (o[b:b + 1], lse[b:b + 1]), ao.attention(*one, mask=mask),
+                                 ao.bounds(*one, HALF_STEP[dt], mask=mask)):
+            _within(x, y, e, f"{name} of length {m}")
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lengths_around_every_tile_without_gradients(dt, D, dev):
+    """The serving forward, which is compiled apart from the one that keeps what a backward needs."""
+    run(dt, D, 2, 1, EDGES, EDGES, dev, seed=D, backward=False)
+    run(dt, D, 4, 2, [5, 64, 1, 130], [5 + 300, 64 + 1, 1 + 511, 130 + 62], dev, seed=D, backward=False)
+    run(dt, D, 4, 2, [40, 3, 7, 0, 9], [8, 0, 7, 5, 9], dev, seed=D, backward=False)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_rows_over_many_keys_without_gradients(dt, D, dev):
+    run(dt, D, 2, 1, [40, 0, 1, 130, 5], [2500, 700, 3000, 130 + 2200, 3], dev, seed=D, backward=False)
+    gen = torch.Generator().manual_seed(D)
+    q, k, v = (_randn(gen, (1, 2400, 1, D), dt, dev) for _ in range(3))
+    check(q, k, v, [2400], [2400], D ** -0.5, cu=False)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_rows_without_gradients(dt, D, dev):
+    """Many turns of the stages' ring in one part: 8 heads of 12 dense sequences leave the keys whole.  Rising and falling
+    scores move the base of the weights."""
+    gen = torch.Generator().manual_seed(8)
+    n, b, h = 1100, 12, 8
+    ramp = torch.linspace(-1, 1, n).view(1, -1, 1, 1).to(dev)
+    q, k, v = (_randn(gen, (b, n, x, D), dt, dev) for x in (h, 2, 2))
+    for kk in (k, (k * (4 + 3 * ramp)).to(dt), (k * (4 - 3 * ramp)).to(dt)):
+        o, lse = A.causal_attention(q, kk, v, return_lse=True)
+        for i in (0, b - 1):
+            one = [_np(t[i]) for t in (q, kk, v)]
+            for name, x, y, e in zip(("o", "lse"), (o[i], lse[i]), ao.attention(*one, D ** -0.5),
+                                     ao.bounds(*one, D ** -0.5, HALF_STEP[dt])):
+                _within(x, y, e, name)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 64), (BF16, 128), (F16, 256)])
+def test_c_abi_backward_without_the_left_over(dt, D, dev):
+    """o_lo may be NULL for the backward: o is then taken as it was rounded, for which delta is off by u |do| |o| more."""
+    import _lib as L
+    gen = torch.Generator().manual_seed(D)
+    n, hq, hk, u, scale = 333, 4, 2, HALF_STEP[dt], D ** -0.5
+    q, k, v, do = (_randn(gen, (n, h, D), dt, dev) for h in (hq, hk, hk, hq))
+    o, lse = A.causal_attention(q, k, v, _ends([n], dev), return_lse=True)
+    shape = L.AttnShape(1, n, n, hq, hk, D, L.dt(q))
+    lse_t, grads_ = lse.t().contiguous(), [torch.empty_like(t) for t in (q, k, v)]
+    ws = L.workspace(L.lib().lsurge_attn_bwd_workspace_bytes(shape), dev)
+    rows = [L.AttnRows(t.data_ptr(), t.stride(0), t.stride(1)) for t in (q, k, v)]
+    L.check(L.lib().lsurge_attn_bwd(shape, *rows, None, None, scale, L.ptr(o), None, L.ptr(lse_t), L.ptr(do), None,
+                                    *(L.ptr(t) for t in grads_), L.ptr(ws), ws.numel(), L.stream(dev)), "attn_bwd")
+    one, g = [_np(t) for t in (q, k, v)], _np(do)
+    bound = ao.bounds(*one, scale, u, do=g)[2:]
+    _, w, _ = ao._weights(*one[:2], scale)
+    ed = w * (np.abs(g) * u * np.abs(_np(o))).sum(-1).T[..., None]  # of ds
+    more = (scale * (ed @ np.abs(ao._heads(one[1], 2))).transpose(1, 0, 2),
+            scale * (ed.transpose(0, 2, 1) @ np.abs(one[0].transpose(1, 0, 2))).reshape(hk, 2, n, D).sum(1).transpose(1, 0, 2), 0.0)
+    for name, x, y, b, m in zip(("dq", "dk", "dv"), grads_, ao.attention_bwd(*one, g, scale), bound, more):
+        _within(x, y, b + m, name)
