@@ -36,8 +36,9 @@ struct CacheArgs {
 constexpr int DW = 4;             // waves of a workgroup; each takes 32 keys at a time
 constexpr int UK = DW * 32;       // keys of a unit
 constexpr int DT_THREADS = DW * 64;
-template <int D> constexpr int DECODE_EU = D == 64 ? 3 : D == 128 ? 2 : 1;  // waves per SIMD that the registers leave
-constexpr int DECODE_GRID = 1024;                             // at most 4 workgroups a CU
+constexpr int64_t decode_eu(int64_t d) { return d == 64 ? 3 : d == 128 ? 2 : 1; }  // waves per SIMD that the registers leave
+constexpr int64_t CUS = 256;
+constexpr int64_t DECODE_GRID = CUS * decode_eu(64);  // workgroups at most: 4 waves each, one a SIMD
 
 struct DecodeArgs {
   CacheArgs c;
@@ -68,7 +69,7 @@ __device__ __forceinline__ int64_t div64(int64_t n, int64_t d) {
 }
 
 template <int D, int DT>
-__global__ __launch_bounds__(DT_THREADS) __attribute__((amdgpu_waves_per_eu(DECODE_EU<D>)))
+__global__ __launch_bounds__(DT_THREADS) __attribute__((amdgpu_waves_per_eu(decode_eu(D))))
 void attn_decode_kernel(DecodeArgs a) {
   constexpr int KC = D / 32, VE = D / 16, VW = VE / 2;  // a lane's 16-byte chunks of a key, columns and registers of a value
   __shared__ int64_t wsum[DW], found;
@@ -462,11 +463,13 @@ int check_new_rows(const char* what, const lsurge_attn_rows* r) {
   return LSURGE_OK;
 }
 
-// Workgroups that the units are dealt to: as many as the registers let a GPU of 256 CUs hold at a time, or one for every
-// unit that the page table's width allows where that is less.
+// Workgroups that the units are dealt to: as many as the registers let the GPU's CUs hold at a time, or one for every unit
+// that the page table's width allows where that is less.  Twice as many at 256 wide, us for 512 and 256 workgroups: 32
+// sequences of 4000, 16 heads over 2: 52.2 and 47.4; 64 of 100 to 8192: 106.6 and 100.5; 2 of 120000: 97.4 and 88.5; 200 of up
+// to 2000: 97.9 and 96.1.
 int64_t decode_grid(int64_t nseq, int64_t heads, int64_t d, int64_t max_pages, int64_t page_size) {
   const double most = (double)nseq * heads * (((double)max_pages * page_size + UK - 1) / UK);
-  const int64_t full = d == 64 ? DECODE_GRID * 3 / 4 : DECODE_GRID / 2;
+  const int64_t full = CUS * decode_eu(d);
   return most < full ? std::max<int64_t>(1, (int64_t)most) : full;
 }
 size_t decode_parts_bytes(int64_t d) { return sizeof(float) * (size_t)DECODE_GRID * 2 * 16 * (size_t)(d + 2); }
