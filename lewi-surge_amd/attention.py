@@ -131,6 +131,8 @@ class _AttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, nseq, scale, want_lse, training):
+        if training is None:
+            training = any(ctx.needs_input_grad[:3])
         o, lse, rows, shape = _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse or training, training)
         if training:
             ctx.save_for_backward(*rows, cu_q, cu_k, o, lse)
@@ -196,7 +198,9 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
     shape = q.shape
     if q.dim() == 4:
         q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
-    training = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    # a trace does not hold what it was recorded for: a replay goes by its own inputs
+    training = None if torch.jit.is_tracing() else \
+        torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     o, lse = _AttnFn.apply(q, k, v, cu_q, cu_k, nseq, scale, return_lse, training)
     o = o.view(shape)
     return (o, lse.t().reshape(shape[:-1])) if return_lse else o

@@ -791,3 +791,19 @@ def test_c_abi_backward_without_the_left_over(dt, D, dev):
             scale * (ed.transpose(0, 2, 1) @ np.abs(one[0].transpose(1, 0, 2))).reshape(hk, 2, n, D).sum(1).transpose(1, 0, 2), 0.0)
     for name, x, y, b, m in zip(("dq", "dk", "dv"), grads_, ao.attention_bwd(*one, g, scale), bound, more):
         _within(x, y, b + m, name)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_traced_without_gradients_then_trained(dev):
+    gen = torch.Generator().manual_seed(24)
+    cu = _ends([20, 33], dev)
+    draw = lambda: [_randn(gen, (53, h, 64), BF16, dev) for h in (4, 2, 2)]  # noqa: E731
+    call = lambda q, k, v: A.causal_attention(q, k, v, cu, return_lse=True)  # noqa: E731
+    with torch.no_grad():
+        traced = torch.jit.trace(call, tuple(draw()), check_trace=False)
+    do, dl = _randn(gen, (53, 4, 64), BF16, dev), torch.randn((53, 4), generator=gen).to(dev)
+    for _ in range(3):
+        x = [t.requires_grad_(True) for t in draw()]
+        got, want = traced(*x), call(*x)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, x, (do, dl)), torch.autograd.grad(want, x, (do, dl))))
