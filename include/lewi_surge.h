@@ -450,9 +450,9 @@ int lsurge_attn_fwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
 /* Backward of lsurge_attn_fwd for upstream dout [total_q, hq, d] (contiguous) and dlse [hq, total_q] f32 (NULL: 0), from
  * the forward's o, o_lo (NULL: the backward takes o as it was rounded, a little less exact) and lse: dq [total_q, hq, d],
  * dk and dv [total_k, hk, d], summed over the heads of a group, all of the shape's dtype and contiguous; 0 in the rows
- * behind the last sequence.  No atomics: results repeat bit for bit.  The workspace holds 8 bytes a query and head, 4 a tile
- * of 128 queries and head in f16, and, where the work is cut into parts, their f32 sums: up to 512 MiB, or 4 times dk and dv
- * where that is more. */
+ * behind the last sequence.  dlse of a row without keys counts for nothing.  No atomics: results repeat bit for bit.  The
+ * workspace holds 8 bytes a query and head, 4 a tile of 128 queries and head in f16, and, where the work is cut into parts,
+ * their f32 sums: up to 512 MiB, or 4 times dk and dv where that is more. */
 size_t lsurge_attn_bwd_workspace_bytes(const lsurge_attn_shape* s);
 int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const lsurge_attn_rows* k,
                     const lsurge_attn_rows* v, const int32_t* cu_q, const int32_t* cu_k, float scale, const void* o,
@@ -467,8 +467,8 @@ int lsurge_attn_bwd(const lsurge_attn_shape* s, const lsurge_attn_rows* q, const
  * slot t and head h at k + p k_page_stride + t k_slot_stride + h k_head_stride (elements, multiples of 8; v alike), 16-byte
  * aligned.  page_table [nseq, max_pages] i32 on the device, rows table_stride apart: entry i of row b is the page of
  * sequence b's tokens i page_size .. + page_size - 1.  An entry outside [0, num_pages) names no page: its tokens take no
- * part in the attention and are not written.  seq_lens [nseq] i32 on the device: tokens of each sequence, held to
- * [0, max_pages page_size]. */
+ * part in the attention and are not written.  seq_lens [nseq] i32 on the device: tokens of each sequence; the attention holds
+ * them to [0, max_pages page_size], and a new token past the table's last page is not written. */
 typedef struct {
   void *k, *v;
   int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;

@@ -16,7 +16,8 @@ others.  The reference leaves them to MaxText (third-party, not vendored), so th
 Query head h reads key head h // (H // Hkv).  Types: bf16 and f16, head dims 64, 128 and 256; scores and sums are f32, and
 every output is rounded once.  Sequence ends, lengths and page tables stay on the device: no call waits for the GPU, and
 all of them can be captured in a graph.  What the device holds is not checked on the host; entries outside their range are
-held to it, so that nothing outside the tensors is read or written.
+held to it, so that nothing outside the tensors is read or written; like any input it has to stay as it is until a call's
+kernels have run.
 """
 from __future__ import annotations
 
@@ -167,11 +168,16 @@ def causal_attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, scale=None, 
     that sees no key gives zeros.  scale (default D ** -0.5) multiplies the scores.
 
     Returns o in q's shape and dtype, and with return_lse also the natural logarithm of each row's sum of exponentials, f32
-    [B, Tq, H] or [Tq, H] (-inf for a row without keys).  Both are differentiable (once); rows of packed tensors behind the
-    last sequence give zeros and get zero gradients.  A masked key never counts, whatever k holds there; a value of v that is
+    [B, Tq, H] or [Tq, H] (-inf for a row without keys, whose upstream gradient counts for nothing).  Both are differentiable
+    (once, in backward mode); rows of packed tensors behind the last sequence give zeros and get zero gradients.  Where a
+    gradient will be taken, o is divided by the sum of the weights as they were rounded, which is a little more exact: its
+    last bits differ from those of a call without gradients, so reentrant activation checkpointing, which makes both, passes
+    on another o than it recomputes.  A masked key never counts, whatever k holds there; a value of v that is
     not finite may also reach queries up to 62 before the first that sees it (its weight there is 0, and 0 x inf is NaN), and
-    in the backward any input that is not finite gradients of rows up to 95 away.  Strides are free as long as the last axis
-    is contiguous: q, k and v may be views of one projection's output.  While a training step is captured in a graph no eager
+    in the backward any input that is not finite gradients of rows up to 95 away, of its own sequence.  Strides are free;
+    q, k and v that are views of one projection's output are read in place, and copied are tensors whose last axis is not
+    contiguous, whose rows or heads do not start on 16 bytes, overlap or lie 2^22 elements apart, or, dense, whose sequences do
+    not follow each other at the rows' stride ([B, H, T, D] transposed).  While a training step is captured in a graph no eager
     autograd graph of the same leaves may live (torch's accumulators of those leaves belong to the other stream)."""
     what = "causal_attention"
     if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape or k.shape[-1] != q.shape[-1]:

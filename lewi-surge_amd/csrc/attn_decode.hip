@@ -8,9 +8,10 @@
 // 4 D flops a query head needs for them are a few percent of the matrix cores' rate even with one head a group.  The keys'
 // fragments come straight from memory; the values are read in whole rows (256 bytes at D = 128, in the order in which the
 // weights lie in their lanes) and turned by byte permutes, 4 for each 4 registers: no LDS on the way, so that every wave
-// keeps one or two tiles of loads in flight.  Measured: 64 sequences of 4150 tokens on average, 8 key heads of 128: 192 us,
-// 5.7 TB/s (a copy reaches 5.0 reading and writing); 2 of 120000, 4 heads: 88 us and 6 for the join, 5.2 TB/s; 96 of 900,
-// 16 heads of 64: 73 us and 5, 4.6 TB/s; one of 777 tokens: 10 us and 4, a chain of trips to memory.
+// keeps one or two tiles of loads in flight.  Measured: 64 sequences of 4150 tokens on average, 8 key heads of 128: 193 us,
+// 5.6 TB/s (a copy reaches 5.0 reading and writing); 2 of them of 256: 107 us and 5 for the join, 5.1 TB/s; 2 of 120000, 4
+// heads of 128: 89 us and 6, 5.1 TB/s; 96 of 900, 16 heads of 64: 71 us and 5, 4.6 TB/s; one of 777 tokens: 10 us and 4, a
+// chain of trips to memory.
 #include <algorithm>
 
 #include "attn_common.h"
