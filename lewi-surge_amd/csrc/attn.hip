@@ -91,6 +91,12 @@ template <int D> constexpr int STAGES = D == 256 ? 3 : 4;
 constexpr int BN = 64;  // keys per stage of the pass over queries
 
 constexpr float LAZY = 8.f;  // log2 of the growth of a row's largest weight that the base lets pass
+// log2 of the f16 weights' room above that: one below 2^-25 of the largest would be none, though thousands of them may hold a
+// share of the row that counts, so the base is taken lower, and the sums have the factor too.  4 is a constant that the fma
+// takes, so it costs nothing (7: an instruction and 1%, or a register, which undoes the loop's schedule, and 7%).  Weights are
+// off by 2^-29 of the largest at most, 2^18 of them by half of f16's step, and stay in its range up to scores of 2^26 (base 2,
+// with an f32 step of 4).
+constexpr float LIFT = 4.f;
 
 // acc *= f.  At D = 256 the accumulators fill half of the registers and have to stay in the accumulation file, which the
 // vector unit cannot work on: written as plain products, the compiler moves all of them to the other file and back in
@@ -289,12 +295,7 @@ void attn_fwd_kernel(AttnArgs a, int parts, float* __restrict__ po, f32x4* __res
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = halves(mx, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
-    if constexpr (DT == LSURGE_F16) {
-      // as an fma it would hold a register more, the one that undoes the schedule below (3 chunks, 128-wide: 222 us, 207 so)
-#pragma clang fp contract(off)
-      mx = mx - (ROOM<DT> - LAZY);
-    }
+    mx = fmaf(halves(mx, [](float x, float y) { return fmaxf(x, y); }), a.scale2, DT == LSURGE_F16 ? -LIFT : 0.f);
     // the weights' base follows the maximum only when it has grown by 2^8: any base does, and f32 sums and 16-bit weights
     // have room for it, so that the accumulators are rescaled in few stages
     mx = mx > m + LAZY ? mx : m;

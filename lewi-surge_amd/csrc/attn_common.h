@@ -63,11 +63,6 @@ __device__ __forceinline__ float add2(uint32_t v, float c) {
                                            false);
 }
 
-// log2 of the room that a row's weights are given, as operands of their product with V: f16 has few exponent bits, and a
-// weight below 2^-25 of the largest would be none, though thousands of them may hold a share of the row that counts, so the
-// base is taken that much below the largest score and the sums of the weights have the same factor.  Not needed in bf16.
-template <int DT> constexpr float ROOM = DT == LSURGE_F16 ? 15.f : 0.f;
-
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // a value's partner in the other half of the wave (lane ^ 32), combined with op; both halves get the result

@@ -69,6 +69,15 @@ __device__ __forceinline__ int64_t div64(int64_t n, int64_t d) {
   return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
 }
 
+// log2 of the room that a row's weights are given above 1, as operands of their product with V: f16 has few exponent bits,
+// and a weight below 2^-25 of the largest would be none, though thousands of them may hold a share of the row that counts.
+// The base is taken that much below the largest scaled score `top`, and the sums of the weights have the same factor.  2^15,
+// less where the roundings of the base (2^-24 of top each, two of them) leave the largest score above it.  Not needed in bf16.
+template <int DT>
+__device__ __forceinline__ float room(float top) {
+  return DT == LSURGE_F16 ? fmaxf(fmaf(fabsf(top), -0x1p-23f, 15.f), 0.f) : 0.f;
+}
+
 template <int D, int DT>
 __global__ __launch_bounds__(DT_THREADS) __attribute__((amdgpu_waves_per_eu(decode_eu(D))))
 void attn_decode_kernel(DecodeArgs a) {
@@ -202,8 +211,9 @@ void attn_decode_kernel(DecodeArgs a) {
     f32x4 acc[VE];
 #pragma unroll
     for (int t = 0; t < VE; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // m: the largest score so far times the scale, less ROOM, as rounded.  Weights, sums and the join all take this one value as their
-    // base: the product formed anew inside an fma would be the unrounded one, a factor of 2^(its rounding) for every tile.
+    // m: the largest score so far times the scale, less its room, as rounded.  Weights, sums and the join all take this one value
+    // as their base: the product formed anew inside an fma would be the unrounded one, a factor of 2^(its rounding) for every
+    // tile.
     float m = -INFINITY, l = 0.f;
 
     auto compute = [&](int key0, Tile& x, auto&& after_scores) {
@@ -227,7 +237,8 @@ void attn_decode_kernel(DecodeArgs a) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(m, halves(mx, [](float p, float q) { return fmaxf(p, q); }) * a.scale2 - ROOM<DT>);
+      mx = halves(mx, [](float p, float q) { return fmaxf(p, q); }) * a.scale2;
+      mx = fmaxf(m, mx - room<DT>(mx));
       const float mc = mx == -INFINITY ? 0.f : mx;
       const float alpha = exp2_hw(m - mc);  // 1 where the largest score stays
       m = mx;

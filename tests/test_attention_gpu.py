@@ -696,8 +696,8 @@ def test_f16_decode_weights_far_below_the_largest(D, dev):
 @pytest.mark.parametrize("grad", [False, True])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_f16_forward_weights_far_below_the_largest(D, grad, dev):
-    """Value -1 for the one: o = (W - 1) / (W + 1), -0.997.  The others' weights are held as 2^-18.5 at least (the base may
-    lag behind the largest score by 2^8), within half a subnormal step, 2^-25, or 2^-6.5 of themselves, which counts twice
+    """Value -1 for the one: o = (W - 1) / (W + 1), -0.997.  The others' weights are held as 2^-21.5 at least (the base may
+    lag behind the largest score by 2^8), within half a subnormal step, 2^-25, or 2^-3.5 of themselves, which counts twice
     in o; o's own rounding is 2^-12 of less than 1, but 2^-11 is allowed, and 2^-20 for f32.  128 rows of 768 heads leave the
     keys in one part; the last rows see up to 127 keys more, of weight e^-1060."""
     k, v, scale = (x.to(dev) if torch.is_tensor(x) else x for x in flat_rows(D, -1.0))
@@ -707,7 +707,7 @@ def test_f16_forward_weights_far_below_the_largest(D, grad, dev):
     o = A.causal_attention(q, *(x[None].detach().requires_grad_(grad) for x in (k, v)), scale=scale).detach()
     assert o.shape == q.shape and (o == o[:, :, :1, :1]).all()
     o = o[0, :, 0, :1]
-    _within(o, np.full(o.shape, (FLAT - 1) / (FLAT + 1)), np.full(o.shape, 2 * FLAT * 2.0 ** -6.5 + 2.0 ** -11 + 2.0 ** -20), "o")
+    _within(o, np.full(o.shape, (FLAT - 1) / (FLAT + 1)), np.full(o.shape, 2 * FLAT * 2.0 ** -3.5 + 2.0 ** -11 + 2.0 ** -20), "o")
 
 
 @pytest.mark.parametrize("dt", [BF16, F16])
@@ -807,3 +807,30 @@ def test_traced_without_gradients_then_trained(dev):
         got, want = traced(*x), call(*x)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, x, (do, dl)), torch.autograd.grad(want, x, (do, dl))))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f16_scores_past_the_roundings_of_their_base(D, dev):
+    """Scores of 2^24 to 2^25.5, in base 2 up to 2^26, where an f32 step is 4.  The scores are exact here (17 bits and the 4 of
+    a sum over D / 16), so each row is the mean of the values at its largest ones, whose weights are alike, rounded to 2^-11 of
+    themselves, and o to 2^-11.  lse has six roundings in f32: log2 e, its product with the score, the room below it, the
+    logarithm of the sum added, log 2, its product."""
+    gen = torch.Generator().manual_seed(D)
+    n, scale = 300, 8 / D
+    k, v = torch.full((n, 1, D), 2048.0, dtype=F16), _randn(gen, (n, 1, D), F16, "cpu")
+    k[7] = k[200] = 3008.0
+    q = (1025.0 + 3 * torch.arange(n)).view(n, 1, 1).repeat(1, 2, D).to(F16)
+    q[:, 1] *= -1  # the largest scores are the small keys'
+    want, want_lse = ao.attention(_np(q), _np(k), _np(v), scale)
+    off = 2.1 * 2.0 ** -11 * ao.attention(_np(q), _np(k), np.abs(_np(v)), scale)[0]
+    step = 6 * 2.0 ** -24 * np.abs(want_lse)
+    for grad in (False, True):
+        o, lse = A.causal_attention(q[None].to(dev), *(t[None].to(dev).requires_grad_(grad) for t in (k, v)), scale=scale,
+                                    return_lse=True)
+        _within(lse[0], want_lse, step, "lse")
+        _within(o[0], want, off, "o")
+    kc, vc, table = shared_cache(k, v, 16, n, F16, dev)
+    lens = torch.arange(1, n + 1, dtype=torch.int32, device=dev)
+    o, lse = A.paged_attention(q.to(dev), kc, vc, table, lens, scale=scale, return_lse=True)
+    _within(lse, want_lse, step, "lse, decode")
+    _within(o, want, off, "o, decode")
