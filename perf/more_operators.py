@@ -160,6 +160,8 @@ def _slots(c, s, r):
     # the sequences, longest first
     s["order"] = sorted(s["used"], key=lambda b: -s["new"][b])
     s["order_gpu"] = torch.tensor(s["order"], device="cuda")
+    s["seq"] = torch.tensor([b for b, n in enumerate(s["new"]) for _ in range(n)], device="cuda")
+    s["pos"] = torch.tensor([p for n in s["new"] for p in range(n)], device="cuda")
 
 
 def _inv_freq(rot):
@@ -192,13 +194,13 @@ def prepare(case, seed):
         s["x"], s["w"] = r(total, c["C"]), r(c["K"], 1, c["C"], std=0.5)
         s["state"], s["silu"] = r(c["n"] + 3, c["K"] - 1, c["C"]), c["silu"]
         _slots(c, s, r)
+        s["heads"] = [(s["pos"] < back).nonzero()[:, 0] for back in range(c["K"])]
         return s
     hq, hk, D = c["hq"], c["hk"], c["D"]
     # each row's position: a sequence's new tokens are its last
     s["pos"] = torch.tensor([p for m, n in zip(new, keys) for p in range(n - m, n)], device="cuda")
+    s["seq"] = torch.tensor([b for b, m in enumerate(new) for _ in range(m)], device="cuda")
     s["rot"], s["inter"], s["inv_freq"] = c["rot"], c["inter"], _inv_freq(c["rot"])
-    if own:
-        s["freqs"] = _module("attention").rotary_frequencies(c["rot"], inv_freq=s["inv_freq"])
     if c["kind"] == "append":
         page, need = c["page"], [-(-n // c["page"]) for n in keys]
         pages = sum(need) + 3
@@ -221,8 +223,7 @@ def prepare(case, seed):
         s["q"], s["k"] = rows[:, :hq], rows[:, hq:hq + hk]
         s["cu"] = torch.tensor(_ends(new), **i32)
     s["dq"], s["dk"] = r(*s["q"].shape), r(*s["k"].shape)
-    if own:
-        s["q"].requires_grad_(True), s["k"].requires_grad_(True)
+    s["q"].requires_grad_(True), s["k"].requires_grad_(True)
     return s
 
 
@@ -253,10 +254,10 @@ def _run_own(s):
         return [y, s["state"]]
     attention = _module("attention")
     if kind == "append":
-        q = attention.rotary_append_kv(s["q"], s["k"], s["v"], s["kc"], s["vc"], s["table"], s["lens"], s["freqs"],
+        q = attention.rotary_append_kv(s["q"], s["k"], s["v"], s["kc"], s["vc"], s["table"], s["lens"], s["inv_freq"],
                                        cu_seqlens=s["cu"], interleaved=s["inter"], return_k=s["keep_k"])
         return [*(q if s["keep_k"] else (q,)), s["kc"], s["vc"]]
-    out = attention.rotary(s["q"], s["k"], s["freqs"], cu_seqlens=s["cu"], interleaved=s["inter"])
+    out = attention.rotary(s["q"], s["k"], s["inv_freq"], cu_seqlens=s["cu"], interleaved=s["inter"])
     grads = torch.autograd.grad(out, (s["q"], s["k"]), (s["dq"], s["dk"]))
     return [*(t.detach() for t in out), *grads]
 
@@ -292,23 +293,25 @@ def _plain_gdn(s):
 def _plain_conv(s):
     x, w, state = s["x"], s["w"][:, 0].float(), s["state"]
     K = w.shape[0]
-    y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+    used = s["order_gpu"]
+    slots = s["slots"].long()
     if s["step"]:
-        used = s["order_gpu"]
-        slots = s["slots"].long()[used]
-        seen = torch.cat([state[slots], x[used][:, None]], 1)
+        seen = torch.cat([state[slots[used]], x[used][:, None]], 1)
+        y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
         y[used] = (seen.float() * w).sum(1)
-        state[slots] = seen[:, 1:]
+        state[slots[used]] = seen[:, 1:]
     else:
-        a = 0
-        for b, n in enumerate(s["new"]):
-            slot = s["slots"][b:b + 1].long()
-            seen = torch.cat([state[slot][0], x[a:a + n]], 0)
-            f = seen.float()
-            for j in range(K):
-                y[a:a + n] += f[j:j + n] * w[j]
-            state[slot] = seen[n:][None]
-            a += n
+        y = x.float() * w[K - 1]
+        last = s["cu"].long()[1:] - 1
+        left = []
+        for back in range(K - 1, 0, -1):  # the input `back` rows before each, a sequence's first ones from its state
+            before = x.roll(back, 0)
+            head = s["heads"][back]
+            before[head] = state[slots[s["seq"][head]], K - 1 + s["pos"][head] - back]
+            y += before.float() * w[K - 1 - back]
+            if back < K - 1:
+                left.append(before[last])
+        state[slots] = torch.stack([*left, x[last]], 1)
     if s["silu"]:
         y = y / (1 + torch.exp(-y))
     return [y.to(x.dtype), state]
@@ -340,13 +343,9 @@ def _run_plain(s):
     rot, inter = s["rot"], s["inter"]
     if s["kind"] == "append":
         q, k = (_rotate(s[n], angle, rot, inter) for n in ("q", "k"))
-        page, at = s["kc"].shape[1], 0
-        for b, (m, n) in enumerate(zip(s["new"], s["keys"])):
-            tok = torch.arange(n - m, n, device=q.device)
-            where = s["table"][b][tok // page].long(), tok % page
-            s["kc"][where] = k[at:at + m]
-            s["vc"][where] = s["v"][at:at + m]
-            at += m
+        page = s["kc"].shape[1]
+        where = s["table"][s["seq"], s["pos"] // page].long(), s["pos"] % page
+        s["kc"][where], s["vc"][where] = k, s["v"]
         return [q, k, s["kc"], s["vc"]] if s["keep_k"] else [q, s["kc"], s["vc"]]
     flat = [s[n].detach().flatten(0, -3) for n in ("q", "k", "dq", "dk")]
     out = [_rotate(t, angle, rot, inter, sg) for t, sg in zip(flat, (1.0, 1.0, -1.0, -1.0))]
@@ -444,8 +443,10 @@ def exact(case, seed):
                 for n, sg in (("q", 1), ("k", 1), ("dq", -1), ("dk", -1))]
     q, k = (_exact_rotated(s[n], pos, c, 1) for n in ("q", "k"))
     kc, vc = s["kc"].double(), s["vc"].double()
-    seq = [b for b, m in enumerate(s["new"]) for _ in range(m)]
-    page = s["table"][seq, pos // c["page"]].long()
-    kc[page, pos % c["page"]] = k
-    vc[page, pos % c["page"]] = s["v"].double()
+    table, at = s["table"].tolist(), 0
+    for b, (m, n) in enumerate(zip(s["new"], s["keys"])):
+        page = torch.tensor([table[b][t // c["page"]] for t in range(n - m, n)], device="cuda")
+        slot = torch.arange(n - m, n, device="cuda") % c["page"]
+        kc[page, slot], vc[page, slot] = k[at:at + m], s["v"][at:at + m].double()
+        at += m
     return [q, k, kc, vc] if c["keep_k"] else [q, kc, vc]
