@@ -496,6 +496,75 @@ int lsurge_kv_append(const lsurge_kv_cache* c, const lsurge_attn_rows* k, const 
                      int64_t nseq, const int32_t* cu, lsurge_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * New tokens of a hybrid model's sequences: the linear layers' states, and the position rotation of the softmax layers' heads
+ * (no reference counterpart: MaxText's decode and attention, third-party and not vendored).
+ * ------------------------------------------------------------------------------------------------ */
+
+/* The convolution of lsurge_causal_conv1d over new rows only.  x: rows of `channels` values x_stride elements apart, packed:
+ * sequence b holds the rows [cu[b], cu[b + 1]) (cu [nseq + 1] i32 on the device, ascending from 0), or with cu = NULL the one
+ * row b (rows = nseq).  Its last taps - 1 inputs before them stand in slot slots[b] (NULL: b) of state, [num_slots] of
+ * [taps - 1, channels], oldest first, slot_stride elements apart; the sequence's last taps - 1 inputs, the new ones counted,
+ * replace them.  y [rows, channels] = f(sum_j w[j] x[t - (taps - 1) + j]), f32 sums, one rounding, f the identity or
+ * f(s) = s / (1 + e^-s).  A sequence without rows keeps its state; a slot outside [0, num_slots) is none: y = 0 and nothing
+ * written, as for rows behind the last sequence.  No two sequences with rows may name one slot.  x, w [taps, channels], state
+ * and y of dtype (LSURGE_BF16, LSURGE_F16), 16-byte aligned; channels, x_stride and slot_stride multiples of 8, 2 to 8 taps. */
+enum { LSURGE_ACT_NONE = 0, LSURGE_ACT_SILU = 1 };
+typedef struct {
+  const void *x, *w;
+  void *state, *y;
+  const int32_t *slots, *cu;
+  int64_t rows, nseq, channels, taps, x_stride, num_slots, slot_stride;
+  int dtype, activation;
+} lsurge_conv_update;
+int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t stream);
+
+/* The gated delta rule token by token, from and to states that are kept:  per sequence and value head h, S [128, 128] f32,
+ *   S <- e^g S,  d = beta (v - S^T k),  S <- S + k d^T,  o = S^T q / sqrt(128),
+ * q and k of head h / (hv / hk).  q, k [rows, hk, 128] and v [rows, hv, 128] by strides (any multiples of 8), dtype LSURGE_BF16
+ * or LSURGE_F16; g [rows, hv] f32 (log decay) and beta [rows, hv] of dtype or LSURGE_F32 (beta_dtype), rows g_stride and
+ * beta_stride elements apart; o [rows, hv, 128] of dtype.  l2_eps >= 0: q and k are first multiplied by rsqrt(sum x^2 + l2_eps)
+ * (not rounded in between); negative: taken as they are.  Packed rows, slots and rows without one as for
+ * lsurge_causal_conv1d_update; state: [num_slots] of [hv, 128, 128] f32, slot_stride elements apart (a multiple of 4),
+ * 16-byte aligned.  Products and states are f32; results of a sequence do not depend on the others.  Workspace (it may be 0)
+ * from lsurge_gdn_recurrent_workspace_bytes. */
+typedef struct {
+  lsurge_attn_rows q, k, v;
+  const float* g;
+  const void* beta;
+  float* state;
+  void* o;
+  const int32_t *slots, *cu;
+  int64_t rows, nseq, hk, hv, g_stride, beta_stride, num_slots, slot_stride;
+  float l2_eps;
+  int dtype, beta_dtype;
+} lsurge_gdn_tokens;
+size_t lsurge_gdn_recurrent_workspace_bytes(const lsurge_gdn_tokens* t);
+int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
+
+/* Rotation of heads by their token's position p: pair i of a head's first rotary_dim values, (x_i, x_{i + rotary_dim / 2}) or,
+ * interleaved, (x_2i, x_{2i + 1}), turned by the angle p inv_freq[i] (inverse != 0: by its negative); the values behind them
+ * stay.  inv_freq [rotary_dim / 2] f64 on the device (angles are formed in 64 bits); rotary_dim a multiple of 16 up to d.
+ * positions [rows] i32 on the device, or NULL: a row's place in its sequence. */
+typedef struct {
+  const double* inv_freq;
+  const int32_t* positions;
+  int64_t rotary_dim;
+  int interleaved, inverse, dtype;
+} lsurge_rotary;
+/* q [rows, hq, d] and k [rows, hk, d] (by strides, any multiples of 8; hq or hk may be 0) to q_out and k_out (contiguous), d 64,
+ * 128 or 256.  Sequences are packed by cu [nseq + 1], or with cu = NULL of rows / nseq rows each (nseq = 0: one).  Rows behind
+ * the last sequence: 0. */
+int lsurge_rotary_rows(const lsurge_rotary* r, const lsurge_attn_rows* q, int64_t hq, const lsurge_attn_rows* k, int64_t hk,
+                       int64_t d, int64_t rows, int64_t nseq, const int32_t* cu, void* q_out, void* k_out,
+                       lsurge_stream_t stream);
+/* lsurge_kv_append with q and k rotated first: q [rows, hq, d] to q_out (contiguous), k to its pages and, where k_out is given,
+ * to it too ([rows, heads, d], contiguous), v to its pages.  Without positions a token's is its place in its sequence.  Rows that
+ * hold no token of a sequence give 0; a token whose table entry names no page is rotated and not written.  */
+int lsurge_rotary_append(const lsurge_kv_cache* c, const lsurge_rotary* r, const lsurge_attn_rows* q, int64_t hq,
+                         const lsurge_attn_rows* k, const lsurge_attn_rows* v, int64_t rows, int64_t nseq, const int32_t* cu,
+                         void* q_out, void* k_out, lsurge_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Test hooks (no reference counterpart): failure injection for the error paths.
  * ------------------------------------------------------------------------------------------------ */
 /* Arm a host-side failure: the nth launch (counting from 1) of the kernel with profiler id kernel_id

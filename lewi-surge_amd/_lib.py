@@ -56,6 +56,23 @@ class KvCache(ctypes.Structure):
                 [(n, _i64) for n in ("num_pages", "page_size", "max_pages", "heads", "d")] + [("dtype", _int)])
 
 
+class ConvUpdate(ctypes.Structure):
+    _fields_ = ([(n, _p) for n in ("x", "w", "state", "y", "slots", "cu")] +
+                [(n, _i64) for n in ("rows", "nseq", "channels", "taps", "x_stride", "num_slots", "slot_stride")] +
+                [("dtype", _int), ("activation", _int)])
+
+
+class GdnTokens(ctypes.Structure):
+    _fields_ = ([(n, AttnRows) for n in "qkv"] + [(n, _p) for n in ("g", "beta", "state", "o", "slots", "cu")] +
+                [(n, _i64) for n in ("rows", "nseq", "hk", "hv", "g_stride", "beta_stride", "num_slots", "slot_stride")] +
+                [("l2_eps", ctypes.c_float), ("dtype", _int), ("beta_dtype", _int)])
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("inv_freq", _p), ("positions", _p), ("rotary_dim", _i64), ("interleaved", _int), ("inverse", _int),
+                ("dtype", _int)]
+
+
 _rows = ctypes.POINTER(AttnRows)
 
 # name -> (restype, argtypes)
@@ -138,6 +155,12 @@ _SIGS = {
     "lsurge_paged_attn_workspace_bytes": (_sz, [_i64] * 3),
     "lsurge_paged_attn": (_int, [ctypes.POINTER(KvCache), _rows, _i64, _i64, ctypes.c_float, _p, _p, _p, _sz, _p]),
     "lsurge_kv_append": (_int, [ctypes.POINTER(KvCache), _rows, _rows, _i64, _i64, _p, _p]),
+    "lsurge_causal_conv1d_update": (_int, [ctypes.POINTER(ConvUpdate), _p]),
+    "lsurge_gdn_recurrent_workspace_bytes": (_sz, [ctypes.POINTER(GdnTokens)]),
+    "lsurge_gdn_recurrent": (_int, [ctypes.POINTER(GdnTokens), _p, _sz, _p]),
+    "lsurge_rotary_rows": (_int, [ctypes.POINTER(Rotary), _rows, _i64, _rows, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "lsurge_rotary_append": (_int, [ctypes.POINTER(KvCache), ctypes.POINTER(Rotary), _rows, _i64, _rows, _rows, _i64, _i64,
+                                    _p, _p, _p, _p]),
     "lsurge_mfma_rate_probe_out_floats": (_sz, []),
     "lsurge_mfma_rate_probe": (_int, [_int, _int, _p, _p]),
     "lsurge_prof_enable": (_int, [_int]),

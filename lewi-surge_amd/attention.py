@@ -1,5 +1,5 @@
 """Softmax attention of the hybrid model's full-attention layers on the HIP library: whole prompts and training, and one
-new token per sequence over a paged key-value cache.
+new token per sequence over a paged key-value cache; and the rotation of its queries and keys by their positions.
 
 The Gated DeltaNet block (fast_conv, gdn_fast) mixes a sequence in the model's linear layers; these operators do it in the
 others.  The reference leaves them to MaxText (third-party, not vendored), so the names are this package's own.
@@ -10,6 +10,13 @@ others.  The reference leaves them to MaxText (third-party, not vendored), so th
       an empty key and value cache [num_pages, page_size, kv_heads, head_dim]
   append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None)
       new tokens' keys and values written to their pages, in place
+  rotary_inv_freq(rotary_dim, theta=10000.0, device="cuda")
+      the rotation's angles a position, float64 [rotary_dim / 2]
+  rotary(q, k, inv_freq, positions=None, cu_seqlens=None, interleaved=False)
+      differentiable; queries and keys of prompts and training turned by their positions, dense or packed
+  rotary_append_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens=None, positions=None,
+                   interleaved=False, return_k=False)
+      append_kv with q and k turned on the way (inference only); returns the turned q
   paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=None, return_lse=False)
       one query token per sequence over its cached tokens (inference only)
 
@@ -25,60 +32,21 @@ import ctypes
 import math
 
 import torch
-from torch.autograd import forward_ad
 
 import _lib as L
+from _calls import aligned as _aligned, call as _call, check_device as _check_device, check_dtype as _check_dtype
+from _calls import check_index as _check_index, check_no_grad as _check_no_grad, ptr as _ptr, rows as _rows
+from _calls import rows_arg as _rows_arg, step as _step
 
 HEAD_DIMS = (64, 128, 256)
 
 
 def _check_heads(what, q_heads, kv_heads, d, *ts):
-    L.require_cuda(*ts)
-    device = ts[0].device
-    for t in ts:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on one device (got {device} and {t.device})")
+    _check_device(what, *ts)
     if d not in HEAD_DIMS:
         raise ValueError(f"{what}: head dim must be one of {HEAD_DIMS} (got {d})")
     if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"{what}: {q_heads} query heads are no multiple of {kv_heads} key heads")
-
-
-def _check_dtype(what, *ts):
-    dt = ts[0].dtype
-    for t in ts:
-        if t.dtype is not dt or dt is not torch.bfloat16 and dt is not torch.float16:
-            raise TypeError(f"{what}: tensors must all be bfloat16 or all float16 (got {[str(t.dtype) for t in ts]})")
-
-
-def _check_no_grad(what, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
-    # no level is open outside of forward-mode code (unpack_dual would say so too, 0.3 us a tensor)
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
-        raise ValueError(f"{what}: no gradient, of the forward mode neither; call it on detached tensors")
-
-
-def _check_index(what, name, t, shape):
-    if t.dtype is not torch.int32 or t.shape != shape:
-        raise ValueError(f"{what}: {name} must be int32 of shape {shape} (got {t.dtype}, {tuple(t.shape)})")
-    return L.contig(t)
-
-
-def _call(what, device, fn, *args):
-    """fn(*args, the current stream of `device`), with `device` current while its kernels are launched.  The stream's bare
-    handle: a Stream object around it costs 2 us, as much as a short call's launch."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
-    L.check(rc, what)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _scale(what, scale, d):
@@ -86,26 +54,6 @@ def _scale(what, scale, d):
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"{what}: scale must be positive and finite (got {scale})")
     return scale
-
-
-def _rows(t, min_row=None):
-    """t [rows, heads, D] as the kernels read it, by strides: a copy only where its last axis is not contiguous, a row or
-    head does not start on 16 bytes, or (min_row) rows overlap or lie too far apart."""
-    if t.is_contiguous():
-        return _aligned(t)
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
-    if min_row is not None:
-        ok = ok and min_row <= t.stride(0) < 1 << 22
-    return t if ok else t.contiguous()
-
-
-def _aligned(t):
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _rows_arg(t):
-    row, head = (t.shape[1] * t.shape[2], t.shape[2]) if t.is_contiguous() else t.stride()[:2]
-    return L.AttnRows(t.data_ptr(), row, head)
 
 
 def _forward(q, k, v, cu_q, cu_k, nseq, scale, want_lse, training):
@@ -245,20 +193,6 @@ def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
     return arg, (table, lens)
 
 
-class _Step(torch.autograd.Function):
-    """fn(*args) as one step of a trace."""
-
-    @staticmethod
-    def forward(ctx, fn, *args):
-        return fn(*args)
-
-
-def _step(fn, *args):
-    """fn(*args), which has no gradient: plainly, 3 us less than an autograd function takes, but as one where torch.jit
-    traces, which would otherwise record the empty output and not the call that fills it."""
-    return _Step.apply(fn, *args) if torch.jit.is_tracing() else fn(*args)
-
-
 def append_kv(k_cache, v_cache, page_table, seq_lens, k, v, cu_seqlens=None):
     """Write new tokens into a paged cache, in place.  k, v [rows, Hkv, D]: one token for each sequence, or with cu_seqlens
     (int32 [sequences + 1]) the rows cu_seqlens[b] .. cu_seqlens[b + 1] of sequence b.  They become the last of its
@@ -321,3 +255,143 @@ def _paged(q, k_cache, v_cache, page_table, seq_lens, scale, return_lse):
           ws.numel())
     del keep
     return o, lse
+
+
+def rotary_inv_freq(rotary_dim, theta=10000.0, device="cuda"):
+    """theta ** (-2 i / rotary_dim) for pair i: the angle that each position adds, float64 [rotary_dim / 2].  Scaled variants
+    are the caller's own tensors of that form."""
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    return torch.pow(torch.full_like(i, float(theta)), -2 * i / rotary_dim)
+
+
+def _rotary_arg(what, d, rows, like, inv_freq, positions, interleaved, inverse=False):
+    """The C call's lsurge_rotary, and what it points at."""
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64:
+        raise ValueError(f"{what}: inv_freq must be float64 [rotary_dim / 2], since float32 loses the angles of far positions "
+                         f"(got {inv_freq.dtype}, {tuple(inv_freq.shape)})")
+    rot = 2 * inv_freq.shape[0]
+    if not 16 <= rot <= d or rot % 16:
+        raise ValueError(f"{what}: rotary_dim must be a multiple of 16 from 16 to the head dim {d} (got {rot})")
+    inv_freq = L.contig(inv_freq)
+    if positions is not None:
+        positions = _check_index(what, "positions", positions, rows).view(-1)
+    arg = L.Rotary(inv_freq.data_ptr(), _ptr(positions), rot, bool(interleaved), inverse, L.dt(like))
+    return arg, (inv_freq, positions)
+
+
+def _rotate(q, k, inv_freq, positions, cu, interleaved, inverse, nseq, shape):
+    """Rows q and k (either may be None) turned, or by `inverse` turned back."""
+    like = k if q is None else q
+    d = like.shape[-1]
+    arg, keep = _rotary_arg("rotary", d, shape, like, inv_freq, positions, interleaved, inverse)
+    ts = [None if t is None else _rows(t) for t in (q, k)]
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
+    rows = [(None, 0) if t is None else (_rows_arg(t), t.shape[1]) for t in ts]
+    _call("rotary", like.device, L.lib().lsurge_rotary_rows, arg, *rows[0], *rows[1], d, like.shape[0], nseq, _ptr(cu),
+          _ptr(outs[0]), _ptr(outs[1]))
+    del keep
+    return outs
+
+
+class _RotaryFn(torch.autograd.Function):
+    """Always called through here, as _AttnFn is.  The backward turns the gradients back."""
+
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, positions, cu, interleaved, nseq, shape):
+        ctx.save_for_backward(inv_freq, positions, cu)
+        ctx.rest = interleaved, nseq, shape
+        ctx.dtype = q.dtype
+        ctx.set_materialize_grads(False)
+        return tuple(_rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq, shape))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        inv_freq, positions, cu = ctx.saved_tensors
+        interleaved, nseq, shape = ctx.rest
+        if dq is not None or dk is not None:
+            dq, dk = (None if t is None else t.to(ctx.dtype) for t in (dq, dk))
+            dq, dk = _rotate(dq, dk, inv_freq, positions, cu, interleaved, True, nseq, shape)
+        return dq, dk, None, None, None, None, None, None
+
+
+def rotary(q, k, inv_freq, positions=None, cu_seqlens=None, interleaved=False):
+    """q and k with the first rotary_dim = 2 len(inv_freq) values of every head turned pair by pair by their token's position p:
+    (a, b) -> (a cos p f_i - b sin p f_i, b cos p f_i + a sin p f_i), where pair i is the values i and i + rotary_dim / 2, or
+    with interleaved 2 i and 2 i + 1.  Dense q [B, T, H, D], k [B, T, Hkv, D], or packed q [T, H, D], k [T, Hkv, D] with
+    cu_seqlens (int32 [sequences + 1] on the device) or positions.  positions: int32 of q.shape[:-2]; without them a token's is
+    its place in its sequence.  inv_freq: float64 [rotary_dim / 2] (rotary_inv_freq), a constant; angles are formed in 64 bits,
+    the rotation in 32, the outputs rounded once.
+
+    Returns new tensors (q, k), differentiable once, in backward mode: the gradients are turned back.  Rows behind the last
+    sequence give zeros and get zero gradients.  Strides are free, as in causal_attention, which takes the result."""
+    what = "rotary"
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        raise ValueError(f"{what}: q [B, T, H, D] or [T, H, D] and k alike with its own heads (got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)})")
+    _check_heads(what, q.shape[-2], q.shape[-2], q.shape[-1], q, k, inv_freq, positions, cu_seqlens)
+    _check_dtype(what, q, k)
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: inv_freq has no gradient; detach it")
+    shape = q.shape
+    if q.dim() == 4:
+        if cu_seqlens is not None:
+            raise ValueError(f"{what}: cu_seqlens go with packed [T, H, D] tensors")
+        nseq, cu = q.shape[0], None
+        qr, kr = q.flatten(0, 1), k.flatten(0, 1)
+    else:
+        if cu_seqlens is None and positions is None:
+            raise ValueError(f"{what}: packed tensors need cu_seqlens or positions")
+        nseq, cu = 0, None
+        if cu_seqlens is not None:
+            nseq = max(cu_seqlens.numel() - 1, 0)
+            cu = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
+        qr, kr = q, k
+    qo, ko = _RotaryFn.apply(qr, kr, inv_freq, positions, cu, interleaved, nseq, shape[:-2])
+    return qo.view(shape), ko.view(k.shape)
+
+
+def rotary_append_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens=None, positions=None,
+                     interleaved=False, return_k=False):
+    """append_kv of new tokens whose queries and keys are turned first, as rotary turns them: q [rows, H, D], k, v
+    [rows, Hkv, D], everything else as append_kv takes it.  A token's position is its place in its sequence, seq_lens counted
+    back from, or positions[row] (int32 [rows]).  The turned k goes to the cache, v as it is.
+
+    Returns the turned q [rows, H, D] for paged_attention (one token a sequence) or, with the turned k [rows, Hkv, D] that
+    return_k adds, for causal_attention (prompts).  Rows that hold no token give zeros; a token whose page the table does not
+    name is turned and not written.  No gradient."""
+    what = "rotary_append_kv"
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or k.shape[1:] != k_cache.shape[2:] or q.dim() != 3 or \
+            q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: q must be [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] of the caches (got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, caches {tuple(k_cache.shape)})")
+    _check_heads(what, q.shape[1], k.shape[1], k.shape[2], q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens,
+                 positions)
+    _check_dtype(what, q, k, v, k_cache, v_cache)
+    _check_no_grad(what, q, k, v, k_cache, v_cache, inv_freq)
+    q, k = _step(_rotary_append, q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens, positions, interleaved,
+                 return_k)
+    return (q, k) if return_k else q
+
+
+def _rotary_append(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens, positions, interleaved, return_k):
+    what = "rotary_append_kv"
+    n, hq, d = q.shape
+    cache, keep = _cache_arg(what, k_cache, v_cache, page_table, seq_lens)
+    nseq = page_table.shape[0]
+    if cu_seqlens is not None:
+        cu_seqlens = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
+    elif n != nseq:
+        raise ValueError(f"{what}: {n} tokens for {nseq} sequences need cu_seqlens")
+    rotation, more = _rotary_arg(what, d, (n,), q, inv_freq, positions, interleaved)
+    q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if return_k else None
+    if nseq == 0:  # no sequence: every row is behind the last
+        q_out.zero_()
+        return q_out, k_out.zero_() if return_k else None
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    _call("rotary_append", q.device, L.lib().lsurge_rotary_append, cache, rotation, _rows_arg(q), hq, _rows_arg(k), _rows_arg(v),
+          n, nseq, _ptr(cu_seqlens), _ptr(q_out), _ptr(k_out))
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+    del keep, more
+    return q_out, k_out

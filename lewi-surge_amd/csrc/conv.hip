@@ -12,7 +12,11 @@
 // covers 512 contiguous channels of a row.  Products accumulate in f32 with one rounding to bf16.  dw: each thread
 // keeps an f32 partial over its steps, a workgroup folds its four segments' partials into one slot, and a second
 // kernel sums the slots in order (deterministic, no atomics).
+//
+// causal_conv_update_kernel is the forward of new tokens only: what a sequence's first rows reach back to are the last
+// K - 1 inputs that its slot of a state keeps, which the new rows replace.
 #include "launchers.h"
+#include "rows16.h"
 
 namespace {
 
@@ -188,6 +192,95 @@ __global__ void causal_conv_dw_reduce_kernel(const float* __restrict__ part, int
   }
 }
 
+// Packed new rows through the states.  One thread owns 8 channels over a tile of `tile` rows, as above.  The thread that
+// meets a sequence's first row computes its first K - 1 rows, also where they pass the end of its tile (the next tile leaves
+// them out), and it alone reads the slot and afterwards writes it: no other thread's row needs what it replaces.  Bound by
+// memory: x and y once, K - 1 rows read again a tile, the states read and written.
+struct UpdateArgs {
+  const bf16_t *x, *w;
+  int64_t x_stride;
+  bf16_t* state;
+  int64_t slot_stride;
+  const int32_t *slots, *cu;
+  bf16_t* y;
+  int rows, nseq, num_slots, groups, tile;
+};
+template <int K, int DT, bool SILU>
+__global__ __launch_bounds__(CT) void causal_conv_update_kernel(UpdateArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * CT + threadIdx.x;
+  const int64_t t0 = id / a.groups * a.tile;
+  if (t0 >= a.rows) return;
+  const int cg = (int)(id % a.groups);
+  const int64_t C = 8 * (int64_t)a.groups;
+  const int first = (int)t0, t1 = (int)min(t0 + a.tile, (int64_t)a.rows);
+  const bf16_t* xb = a.x + 8 * cg;
+  bf16_t* yb = a.y + 8 * cg;
+  float wk[K][8];
+#pragma unroll
+  for (int j = 0; j < K; ++j) lsrows::unpack8<DT>(*reinterpret_cast<const u32x4*>(a.w + j * C + 8 * cg), wk[j]);
+  auto x_row = [&](int64_t t) { return *reinterpret_cast<const u32x4*>(xb + t * a.x_stride); };
+
+  for (int r = first; r < t1;) {
+    const lsrows::Seq s = lsrows::seq_of(a.cu, a.nseq, a.rows, r);
+    const int slot = s.seq < 0 ? -1 : a.slots ? a.slots[s.seq] : s.seq;
+    const bool owner = s.begin >= first;  // of the sequence's first rows
+    int t = owner ? r : max(r, s.begin + K - 1);
+    const int end = owner ? min(s.end, max(t1, s.begin + K - 1)) : min(s.end, t1);
+    r = min(s.end, t1);
+    if (t >= end) continue;
+    if ((unsigned)slot >= (unsigned)a.num_slots) {
+      for (; t < end; ++t) *reinterpret_cast<u32x4*>(yb + t * C) = u32x4{0u, 0u, 0u, 0u};
+      continue;
+    }
+    u32x4 raw[K - 1];  // the K - 1 inputs before row t
+    if (owner) {
+      bf16_t* sb = a.state + slot * a.slot_stride + 8 * cg;
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) raw[j] = *reinterpret_cast<const u32x4*>(sb + j * C);
+      const int n = s.end - s.begin;
+#pragma unroll
+      for (int i = 0; i < K - 1; ++i) {  // the last K - 1 of the kept inputs and the n new ones
+        u32x4 keep = raw[K - 2];
+#pragma unroll
+        for (int j = K - 2; j > i; --j)
+          if (i + n == j) keep = raw[j];
+        if (i + n >= K - 1) keep = x_row(s.end - (K - 1) + i);
+        *reinterpret_cast<u32x4*>(sb + i * C) = keep;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) raw[j] = x_row(t - (K - 1) + j);
+    }
+    float win[K][8];
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) lsrows::unpack8<DT>(raw[j], win[j]);
+    constexpr int U = 4;  // rows loaded ahead
+    for (; t < end; t += U) {
+      u32x4 row[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) row[u] = x_row(min(t + u, end - 1));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (t + u >= end) break;
+        lsrows::unpack8<DT>(row[u], win[K - 1]);
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float acc = wk[0][i] * win[0][i];
+#pragma unroll
+          for (int j = 1; j < K; ++j) acc = fmaf(wk[j][i], win[j][i], acc);
+          o[i] = SILU ? acc * __builtin_amdgcn_rcpf(1.f + __expf(-acc)) : acc;
+        }
+        *reinterpret_cast<u32x4*>(yb + (int64_t)(t + u) * C) = lsrows::pack8<DT>(o);
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) win[j][i] = win[j + 1][i];
+      }
+    }
+  }
+}
+
 int check_conv(const void* x, const void* w, int64_t b, int64_t t, int64_t c, int64_t k) {
   LSURGE_REQUIRE(x && w, "causal_conv1d: null pointer");
   LSURGE_REQUIRE(b >= 1 && b < 65536 && t >= 1 && t < (1ll << 31) && c >= 8 && c % 8 == 0 && c < (1ll << 31) &&
@@ -196,6 +289,13 @@ int check_conv(const void* x, const void* w, int64_t b, int64_t t, int64_t c, in
                  (long long)t, (long long)c, (long long)k, CONV_KMAX);
   LSURGE_REQUIRE((t + CT_STEPS - 1) / CT_STEPS < 65536, "causal_conv1d: t=%lld too long", (long long)t);
   return LSURGE_OK;
+}
+
+// Rows a thread of the update walks: one while that leaves threads for every SIMD, then more, which reads fewer rows twice.
+int update_tile(int64_t rows, int64_t groups) {
+  int tile = 1;
+  while (tile < 32 && rows * groups / (2 * tile) >= (1 << 18)) tile *= 2;
+  return tile;
 }
 
 #define CONV_K_CASES(M) M(1) M(2) M(3) M(4) M(5) M(6) M(7) M(8)
@@ -257,6 +357,54 @@ int lsurge_causal_conv1d_bwd(const void* x, const void* w, const void* dy, int64
   const unsigned rgrid = (unsigned)std::min<int64_t>((KC + 255) / 256, 1024);
   LSURGE_LAUNCH(KID_MISC, s, hipLaunchKernelGGL(causal_conv_dw_reduce_kernel, dim3(rgrid), dim3(256), 0, s,
                                                 (const float*)part, (int)(b * groups), KC, dw));
+  return LSURGE_OK;
+}
+
+int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t stream) {
+  LSURGE_REQUIRE(u, "causal_conv1d_update: null arguments");
+  const int64_t c = u->channels, k = u->taps, rows = u->rows;
+  LSURGE_REQUIRE(c >= 8 && c % 8 == 0 && c < (1ll << 31) && k >= 2 && k <= CONV_KMAX,
+                 "causal_conv1d_update: %lld channels (a multiple of 8) and %lld taps (2 to %d)", (long long)c, (long long)k,
+                 CONV_KMAX);
+  LSURGE_REQUIRE(rows >= 0 && rows < (1ll << 30) && u->nseq >= 0 && u->nseq < (1ll << 30) && (u->cu || rows == u->nseq),
+                 "causal_conv1d_update: %lld rows of %lld sequences", (long long)rows, (long long)u->nseq);
+  if (u->dtype != LSURGE_BF16 && u->dtype != LSURGE_F16)
+    return lsurge::set_error(LSURGE_ERR_DTYPE, "causal_conv1d_update: bf16 or f16");
+  LSURGE_REQUIRE(u->activation == LSURGE_ACT_NONE || u->activation == LSURGE_ACT_SILU, "causal_conv1d_update: activation %d",
+                 u->activation);
+  if (rows == 0) return LSURGE_OK;
+  LSURGE_REQUIRE(u->num_slots >= 0 && u->num_slots < (1ll << 31) && u->slot_stride >= 0 && u->slot_stride < (1ll << 40) &&
+                     u->slot_stride % 8 == 0 && u->x_stride >= 0 && u->x_stride < (1ll << 32) && u->x_stride % 8 == 0,
+                 "causal_conv1d_update: %lld slots, strides of a slot %lld and a row %lld (multiples of 8)",
+                 (long long)u->num_slots, (long long)u->slot_stride, (long long)u->x_stride);
+  LSURGE_REQUIRE(u->x && u->w && u->y && (u->state || u->num_slots == 0), "causal_conv1d_update: null pointer");
+  LSURGE_REQUIRE(((uintptr_t)u->x | (uintptr_t)u->w | (uintptr_t)u->y | (uintptr_t)u->state) % 16 == 0,
+                 "causal_conv1d_update: buffers must be 16-byte aligned");
+  UpdateArgs a;
+  a.x = (const bf16_t*)u->x, a.w = (const bf16_t*)u->w, a.x_stride = u->x_stride;
+  a.state = (bf16_t*)u->state, a.slot_stride = u->slot_stride;
+  a.slots = u->slots, a.cu = u->cu, a.y = (bf16_t*)u->y;
+  a.rows = (int)rows, a.nseq = (int)u->nseq, a.num_slots = (int)u->num_slots, a.groups = (int)(c / 8);
+  a.tile = update_tile(rows, a.groups);
+  const int64_t threads = (rows + a.tile - 1) / a.tile * a.groups;
+  LSURGE_REQUIRE(threads < (1ll << 32), "causal_conv1d_update: %lld rows of %lld channels", (long long)rows, (long long)c);
+  const unsigned grid = (unsigned)((threads + CT - 1) / CT);
+  hipStream_t s = (hipStream_t)stream;
+#define CONV_UPDATE(KK, DT, SILU)                                                                          \
+  LSURGE_LAUNCH(KID_MISC, s, hipLaunchKernelGGL((causal_conv_update_kernel<KK, DT, SILU>), dim3(grid), dim3(CT), 0, s, a))
+#define CONV_UPDATE_K(KK)                                                      \
+  case KK:                                                                     \
+    if (u->dtype == LSURGE_BF16) {                                             \
+      if (u->activation) { CONV_UPDATE(KK, LSURGE_BF16, true); }               \
+      else { CONV_UPDATE(KK, LSURGE_BF16, false); }                            \
+    } else {                                                                   \
+      if (u->activation) { CONV_UPDATE(KK, LSURGE_F16, true); }                \
+      else { CONV_UPDATE(KK, LSURGE_F16, false); }                             \
+    }                                                                          \
+    break;
+  switch (k) { CONV_UPDATE_K(2) CONV_UPDATE_K(3) CONV_UPDATE_K(4) CONV_UPDATE_K(5) CONV_UPDATE_K(6) CONV_UPDATE_K(7) CONV_UPDATE_K(8) }
+#undef CONV_UPDATE_K
+#undef CONV_UPDATE
   return LSURGE_OK;
 }
 

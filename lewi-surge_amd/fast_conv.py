@@ -7,12 +7,20 @@ products accumulated in f32 with one rounding.
 
   applies(...)                 the reference's eligibility test (fast_conv.py:17-22)
   causal_conv1d(inputs, kernel) differentiable op: inputs [B, T, C] bf16, kernel [K, 1, C] (or [K, C]) bf16
+
+Serving keeps each sequence's last K - 1 inputs between calls and takes new ones after them (the reference leaves decoding to
+MaxText, third-party and not vendored):
+
+  alloc_conv_state(slots, taps, channels, dtype, device)  empty states [slots, K - 1, C]
+  causal_conv1d_update(inputs, kernel, state, state_slots=None, cu_seqlens=None, activation=None)
+      the convolution of packed new rows, one of each sequence or any number, the states updated in place (inference only)
 """
 from __future__ import annotations
 
 
 import torch
 
+import _calls as calls
 import _lib as L
 
 
@@ -65,4 +73,58 @@ def causal_conv1d(inputs, kernel):
     """y = causal depthwise conv of inputs [B, T, C] with kernel [K, 1, C] (modal/fast_conv.py:24-31)."""
     x, w = _check(inputs, kernel)
     y = _ConvFn.apply(x, w)
+    return y
+
+
+def alloc_conv_state(slots, taps, channels, dtype=torch.bfloat16, device="cuda"):
+    """The kept inputs of sequences that have no row yet, zeros [slots, taps - 1, channels]."""
+    return torch.zeros((slots, taps - 1, channels), dtype=dtype, device=device)
+
+
+_ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def causal_conv1d_update(inputs, kernel, state, state_slots=None, cu_seqlens=None, activation=None):
+    """causal_conv1d of new rows of sequences whose last inputs are kept.  inputs [rows, C] and kernel [K, 1, C] or [K, C],
+    2 <= K <= 8, all bfloat16 or all float16, C a multiple of 8.  Row b is the one new row of sequence b, or with cu_seqlens
+    (int32 [sequences + 1] on the device, ascending from 0) sequence b has the rows cu_seqlens[b] .. cu_seqlens[b + 1].  state
+    [slots, K - 1, C] (alloc_conv_state), oldest first, of the same dtype: sequence b's last K - 1 inputs before its new rows are
+    in slot state_slots[b] (int32 on the device; None: b), and its last K - 1 with them replace them, in place.  activation:
+    None, or "silu", y = s / (1 + exp(-s)) of the float32 sum s.  Returns y [rows, C].
+
+    A sequence without rows keeps its state.  One whose slot is outside [0, slots), such as -1 for a place of the batch that is
+    not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one slot.
+    inputs may be a view with rows of any stride.  No gradient."""
+    what = "causal_conv1d_update"
+    if kernel.dim() == 3 and kernel.shape[1] == 1:
+        kernel = kernel[:, 0]
+    if inputs.dim() != 2 or kernel.dim() != 2 or kernel.shape[1] != inputs.shape[1]:
+        raise ValueError(f"{what}: inputs must be [rows, C], kernel [K, 1, C] or [K, C] (got {tuple(inputs.shape)}, "
+                         f"{tuple(kernel.shape)})")
+    K, channels = kernel.shape
+    if not 2 <= K <= 8 or channels < 8 or channels % 8:
+        raise ValueError(f"{what}: 2 to 8 taps and a multiple of 8 channels (got {K}, {channels})")
+    if state.dim() != 3 or state.shape[1:] != (K - 1, channels):
+        raise ValueError(f"{what}: state must be [slots, {K - 1}, {channels}] (got {tuple(state.shape)})")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be None or 'silu' (got {activation!r})")
+    calls.check_device(what, inputs, kernel, state, state_slots, cu_seqlens)
+    calls.check_dtype(what, inputs, kernel, state)
+    calls.check_no_grad(what, inputs, kernel, state)
+    return calls.step(_update, inputs, kernel, state, state_slots, cu_seqlens, activation)
+
+
+def _update(x, w, state, state_slots, cu_seqlens, activation):
+    what = "causal_conv1d_update"
+    rows, channels = x.shape
+    nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
+    stride = calls.slot_stride(what, state, 8)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    w = calls.aligned(L.contig(w))
+    y = torch.empty((rows, channels), dtype=x.dtype, device=x.device)
+    arg = L.ConvUpdate(x.data_ptr(), w.data_ptr(), state.data_ptr(), y.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, channels,
+                       w.shape[0], x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
+    calls.call("causal_conv1d_update", x.device, L.lib().lsurge_causal_conv1d_update, arg)
+    torch.autograd.graph.increment_version(state)
     return y

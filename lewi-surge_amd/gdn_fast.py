@@ -15,11 +15,20 @@ work); the results are bitwise the same.  Without gradients the forward is lsurg
       f32 with the exact inverse
 With use_qk_norm_in_gdn the query and key heads are l2-normalised first (gdn_fast.py:43-46) by lsurge_l2norm_rows,
 whose backward is lsurge_l2norm_rows_bwd.
+
+Serving keeps each sequence's state between calls, in float32, and takes new tokens through it:
+
+  alloc_delta_state(slots, heads, device="cuda")
+      empty states [slots, heads, 128, 128]
+  recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=None, cu_seqlens=None, use_qk_norm_in_gdn=False)
+      the rule over packed new tokens, one of each sequence or any number, the states updated in place (inference only)
+The reference leaves decoding to MaxText (third-party, not vendored), so these names are this package's own.
 """
 from __future__ import annotations
 
 import torch
 
+import _calls as calls
 import _lib as L
 
 SAVE_RESIDUALS = True
@@ -131,6 +140,69 @@ def fast_chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initi
     res = _GdnFn.apply(q, k, v, gf, bt, h0, initial_state is not None)
     o = res[0].to(out_dtype)
     return o, (res[1].to(compute_dtype) if initial_state is not None else None)
+
+
+def alloc_delta_state(slots, heads, device="cuda"):
+    """States of sequences that have no token yet, zeros [slots, heads, 128, 128] float32."""
+    return torch.zeros((slots, heads, D, D), dtype=torch.float32, device=device)
+
+
+def recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=None, cu_seqlens=None,
+                               use_qk_norm_in_gdn=False):
+    """The gated delta rule over new tokens of sequences whose states are kept: per sequence and value head
+    S <- e^g S, d = beta (v - S^T k), S <- S + k d^T, o = S^T q / sqrt(128).
+
+    query, key [rows, Hk, 128] and value [rows, H, 128], bfloat16 or float16, head h reading query and key head
+    h // (H // Hk); g [rows, H] float32, the log decay; beta [rows, H] float32 or the others' dtype.  Row b is the one new
+    token of sequence b, or with cu_seqlens (int32 [sequences + 1] on the device, ascending from 0) sequence b has the rows
+    cu_seqlens[b] .. cu_seqlens[b + 1].  state [slots, H, 128, 128] float32 (alloc_delta_state, or the final states of
+    fast_chunk_gated_delta_rule) is updated in place: sequence b's in slot state_slots[b] (int32 on the device; None: b).
+    Returns o [rows, H, 128] in value's dtype.
+
+    A sequence without rows keeps its state.  One whose slot is outside [0, slots), such as -1 for a place of the batch that
+    is not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one
+    slot.  use_qk_norm_in_gdn: query and key heads are l2-normalised first (eps 1e-6), without the rounding of the normalised
+    heads that fast_chunk_gated_delta_rule makes.  Everything between the inputs and o is float32, so a prompt's state comes
+    out exact to float32, where the chunked form rounds as the reference does.  Strides are free: views of one projection are
+    read in place.  No gradient."""
+    what = "recurrent_gated_delta_rule"
+    if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[0] != query.shape[0] or \
+            query.shape[2] != D or value.shape[2] != D:
+        raise ValueError(f"{what}: query and key must be [rows, key heads, {D}], value [rows, heads, {D}] (got "
+                         f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)})")
+    rows, hk, hv = query.shape[0], query.shape[1], value.shape[1]
+    if hk < 1 or hv < 1 or hv % hk:
+        raise ValueError(f"{what}: {hv} value heads are no multiple of {hk} key heads")
+    if g.shape != (rows, hv) or beta.shape != (rows, hv):
+        raise ValueError(f"{what}: g and beta must be [{rows}, {hv}] (got {tuple(g.shape)}, {tuple(beta.shape)})")
+    if state.dim() != 4 or state.shape[1:] != (hv, D, D):
+        raise ValueError(f"{what}: state must be [slots, {hv}, {D}, {D}] (got {tuple(state.shape)})")
+    calls.check_device(what, query, key, value, g, beta, state, state_slots, cu_seqlens)
+    calls.check_dtype(what, query, key, value)
+    if g.dtype is not torch.float32 or state.dtype is not torch.float32 or beta.dtype not in (torch.float32, query.dtype):
+        raise TypeError(f"{what}: g and state must be float32, beta float32 or {query.dtype} (got {g.dtype}, {state.dtype}, "
+                        f"{beta.dtype})")
+    calls.check_no_grad(what, query, key, value, g, beta, state)
+    return calls.step(_recurrent, query, key, value, g, beta, state, state_slots, cu_seqlens, use_qk_norm_in_gdn)
+
+
+def _recurrent(query, key, value, g, beta, state, state_slots, cu_seqlens, norm):
+    what = "recurrent_gated_delta_rule"
+    rows, hv, _ = value.shape
+    nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
+    stride = calls.slot_stride(what, state, 4)
+    q, k, v = calls.rows(query), calls.rows(key), calls.rows(value)
+    g, beta = (t if t.stride(1) == 1 or hv == 1 else t.contiguous() for t in (g, beta))
+    o = torch.empty((rows, hv, D), dtype=v.dtype, device=v.device)
+    arg = L.GdnTokens(calls.rows_arg(q), calls.rows_arg(k), calls.rows_arg(v), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+                      o.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, q.shape[1], hv, g.stride(0), beta.stride(0),
+                      state.shape[0], stride, 1e-6 if norm else -1.0, L.dt(v), L.dt(beta))
+    lib = L.lib()
+    nbytes = lib.lsurge_gdn_recurrent_workspace_bytes(arg)
+    ws = L.workspace(nbytes, v.device) if nbytes else None
+    calls.call("gdn_recurrent", v.device, lib.lsurge_gdn_recurrent, arg, calls.ptr(ws), nbytes)
+    torch.autograd.graph.increment_version(state)
+    return o
 
 
 def install(prec="high", inv="neumann", unroll=1):
