@@ -12,6 +12,7 @@
 // Bound by memory for a token or a few (the state's 128 KiB a sequence and head), by the vector unit from about ten tokens on:
 // 4 x 128 x 128 multiply-adds a token and head, which have to follow each other.
 #include <algorithm>
+#include <type_traits>
 
 #include "launchers.h"
 #include "rows16.h"
@@ -62,43 +63,62 @@ __device__ __forceinline__ float scalar_at(const void* p, int64_t i, int f32) {
   return DT == LSURGE_F16 ? f16_to_f32(x) : bf16_to_f32(x);
 }
 
-// CB columns a wave: lane l holds the rows R (l % RG) .. + R - 1 of the columns 4 (l / RG) .. + 3, RG = 256 / CB lanes a column
-template <int DT, int CB, bool BETA32>
-__global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
-  constexpr int RG = 256 / CB, R = D / RG, V = R / 8 > 0 ? R / 8 : 1;  // V: 16-byte loads of a lane's rows of q or k
-  constexpr int BLOCKS = D / CB / WAVES;  // workgroups a (sequence, head)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x >= a.units) {  // rows behind the last sequence
-    const int64_t first = a.nseq ? lsrows::end_at(a.cu, a.nseq, a.rows) : 0;
-    const int64_t n = (a.rows - first) * a.hv * (D / 8), step = (int64_t)(gridDim.x - a.units) * 64 * WAVES;
-    u32x4* o = reinterpret_cast<u32x4*>(a.o + first * a.hv * D);
-    for (int64_t i = (int64_t)(blockIdx.x - a.units) * 64 * WAVES + threadIdx.x; i < n; i += step) o[i] = u32x4{0u, 0u, 0u, 0u};
-    return;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t x, float& lo, float& hi) {
+  if constexpr (DT == LSURGE_F16) {
+    lo = f16_to_f32((uint16_t)x);
+    hi = f16_to_f32((uint16_t)(x >> 16));
+  } else {
+    lo = __uint_as_float(x << 16);
+    hi = __uint_as_float(x & 0xffff0000u);
   }
-  const int block = blockIdx.x % BLOCKS, sh = blockIdx.x / BLOCKS, h = sh % a.hv, b = sh / a.hv;
-  const int rg = lane % RG, col = (block * WAVES + wave) * CB + lane / RG * 4;
-  const int begin = a.cu ? lsrows::end_at(a.cu, b, a.rows) : b;
-  const int end = a.cu ? lsrows::end_at(a.cu, b + 1, a.rows) : b + 1;
-  const int slot = a.slots ? a.slots[b] : b;
-  if (begin >= end) return;
+}
+
+// One (sequence, value head), its rows [begin, end) and slot.
+struct Unit {
+  int b, h, begin, end, slot;
+};
+__device__ __forceinline__ Unit unit_of(const TokenArgs& a, int sh) {
+  Unit u;
+  u.h = sh % a.hv, u.b = sh / a.hv;
+  u.begin = a.cu ? lsrows::end_at(a.cu, u.b, a.rows) : u.b;
+  u.end = a.cu ? lsrows::end_at(a.cu, u.b + 1, a.rows) : u.b + 1;
+  u.slot = a.slots ? a.slots[u.b] : u.b;
+  return u;
+}
+// workgroup i of n: the rows behind the last sequence give zeros
+__device__ __forceinline__ void clear_tail(const TokenArgs& a, int i, int n) {
+  const int64_t first = a.nseq ? lsrows::end_at(a.cu, a.nseq, a.rows) : 0;
+  const int64_t count = (a.rows - first) * a.hv * (D / 8);
+  u32x4* o = reinterpret_cast<u32x4*>(a.o + first * a.hv * D);
+  for (int64_t j = (int64_t)i * blockDim.x + threadIdx.x; j < count; j += (int64_t)n * blockDim.x) o[j] = u32x4{0u, 0u, 0u, 0u};
+}
+
+// Columns `col0` .. + CB - 1 through a unit's tokens by one wave, token by token: lane l holds the rows R (l % RG) .. + R - 1 of
+// the columns 4 (l / RG) .. + 3, RG = 256 / CB lanes a column.
+template <int DT, int CB, bool BETA32>
+__device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, int col0, int lane) {
+  constexpr int RG = 256 / CB, R = D / RG, V = R / 8 > 0 ? R / 8 : 1;  // V: 16-byte loads of a lane's rows of q or k
+  const int rg = lane % RG, col = col0 + lane / RG * 4, h = u.h;
   uint16_t* o = a.o + (int64_t)h * D + col;
   const int64_t o_row = (int64_t)a.hv * D;
-  if ((unsigned)slot >= (unsigned)a.num_slots) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  if ((unsigned)u.slot >= (unsigned)a.num_slots) {
     if (rg == 0)
-      for (int t = begin; t < end; ++t) *reinterpret_cast<u32x2*>(o + t * o_row) = u32x2{0u, 0u};
+      for (int t = u.begin; t < u.end; ++t) *reinterpret_cast<u32x2*>(o + t * o_row) = u32x2{0u, 0u};
     return;
   }
-  float* sp = a.state + slot * a.slot_stride + (int64_t)h * D * D + (int64_t)rg * R * D + col;
-  f32x4 S[R];
+  float* sp = a.state + u.slot * a.slot_stride + (int64_t)h * D * D + (int64_t)rg * R * D + col;
+  f32x4 S[R];  // the state divided by `c`
 #pragma unroll
   for (int i = 0; i < R; ++i) S[i] = *reinterpret_cast<const f32x4*>(sp + i * D);
+  float c = 1.f;
 
   const int kh = h / (a.hv / a.hk);
   const uint16_t* qp = a.q + kh * a.q_head + rg * R;
   const uint16_t* kp = a.k + kh * a.k_head + rg * R;
   const uint16_t* vp = a.v + h * a.v_head + col;
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   struct Token {
     u32x4 q[V], k[V];
     u32x2 v;
@@ -121,10 +141,10 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
     x.beta = scalar_at<DT>(a.beta, t * a.beta_row + h, BETA32);
   };
   Token cur, next;
-  load(begin, next);
-  for (int t = begin; t < end; ++t) {
+  load(u.begin, next);
+  for (int t = u.begin; t < u.end; ++t) {
     cur = next;
-    load(min(t + 1, end - 1), next);
+    load(min(t + 1, u.end - 1), next);
     float q[8 * V], k[8 * V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -139,9 +159,9 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
       qq = fmaf(q[i], q[i], qq);
       kq = fmaf(k[i], q[i], kq);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        kS[c] = fmaf(k[i], S[i][c], kS[c]);
-        qS[c] = fmaf(q[i], S[i][c], qS[c]);
+      for (int j = 0; j < 4; ++j) {
+        kS[j] = fmaf(k[i], S[i][j], kS[j]);
+        qS[j] = fmaf(q[i], S[i][j], qS[j]);
       }
     }
     kq = group_sum<RG>(kq);
@@ -150,26 +170,486 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
       rk = rsqrtf(group_sum<RG>(kk) + a.l2_eps);
       rq *= rsqrtf(group_sum<RG>(qq) + a.l2_eps);
     }
-    const float decay = expf(cur.g);
-    float v[4], out[4], kd[4];
-    v[0] = DT == LSURGE_F16 ? f16_to_f32((uint16_t)cur.v[0]) : bf16_to_f32((uint16_t)cur.v[0]);
-    v[1] = DT == LSURGE_F16 ? f16_to_f32((uint16_t)(cur.v[0] >> 16)) : bf16_to_f32((uint16_t)(cur.v[0] >> 16));
-    v[2] = DT == LSURGE_F16 ? f16_to_f32((uint16_t)cur.v[1]) : bf16_to_f32((uint16_t)cur.v[1]);
-    v[3] = DT == LSURGE_F16 ? f16_to_f32((uint16_t)(cur.v[1] >> 16)) : bf16_to_f32((uint16_t)(cur.v[1] >> 16));
+    // The decay goes to the factor c, one multiplication for the whole state, until c is far from 1.
+    c *= expf(cur.g);
+    if (!(c > 0x1p-40f && c < 0x1p40f)) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      kd[c] = rk * (cur.beta * fmaf(-decay * rk, group_sum<RG>(kS[c]), v[c]));  // rk d
-      out[c] = rq * fmaf(decay, group_sum<RG>(qS[c]), kq * kd[c]);
+      for (int i = 0; i < R; ++i) S[i] *= c;
+      kS *= c, qS *= c;
+      c = 1.f;
+    }
+    float v[4], out[4], kd[4];
+    unpack2<DT>(cur.v[0], v[0], v[1]);
+    unpack2<DT>(cur.v[1], v[2], v[3]);
+    const float ic = 1.f / c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      kd[j] = rk * (cur.beta * fmaf(-c * rk, group_sum<RG>(kS[j]), v[j]));  // rk d
+      out[j] = rq * fmaf(c, group_sum<RG>(qS[j]), kq * kd[j]);
+      kd[j] *= ic;
     }
     if (rg == 0)
       *reinterpret_cast<u32x2*>(o + t * o_row) = u32x2{lsrows::pack2<DT>(out[0], out[1]), lsrows::pack2<DT>(out[2], out[3])};
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) S[i][c] = fmaf(k[i], kd[c], decay * S[i][c]);
+      for (int j = 0; j < 4; ++j) S[i][j] = fmaf(k[i], kd[j], S[i][j]);
   }
 #pragma unroll
-  for (int i = 0; i < R; ++i) *reinterpret_cast<f32x4*>(sp + i * D) = S[i];
+  for (int i = 0; i < R; ++i) *reinterpret_cast<f32x4*>(sp + i * D) = S[i] * c;
+}
+
+// One token for each sequence.
+template <int DT, int CB, bool BETA32>
+__global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
+  constexpr int BLOCKS = D / CB / WAVES;  // workgroups a (sequence, head)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Unit u = unit_of(a, blockIdx.x / BLOCKS);
+  if (u.begin < u.end) walk_tokens<DT, CB, BETA32>(a, u, (blockIdx.x % BLOCKS * WAVES + wave) * CB, lane);
+}
+
+// ------------------------------------------------------------------------------------ runs of tokens
+// Sequences of any length, packed.  From CHUNKED tokens on a sequence goes in chunks of C = 32.  With G_i the sum of the log
+// decays up to token i of a chunk, S0 the state before it, and k and q normalised,
+//   (I + A) X = R,  R_i = beta_i (v_i - e^{G_i} S0^T k_i),  A_ij = beta_i e^{G_i - G_j} k_i.k_j (j < i),
+//   o_i = (e^{G_i} S0^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i.k_j) x_j) / sqrt(128),
+//   S = e^{G_C} S0 + sum_j e^{G_C - G_j} k_j x_j^T
+// (row i of X is the token's d).  A and the weights of o do not depend on the state: a fifth wave forms them for the next chunk
+// while four waves of 16 columns each take this one, with one barrier a chunk.
+//
+// Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
+// terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
+// the state is kept times a power of two there, its largest value between 2^8 and 2^15: what is lost is below 2^-33 of it).
+// The 16 x 16 matrices R, X, A and the inverse of A's diagonal blocks are three bf16 terms, and two where they reach o alone,
+// which is rounded to 11 bits or fewer.  A wave's 16 columns of every matrix lie in its lanes (lane l: column l % 16), so that
+// each product's result is in place as the next one's operand: the state, R and X never leave their lane.  (I + A) is solved by
+// blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
+// since differences of sums go into exponents.
+constexpr int C = 32;
+constexpr int CHUNKED = 4;
+constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
+constexpr int RUN_THREADS = 64 * 5;
+constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
+
+struct ChunkTiles {
+  uint16_t k[C][PITCH], q[C][PITCH];
+};
+struct ChunkTerms {
+  // operands of 16 x 16 x 16 products, lane l's four values (row l % 16, columns 4 (l / 16) .. + 3) at [l]
+  u32x2 inv[2][3][64];  // the inverses of the diagonal blocks of I + A
+  u32x2 a10[3][64];     // -A, rows 16.., columns ..15
+  u32x2 m00[2][64];     // the weights of o
+  u32x2 m1[2][2][64];   // their rows 16.., columns by halves
+  // by token: R = beta v - c1 (S0^T k), o = c2 (S0^T q) + .., the factor of k in the state's update
+  float beta[C], c1[C], c2[C], w[C];
+  float decay;
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mma_16(u32x2 p, u32x2 q, f32x4 c) {  // D[16 x 16] += P[16 x 16] Q[16 x 16], bf16
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, p), __builtin_bit_cast(s16x4_t, q), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ f32x4 mma_32(u32x4 p, u32x4 q, f32x4 c) {  // D[16 x 16] += P[16 x 32] Q[32 x 16]
+  typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+  if constexpr (DT == LSURGE_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, p), __builtin_bit_cast(f16x8_t, q), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+// x as a sum of N terms of DT, four values each
+template <int DT, int N>
+__device__ __forceinline__ void split(f32x4 x, u32x2* t) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    t[n] = u32x2{lsrows::pack2<DT>(x[0], x[1]), lsrows::pack2<DT>(x[2], x[3])};
+    if (n + 1 < N) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float lo, hi;
+        unpack2<DT>(t[n][i], lo, hi);
+        x[2 * i] -= lo;
+        x[2 * i + 1] -= hi;
+      }
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void split(f32x4 x, u32x2* t) { split<LSURGE_BF16, N>(x, t); }
+// orders a wave's accesses to LDS between its lanes
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// c + P Q of operands of three terms: the six products of 2^-24 and more
+__device__ __forceinline__ f32x4 mma_16_f32(const u32x2* p, const u32x2* q, f32x4 c) {
+  c = mma_16(p[2], q[0], c);
+  c = mma_16(p[1], q[1], c);
+  c = mma_16(p[0], q[2], c);
+  c = mma_16(p[1], q[0], c);
+  c = mma_16(p[0], q[1], c);
+  return mma_16(p[0], q[0], c);
+}
+__device__ __forceinline__ u32x4 join(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
+
+struct PrepareScratch {
+  double G[C];        // sums of the log2 decays
+  float rk[C], rq[C], beta[C];
+  float A[2][16][20];  // the diagonal blocks, rows 16 bytes apart
+};
+// What a chunk's products need besides the state, by one wave: its k and q from their tiles, the log decay and beta of token
+// lane % 32 (0 behind the end).
+template <int DT>
+__device__ __forceinline__ void prepare_chunk(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane,
+                                              PrepareScratch& s, ChunkTerms& out) {
+  const int c = lane & 15, g = lane >> 4;
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+  // products [token j][token i], lane: i = c, j = 4 g + r
+  f32x4 kk[3] = {zero, zero, zero}, kq[3] = {zero, zero, zero}, qq[2] = {zero, zero};  // blocks (0, 0), (1, 1), (0, 1)
+#pragma unroll
+  for (int st = 0; st < 4; ++st) {
+    u32x4 k[2], q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      k[i] = *reinterpret_cast<const u32x4*>(&x.k[16 * i + c][32 * st + 8 * g]);
+      q[i] = *reinterpret_cast<const u32x4*>(&x.q[16 * i + c][32 * st + 8 * g]);
+    }
+    kk[0] = mma_32<DT>(k[0], k[0], kk[0]);
+    kk[1] = mma_32<DT>(k[1], k[1], kk[1]);
+    kk[2] = mma_32<DT>(k[0], k[1], kk[2]);
+    kq[0] = mma_32<DT>(k[0], q[0], kq[0]);
+    kq[1] = mma_32<DT>(k[1], q[1], kq[1]);
+    kq[2] = mma_32<DT>(k[0], q[1], kq[2]);
+    qq[0] = mma_32<DT>(q[0], q[0], qq[0]);
+    qq[1] = mma_32<DT>(q[1], q[1], qq[1]);
+  }
+  // A decay below e^-104 is 0 in f32 whatever it is.
+  const int t = lane & 31;
+  double G = (double)(decay < -104.f ? -104.f : decay) * 1.4426950408889634;
+#pragma unroll
+  for (int d = 1; d < C; d *= 2) {
+    const double before = __shfl_up(G, d, C);
+    if (t >= d) G += before;
+  }
+  const double last = __shfl(G, C - 1, C);
+  if (lane < C) s.G[t] = G, s.beta[t] = beta;
+  if (g == c >> 2) {  // the diagonals hold the norms
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float k2 = kk[i][0], q2 = qq[i][0];
+#pragma unroll
+      for (int r = 1; r < 4; ++r)
+        if ((c & 3) == r) k2 = kk[i][r], q2 = qq[i][r];
+      s.rk[16 * i + c] = l2_eps >= 0.f ? rsqrtf(k2 + l2_eps) : 1.f;
+      s.rq[16 * i + c] = QSCALE * (l2_eps >= 0.f ? rsqrtf(q2 + l2_eps) : 1.f);
+    }
+  }
+  wave_sync();
+  if (lane < C) {
+    const float e = __builtin_amdgcn_exp2f((float)G), rk = s.rk[t];
+    out.beta[t] = beta;
+    out.c1[t] = beta * e * rk;
+    out.c2[t] = e * s.rq[t];
+    out.w[t] = rk * __builtin_amdgcn_exp2f((float)(last - G));
+    if (t == 0) out.decay = __builtin_amdgcn_exp2f((float)last);
+  }
+  f32x4 m[3], a10;
+#pragma unroll
+  for (int b = 0; b < 3; ++b) {
+    const int i = (b == 0 ? 0 : 16) + c, j0 = (b == 1 ? 16 : 0) + 4 * g;
+    const double Gi = s.G[i];
+    const float fa = s.beta[i] * s.rk[i], fm = s.rq[i];
+    f32x4 A;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = j0 + r;
+      const float e = j <= i ? s.rk[j] * __builtin_amdgcn_exp2f((float)(Gi - s.G[j])) : 0.f;
+      A[r] = j < i ? fa * (e * kk[b][r]) : 0.f;
+      m[b][r] = j <= i ? fm * (e * kq[b][r]) : 0.f;
+    }
+    if (b < 2) *reinterpret_cast<f32x4*>(&s.A[b][c][4 * g]) = A;
+    else a10 = -A;
+  }
+  u32x2 terms[3];
+  split<3>(a10, terms);
+#pragma unroll
+  for (int n3 = 0; n3 < 3; ++n3) out.a10[n3][lane] = terms[n3];
+#pragma unroll
+  for (int b = 0; b < 3; ++b) {
+    split<2>(m[b], terms);
+#pragma unroll
+    for (int n2 = 0; n2 < 2; ++n2) (b == 0 ? out.m00[n2] : out.m1[n2][b == 1])[lane] = terms[n2];
+  }
+  wave_sync();
+  // Row c of a block's inverse, x (I + A) = e_c, from its last value on; lanes below 32 the first block, the others the second.
+  const int blk = lane >> 5;
+  float y[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) y[j] = j == c ? 1.f : 0.f;
+#pragma unroll
+  for (int k = 15; k > 0; --k) {
+#pragma unroll
+    for (int j4 = 0; j4 < k; j4 += 4) {
+      const f32x4 row = *reinterpret_cast<const f32x4*>(&s.A[blk][k][j4]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (j4 + r < k) y[j4 + r] = fmaf(-y[k], row[r], y[j4 + r]);
+    }
+    if (k % 4 == 0) asm volatile("" ::: "memory");  // a few rows are read ahead: all of them would take 160 registers
+  }
+  // its columns 8 (g % 2) .. + 7 as operands
+  f32x4 z[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[h][r] = g & 1 ? y[8 + 4 * h + r] : y[4 * h + r];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    split<3>(z[h], terms);
+#pragma unroll
+    for (int n3 = 0; n3 < 3; ++n3) out.inv[blk][n3][c + 16 * (2 * (g & 1) + h)] = terms[n3];
+  }
+}
+
+// the largest of a column's values, from each of the four lanes that hold it
+__device__ __forceinline__ float column_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// S and its scale changed by a power of two that brings a column's `most` to 2^12 .. 2^13, where it is outside [least, 2^15)
+__device__ __forceinline__ void rescale(float most, float least, f32x4* S, float& scale, float& unscale) {
+  const bool out = most < least || most >= 0x1p15f;
+  if (__ballot(out) == 0) return;
+  const int e = out && most > 0.f ? (int)(__float_as_uint(most) >> 23) - 127 : 12;  // 2^e <= most < 2^(e + 1)
+  const int now = (int)(__float_as_uint(scale) >> 23) - 127;
+  const int n = min(max(12 - e, -60 - now), 60 - now);  // the scale within 2^-60 .. 2^60
+  const float up = __uint_as_float((uint32_t)(127 + n) << 23), down = __uint_as_float((uint32_t)(127 - n) << 23);
+#pragma unroll
+  for (int m = 0; m < 8; ++m) S[m] *= up;
+  scale *= up, unscale *= down;
+}
+
+template <int DT, bool BETA32>
+__global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
+  constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
+  __shared__ ChunkTiles tiles[3];
+  __shared__ ChunkTerms terms[2];
+  __shared__ PrepareScratch scratch;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
+  const Unit u = unit_of(a, blockIdx.x >> 1);
+  const int col0 = (blockIdx.x & 1) * 64 + wave * 16;
+  const int total = u.end - u.begin;
+  if (total <= 0) return;
+  if (total < CHUNKED || (unsigned)u.slot >= (unsigned)a.num_slots) {
+    if (wave < 4) walk_tokens<DT, 16, BETA32>(a, u, col0, lane);
+    return;
+  }
+  const int chunks = (total + C - 1) / C;
+  const int c = lane & 15, g = lane >> 4;
+
+  // Chunk n's tiles are staged two chunks ahead of its products, its terms prepared one ahead.
+  if (wave == 4) {
+    auto load = [&](int t0, float& decay, float& beta) {
+      const int t = t0 + (lane & 31);
+      const bool live = t < u.end;
+      decay = live ? a.g[t * a.g_row + u.h] : 0.f;
+      beta = live ? scalar_at<DT>(a.beta, t * a.beta_row + u.h, BETA32) : 0.f;
+    };
+    float decay, beta, decay1, beta1;
+    load(u.begin, decay, beta);
+    __syncthreads();  // the first tiles are there
+    for (int n = 0; n < chunks; ++n) {
+      load(u.begin + (n + 1) * C, decay1, beta1);
+      prepare_chunk<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch, terms[n & 1]);
+      decay = decay1, beta = beta1;
+      __syncthreads();  // chunk n may start
+    }
+    return;
+  }
+
+  // wave < 4: the columns col0 .. + 15 of the state: tile m, register r: row 16 m + 4 g + r, column c
+  float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + col0 + c;
+  f32x4 S[8];
+  float scale = 1.f, unscale = 1.f;  // f16: S holds the state times `scale`, a power of two of the column's own
+#pragma unroll
+  for (int m = 0; m < 8; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[m][r] = sp[(16 * m + 4 * g + r) * D];
+
+  const int kh = u.h / (a.hv / a.hk);
+  const uint16_t* kp = a.k + kh * a.k_head;
+  const uint16_t* qp = a.q + kh * a.q_head;
+  const uint16_t* vp = a.v + u.h * a.v_head + col0 + c;
+  uint16_t* op = a.o + (int64_t)u.h * D + col0 + c;
+  const int64_t o_row = (int64_t)a.hv * D;
+  // this thread's part of the tiles: two pieces of 8 values of k and of q
+  const int srow = threadIdx.x >> 4, scol = (threadIdx.x & 15) * 8;
+  u32x4 kr[2], qr[2];
+  uint16_t vr[8], vnext[8];
+  auto load_tiles = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = min(t0 + srow + 16 * i, u.end - 1);
+      kr[i] = *reinterpret_cast<const u32x4*>(kp + t * a.k_row + scol);
+      qr[i] = *reinterpret_cast<const u32x4*>(qp + t * a.q_row + scol);
+    }
+  };
+  auto store_tiles = [&](int t0, ChunkTiles& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = srow + 16 * i;
+      const bool live = t0 + row < u.end;  // rows behind the end are 0
+      *reinterpret_cast<u32x4*>(&x.k[row][scol]) = live ? kr[i] : u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(&x.q[row][scol]) = live ? qr[i] : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  auto load_v = [&](int t0, uint16_t* v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = vp[min(t0 + 16 * (i >> 2) + 4 * g + (i & 3), u.end - 1) * a.v_row];
+  };
+  load_tiles(u.begin);
+  load_v(u.begin, vnext);
+  store_tiles(u.begin, tiles[0]);
+  if (chunks > 1) load_tiles(u.begin + C);
+  __syncthreads();
+  if (chunks > 1) store_tiles(u.begin + C, tiles[1]);
+  if (chunks > 2) load_tiles(u.begin + 2 * C);
+
+  int ring = 0;  // n % 3
+  for (int n = 0; n < chunks; ++n) {
+    const int t0 = u.begin + n * C;
+    __syncthreads();  // chunk n is prepared, chunk n + 1 staged; chunk n - 1 is no longer read
+    const ChunkTiles& tile = tiles[ring];
+    const ChunkTerms& x = terms[n & 1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vr[i] = vnext[i];
+    if (n + 1 < chunks) load_v(t0 + C, vnext);
+    if (n + 2 < chunks) store_tiles(t0 + 2 * C, tiles[ring == 0 ? 2 : ring - 1]);
+    if (n + 3 < chunks) load_tiles(t0 + 3 * C);
+    ring = ring == 2 ? 0 : ring + 1;
+    if constexpr (DT == LSURGE_F16) {
+      float most = 0.f;
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(S[m][r]));
+      rescale(column_max(most), 0x1p8f, S, scale, unscale);
+    }
+    // P = K S0, O = Q S0 by halves of the tokens
+    f32x4 P[2], O[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) P[i] = O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x2 s0[NT], s1[NT];
+      split<DT, NT>(S[2 * st], s0);
+      split<DT, NT>(S[2 * st + 1], s1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // the state's rows 32 st + {4 g .. + 3, 16 + 4 g .. + 3}, in that order
+        auto frag = [&](const uint16_t (*rows)[PITCH]) {
+          const uint16_t* p = &rows[16 * i + c][32 * st + 4 * g];
+          return join(*reinterpret_cast<const u32x2*>(p), *reinterpret_cast<const u32x2*>(p + 16));
+        };
+        const u32x4 k = frag(tile.k), q = frag(tile.q);
+#pragma unroll
+        for (int j = NT - 1; j >= 0; --j) {
+          P[i] = mma_32<DT>(k, join(s0[j], s1[j]), P[i]);
+          if (j < 2) O[i] = mma_32<DT>(q, join(s0[j], s1[j]), O[i]);
+        }
+      }
+    }
+    // R, and X by blocks of 16 tokens
+    f32x4 R[2], X[2], w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 16 * i + 4 * g;
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(&x.beta[t]), c1 = *reinterpret_cast<const f32x4*>(&x.c1[t]);
+      const f32x4 c2 = *reinterpret_cast<const f32x4*>(&x.c2[t]);
+      w[i] = *reinterpret_cast<const f32x4*>(&x.w[t]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = DT == LSURGE_F16 ? f16_to_f32(vr[4 * i + r]) : bf16_to_f32(vr[4 * i + r]);
+        R[i][r] = t0 + t + r < u.end ? fmaf(-c1[r] * unscale, P[i][r], beta[r] * v) : 0.f;
+        O[i][r] *= c2[r] * unscale;
+      }
+    }
+    auto terms3 = [&](const u32x2 (*p)[64], u32x2* q) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) q[i] = p[i][lane];
+    };
+    u32x2 op3[3], x3[3], m0[2], m1[2];
+    const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+    split<3>(R[0], x3);
+    terms3(x.inv[0], op3);
+    X[0] = mma_16_f32(op3, x3, zero);
+    split<3>(X[0], x3);
+    terms3(x.a10, op3);
+    X[1] = mma_16_f32(op3, x3, R[1]);
+    // o of the first tokens; products of two terms
+    auto add_o = [&](const u32x2 (*p)[64], const u32x2* q, f32x4 acc) {
+      m0[0] = p[0][lane], m0[1] = p[1][lane];
+      acc = mma_16(m0[1], q[0], acc);
+      acc = mma_16(m0[0], q[1], acc);
+      return mma_16(m0[0], q[0], acc);
+    };
+    O[0] = add_o(x.m00, x3, O[0]);
+    auto add_o1 = [&](int half, const u32x2* q, f32x4 acc) {
+      m1[0] = x.m1[0][half][lane], m1[1] = x.m1[1][half][lane];
+      acc = mma_16(m1[1], q[0], acc);
+      acc = mma_16(m1[0], q[1], acc);
+      return mma_16(m1[0], q[0], acc);
+    };
+    O[1] = add_o1(0, x3, O[1]);
+    split<3>(X[1], x3);
+    terms3(x.inv[1], op3);
+    X[1] = mma_16_f32(op3, x3, zero);
+    split<2>(X[1], x3);
+    O[1] = add_o1(1, x3, O[1]);
+    // the state's update
+    f32x4 E[2] = {X[0] * w[0], X[1] * w[1]};
+    if constexpr (DT == LSURGE_F16) {
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(E[i][r]));
+      rescale(column_max(most) * scale, 0.f, S, scale, unscale);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) E[i] *= scale;
+    }
+    u32x2 e0[NT], e1[NT];
+    split<DT, NT>(E[0], e0);
+    split<DT, NT>(E[1], e1);
+    const float decay = x.decay;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+      // k's values 16 m + c of the tokens 4 g .. + 3 and 16 + 4 g .. + 3
+      const uint16_t* p = &tile.k[4 * g + (c >> 2)][16 * m + 4 * (c & 3)];
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p + 16 * PITCH));
+      const u32x4 k = join(__builtin_bit_cast(u32x2, lo), __builtin_bit_cast(u32x2, hi));
+      S[m] *= decay;
+#pragma unroll
+      for (int j = NT - 1; j >= 0; --j) S[m] = mma_32<DT>(k, join(e0[j], e1[j]), S[m]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = t0 + 16 * i + 4 * g + r;
+        if (t < u.end) op[t * o_row] = DT == LSURGE_F16 ? f32_to_f16(O[i][r]) : f32_to_bf16(O[i][r]);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < 8; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sp[(16 * m + 4 * g + r) * D] = S[m][r] * unscale;
 }
 
 int check_tokens(const lsurge_gdn_tokens* t) {
@@ -233,25 +713,39 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, void* workspace, size_t wor
   if (t->rows == 0) return LSURGE_OK;
   TokenArgs a = token_args(t);
   const int64_t sh = t->nseq * t->hv;
-  const int cb = columns(sh);
-  const int64_t units = sh * (D / cb / WAVES);
-  const int64_t tail = t->cu ? std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17)) : 0;
-  LSURGE_REQUIRE(units < (1ll << 24) - 256, "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
-  a.units = (int)units;
-  const unsigned grid = (unsigned)(units + tail);
   hipStream_t s = (hipStream_t)stream;
+  LSURGE_REQUIRE(sh < (1ll << 20), "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
+  const bool b32 = t->beta_dtype == LSURGE_F32;
+  if (t->cu) {  // runs of any length, two workgroups a (sequence, head)
+    const int64_t tail = std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17));
+    a.units = (int)(2 * sh);
+#define RUNS(DT, B32)                                                                                                   \
+  LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                                        \
+                hipLaunchKernelGGL((gdn_run_kernel<DT, B32>), dim3((unsigned)(a.units + tail)), dim3(RUN_THREADS), 0, s, a))
+    if (t->dtype == LSURGE_BF16) {
+      if (b32) { RUNS(LSURGE_BF16, true); }
+      else { RUNS(LSURGE_BF16, false); }
+    } else {
+      if (b32) { RUNS(LSURGE_F16, true); }
+      else { RUNS(LSURGE_F16, false); }
+    }
+#undef RUNS
+    return LSURGE_OK;
+  }
+  const int cb = columns(sh);
+  a.units = (int)(sh * (D / cb / WAVES));
 #define TOKENS(DT, CB, B32)                                                                                   \
   LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                              \
-                hipLaunchKernelGGL((gdn_token_kernel<DT, CB, B32>), dim3(grid), dim3(64 * WAVES), 0, s, a))
+                hipLaunchKernelGGL((gdn_token_kernel<DT, CB, B32>), dim3((unsigned)a.units), dim3(64 * WAVES), 0, s, a))
 #define TOKENS_CB(DT, B32)                        \
   if (cb == 32) { TOKENS(DT, 32, B32); }          \
   else if (cb == 16) { TOKENS(DT, 16, B32); }     \
   else { TOKENS(DT, 8, B32); }
   if (t->dtype == LSURGE_BF16) {
-    if (t->beta_dtype == LSURGE_F32) { TOKENS_CB(LSURGE_BF16, true) }
+    if (b32) { TOKENS_CB(LSURGE_BF16, true) }
     else { TOKENS_CB(LSURGE_BF16, false) }
   } else {
-    if (t->beta_dtype == LSURGE_F32) { TOKENS_CB(LSURGE_F16, true) }
+    if (b32) { TOKENS_CB(LSURGE_F16, true) }
     else { TOKENS_CB(LSURGE_F16, false) }
   }
 #undef TOKENS_CB
