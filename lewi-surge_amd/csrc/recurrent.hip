@@ -13,6 +13,7 @@
 // 4 x 128 x 128 multiply-adds a token and head, which have to follow each other.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "launchers.h"
 #include "rows16.h"
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 //   (I + A) X = R,  R_i = beta_i (v_i - e^{G_i} S0^T k_i),  A_ij = beta_i e^{G_i - G_j} k_i.k_j (j < i),
 //   o_i = (e^{G_i} S0^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i.k_j) x_j) / sqrt(128),
 //   S = e^{G_C} S0 + sum_j e^{G_C - G_j} k_j x_j^T
-// (row i of X is the token's d).  A and the weights of o do not depend on the state: a fifth wave forms them for the next chunk
+// (row i of X is the token's d).  A and the weights of o do not depend on the state: two waves form them for the next chunk
 // while four waves of 16 columns each take this one, with one barrier a chunk.
 //
 // Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
@@ -228,8 +229,16 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 constexpr int C = 32;
 constexpr int CHUNKED = 4;
 constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
-constexpr int RUN_THREADS = 64 * 5;
+constexpr int RUN_THREADS = 64 * 6;
+constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
 constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
+
+// a barrier behind this wave's writes to LDS; loads from memory go on across it
+__device__ __forceinline__ void stage_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 struct ChunkTiles {
   uint16_t k[C][PITCH], q[C][PITCH];
@@ -283,132 +292,214 @@ __device__ __forceinline__ void wave_sync() {
 }
 // c + P Q of operands of three terms: the six products of 2^-24 and more
 __device__ __forceinline__ f32x4 mma_16_f32(const u32x2* p, const u32x2* q, f32x4 c) {
-  c = mma_16(p[2], q[0], c);
-  c = mma_16(p[1], q[1], c);
-  c = mma_16(p[0], q[2], c);
-  c = mma_16(p[1], q[0], c);
-  c = mma_16(p[0], q[1], c);
-  return mma_16(p[0], q[0], c);
+  f32x4 small = mma_16(p[2], q[0], f32x4{0.f, 0.f, 0.f, 0.f});  // two chains: each product waits for the one before it
+  c = mma_16(p[0], q[0], c);
+  small = mma_16(p[1], q[1], small);
+  small = mma_16(p[0], q[2], small);
+  small = mma_16(p[1], q[0], small);
+  small = mma_16(p[0], q[1], small);
+  return c + small;
 }
 __device__ __forceinline__ u32x4 join(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
 
-struct PrepareScratch {
-  double G[C];        // sums of the log2 decays
-  float rk[C], rq[C], beta[C];
-  float A[2][16][20];  // the diagonal blocks, rows 16 bytes apart
+// Two waves form a chunk's terms from its tiles: one all that concerns A, the other the weights of o.
+struct Scratch {
+  double G[C];  // sums of the log2 decays
+  float rk[C];  // factors of k
 };
-// What a chunk's products need besides the state, by one wave: its k and q from their tiles, the log decay and beta of token
-// lane % 32 (0 behind the end).
+struct ScratchA : Scratch {
+  float beta[C];
+  float A[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
+};
+struct ScratchO : Scratch {
+  float rq[C];  // factors of q
+};
+// operand of a tile's tokens 16 i .. + 15, values 32 s .. + 31
+__device__ __forceinline__ u32x4 token_frag(const uint16_t (*rows)[PITCH], int i, int s, int lane) {
+  return *reinterpret_cast<const u32x4*>(&rows[16 * i + (lane & 15)][32 * s + 8 * (lane >> 4)]);
+}
+// The sum of the log2 decays up to token lane % 32, and of all.  A decay below e^-104 is 0 in f32 whatever it is.
+__device__ __forceinline__ double decay_sums(float decay, double& last) {
+  const double x = (double)(decay < -104.f ? -104.f : decay) * 1.4426950408889634;
+  auto add = [](double v, auto ctrl, auto rows) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    constexpr int CT = decltype(ctrl)::value, RM = decltype(rows)::value;
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CT, RM, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CT, RM, 0xf, true);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  typedef std::integral_constant<int, 0xf> All;
+  double G = x;
+  G = add(G, std::integral_constant<int, 0x111>(), All());  // the lane 1, 2, 4, 8 before it in a row of 16
+  G = add(G, std::integral_constant<int, 0x112>(), All());
+  G = add(G, std::integral_constant<int, 0x114>(), All());
+  G = add(G, std::integral_constant<int, 0x118>(), All());
+  G = add(G, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // the last lane of the row before
+  const uint64_t u = __builtin_bit_cast(uint64_t, G);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, C - 1), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), C - 1);
+  last = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  return G;
+}
+// the element of a diagonal block's product that lies on its diagonal, in the lanes that hold one (on_diagonal)
+__device__ __forceinline__ bool on_diagonal(int lane) { return lane >> 4 == (lane & 15) >> 2; }
+__device__ __forceinline__ float diagonal(f32x4 x, int lane) {
+  float d = x[0];
+#pragma unroll
+  for (int r = 1; r < 4; ++r)
+    if ((lane & 3) == r) d = x[r];
+  return d;
+}
+__device__ __forceinline__ float norm_factor(float square, float eps) { return eps >= 0.f ? rsqrtf(square + eps) : 1.f; }
+
+// e^{G_i - G_j} times k's factor, j = j0 .. + 3; without branches, whose loads would wait one after the other
+__device__ __forceinline__ f32x4 decays(const Scratch& s, int i, int j0) {
+  typedef double f64x2 __attribute__((ext_vector_type(2)));
+  const double Gi = s.G[i];
+  const f64x2 a = *reinterpret_cast<const f64x2*>(&s.G[j0]), b = *reinterpret_cast<const f64x2*>(&s.G[j0 + 2]);
+  const f32x4 rk = *reinterpret_cast<const f32x4*>(&s.rk[j0]);
+  return f32x4{rk[0] * __builtin_amdgcn_exp2f((float)(Gi - a[0])), rk[1] * __builtin_amdgcn_exp2f((float)(Gi - a[1])),
+               rk[2] * __builtin_amdgcn_exp2f((float)(Gi - b[0])), rk[3] * __builtin_amdgcn_exp2f((float)(Gi - b[1]))};
+}
+// y[j] += y[k] A_kj for j < k, A_kj from lane k of the row of 16; k = 15 - STEP in turn
+template <int STEP>
+__device__ __forceinline__ void subtract_row(float* y, const float* A) {
+  constexpr int K = 15 - STEP;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int a = __builtin_amdgcn_update_dpp(0, __float_as_int(A[j]), 0x150 + K, 0xf, 0xf, true);
+    y[j] = fmaf(y[K], __int_as_float(a), y[j]);
+  }
+}
+template <int... STEP>
+__device__ __forceinline__ void subtract_rows(float* y, const float* A, std::integer_sequence<int, STEP...>) {
+  (subtract_row<STEP>(y, A), ...);
+}
+
+// All that concerns A; the log decay and beta are those of token lane % 32 (0 behind the end).
 template <int DT>
-__device__ __forceinline__ void prepare_chunk(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane,
-                                              PrepareScratch& s, ChunkTerms& out) {
+__device__ __forceinline__ void prepare_a(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, ScratchA& s,
+                                          ChunkTerms& out) {
+  asm volatile("" : "+v"(lane));  // LDS addresses are formed again in every chunk, not kept in registers that spill
   const int c = lane & 15, g = lane >> 4;
   const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-  // products [token j][token i], lane: i = c, j = 4 g + r
-  f32x4 kk[3] = {zero, zero, zero}, kq[3] = {zero, zero, zero}, qq[2] = {zero, zero};  // blocks (0, 0), (1, 1), (0, 1)
+  f32x4 kk[3] = {zero, zero, zero};  // blocks (0, 0), (1, 1), (0, 1) of products [token j][token i], lane: i = c, j = 4 g + r
 #pragma unroll
   for (int st = 0; st < 4; ++st) {
-    u32x4 k[2], q[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      k[i] = *reinterpret_cast<const u32x4*>(&x.k[16 * i + c][32 * st + 8 * g]);
-      q[i] = *reinterpret_cast<const u32x4*>(&x.q[16 * i + c][32 * st + 8 * g]);
-    }
-    kk[0] = mma_32<DT>(k[0], k[0], kk[0]);
-    kk[1] = mma_32<DT>(k[1], k[1], kk[1]);
-    kk[2] = mma_32<DT>(k[0], k[1], kk[2]);
-    kq[0] = mma_32<DT>(k[0], q[0], kq[0]);
-    kq[1] = mma_32<DT>(k[1], q[1], kq[1]);
-    kq[2] = mma_32<DT>(k[0], q[1], kq[2]);
-    qq[0] = mma_32<DT>(q[0], q[0], qq[0]);
-    qq[1] = mma_32<DT>(q[1], q[1], qq[1]);
+    const u32x4 k0 = token_frag(x.k, 0, st, lane), k1 = token_frag(x.k, 1, st, lane);
+    kk[0] = mma_32<DT>(k0, k0, kk[0]);
+    kk[1] = mma_32<DT>(k1, k1, kk[1]);
+    kk[2] = mma_32<DT>(k0, k1, kk[2]);
   }
-  // A decay below e^-104 is 0 in f32 whatever it is.
   const int t = lane & 31;
-  double G = (double)(decay < -104.f ? -104.f : decay) * 1.4426950408889634;
-#pragma unroll
-  for (int d = 1; d < C; d *= 2) {
-    const double before = __shfl_up(G, d, C);
-    if (t >= d) G += before;
-  }
-  const double last = __shfl(G, C - 1, C);
+  double last;
+  const double G = decay_sums(decay, last);
   if (lane < C) s.G[t] = G, s.beta[t] = beta;
-  if (g == c >> 2) {  // the diagonals hold the norms
+  if (on_diagonal(lane)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float k2 = kk[i][0], q2 = qq[i][0];
-#pragma unroll
-      for (int r = 1; r < 4; ++r)
-        if ((c & 3) == r) k2 = kk[i][r], q2 = qq[i][r];
-      s.rk[16 * i + c] = l2_eps >= 0.f ? rsqrtf(k2 + l2_eps) : 1.f;
-      s.rq[16 * i + c] = QSCALE * (l2_eps >= 0.f ? rsqrtf(q2 + l2_eps) : 1.f);
-    }
+    for (int i = 0; i < 2; ++i) s.rk[16 * i + c] = norm_factor(diagonal(kk[i], lane), l2_eps);
   }
   wave_sync();
   if (lane < C) {
-    const float e = __builtin_amdgcn_exp2f((float)G), rk = s.rk[t];
+    const float rk = s.rk[t];
     out.beta[t] = beta;
-    out.c1[t] = beta * e * rk;
-    out.c2[t] = e * s.rq[t];
+    out.c1[t] = beta * __builtin_amdgcn_exp2f((float)G) * rk;
     out.w[t] = rk * __builtin_amdgcn_exp2f((float)(last - G));
     if (t == 0) out.decay = __builtin_amdgcn_exp2f((float)last);
   }
-  f32x4 m[3], a10;
+  f32x4 a10;
 #pragma unroll
   for (int b = 0; b < 3; ++b) {
     const int i = (b == 0 ? 0 : 16) + c, j0 = (b == 1 ? 16 : 0) + 4 * g;
-    const double Gi = s.G[i];
-    const float fa = s.beta[i] * s.rk[i], fm = s.rq[i];
+    const f32x4 e = decays(s, i, j0);
+    const float f = -s.beta[i] * s.rk[i];
     f32x4 A;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = j0 + r;
-      const float e = j <= i ? s.rk[j] * __builtin_amdgcn_exp2f((float)(Gi - s.G[j])) : 0.f;
-      A[r] = j < i ? fa * (e * kk[b][r]) : 0.f;
-      m[b][r] = j <= i ? fm * (e * kq[b][r]) : 0.f;
-    }
+    for (int r = 0; r < 4; ++r) A[r] = j0 + r < i ? f * (e[r] * kk[b][r]) : 0.f;
     if (b < 2) *reinterpret_cast<f32x4*>(&s.A[b][c][4 * g]) = A;
-    else a10 = -A;
+    else a10 = A;
   }
   u32x2 terms[3];
   split<3>(a10, terms);
 #pragma unroll
-  for (int n3 = 0; n3 < 3; ++n3) out.a10[n3][lane] = terms[n3];
-#pragma unroll
-  for (int b = 0; b < 3; ++b) {
-    split<2>(m[b], terms);
-#pragma unroll
-    for (int n2 = 0; n2 < 2; ++n2) (b == 0 ? out.m00[n2] : out.m1[n2][b == 1])[lane] = terms[n2];
-  }
+  for (int n = 0; n < 3; ++n) out.a10[n][lane] = terms[n];
   wave_sync();
-  // Row c of a block's inverse, x (I + A) = e_c, from its last value on; lanes below 32 the first block, the others the second.
+  // Row c of a block's inverse, y (I + A) = e_c, from its last value on; lanes below 32 the first block, the others the second.
+  // Lane k of a row of 16 holds row k of -A, which the others read from its register as they go: 120 multiply-adds, no LDS.
   const int blk = lane >> 5;
-  float y[16];
+  float y[16], A[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) y[j] = j == c ? 1.f : 0.f;
+  for (int j = 0; j < 16; j += 4) {
+    const f32x4 x4 = *reinterpret_cast<const f32x4*>(&s.A[blk][c][j]);
 #pragma unroll
-  for (int k = 15; k > 0; --k) {
-#pragma unroll
-    for (int j4 = 0; j4 < k; j4 += 4) {
-      const f32x4 row = *reinterpret_cast<const f32x4*>(&s.A[blk][k][j4]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (j4 + r < k) y[j4 + r] = fmaf(-y[k], row[r], y[j4 + r]);
-    }
-    if (k % 4 == 0) asm volatile("" ::: "memory");  // a few rows are read ahead: all of them would take 160 registers
+    for (int r = 0; r < 4; ++r) A[j + r] = x4[r], y[j + r] = j + r == c ? 1.f : 0.f;
   }
+  subtract_rows(y, A, std::make_integer_sequence<int, 15>());
   // its columns 8 (g % 2) .. + 7 as operands
-  f32x4 z[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) z[h][r] = g & 1 ? y[8 + 4 * h + r] : y[4 * h + r];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    split<3>(z[h], terms);
+    f32x4 z;
 #pragma unroll
-    for (int n3 = 0; n3 < 3; ++n3) out.inv[blk][n3][c + 16 * (2 * (g & 1) + h)] = terms[n3];
+    for (int r = 0; r < 4; ++r) z[r] = g & 1 ? y[8 + 4 * h + r] : y[4 * h + r];
+    split<3>(z, terms);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) out.inv[blk][n][c + 16 * (2 * (g & 1) + h)] = terms[n];
   }
+}
+
+// The weights of o.
+template <int DT>
+__device__ __forceinline__ void prepare_o(const ChunkTiles& x, float decay, float l2_eps, int lane, ScratchO& s, ChunkTerms& out) {
+  asm volatile("" : "+v"(lane));
+  const int c = lane & 15, g = lane >> 4;
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+  f32x4 kk[2] = {zero, zero}, qq[2] = {zero, zero}, kq[3] = {zero, zero, zero};
+#pragma unroll
+  for (int st = 0; st < 4; ++st) {
+    u32x4 k[2], q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) k[i] = token_frag(x.k, i, st, lane), q[i] = token_frag(x.q, i, st, lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      kq[i] = mma_32<DT>(k[i], q[i], kq[i]);
+      kk[i] = mma_32<DT>(k[i], k[i], kk[i]);
+      qq[i] = mma_32<DT>(q[i], q[i], qq[i]);
+    }
+    kq[2] = mma_32<DT>(k[0], q[1], kq[2]);
+  }
+  const int t = lane & 31;
+  double last;
+  const double G = decay_sums(decay, last);
+  if (lane < C) s.G[t] = G;
+  if (on_diagonal(lane)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s.rk[16 * i + c] = norm_factor(diagonal(kk[i], lane), l2_eps);
+      s.rq[16 * i + c] = QSCALE * norm_factor(diagonal(qq[i], lane), l2_eps);
+    }
+  }
+  wave_sync();
+  if (lane < C) out.c2[t] = __builtin_amdgcn_exp2f((float)G) * s.rq[t];
+#pragma unroll
+  for (int b = 0; b < 3; ++b) {
+    const int i = (b == 0 ? 0 : 16) + c, j0 = (b == 1 ? 16 : 0) + 4 * g;
+    const f32x4 e = decays(s, i, j0);
+    const float f = s.rq[i];
+    f32x4 m;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[r] = j0 + r <= i ? f * (e[r] * kq[b][r]) : 0.f;
+    u32x2 terms[2];
+    split<2>(m, terms);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) (b == 0 ? out.m00[n] : out.m1[n][b == 1])[lane] = terms[n];
+  }
+}
+
+// Chunk n of u's rows, `width` values of `size` bytes each and `row` values apart, as a buffer that ends with the sequence:
+// behind it reads give 0 and writes are dropped.
+__device__ __forceinline__ auto chunk_rows(const Unit& u, const void* head, int64_t row, int n, int width, int size) {
+  const int t0 = u.begin + n * C, left = min(u.end - t0, C);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)head + t0 * row * size), (short)0,
+                                           left > 0 ? (int)(((left - 1) * row + width) * size) : 0, 0x00027000);
 }
 
 // the largest of a column's values, from each of the four lanes that hold it
@@ -436,7 +527,8 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
   __shared__ ChunkTiles tiles[3];
   __shared__ ChunkTerms terms[2];
-  __shared__ PrepareScratch scratch;
+  __shared__ ScratchA scratch_a;
+  __shared__ ScratchO scratch_o;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
   const Unit u = unit_of(a, blockIdx.x >> 1);
@@ -450,85 +542,91 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   const int chunks = (total + C - 1) / C;
   const int c = lane & 15, g = lane >> 4;
 
-  // Chunk n's tiles are staged two chunks ahead of its products, its terms prepared one ahead.
-  if (wave == 4) {
-    auto load = [&](int t0, float& decay, float& beta) {
-      const int t = t0 + (lane & 31);
-      const bool live = t < u.end;
-      decay = live ? a.g[t * a.g_row + u.h] : 0.f;
-      beta = live ? scalar_at<DT>(a.beta, t * a.beta_row + u.h, BETA32) : 0.f;
+  // While four waves take chunk n, two prepare chunk n + 1 from its tiles, which the four staged during chunk n - 1.
+  if (wave >= 4) {
+    const int g_off = (lane & 31) * (int)a.g_row * 4, b_size = BETA32 ? 4 : 2, b_off = (lane & 31) * (int)a.beta_row * b_size;
+    auto load = [&](int n, float& decay, float& beta) {
+      const auto gb = chunk_rows(u, a.g + u.h, a.g_row, n, 1, 4);
+      const auto bb = chunk_rows(u, (const char*)a.beta + u.h * b_size, a.beta_row, n, 1, b_size);
+      decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gb, g_off, 0, 0));
+      if constexpr (BETA32) {
+        beta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bb, b_off, 0, 0));
+      } else {
+        const uint16_t x = __builtin_amdgcn_raw_buffer_load_b16(bb, b_off, 0, 0);
+        beta = DT == LSURGE_F16 ? f16_to_f32(x) : bf16_to_f32(x);
+      }
     };
     float decay, beta, decay1, beta1;
-    load(u.begin, decay, beta);
-    __syncthreads();  // the first tiles are there
+    load(0, decay, beta);
+    stage_barrier();  // the first chunk is staged
     for (int n = 0; n < chunks; ++n) {
-      load(u.begin + (n + 1) * C, decay1, beta1);
-      prepare_chunk<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch, terms[n & 1]);
+      load(n + 1, decay1, beta1);
+      if (wave == 4) prepare_a<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch_a, terms[n & 1]);
+      else prepare_o<DT>(tiles[n % 3], decay, a.l2_eps, lane, scratch_o, terms[n & 1]);
       decay = decay1, beta = beta1;
-      __syncthreads();  // chunk n may start
+      stage_barrier();  // chunk n is prepared
     }
     return;
   }
 
   // wave < 4: the columns col0 .. + 15 of the state: tile m, register r: row 16 m + 4 g + r, column c
-  float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + col0 + c;
+  float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + 4 * g * D + col0 + c;
   f32x4 S[8];
   float scale = 1.f, unscale = 1.f;  // f16: S holds the state times `scale`, a power of two of the column's own
 #pragma unroll
   for (int m = 0; m < 8; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) S[m][r] = sp[(16 * m + 4 * g + r) * D];
+    for (int r = 0; r < 4; ++r) S[m][r] = sp[(16 * m + r) * D];
 
   const int kh = u.h / (a.hv / a.hk);
-  const uint16_t* kp = a.k + kh * a.k_head;
-  const uint16_t* qp = a.q + kh * a.q_head;
-  const uint16_t* vp = a.v + u.h * a.v_head + col0 + c;
-  uint16_t* op = a.o + (int64_t)u.h * D + col0 + c;
-  const int64_t o_row = (int64_t)a.hv * D;
   // this thread's part of the tiles: two pieces of 8 values of k and of q
   const int srow = threadIdx.x >> 4, scol = (threadIdx.x & 15) * 8;
+  int k_off = (srow * (int)a.k_row + scol) * 2, q_off = (srow * (int)a.q_row + scol) * 2;
+  const int o_row = a.hv * D;
+  int v_off = (4 * g * (int)a.v_row + col0 + c) * 2, o_off = (4 * g * o_row + col0 + c) * 2;
   u32x4 kr[2], qr[2];
-  uint16_t vr[8], vnext[8];
-  auto load_tiles = [&](int t0) {
+  uint16_t vr[8];
+  auto load_tiles = [&](int n) {
+    const auto kb = chunk_rows(u, a.k + kh * a.k_head, a.k_row, n, D, 2), qb = chunk_rows(u, a.q + kh * a.q_head, a.q_row, n, D, 2);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int t = min(t0 + srow + 16 * i, u.end - 1);
-      kr[i] = *reinterpret_cast<const u32x4*>(kp + t * a.k_row + scol);
-      qr[i] = *reinterpret_cast<const u32x4*>(qp + t * a.q_row + scol);
+      kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kb, k_off + 32 * i * (int)a.k_row, 0, 0));
+      qr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(qb, q_off + 32 * i * (int)a.q_row, 0, 0));
     }
   };
-  auto store_tiles = [&](int t0, ChunkTiles& x) {
+  auto store_tiles = [&](ChunkTiles& x) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = srow + 16 * i;
-      const bool live = t0 + row < u.end;  // rows behind the end are 0
-      *reinterpret_cast<u32x4*>(&x.k[row][scol]) = live ? kr[i] : u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(&x.q[row][scol]) = live ? qr[i] : u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(&x.k[srow + 16 * i][scol]) = kr[i];
+      *reinterpret_cast<u32x4*>(&x.q[srow + 16 * i][scol]) = qr[i];
     }
   };
-  auto load_v = [&](int t0, uint16_t* v) {
+  auto load_v = [&](int n) {
+    const auto vb = chunk_rows(u, a.v + u.h * a.v_head, a.v_row, n, D, 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = vp[min(t0 + 16 * (i >> 2) + 4 * g + (i & 3), u.end - 1) * a.v_row];
+    for (int i = 0; i < 8; ++i)
+      vr[i] = __builtin_amdgcn_raw_buffer_load_b16(vb, v_off + (32 * (i >> 2) + 2 * (i & 3)) * (int)a.v_row, 0, 0);
   };
-  load_tiles(u.begin);
-  load_v(u.begin, vnext);
-  store_tiles(u.begin, tiles[0]);
-  if (chunks > 1) load_tiles(u.begin + C);
-  __syncthreads();
-  if (chunks > 1) store_tiles(u.begin + C, tiles[1]);
-  if (chunks > 2) load_tiles(u.begin + 2 * C);
+  load_tiles(0);
+  load_v(0);
+  store_tiles(tiles[0]);
+  load_tiles(1);
+  stage_barrier();  // the first chunk is staged
+  store_tiles(tiles[1]);
+  load_tiles(2);
 
   int ring = 0;  // n % 3
   for (int n = 0; n < chunks; ++n) {
-    const int t0 = u.begin + n * C;
-    __syncthreads();  // chunk n is prepared, chunk n + 1 staged; chunk n - 1 is no longer read
+    stage_barrier();  // chunk n is prepared, chunk n + 1 staged, chunk n - 1 no longer read
     const ChunkTiles& tile = tiles[ring];
     const ChunkTerms& x = terms[n & 1];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vr[i] = vnext[i];
-    if (n + 1 < chunks) load_v(t0 + C, vnext);
-    if (n + 2 < chunks) store_tiles(t0 + 2 * C, tiles[ring == 0 ? 2 : ring - 1]);
-    if (n + 3 < chunks) load_tiles(t0 + 3 * C);
+    // the addresses' multiples of the rows are added again in every chunk: kept, they spill, and a spill's reload waits for
+    // all loads before it
+    asm volatile("" : "+v"(k_off), "+v"(q_off), "+v"(v_off), "+v"(o_off));
+    if (n + 2 < chunks) {
+      store_tiles(tiles[ring == 0 ? 2 : ring - 1]);
+      load_tiles(n + 3);
+    }
     ring = ring == 2 ? 0 : ring + 1;
     if constexpr (DT == LSURGE_F16) {
       float most = 0.f;
@@ -544,7 +642,6 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
     for (int i = 0; i < 2; ++i) P[i] = O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
-      __builtin_amdgcn_sched_barrier(0);
       u32x2 s0[NT], s1[NT];
       split<DT, NT>(S[2 * st], s0);
       split<DT, NT>(S[2 * st + 1], s1);
@@ -574,10 +671,11 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float v = DT == LSURGE_F16 ? f16_to_f32(vr[4 * i + r]) : bf16_to_f32(vr[4 * i + r]);
-        R[i][r] = t0 + t + r < u.end ? fmaf(-c1[r] * unscale, P[i][r], beta[r] * v) : 0.f;
+        R[i][r] = fmaf(-c1[r] * unscale, P[i][r], beta[r] * v);  // 0 behind the end, as beta is
         O[i][r] *= c2[r] * unscale;
       }
     }
+    load_v(n + 1);
     auto terms3 = [&](const u32x2 (*p)[64], u32x2* q) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) q[i] = p[i][lane];
@@ -628,7 +726,6 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
     const float decay = x.decay;
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       // k's values 16 m + c of the tokens 4 g .. + 3 and 16 + 4 g .. + 3
       const uint16_t* p = &tile.k[4 * g + (c >> 2)][16 * m + 4 * (c & 3)];
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
@@ -638,18 +735,19 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
 #pragma unroll
       for (int j = NT - 1; j >= 0; --j) S[m] = mma_32<DT>(k, join(e0[j], e1[j]), S[m]);
     }
+    const auto ob = chunk_rows(u, a.o + (int64_t)u.h * D, o_row, n, D, 2);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * i + 4 * g + r;
-        if (t < u.end) op[t * o_row] = DT == LSURGE_F16 ? f32_to_f16(O[i][r]) : f32_to_bf16(O[i][r]);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float o = O[i >> 2][i & 3];
+      __builtin_amdgcn_raw_buffer_store_b16(DT == LSURGE_F16 ? f32_to_f16(o) : f32_to_bf16(o), ob,
+                                            o_off + (32 * (i >> 2) + 2 * (i & 3)) * o_row, 0, 0);
+    }
   }
+  asm volatile("" : "+v"(sp));  // its 32 addresses are formed again, not kept in 64 registers through the loop
 #pragma unroll
   for (int m = 0; m < 8; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sp[(16 * m + 4 * g + r) * D] = S[m][r] * unscale;
+    for (int r = 0; r < 4; ++r) sp[(16 * m + r) * D] = S[m][r] * unscale;
 }
 
 int check_tokens(const lsurge_gdn_tokens* t) {
@@ -664,14 +762,14 @@ int check_tokens(const lsurge_gdn_tokens* t) {
   if (t->rows == 0) return LSURGE_OK;
   for (const lsurge_attn_rows* r : {&t->q, &t->k, &t->v}) {
     LSURGE_REQUIRE(r->data && (uintptr_t)r->data % 16 == 0, "%s: null or misaligned rows", what);
-    LSURGE_REQUIRE(r->row_stride >= 0 && r->row_stride < (1ll << 32) && r->head_stride >= 0 && r->head_stride < (1ll << 32) &&
+    LSURGE_REQUIRE(r->row_stride >= 0 && r->row_stride < MOST_ROW && r->head_stride >= 0 && r->head_stride < (1ll << 32) &&
                        r->row_stride % 8 == 0 && r->head_stride % 8 == 0,
-                   "%s: row and head strides (%lld, %lld elements) must be multiples of 8 in [0, 2^32)", what,
+                   "%s: row and head strides (%lld, %lld elements) must be multiples of 8 in [0, 2^22) and [0, 2^32)", what,
                    (long long)r->row_stride, (long long)r->head_stride);
   }
   LSURGE_REQUIRE(t->g && t->beta && t->o && (t->state || t->num_slots == 0), "%s: null pointer", what);
   LSURGE_REQUIRE(((uintptr_t)t->state | (uintptr_t)t->o) % 16 == 0 && (uintptr_t)t->g % 4 == 0, "%s: misaligned pointer", what);
-  LSURGE_REQUIRE(t->g_stride >= 0 && t->g_stride < (1ll << 32) && t->beta_stride >= 0 && t->beta_stride < (1ll << 32) &&
+  LSURGE_REQUIRE(t->g_stride >= 0 && t->g_stride < MOST_ROW && t->beta_stride >= 0 && t->beta_stride < MOST_ROW &&
                      t->num_slots >= 0 && t->num_slots < (1ll << 31) && t->slot_stride >= 0 && t->slot_stride < (1ll << 40) &&
                      t->slot_stride % 4 == 0,
                  "%s: strides of g, beta and a slot (%lld, %lld, %lld), %lld slots", what, (long long)t->g_stride,

@@ -191,8 +191,8 @@ def _recurrent(query, key, value, g, beta, state, state_slots, cu_seqlens, norm)
     rows, hv, _ = value.shape
     nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
     stride = calls.slot_stride(what, state, 4)
-    q, k, v = calls.rows(query), calls.rows(key), calls.rows(value)
-    g, beta = (t if t.stride(1) == 1 or hv == 1 else t.contiguous() for t in (g, beta))
+    q, k, v = calls.rows(query, D), calls.rows(key, D), calls.rows(value, D)
+    g, beta = (t if t.stride(1) == 1 and t.stride(0) < 1 << 22 else t.contiguous() for t in (g, beta))
     o = torch.empty((rows, hv, D), dtype=v.dtype, device=v.device)
     arg = L.GdnTokens(calls.rows_arg(q), calls.rows_arg(k), calls.rows_arg(v), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
                       o.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, q.shape[1], hv, g.stride(0), beta.stride(0),
