@@ -244,7 +244,7 @@ struct ChunkTiles {
   uint16_t k[C][PITCH], q[C][PITCH];
 };
 struct ChunkTerms {
-  // operands of 16 x 16 x 16 products, lane l's four values (row l % 16, columns 4 (l / 16) .. + 3) at [l]
+  // operands of products over 16 tokens, lane l's four values (row l % 16, columns 4 (l / 16) .. + 3) at [l]
   u32x2 inv[2][3][64];  // the inverses of the diagonal blocks of I + A
   u32x2 a10[3][64];     // -A, rows 16.., columns ..15
   u32x2 m00[2][64];     // the weights of o
@@ -254,10 +254,6 @@ struct ChunkTerms {
   float decay;
 };
 
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f32x4 mma_16(u32x2 p, u32x2 q, f32x4 c) {  // D[16 x 16] += P[16 x 16] Q[16 x 16], bf16
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, p), __builtin_bit_cast(s16x4_t, q), c, 0, 0, 0);
-}
 template <int DT>
 __device__ __forceinline__ f32x4 mma_32(u32x4 p, u32x4 q, f32x4 c) {  // D[16 x 16] += P[16 x 32] Q[32 x 16]
   typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -290,29 +286,24 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// c + P Q of operands of three terms: the six products of 2^-24 and more
-__device__ __forceinline__ f32x4 mma_16_f32(const u32x2* p, const u32x2* q, f32x4 c) {
-  f32x4 small = mma_16(p[2], q[0], f32x4{0.f, 0.f, 0.f, 0.f});  // two chains: each product waits for the one before it
-  c = mma_16(p[0], q[0], c);
-  small = mma_16(p[1], q[1], small);
-  small = mma_16(p[0], q[2], small);
-  small = mma_16(p[1], q[0], small);
-  small = mma_16(p[0], q[1], small);
-  return c + small;
-}
 __device__ __forceinline__ u32x4 join(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
+// P0 Q0 + P1 Q1 of 16 x 16 operands (lane l: row / column l % 16 at 4 (l / 16) .. + 3), added to c
+__device__ __forceinline__ f32x4 mma_pair(u32x2 p0, u32x2 q0, u32x2 p1, u32x2 q1, f32x4 c) {
+  return mma_32<LSURGE_BF16>(join(p0, p1), join(q0, q1), c);
+}
+// c + P Q of such operands of three terms: the six products of 2^-24 and more
+__device__ __forceinline__ f32x4 mma_f32(const u32x2* p, const u32x2* q, f32x4 c) {
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+  f32x4 less = mma_pair(p[2], q[0], p[0], q[2], zero);
+  c = mma_pair(p[1], q[1], p[0], q[0], c);
+  less = mma_pair(p[1], q[0], p[0], q[1], less);
+  return c + less;
+}
 
-// Two waves form a chunk's terms from its tiles: one all that concerns A, the other the weights of o.
+// Two waves form a chunk's terms from its tiles.
 struct Scratch {
   double G[C];  // sums of the log2 decays
-  float rk[C];  // factors of k
-};
-struct ScratchA : Scratch {
-  float beta[C];
-  float A[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
-};
-struct ScratchO : Scratch {
-  float rq[C];  // factors of q
+  float rk[C], rq[C], beta[C];
 };
 // operand of a tile's tokens 16 i .. + 15, values 32 s .. + 31
 __device__ __forceinline__ u32x4 token_frag(const uint16_t (*rows)[PITCH], int i, int s, int lane) {
@@ -360,68 +351,64 @@ __device__ __forceinline__ f32x4 decays(const Scratch& s, int i, int j0) {
   return f32x4{rk[0] * __builtin_amdgcn_exp2f((float)(Gi - a[0])), rk[1] * __builtin_amdgcn_exp2f((float)(Gi - a[1])),
                rk[2] * __builtin_amdgcn_exp2f((float)(Gi - b[0])), rk[3] * __builtin_amdgcn_exp2f((float)(Gi - b[1]))};
 }
-// y[j] += y[k] A_kj for j < k, A_kj from lane k of the row of 16; k = 15 - STEP in turn
-template <int STEP>
-__device__ __forceinline__ void subtract_row(float* y, const float* A) {
-  constexpr int K = 15 - STEP;
+// y[j] += y[k] A_kj for four j from J on (those below k), A_kj from lane k of the row of 16.  In assembly, since the compiler
+// takes a move and a multiply-add for each; the nop is what a register needs between its last write and a read across lanes.
+template <int K, int J>
+__device__ __forceinline__ void subtract_4(float* y, const float* A) {
+  if constexpr (J + 4 <= K)
+    asm("s_nop 1\n\t"
+        "v_fmac_f32_dpp %0, %4, %8 row_newbcast:%c9 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %1, %5, %8 row_newbcast:%c9 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %6, %8 row_newbcast:%c9 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %3, %7, %8 row_newbcast:%c9 row_mask:0xf bank_mask:0xf"
+        : "+&v"(y[J]), "+&v"(y[J + 1]), "+&v"(y[J + 2]), "+&v"(y[J + 3])
+        : "v"(A[J]), "v"(A[J + 1]), "v"(A[J + 2]), "v"(A[J + 3]), "v"(y[K]), "n"(K));
+  else
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    const int a = __builtin_amdgcn_update_dpp(0, __float_as_int(A[j]), 0x150 + K, 0xf, 0xf, true);
-    y[j] = fmaf(y[K], __int_as_float(a), y[j]);
-  }
+    for (int j = J; j < K; ++j)
+      asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%c3 row_mask:0xf bank_mask:0xf"
+          : "+v"(y[j]) : "v"(A[j]), "v"(y[K]), "n"(K));
 }
 template <int... STEP>
 __device__ __forceinline__ void subtract_rows(float* y, const float* A, std::integer_sequence<int, STEP...>) {
-  (subtract_row<STEP>(y, A), ...);
+  ((subtract_4<15 - STEP, 0>(y, A), subtract_4<15 - STEP, 4>(y, A), subtract_4<15 - STEP, 8>(y, A),
+    subtract_4<15 - STEP, 12>(y, A)), ...);
 }
 
-// All that concerns A; the log decay and beta are those of token lane % 32 (0 behind the end).
+// The inverses of A's diagonal blocks; the log decay and beta are those of token lane % 32 (0 behind the end).
 template <int DT>
-__device__ __forceinline__ void prepare_a(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, ScratchA& s,
-                                          ChunkTerms& out) {
+__device__ __forceinline__ void prepare_inverse(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, Scratch& s,
+                                                float (*blocks)[16][20], ChunkTerms& out) {
   asm volatile("" : "+v"(lane));  // LDS addresses are formed again in every chunk, not kept in registers that spill
-  const int c = lane & 15, g = lane >> 4;
-  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-  f32x4 kk[3] = {zero, zero, zero};  // blocks (0, 0), (1, 1), (0, 1) of products [token j][token i], lane: i = c, j = 4 g + r
+  const int c = lane & 15, g = lane >> 4, t = lane & 31;
+  u32x4 k[2][4];
 #pragma unroll
-  for (int st = 0; st < 4; ++st) {
-    const u32x4 k0 = token_frag(x.k, 0, st, lane), k1 = token_frag(x.k, 1, st, lane);
-    kk[0] = mma_32<DT>(k0, k0, kk[0]);
-    kk[1] = mma_32<DT>(k1, k1, kk[1]);
-    kk[2] = mma_32<DT>(k0, k1, kk[2]);
-  }
-  const int t = lane & 31;
+  for (int st = 0; st < 4; ++st) k[0][st] = token_frag(x.k, 0, st, lane), k[1][st] = token_frag(x.k, 1, st, lane);
   double last;
   const double G = decay_sums(decay, last);
   if (lane < C) s.G[t] = G, s.beta[t] = beta;
+  f32x4 kk[2];  // blocks (0, 0), (1, 1) of products [token j][token i], lane: i = c, j = 4 g + r
+#pragma unroll
+  for (int i = 0; i < 2; ++i) kk[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int st = 0; st < 4; ++st)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) kk[i] = mma_32<DT>(k[i][st], k[i][st], kk[i]);
   if (on_diagonal(lane)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) s.rk[16 * i + c] = norm_factor(diagonal(kk[i], lane), l2_eps);
   }
   wave_sync();
-  if (lane < C) {
-    const float rk = s.rk[t];
-    out.beta[t] = beta;
-    out.c1[t] = beta * __builtin_amdgcn_exp2f((float)G) * rk;
-    out.w[t] = rk * __builtin_amdgcn_exp2f((float)(last - G));
-    if (t == 0) out.decay = __builtin_amdgcn_exp2f((float)last);
-  }
-  f32x4 a10;
 #pragma unroll
-  for (int b = 0; b < 3; ++b) {
-    const int i = (b == 0 ? 0 : 16) + c, j0 = (b == 1 ? 16 : 0) + 4 * g;
+  for (int b = 0; b < 2; ++b) {
+    const int i = 16 * b + c, j0 = 16 * b + 4 * g;
     const f32x4 e = decays(s, i, j0);
     const float f = -s.beta[i] * s.rk[i];
     f32x4 A;
 #pragma unroll
     for (int r = 0; r < 4; ++r) A[r] = j0 + r < i ? f * (e[r] * kk[b][r]) : 0.f;
-    if (b < 2) *reinterpret_cast<f32x4*>(&s.A[b][c][4 * g]) = A;
-    else a10 = A;
+    *reinterpret_cast<f32x4*>(&blocks[b][c][4 * g]) = A;
   }
-  u32x2 terms[3];
-  split<3>(a10, terms);
-#pragma unroll
-  for (int n = 0; n < 3; ++n) out.a10[n][lane] = terms[n];
   wave_sync();
   // Row c of a block's inverse, y (I + A) = e_c, from its last value on; lanes below 32 the first block, the others the second.
   // Lane k of a row of 16 holds row k of -A, which the others read from its register as they go: 120 multiply-adds, no LDS.
@@ -429,12 +416,13 @@ __device__ __forceinline__ void prepare_a(const ChunkTiles& x, float decay, floa
   float y[16], A[16];
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    const f32x4 x4 = *reinterpret_cast<const f32x4*>(&s.A[blk][c][j]);
+    const f32x4 x4 = *reinterpret_cast<const f32x4*>(&blocks[blk][c][j]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) A[j + r] = x4[r], y[j + r] = j + r == c ? 1.f : 0.f;
   }
   subtract_rows(y, A, std::make_integer_sequence<int, 15>());
   // its columns 8 (g % 2) .. + 7 as operands
+  u32x2 terms[3];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     f32x4 z;
@@ -446,13 +434,18 @@ __device__ __forceinline__ void prepare_a(const ChunkTiles& x, float decay, floa
   }
 }
 
-// The weights of o.
+// Everything else: A's block (1, 0), the weights of o, the factors by token.
 template <int DT>
-__device__ __forceinline__ void prepare_o(const ChunkTiles& x, float decay, float l2_eps, int lane, ScratchO& s, ChunkTerms& out) {
+__device__ __forceinline__ void prepare_rest(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, Scratch& s,
+                                             ChunkTerms& out) {
   asm volatile("" : "+v"(lane));
-  const int c = lane & 15, g = lane >> 4;
+  const int c = lane & 15, g = lane >> 4, t = lane & 31;
+  double last;
+  const double G = decay_sums(decay, last);
+  if (lane < C) s.G[t] = G, s.beta[t] = beta;
   const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-  f32x4 kk[2] = {zero, zero}, qq[2] = {zero, zero}, kq[3] = {zero, zero, zero};
+  // blocks (0, 0), (1, 1), (0, 1) of products [token j][token i], lane: i = c, j = 4 g + r
+  f32x4 kk[3] = {zero, zero, zero}, kq[3] = {zero, zero, zero}, qq[2] = {zero, zero};
 #pragma unroll
   for (int st = 0; st < 4; ++st) {
     u32x4 k[2], q[2];
@@ -460,16 +453,13 @@ __device__ __forceinline__ void prepare_o(const ChunkTiles& x, float decay, floa
     for (int i = 0; i < 2; ++i) k[i] = token_frag(x.k, i, st, lane), q[i] = token_frag(x.q, i, st, lane);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      kq[i] = mma_32<DT>(k[i], q[i], kq[i]);
       kk[i] = mma_32<DT>(k[i], k[i], kk[i]);
+      kq[i] = mma_32<DT>(k[i], q[i], kq[i]);
       qq[i] = mma_32<DT>(q[i], q[i], qq[i]);
     }
+    kk[2] = mma_32<DT>(k[0], k[1], kk[2]);
     kq[2] = mma_32<DT>(k[0], q[1], kq[2]);
   }
-  const int t = lane & 31;
-  double last;
-  const double G = decay_sums(decay, last);
-  if (lane < C) s.G[t] = G;
   if (on_diagonal(lane)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -478,7 +468,14 @@ __device__ __forceinline__ void prepare_o(const ChunkTiles& x, float decay, floa
     }
   }
   wave_sync();
-  if (lane < C) out.c2[t] = __builtin_amdgcn_exp2f((float)G) * s.rq[t];
+  if (lane < C) {
+    const float rk = s.rk[t], e = __builtin_amdgcn_exp2f((float)G);
+    out.beta[t] = beta;
+    out.c1[t] = beta * e * rk;
+    out.c2[t] = e * s.rq[t];
+    out.w[t] = rk * __builtin_amdgcn_exp2f((float)(last - G));
+    if (t == 0) out.decay = __builtin_amdgcn_exp2f((float)last);
+  }
 #pragma unroll
   for (int b = 0; b < 3; ++b) {
     const int i = (b == 0 ? 0 : 16) + c, j0 = (b == 1 ? 16 : 0) + 4 * g;
@@ -487,20 +484,34 @@ __device__ __forceinline__ void prepare_o(const ChunkTiles& x, float decay, floa
     f32x4 m;
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = j0 + r <= i ? f * (e[r] * kq[b][r]) : 0.f;
-    u32x2 terms[2];
+    u32x2 terms[3];
     split<2>(m, terms);
 #pragma unroll
     for (int n = 0; n < 2; ++n) (b == 0 ? out.m00[n] : out.m1[n][b == 1])[lane] = terms[n];
+    if (b == 2) {
+      split<3>(-s.beta[i] * s.rk[i] * (e * kk[2]), terms);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) out.a10[n][lane] = terms[n];
+    }
   }
 }
 
-// Chunk n of u's rows, `width` values of `size` bytes each and `row` values apart, as a buffer that ends with the sequence:
-// behind it reads give 0 and writes are dropped.
-__device__ __forceinline__ auto chunk_rows(const Unit& u, const void* head, int64_t row, int n, int width, int size) {
-  const int t0 = u.begin + n * C, left = min(u.end - t0, C);
-  return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)head + t0 * row * size), (short)0,
-                                           left > 0 ? (int)(((left - 1) * row + width) * size) : 0, 0x00027000);
-}
+// A unit's rows chunk by chunk, `width` values of `size` bytes each and `row` values apart, as buffers that end with the
+// sequence: behind it reads give 0 and writes are dropped.
+struct ChunkRows {
+  const char* at;
+  int64_t step;        // bytes a chunk
+  int left, row, tail;  // rows left; bytes a row, and of the last one short of that
+  __device__ __forceinline__ ChunkRows(const Unit& u, const void* head, int64_t row_, int width, int size)
+      : at((const char*)head + u.begin * row_ * size), step(C * row_ * size), left(u.end - u.begin), row((int)row_ * size),
+        tail((int)row_ * size - width * size) {}
+  __device__ __forceinline__ auto next() {
+    const int bytes = max(min(left, C) * row - tail, 0);
+    const auto b = __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, left > 0 ? bytes : 0, 0x00027000);
+    at += step, left -= C;
+    return b;
+  }
+};
 
 // the largest of a column's values, from each of the four lanes that hold it
 __device__ __forceinline__ float column_max(float x) {
@@ -527,8 +538,8 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
   __shared__ ChunkTiles tiles[3];
   __shared__ ChunkTerms terms[2];
-  __shared__ ScratchA scratch_a;
-  __shared__ ScratchO scratch_o;
+  __shared__ Scratch scratch[2];
+  __shared__ float blocks[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
   const Unit u = unit_of(a, blockIdx.x >> 1);
@@ -545,9 +556,9 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   // While four waves take chunk n, two prepare chunk n + 1 from its tiles, which the four staged during chunk n - 1.
   if (wave >= 4) {
     const int g_off = (lane & 31) * (int)a.g_row * 4, b_size = BETA32 ? 4 : 2, b_off = (lane & 31) * (int)a.beta_row * b_size;
-    auto load = [&](int n, float& decay, float& beta) {
-      const auto gb = chunk_rows(u, a.g + u.h, a.g_row, n, 1, 4);
-      const auto bb = chunk_rows(u, (const char*)a.beta + u.h * b_size, a.beta_row, n, 1, b_size);
+    ChunkRows gs(u, a.g + u.h, a.g_row, 1, 4), bs(u, (const char*)a.beta + u.h * b_size, a.beta_row, 1, b_size);
+    auto load = [&](float& decay, float& beta) {
+      const auto gb = gs.next(), bb = bs.next();
       decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gb, g_off, 0, 0));
       if constexpr (BETA32) {
         beta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bb, b_off, 0, 0));
@@ -557,12 +568,12 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
       }
     };
     float decay, beta, decay1, beta1;
-    load(0, decay, beta);
+    load(decay, beta);
     stage_barrier();  // the first chunk is staged
     for (int n = 0; n < chunks; ++n) {
-      load(n + 1, decay1, beta1);
-      if (wave == 4) prepare_a<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch_a, terms[n & 1]);
-      else prepare_o<DT>(tiles[n % 3], decay, a.l2_eps, lane, scratch_o, terms[n & 1]);
+      load(decay1, beta1);
+      if (wave == 4) prepare_inverse<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch[0], blocks, terms[n & 1]);
+      else prepare_rest<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch[1], terms[n & 1]);
       decay = decay1, beta = beta1;
       stage_barrier();  // chunk n is prepared
     }
@@ -586,8 +597,10 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   int v_off = (4 * g * (int)a.v_row + col0 + c) * 2, o_off = (4 * g * o_row + col0 + c) * 2;
   u32x4 kr[2], qr[2];
   uint16_t vr[8];
-  auto load_tiles = [&](int n) {
-    const auto kb = chunk_rows(u, a.k + kh * a.k_head, a.k_row, n, D, 2), qb = chunk_rows(u, a.q + kh * a.q_head, a.q_row, n, D, 2);
+  ChunkRows ks(u, a.k + kh * a.k_head, a.k_row, D, 2), qs(u, a.q + kh * a.q_head, a.q_row, D, 2);
+  ChunkRows vs(u, a.v + u.h * a.v_head, a.v_row, D, 2), os(u, a.o + (int64_t)u.h * D, o_row, D, 2);
+  auto load_tiles = [&]() {
+    const auto kb = ks.next(), qb = qs.next();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kb, k_off + 32 * i * (int)a.k_row, 0, 0));
@@ -601,19 +614,22 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
       *reinterpret_cast<u32x4*>(&x.q[srow + 16 * i][scol]) = qr[i];
     }
   };
-  auto load_v = [&](int n) {
-    const auto vb = chunk_rows(u, a.v + u.h * a.v_head, a.v_row, n, D, 2);
+  auto load_v = [&]() {
+    const auto vb = vs.next();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       vr[i] = __builtin_amdgcn_raw_buffer_load_b16(vb, v_off + (32 * (i >> 2) + 2 * (i & 3)) * (int)a.v_row, 0, 0);
   };
-  load_tiles(0);
-  load_v(0);
+  load_tiles();
   store_tiles(tiles[0]);
-  load_tiles(1);
+  load_tiles();
   stage_barrier();  // the first chunk is staged
   store_tiles(tiles[1]);
-  load_tiles(2);
+  load_tiles();
+  __builtin_amdgcn_sched_barrier(0);  // in the loop's order, or its first wait is for all of them in every turn
+  load_v();
+  u32x2 s[2][2][NT];  // two tiles of the state by terms, and the next two
+  if constexpr (DT == LSURGE_BF16) split<DT, NT>(S[0], s[0][0]), split<DT, NT>(S[1], s[0][1]);
 
   int ring = 0;  // n % 3
   for (int n = 0; n < chunks; ++n) {
@@ -623,10 +639,20 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
     // the addresses' multiples of the rows are added again in every chunk: kept, they spill, and a spill's reload waits for
     // all loads before it
     asm volatile("" : "+v"(k_off), "+v"(q_off), "+v"(v_off), "+v"(o_off));
-    if (n + 2 < chunks) {
-      store_tiles(tiles[ring == 0 ? 2 : ring - 1]);
-      load_tiles(n + 3);
-    }
+    // Operands are read from LDS a step before their products: k and q of the tokens 16 i + c, at the state's rows
+    // 32 st + {4 g .. + 3, 16 + 4 g .. + 3}, in that order.
+    u32x4 kf[2][2], qf[2][2];
+    auto frags = [&](int st) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint16_t *k = &tile.k[16 * i + c][32 * st + 4 * g], *q = &tile.q[16 * i + c][32 * st + 4 * g];
+        kf[st & 1][i] = join(*reinterpret_cast<const u32x2*>(k), *reinterpret_cast<const u32x2*>(k + 16));
+        qf[st & 1][i] = join(*reinterpret_cast<const u32x2*>(q), *reinterpret_cast<const u32x2*>(q + 16));
+      }
+    };
+    frags(0);
+    store_tiles(tiles[ring == 0 ? 2 : ring - 1]);  // of chunk n + 2, zeros behind the last
+    load_tiles();
     ring = ring == 2 ? 0 : ring + 1;
     if constexpr (DT == LSURGE_F16) {
       float most = 0.f;
@@ -635,79 +661,83 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(S[m][r]));
       rescale(column_max(most), 0x1p8f, S, scale, unscale);
+      split<DT, NT>(S[0], s[0][0]);
+      split<DT, NT>(S[1], s[0][1]);
     }
-    // P = K S0, O = Q S0 by halves of the tokens
+    // P = K S0, O = Q S0 by halves of the tokens; the next step's state is split between this one's products
     f32x4 P[2], O[2];
+    const f32x4 zero{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) P[i] = O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 2; ++i) P[i] = O[i] = zero;
+    u32x2 inv0[3], inv1[3], a10[3], m00[2], m1[2][2];
+    f32x4 beta[2], c1[2], c2[2], w[2];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
-      u32x2 s0[NT], s1[NT];
-      split<DT, NT>(S[2 * st], s0);
-      split<DT, NT>(S[2 * st + 1], s1);
+      if (st < 3) {
+        frags(st + 1);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // the state's rows 32 st + {4 g .. + 3, 16 + 4 g .. + 3}, in that order
-        auto frag = [&](const uint16_t (*rows)[PITCH]) {
-          const uint16_t* p = &rows[16 * i + c][32 * st + 4 * g];
-          return join(*reinterpret_cast<const u32x2*>(p), *reinterpret_cast<const u32x2*>(p + 16));
-        };
-        const u32x4 k = frag(tile.k), q = frag(tile.q);
-#pragma unroll
-        for (int j = NT - 1; j >= 0; --j) {
-          P[i] = mma_32<DT>(k, join(s0[j], s1[j]), P[i]);
-          if (j < 2) O[i] = mma_32<DT>(q, join(s0[j], s1[j]), O[i]);
+        for (int i = 0; i < 2; ++i) {
+          const int t = 16 * i + 4 * g;
+          beta[i] = *reinterpret_cast<const f32x4*>(&x.beta[t]), c1[i] = *reinterpret_cast<const f32x4*>(&x.c1[t]);
         }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) inv0[j] = x.inv[0][j][lane], a10[j] = x.a10[j][lane], inv1[j] = x.inv[1][j][lane];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) m00[j] = x.m00[j][lane], m1[j][0] = x.m1[j][0][lane], m1[j][1] = x.m1[j][1][lane];
+      }
+      const u32x2(*now)[NT] = s[st & 1];
+#pragma unroll
+      for (int j = NT - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          P[i] = mma_32<DT>(kf[st & 1][i], join(now[0][j], now[1][j]), P[i]);
+          if (j < 2) O[i] = mma_32<DT>(qf[st & 1][i], join(now[0][j], now[1][j]), O[i]);
+        }
+      if (st < 3) {
+        split<DT, NT>(S[2 * st + 2], s[(st + 1) & 1][0]);
+        split<DT, NT>(S[2 * st + 3], s[(st + 1) & 1][1]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);  // LDS reads, then a product and a part of the splits in turn
+#pragma unroll
+        for (int i = 0; i < 2 * (NT + 2); ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
     // R, and X by blocks of 16 tokens
-    f32x4 R[2], X[2], w[2];
+    f32x4 R[2], X[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int t = 16 * i + 4 * g;
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(&x.beta[t]), c1 = *reinterpret_cast<const f32x4*>(&x.c1[t]);
-      const f32x4 c2 = *reinterpret_cast<const f32x4*>(&x.c2[t]);
-      w[i] = *reinterpret_cast<const f32x4*>(&x.w[t]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float v = DT == LSURGE_F16 ? f16_to_f32(vr[4 * i + r]) : bf16_to_f32(vr[4 * i + r]);
-        R[i][r] = fmaf(-c1[r] * unscale, P[i][r], beta[r] * v);  // 0 behind the end, as beta is
-        O[i][r] *= c2[r] * unscale;
+        R[i][r] = fmaf(-c1[i][r] * unscale, P[i][r], beta[i][r] * v);  // 0 behind the end, as beta is
       }
+      c2[i] = *reinterpret_cast<const f32x4*>(&x.c2[16 * i + 4 * g]), w[i] = *reinterpret_cast<const f32x4*>(&x.w[16 * i + 4 * g]);
     }
-    load_v(n + 1);
-    auto terms3 = [&](const u32x2 (*p)[64], u32x2* q) {
+    const float decay = x.decay;
+    load_v();
+    u32x2 r0[3], x0[3], r1[3], x1[3];
+    split<3>(R[0], r0);
+    X[0] = mma_f32(inv0, r0, zero);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) q[i] = p[i][lane];
-    };
-    u32x2 op3[3], x3[3], m0[2], m1[2];
-    const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-    split<3>(R[0], x3);
-    terms3(x.inv[0], op3);
-    X[0] = mma_16_f32(op3, x3, zero);
-    split<3>(X[0], x3);
-    terms3(x.a10, op3);
-    X[1] = mma_16_f32(op3, x3, R[1]);
-    // o of the first tokens; products of two terms
-    auto add_o = [&](const u32x2 (*p)[64], const u32x2* q, f32x4 acc) {
-      m0[0] = p[0][lane], m0[1] = p[1][lane];
-      acc = mma_16(m0[1], q[0], acc);
-      acc = mma_16(m0[0], q[1], acc);
-      return mma_16(m0[0], q[0], acc);
-    };
-    O[0] = add_o(x.m00, x3, O[0]);
-    auto add_o1 = [&](int half, const u32x2* q, f32x4 acc) {
-      m1[0] = x.m1[0][half][lane], m1[1] = x.m1[1][half][lane];
-      acc = mma_16(m1[1], q[0], acc);
-      acc = mma_16(m1[0], q[1], acc);
-      return mma_16(m1[0], q[0], acc);
-    };
-    O[1] = add_o1(0, x3, O[1]);
-    split<3>(X[1], x3);
-    terms3(x.inv[1], op3);
-    X[1] = mma_16_f32(op3, x3, zero);
-    split<2>(X[1], x3);
-    O[1] = add_o1(1, x3, O[1]);
+    for (int m = 0; m < 4; ++m) S[m] *= decay;  // beside the chain of products
+    split<3>(X[0], x0);
+    X[1] = mma_f32(a10, x0, R[1]);
+#pragma unroll
+    for (int m = 4; m < 8; ++m) S[m] *= decay;
+    split<3>(X[1], r1);
+    X[1] = mma_f32(inv1, r1, zero);
+    // o's products of two terms, 2^-16 of them
+#pragma unroll
+    for (int i = 0; i < 2; ++i) O[i] *= c2[i] * unscale;
+    O[0] = mma_pair(m00[0], x0[1], m00[1], x0[0], O[0]);
+    O[0] = mma_pair(m00[0], x0[0], u32x2{0u, 0u}, x0[0], O[0]);
+    O[1] = mma_pair(m1[0][0], x0[0], m1[1][0], x0[0], O[1]);
     // the state's update
     f32x4 E[2] = {X[0] * w[0], X[1] * w[1]};
     if constexpr (DT == LSURGE_F16) {
@@ -720,22 +750,29 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) E[i] *= scale;
     }
-    u32x2 e0[NT], e1[NT];
-    split<DT, NT>(E[0], e0);
-    split<DT, NT>(E[1], e1);
-    const float decay = x.decay;
+    u32x4 kt[8];  // k's values 16 m + c of the tokens 4 g .. + 3 and 16 + 4 g .. + 3
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      // k's values 16 m + c of the tokens 4 g .. + 3 and 16 + 4 g .. + 3
       const uint16_t* p = &tile.k[4 * g + (c >> 2)][16 * m + 4 * (c & 3)];
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p + 16 * PITCH));
-      const u32x4 k = join(__builtin_bit_cast(u32x2, lo), __builtin_bit_cast(u32x2, hi));
-      S[m] *= decay;
-#pragma unroll
-      for (int j = NT - 1; j >= 0; --j) S[m] = mma_32<DT>(k, join(e0[j], e1[j]), S[m]);
+      kt[m] = join(__builtin_bit_cast(u32x2, lo), __builtin_bit_cast(u32x2, hi));
     }
-    const auto ob = chunk_rows(u, a.o + (int64_t)u.h * D, o_row, n, D, 2);
+    u32x2 e0[NT], e1[NT];
+    split<DT, NT>(E[0], e0);
+    split<DT, NT>(E[1], e1);
+    split<2>(X[1], x1);
+#pragma unroll
+    for (int m = 0; m < 8; m += 2)  // two tiles in turn: a product waits for the one before it
+#pragma unroll
+      for (int j = NT - 1; j >= 0; --j) {
+        S[m] = mma_32<DT>(kt[m], join(e0[j], e1[j]), S[m]);
+        S[m + 1] = mma_32<DT>(kt[m + 1], join(e0[j], e1[j]), S[m + 1]);
+      }
+    if constexpr (DT == LSURGE_BF16) split<DT, NT>(S[0], s[0][0]), split<DT, NT>(S[1], s[0][1]);
+    O[1] = mma_pair(m1[0][0], x0[1], m1[0][1], x1[1], O[1]);
+    O[1] = mma_pair(m1[0][1], x1[0], m1[1][1], x1[0], O[1]);
+    const auto ob = os.next();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float o = O[i >> 2][i & 3];
@@ -762,14 +799,14 @@ int check_tokens(const lsurge_gdn_tokens* t) {
   if (t->rows == 0) return LSURGE_OK;
   for (const lsurge_attn_rows* r : {&t->q, &t->k, &t->v}) {
     LSURGE_REQUIRE(r->data && (uintptr_t)r->data % 16 == 0, "%s: null or misaligned rows", what);
-    LSURGE_REQUIRE(r->row_stride >= 0 && r->row_stride < MOST_ROW && r->head_stride >= 0 && r->head_stride < (1ll << 32) &&
+    LSURGE_REQUIRE(r->row_stride >= D && r->row_stride < MOST_ROW && r->head_stride >= 0 && r->head_stride < (1ll << 32) &&
                        r->row_stride % 8 == 0 && r->head_stride % 8 == 0,
-                   "%s: row and head strides (%lld, %lld elements) must be multiples of 8 in [0, 2^22) and [0, 2^32)", what,
+                   "%s: row and head strides (%lld, %lld elements) must be multiples of 8 in [128, 2^22) and [0, 2^32)", what,
                    (long long)r->row_stride, (long long)r->head_stride);
   }
   LSURGE_REQUIRE(t->g && t->beta && t->o && (t->state || t->num_slots == 0), "%s: null pointer", what);
   LSURGE_REQUIRE(((uintptr_t)t->state | (uintptr_t)t->o) % 16 == 0 && (uintptr_t)t->g % 4 == 0, "%s: misaligned pointer", what);
-  LSURGE_REQUIRE(t->g_stride >= 0 && t->g_stride < MOST_ROW && t->beta_stride >= 0 && t->beta_stride < MOST_ROW &&
+  LSURGE_REQUIRE(t->g_stride >= t->hv && t->g_stride < MOST_ROW && t->beta_stride >= t->hv && t->beta_stride < MOST_ROW &&
                      t->num_slots >= 0 && t->num_slots < (1ll << 31) && t->slot_stride >= 0 && t->slot_stride < (1ll << 40) &&
                      t->slot_stride % 4 == 0,
                  "%s: strides of g, beta and a slot (%lld, %lld, %lld), %lld slots", what, (long long)t->g_stride,

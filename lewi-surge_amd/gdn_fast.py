@@ -192,10 +192,13 @@ def _recurrent(query, key, value, g, beta, state, state_slots, cu_seqlens, norm)
     nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
     stride = calls.slot_stride(what, state, 4)
     q, k, v = calls.rows(query, D), calls.rows(key, D), calls.rows(value, D)
-    g, beta = (t if t.stride(1) == 1 and t.stride(0) < 1 << 22 else t.contiguous() for t in (g, beta))
+    if not g.is_contiguous() and not (g.stride(1) == 1 and hv <= g.stride(0) < 1 << 22):
+        g = g.contiguous()
+    if not beta.is_contiguous() and not (beta.stride(1) == 1 and hv <= beta.stride(0) < 1 << 22):
+        beta = beta.contiguous()
     o = torch.empty((rows, hv, D), dtype=v.dtype, device=v.device)
     arg = L.GdnTokens(calls.rows_arg(q), calls.rows_arg(k), calls.rows_arg(v), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
-                      o.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, q.shape[1], hv, g.stride(0), beta.stride(0),
+                      o.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, q.shape[1], hv, hv if g.is_contiguous() else g.stride(0), hv if beta.is_contiguous() else beta.stride(0),
                       state.shape[0], stride, 1e-6 if norm else -1.0, L.dt(v), L.dt(beta))
     lib = L.lib()
     nbytes = lib.lsurge_gdn_recurrent_workspace_bytes(arg)
