@@ -520,13 +520,13 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
 
 /* The gated delta rule token by token, from and to states that are kept:  per sequence and value head h, S [128, 128] f32,
  *   S <- e^g S,  d = beta (v - S^T k),  S <- S + k d^T,  o = S^T q / sqrt(128),
- * q and k of head h / (hv / hk).  q, k [rows, hk, 128] and v [rows, hv, 128] by strides (any multiples of 8), dtype LSURGE_BF16
- * or LSURGE_F16; g [rows, hv] f32 (log decay) and beta [rows, hv] of dtype or LSURGE_F32 (beta_dtype), rows g_stride and
+ * q and k of head h / (hv / hk).  q, k [rows, hk, 128] and v [rows, hv, 128] by strides (multiples of 8, rows 128 to 2^22 apart),
+ * dtype LSURGE_BF16 or LSURGE_F16; g [rows, hv] f32 (log decay) and beta [rows, hv] of dtype or LSURGE_F32 (beta_dtype), rows g_stride and
  * beta_stride elements apart; o [rows, hv, 128] of dtype.  l2_eps >= 0: q and k are first multiplied by rsqrt(sum x^2 + l2_eps)
  * (not rounded in between); negative: taken as they are.  Packed rows, slots and rows without one as for
  * lsurge_causal_conv1d_update; state: [num_slots] of [hv, 128, 128] f32, slot_stride elements apart (a multiple of 4),
- * 16-byte aligned.  Products and states are f32; results of a sequence do not depend on the others.  Workspace (it may be 0)
- * from lsurge_gdn_recurrent_workspace_bytes. */
+ * 16-byte aligned.  Products and states are f32; results repeat bit for bit for the same batch, and the last bits of a single token
+ * depend on the batch's size. */
 typedef struct {
   lsurge_attn_rows q, k, v;
   const float* g;
@@ -538,8 +538,7 @@ typedef struct {
   float l2_eps;
   int dtype, beta_dtype;
 } lsurge_gdn_tokens;
-size_t lsurge_gdn_recurrent_workspace_bytes(const lsurge_gdn_tokens* t);
-int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, void* workspace, size_t workspace_bytes, lsurge_stream_t stream);
+int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream);
 
 /* Rotation of heads by their token's position p: pair i of a head's first rotary_dim values, (x_i, x_{i + rotary_dim / 2}) or,
  * interleaved, (x_2i, x_{2i + 1}), turned by the angle p inv_freq[i] (inverse != 0: by its negative); the values behind them

@@ -2,18 +2,22 @@
 without a gradient as steps of a trace."""
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd import forward_ad
 
 import _lib as L
 
 
-def check_device(what, *ts):
-    L.require_cuda(*ts)
-    device = ts[0].device
-    for t in ts:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on one device (got {device} and {t.device})")
+def check_device(what, first, *rest):
+    device = first.get_device()  # a number; a device object for each tensor would take as long as a short call's launch
+    if device < 0:
+        L.require_cuda(first)
+    for t in rest:
+        if t is not None and t.get_device() != device:
+            L.require_cuda(t)
+            raise ValueError(f"{what}: all tensors must be on one device (got {first.device} and {t.device})")
 
 
 def check_dtype(what, *ts):
@@ -24,8 +28,10 @@ def check_dtype(what, *ts):
 
 
 def check_no_grad(what, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise ValueError(f"{what}: no gradient; call it under torch.no_grad() or on detached tensors")
     # no level is open outside of forward-mode code (unpack_dual would say so too, 0.3 us a tensor)
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise ValueError(f"{what}: no gradient, of the forward mode neither; call it on detached tensors")
@@ -54,9 +60,13 @@ def packed(what, rows, cu_seqlens, state, state_slots):
 
 def slot_stride(what, state, unit):
     """Elements from one slot of `state` to the next; a slot's must be contiguous, 16-byte aligned and apart from the others."""
-    size = state[0].numel() if state.shape[0] else 0
-    apart = state.stride(0) if state.shape[0] > 1 else size
-    if state.shape[0] and not state[0].is_contiguous() or state.data_ptr() % 16 or apart < size or apart % unit:
+    if state.is_contiguous():
+        size = apart = math.prod(state.shape[1:])
+        ok = apart % unit == 0
+    else:
+        size, apart = state[0].numel(), state.stride(0)
+        ok = state[0].is_contiguous() and apart >= size and apart % unit == 0
+    if not ok or state.data_ptr() % 16:
         raise ValueError(f"{what}: a slot's state must be contiguous, 16-byte aligned and apart from the others "
                          f"(shape {tuple(state.shape)}, strides {state.stride()})")
     return apart
@@ -71,7 +81,8 @@ def call(what, device, fn, *args):
     else:
         with torch.cuda.device(device):
             rc = fn(*args, stream)
-    L.check(rc, what)
+    if rc:
+        L.check(rc, what)
 
 
 def ptr(t):
@@ -96,6 +107,18 @@ def aligned(t):
 def rows_arg(t):
     row, head = (t.shape[1] * t.shape[2], t.shape[2]) if t.is_contiguous() else t.stride()[:2]
     return L.AttnRows(t.data_ptr(), row, head)
+
+
+def row_args(t, min_row=0, most=1 << 40):
+    """rows(t) and its pointer, row stride and head stride, with as few calls as that takes."""
+    row, head, one = t.stride()
+    p = t.data_ptr()
+    if one == 1 and (p | row << 1 | head << 1) % 16 == 0 and min_row <= row < most:
+        return t, p, row, head
+    t = t.contiguous()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return t, t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]
 
 
 class _Step(torch.autograd.Function):

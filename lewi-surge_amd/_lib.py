@@ -63,7 +63,7 @@ class ConvUpdate(ctypes.Structure):
 
 
 class GdnTokens(ctypes.Structure):
-    _fields_ = ([(n, AttnRows) for n in "qkv"] + [(n, _p) for n in ("g", "beta", "state", "o", "slots", "cu")] +
+    _fields_ = ([(t + n, c) for t in "qkv" for n, c in AttnRows._fields_] + [(n, _p) for n in ("g", "beta", "state", "o", "slots", "cu")] +
                 [(n, _i64) for n in ("rows", "nseq", "hk", "hv", "g_stride", "beta_stride", "num_slots", "slot_stride")] +
                 [("l2_eps", ctypes.c_float), ("dtype", _int), ("beta_dtype", _int)])
 
@@ -156,8 +156,7 @@ _SIGS = {
     "lsurge_paged_attn": (_int, [ctypes.POINTER(KvCache), _rows, _i64, _i64, ctypes.c_float, _p, _p, _p, _sz, _p]),
     "lsurge_kv_append": (_int, [ctypes.POINTER(KvCache), _rows, _rows, _i64, _i64, _p, _p]),
     "lsurge_causal_conv1d_update": (_int, [ctypes.POINTER(ConvUpdate), _p]),
-    "lsurge_gdn_recurrent_workspace_bytes": (_sz, [ctypes.POINTER(GdnTokens)]),
-    "lsurge_gdn_recurrent": (_int, [ctypes.POINTER(GdnTokens), _p, _sz, _p]),
+    "lsurge_gdn_recurrent": (_int, [ctypes.POINTER(GdnTokens), _p]),
     "lsurge_rotary_rows": (_int, [ctypes.POINTER(Rotary), _rows, _i64, _rows, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
     "lsurge_rotary_append": (_int, [ctypes.POINTER(KvCache), ctypes.POINTER(Rotary), _rows, _i64, _rows, _rows, _i64, _i64,
                                     _p, _p, _p, _p]),

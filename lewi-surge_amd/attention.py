@@ -36,7 +36,7 @@ import torch
 import _lib as L
 from _calls import aligned as _aligned, call as _call, check_device as _check_device, check_dtype as _check_dtype
 from _calls import check_index as _check_index, check_no_grad as _check_no_grad, ptr as _ptr, rows as _rows
-from _calls import rows_arg as _rows_arg, step as _step
+from _calls import row_args as _row_args, rows_arg as _rows_arg, step as _step
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -167,29 +167,33 @@ def alloc_kv_cache(num_pages, page_size, kv_heads, head_dim, dtype=torch.bfloat1
     return tuple(torch.empty(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
 
 
-def _cache_strides(what, t):
-    st = t.stride()
-    if 1 in t.shape:  # the stride of an axis of one means nothing
-        st = [0 if n == 1 else s for n, s in zip(t.shape, st)]
-    if t.stride(3) != 1 or (st[0] | st[1] | st[2]) % 8 or t.data_ptr() % 16:
+def _cache_strides(what, t, shape):
+    page, slot, head, one = t.stride()
+    if 1 in shape:  # the stride of an axis of one means nothing
+        page, slot, head = (0 if n == 1 else s for n, s in zip(shape, (page, slot, head)))
+    p = t.data_ptr()
+    if one != 1 or (page | slot | head) % 8 or p % 16:
         raise ValueError(f"{what}: a token's values in a cache must be contiguous and 16-byte aligned (strides {t.stride()})")
-    return st[:3]
+    return p, page, slot, head
 
 
 def _cache_arg(what, k_cache, v_cache, page_table, seq_lens):
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    shape, tshape = k_cache.shape, page_table.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"{what}: caches must be [num_pages, page_size, kv_heads, head_dim] (got {tuple(k_cache.shape)}, "
                          f"{tuple(v_cache.shape)})")
-    pages, size, heads, d = k_cache.shape
+    pages, size, heads, d = shape
     if pages < 1 or size < 8 or size > 4096 or size & (size - 1):
         raise ValueError(f"{what}: at least one page, of a power of two from 8 to 4096 tokens (got {pages} of {size})")
-    if page_table.dim() != 2 or page_table.shape[1] < 1:
-        raise ValueError(f"{what}: page_table must be [sequences, pages] (got {tuple(page_table.shape)})")
-    nseq, most = page_table.shape
-    table = _check_index(what, "page_table", page_table, (nseq, most))
+    if len(tshape) != 2 or tshape[1] < 1:
+        raise ValueError(f"{what}: page_table must be [sequences, pages] (got {tuple(tshape)})")
+    nseq, most = tshape
+    table = _check_index(what, "page_table", page_table, tshape)
     lens = _check_index(what, "seq_lens", seq_lens, (nseq,))
-    arg = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), *_cache_strides(what, k_cache), *_cache_strides(what, v_cache),
-                    table.data_ptr(), most, lens.data_ptr(), pages, size, most, heads, d, L.dt(k_cache))
+    k, *k_strides = _cache_strides(what, k_cache, shape)
+    v, *v_strides = _cache_strides(what, v_cache, shape)
+    arg = L.KvCache(k, v, *k_strides, *v_strides, table.data_ptr(), most, lens.data_ptr(), pages, size, most, heads, d,
+                    L.dt(k_cache))
     return arg, (table, lens)
 
 
@@ -282,13 +286,19 @@ def _rotary_arg(what, d, rows, like, inv_freq, positions, interleaved, inverse=F
 def _rotate(q, k, inv_freq, positions, cu, interleaved, inverse, nseq, shape):
     """Rows q and k (either may be None) turned, or by `inverse` turned back."""
     like = k if q is None else q
-    d = like.shape[-1]
+    rows, _, d = like.shape
     arg, keep = _rotary_arg("rotary", d, shape, like, inv_freq, positions, interleaved, inverse)
-    ts = [None if t is None else _rows(t) for t in (q, k)]
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
-    rows = [(None, 0) if t is None else (_rows_arg(t), t.shape[1]) for t in ts]
-    _call("rotary", like.device, L.lib().lsurge_rotary_rows, arg, *rows[0], *rows[1], d, like.shape[0], nseq, _ptr(cu),
-          _ptr(outs[0]), _ptr(outs[1]))
+    outs, args = [], []
+    for t in (q, k):
+        if t is None:
+            outs.append(None)
+            args += (None, 0)
+        else:
+            outs.append(t.new_empty(t.shape))
+            t, *where = _row_args(t)
+            keep += (t,)
+            args += (L.AttnRows(*where), t.shape[1])
+    _call("rotary", like.device, L.lib().lsurge_rotary_rows, arg, *args, d, rows, nseq, _ptr(cu), _ptr(outs[0]), _ptr(outs[1]))
     del keep
     return outs
 
@@ -299,19 +309,19 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, inv_freq, positions, cu, interleaved, nseq, shape):
         ctx.save_for_backward(inv_freq, positions, cu)
-        ctx.rest = interleaved, nseq, shape
-        ctx.dtype = q.dtype
+        ctx.rest = interleaved, nseq, shape, q.dtype
         ctx.set_materialize_grads(False)
         return tuple(_rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq, shape))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        inv_freq, positions, cu = ctx.saved_tensors
-        interleaved, nseq, shape = ctx.rest
+        interleaved, nseq, shape, dtype = ctx.rest
+        want_q, want_k = ctx.needs_input_grad[:2]
+        dq = dq.to(dtype) if want_q and dq is not None else None
+        dk = dk.to(dtype) if want_k and dk is not None else None
         if dq is not None or dk is not None:
-            dq, dk = (None if t is None else t.to(ctx.dtype) for t in (dq, dk))
-            dq, dk = _rotate(dq, dk, inv_freq, positions, cu, interleaved, True, nseq, shape)
+            dq, dk = _rotate(dq, dk, *ctx.saved_tensors, interleaved, True, nseq, shape)
         return dq, dk, None, None, None, None, None, None
 
 
@@ -333,22 +343,19 @@ def rotary(q, k, inv_freq, positions=None, cu_seqlens=None, interleaved=False):
     _check_dtype(what, q, k)
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: inv_freq has no gradient; detach it")
-    shape = q.shape
-    if q.dim() == 4:
+    shape, kshape = q.shape, k.shape
+    if len(shape) == 4:
         if cu_seqlens is not None:
             raise ValueError(f"{what}: cu_seqlens go with packed [T, H, D] tensors")
-        nseq, cu = q.shape[0], None
-        qr, kr = q.flatten(0, 1), k.flatten(0, 1)
-    else:
-        if cu_seqlens is None and positions is None:
-            raise ValueError(f"{what}: packed tensors need cu_seqlens or positions")
-        nseq, cu = 0, None
-        if cu_seqlens is not None:
-            nseq = max(cu_seqlens.numel() - 1, 0)
-            cu = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
-        qr, kr = q, k
-    qo, ko = _RotaryFn.apply(qr, kr, inv_freq, positions, cu, interleaved, nseq, shape[:-2])
-    return qo.view(shape), ko.view(k.shape)
+        qo, ko = _RotaryFn.apply(q.flatten(0, 1), k.flatten(0, 1), inv_freq, positions, None, interleaved, shape[0], shape[:-2])
+        return qo.view(shape), ko.view(kshape)
+    if cu_seqlens is None and positions is None:
+        raise ValueError(f"{what}: packed tensors need cu_seqlens or positions")
+    nseq = 0
+    if cu_seqlens is not None:
+        nseq = max(cu_seqlens.numel() - 1, 0)
+        cu_seqlens = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
+    return _RotaryFn.apply(q, k, inv_freq, positions, cu_seqlens, interleaved, nseq, shape[:-2])
 
 
 def rotary_append_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens=None, positions=None,
@@ -361,11 +368,12 @@ def rotary_append_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, 
     return_k adds, for causal_attention (prompts).  Rows that hold no token give zeros; a token whose page the table does not
     name is turned and not written.  No gradient."""
     what = "rotary_append_kv"
-    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or k.shape[1:] != k_cache.shape[2:] or q.dim() != 3 or \
-            q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    n, kv, d = k.shape if k.dim() == 3 else (-1, -1, -1)
+    if v.shape != k.shape or k_cache.dim() != 4 or k_cache.shape[2:] != (kv, d) or q.dim() != 3 or q.shape[0] != n or \
+            q.shape[2] != d:
         raise ValueError(f"{what}: q must be [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] of the caches (got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, caches {tuple(k_cache.shape)})")
-    _check_heads(what, q.shape[1], k.shape[1], k.shape[2], q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens,
+    _check_heads(what, q.shape[1], kv, d, q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens,
                  positions)
     _check_dtype(what, q, k, v, k_cache, v_cache)
     _check_no_grad(what, q, k, v, k_cache, v_cache, inv_freq)
@@ -384,14 +392,14 @@ def _rotary_append(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu
     elif n != nseq:
         raise ValueError(f"{what}: {n} tokens for {nseq} sequences need cu_seqlens")
     rotation, more = _rotary_arg(what, d, (n,), q, inv_freq, positions, interleaved)
-    q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if return_k else None
+    q_out = q.new_empty((n, hq, d))
+    k_out = k.new_empty(k.shape) if return_k else None
     if nseq == 0:  # no sequence: every row is behind the last
         q_out.zero_()
         return q_out, k_out.zero_() if return_k else None
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    _call("rotary_append", q.device, L.lib().lsurge_rotary_append, cache, rotation, _rows_arg(q), hq, _rows_arg(k), _rows_arg(v),
-          n, nseq, _ptr(cu_seqlens), _ptr(q_out), _ptr(k_out))
+    q, k, v = _row_args(q), _row_args(k), _row_args(v)
+    _call("rotary_append", q_out.device, L.lib().lsurge_rotary_append, cache, rotation, L.AttnRows(*q[1:]), hq,
+          L.AttnRows(*k[1:]), L.AttnRows(*v[1:]), n, nseq, _ptr(cu_seqlens), q_out.data_ptr(), _ptr(k_out))
     torch.autograd.graph.increment_version((k_cache, v_cache))
     del keep, more
     return q_out, k_out

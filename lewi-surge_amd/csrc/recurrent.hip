@@ -837,14 +837,8 @@ using namespace lsgdn;
 
 extern "C" {
 
-size_t lsurge_gdn_recurrent_workspace_bytes(const lsurge_gdn_tokens* t) {
-  (void)t;
-  return 0;
-}
-
-int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, void* workspace, size_t workspace_bytes, lsurge_stream_t stream) {
+int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   if (int rc = check_tokens(t)) return rc;
-  (void)workspace, (void)workspace_bytes;
   if (t->rows == 0) return LSURGE_OK;
   TokenArgs a = token_args(t);
   const int64_t sh = t->nseq * t->hv;

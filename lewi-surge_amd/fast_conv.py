@@ -122,7 +122,7 @@ def _update(x, w, state, state_slots, cu_seqlens, activation):
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     w = calls.aligned(L.contig(w))
-    y = torch.empty((rows, channels), dtype=x.dtype, device=x.device)
+    y = x.new_empty((rows, channels))
     arg = L.ConvUpdate(x.data_ptr(), w.data_ptr(), state.data_ptr(), y.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, channels,
                        w.shape[0], x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
     calls.call("causal_conv1d_update", x.device, L.lib().lsurge_causal_conv1d_update, arg)

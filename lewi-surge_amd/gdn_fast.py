@@ -166,11 +166,11 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=No
     out exact to float32, where the chunked form rounds as the reference does.  Strides are free: views of one projection are
     read in place.  No gradient."""
     what = "recurrent_gated_delta_rule"
-    if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[0] != query.shape[0] or \
-            query.shape[2] != D or value.shape[2] != D:
+    shape, vshape = query.shape, value.shape
+    if len(shape) != 3 or key.shape != shape or len(vshape) != 3 or vshape[0] != shape[0] or shape[2] != D or vshape[2] != D:
         raise ValueError(f"{what}: query and key must be [rows, key heads, {D}], value [rows, heads, {D}] (got "
                          f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)})")
-    rows, hk, hv = query.shape[0], query.shape[1], value.shape[1]
+    rows, hk, hv = shape[0], shape[1], vshape[1]
     if hk < 1 or hv < 1 or hv % hk:
         raise ValueError(f"{what}: {hv} value heads are no multiple of {hk} key heads")
     if g.shape != (rows, hv) or beta.shape != (rows, hv):
@@ -191,19 +191,17 @@ def _recurrent(query, key, value, g, beta, state, state_slots, cu_seqlens, norm)
     rows, hv, _ = value.shape
     nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
     stride = calls.slot_stride(what, state, 4)
-    q, k, v = calls.rows(query, D), calls.rows(key, D), calls.rows(value, D)
+    q, k, v = (calls.row_args(t, D, 1 << 22) for t in (query, key, value))
     if not g.is_contiguous() and not (g.stride(1) == 1 and hv <= g.stride(0) < 1 << 22):
         g = g.contiguous()
     if not beta.is_contiguous() and not (beta.stride(1) == 1 and hv <= beta.stride(0) < 1 << 22):
         beta = beta.contiguous()
-    o = torch.empty((rows, hv, D), dtype=v.dtype, device=v.device)
-    arg = L.GdnTokens(calls.rows_arg(q), calls.rows_arg(k), calls.rows_arg(v), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
-                      o.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, q.shape[1], hv, hv if g.is_contiguous() else g.stride(0), hv if beta.is_contiguous() else beta.stride(0),
-                      state.shape[0], stride, 1e-6 if norm else -1.0, L.dt(v), L.dt(beta))
-    lib = L.lib()
-    nbytes = lib.lsurge_gdn_recurrent_workspace_bytes(arg)
-    ws = L.workspace(nbytes, v.device) if nbytes else None
-    calls.call("gdn_recurrent", v.device, lib.lsurge_gdn_recurrent, arg, calls.ptr(ws), nbytes)
+    o = value.new_empty((rows, hv, D))
+    arg = L.GdnTokens(*q[1:], *k[1:], *v[1:], g.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), calls.ptr(slots),
+                      calls.ptr(cu), rows, nseq, key.shape[1], hv, hv if g.is_contiguous() else g.stride(0),
+                      hv if beta.is_contiguous() else beta.stride(0), state.shape[0], stride, 1e-6 if norm else -1.0, L.dt(o),
+                      L.dt(beta))
+    calls.call("gdn_recurrent", o.device, L.lib().lsurge_gdn_recurrent, arg)
     torch.autograd.graph.increment_version(state)
     return o
 

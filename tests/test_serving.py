@@ -279,29 +279,33 @@ def _rows(stride=128, head=128, data=FAKE):
 
 
 def _tokens(**kw):
-    a = dict(q=_rows(), k=_rows(), v=_rows(), g=FAKE, beta=FAKE, state=FAKE, o=FAKE, rows=4, nseq=4, hk=1, hv=2, g_stride=2,
+    a = dict(g=FAKE, beta=FAKE, state=FAKE, o=FAKE, rows=4, nseq=4, hk=1, hv=2, g_stride=2,
              beta_stride=2, num_slots=4, slot_stride=32768, l2_eps=-1.0, dtype=L.BF16, beta_dtype=L.BF16)
     a.update(kw)
+    for n in "qkv":
+        r = a.pop(n, _rows())
+        a.update({n + f: getattr(r, f) for f, _ in L.AttnRows._fields_})
     return L.GdnTokens(**a)
 
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(rows=5), b"5 rows of 4"), (dict(rows=-1, cu=FAKE), b"-1 rows"), (dict(hv=3, hk=2), b"3 value heads over 2"),
     (dict(hk=0), b"value heads over 0"), (dict(dtype=L.F32), b"bf16 or f16"), (dict(beta_dtype=L.F16), b"beta alike"),
-    (dict(q=_rows(stride=100)), b"multiples of 8"), (dict(k=_rows(data=264)), b"misaligned rows"), (dict(v=_rows(data=0)), b"null"),
+    (dict(q=_rows(stride=132)), b"multiples of 8"), (dict(k=_rows(stride=120)), b"multiples of 8"),
+    (dict(v=_rows(stride=1 << 22)), b"multiples of 8"), (dict(g_stride=1), b"strides"), (dict(beta_stride=1 << 22), b"strides"), (dict(k=_rows(data=264)), b"misaligned rows"), (dict(v=_rows(data=0)), b"null"),
     (dict(o=0), b"null pointer"), (dict(state=0), b"null pointer"), (dict(state=264), b"misaligned"),
     (dict(slot_stride=32770), b"strides"), (dict(num_slots=-1), b"slots"), (dict(rows=1 << 30, nseq=1 << 30), b"rows of"),
 ])
 def test_recurrent_abi_refusals(kw, msg):
     lib, t = L.lib(), _tokens(**kw)
-    assert lib.lsurge_gdn_recurrent(ctypes.byref(t), None, 0, None) != 0
+    assert lib.lsurge_gdn_recurrent(ctypes.byref(t), None) != 0
     assert msg in lib.lsurge_last_error(), lib.lsurge_last_error()
 
 
 def test_recurrent_abi_empty():
     lib, t = L.lib(), _tokens(rows=0, nseq=0)
-    assert lib.lsurge_gdn_recurrent(ctypes.byref(t), None, 0, None) == 0
-    assert lib.lsurge_gdn_recurrent(None, None, 0, None) != 0
+    assert lib.lsurge_gdn_recurrent(ctypes.byref(t), None) == 0
+    assert lib.lsurge_gdn_recurrent(None, None) != 0
 
 
 def _update(**kw):
