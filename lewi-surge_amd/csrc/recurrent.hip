@@ -227,6 +227,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
 // since differences of sums go into exponents.
 constexpr int C = 32;
+// us for 100 sequences of 8 heads, token by token and in a chunk: 2 tokens each 27.5 and 31.0, 3 30.5 and 31.0, 4 32.8 and 31.1,
+// 5 35.3 and 31.3, 7 41.6 and 31.4.
 constexpr int CHUNKED = 4;
 constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
 constexpr int RUN_THREADS = 64 * 6;
@@ -827,8 +829,10 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
   return a;
 }
 
-// Columns a wave takes: 32 while that leaves four waves for every SIMD, then 16, then 8, whose shorter walks end sooner.
-int columns(int64_t seq_heads) { return seq_heads * 4 >= 4096 ? 32 : seq_heads * 8 >= 2048 ? 16 : 8; }
+// Columns a wave takes: 8 where there are few (sequence, head) pairs, whose one walk over a state is then shorter, else 32,
+// which reads whole lines.  us for 8 and 32, states in the caches: 64 pairs 4.2 and 6.1, 128 5.6 and 6.7, 256 8.8 and 7.3; from
+// memory: 128 7.7 and 7.7, 256 12.1 and 10.1, 2048 70 and 55.6 (16 columns: 61), where a copy of the states takes 52.3.
+int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 
 }  // namespace
 }  // namespace lsgdn
@@ -868,7 +872,6 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
                 hipLaunchKernelGGL((gdn_token_kernel<DT, CB, B32>), dim3((unsigned)a.units), dim3(64 * WAVES), 0, s, a))
 #define TOKENS_CB(DT, B32)                        \
   if (cb == 32) { TOKENS(DT, 32, B32); }          \
-  else if (cb == 16) { TOKENS(DT, 16, B32); }     \
   else { TOKENS(DT, 8, B32); }
   if (t->dtype == LSURGE_BF16) {
     if (b32) { TOKENS_CB(LSURGE_BF16, true) }
