@@ -283,22 +283,23 @@ def _rotary_arg(what, d, rows, like, inv_freq, positions, interleaved, inverse=F
     return arg, (inv_freq, positions)
 
 
-def _rotate(q, k, inv_freq, positions, cu, interleaved, inverse, nseq, shape):
-    """Rows q and k (either may be None) turned, or by `inverse` turned back."""
+def _rotate(q, k, inv_freq, positions, cu, interleaved, inverse, nseq):
+    """Dense or packed q and k (either may be None) turned, or by `inverse` turned back."""
     like = k if q is None else q
-    rows, _, d = like.shape
-    arg, keep = _rotary_arg("rotary", d, shape, like, inv_freq, positions, interleaved, inverse)
-    outs, args = [], []
+    arg, keep = _rotary_arg("rotary", like.shape[-1], like.shape[:-2], like, inv_freq, positions, interleaved, inverse)
+    outs, args, rows = [], [], 0
     for t in (q, k):
         if t is None:
             outs.append(None)
             args += (None, 0)
         else:
             outs.append(t.new_empty(t.shape))
-            t, *where = _row_args(t)
+            t, *where = _row_args(t if t.dim() == 3 else t.flatten(0, 1))
             keep += (t,)
-            args += (L.AttnRows(*where), t.shape[1])
-    _call("rotary", like.device, L.lib().lsurge_rotary_rows, arg, *args, d, rows, nseq, _ptr(cu), _ptr(outs[0]), _ptr(outs[1]))
+            rows, heads, _ = t.shape
+            args += (L.AttnRows(*where), heads)
+    _call("rotary", like.device, L.lib().lsurge_rotary_rows, arg, *args, like.shape[-1], rows, nseq, _ptr(cu), _ptr(outs[0]),
+          _ptr(outs[1]))
     del keep
     return outs
 
@@ -307,22 +308,22 @@ class _RotaryFn(torch.autograd.Function):
     """Always called through here, as _AttnFn is.  The backward turns the gradients back."""
 
     @staticmethod
-    def forward(ctx, q, k, inv_freq, positions, cu, interleaved, nseq, shape):
+    def forward(ctx, q, k, inv_freq, positions, cu, interleaved, nseq):
         ctx.save_for_backward(inv_freq, positions, cu)
-        ctx.rest = interleaved, nseq, shape, q.dtype
+        ctx.rest = interleaved, nseq, q.dtype
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq, shape))
+        return tuple(_rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        interleaved, nseq, shape, dtype = ctx.rest
+        interleaved, nseq, dtype = ctx.rest
         want_q, want_k = ctx.needs_input_grad[:2]
         dq = dq.to(dtype) if want_q and dq is not None else None
         dk = dk.to(dtype) if want_k and dk is not None else None
         if dq is not None or dk is not None:
-            dq, dk = _rotate(dq, dk, *ctx.saved_tensors, interleaved, True, nseq, shape)
-        return dq, dk, None, None, None, None, None, None
+            dq, dk = _rotate(dq, dk, *ctx.saved_tensors, interleaved, True, nseq)
+        return dq, dk, None, None, None, None, None
 
 
 def rotary(q, k, inv_freq, positions=None, cu_seqlens=None, interleaved=False):
@@ -343,19 +344,18 @@ def rotary(q, k, inv_freq, positions=None, cu_seqlens=None, interleaved=False):
     _check_dtype(what, q, k)
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: inv_freq has no gradient; detach it")
-    shape, kshape = q.shape, k.shape
-    if len(shape) == 4:
+    if q.dim() == 4:
         if cu_seqlens is not None:
             raise ValueError(f"{what}: cu_seqlens go with packed [T, H, D] tensors")
-        qo, ko = _RotaryFn.apply(q.flatten(0, 1), k.flatten(0, 1), inv_freq, positions, None, interleaved, shape[0], shape[:-2])
-        return qo.view(shape), ko.view(kshape)
-    if cu_seqlens is None and positions is None:
-        raise ValueError(f"{what}: packed tensors need cu_seqlens or positions")
-    nseq = 0
-    if cu_seqlens is not None:
+        nseq = q.shape[0]
+    elif cu_seqlens is None:
+        if positions is None:
+            raise ValueError(f"{what}: packed tensors need cu_seqlens or positions")
+        nseq = 0
+    else:
         nseq = max(cu_seqlens.numel() - 1, 0)
         cu_seqlens = _check_index(what, "cu_seqlens", cu_seqlens, (nseq + 1,))
-    return _RotaryFn.apply(q, k, inv_freq, positions, cu_seqlens, interleaved, nseq, shape[:-2])
+    return _RotaryFn.apply(q, k, inv_freq, positions, cu_seqlens, interleaved, nseq)
 
 
 def rotary_append_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens=None, positions=None,
