@@ -96,12 +96,10 @@ def causal_conv1d_update(inputs, kernel, state, state_slots=None, cu_seqlens=Non
     not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one slot.
     inputs may be a view with rows of any stride.  No gradient."""
     what = "causal_conv1d_update"
-    if kernel.dim() == 3 and kernel.shape[1] == 1:
-        kernel = kernel[:, 0]
-    if inputs.dim() != 2 or kernel.dim() != 2 or kernel.shape[1] != inputs.shape[1]:
+    K, *one, channels = kernel.shape if kernel.dim() in (2, 3) else (0, 0, 0)
+    if inputs.dim() != 2 or one not in ([], [1]) or inputs.shape[1] != channels:
         raise ValueError(f"{what}: inputs must be [rows, C], kernel [K, 1, C] or [K, C] (got {tuple(inputs.shape)}, "
                          f"{tuple(kernel.shape)})")
-    K, channels = kernel.shape
     if not 2 <= K <= 8 or channels < 8 or channels % 8:
         raise ValueError(f"{what}: 2 to 8 taps and a multiple of 8 channels (got {K}, {channels})")
     if state.dim() != 3 or state.shape[1:] != (K - 1, channels):
@@ -111,10 +109,10 @@ def causal_conv1d_update(inputs, kernel, state, state_slots=None, cu_seqlens=Non
     calls.check_device(what, inputs, kernel, state, state_slots, cu_seqlens)
     calls.check_dtype(what, inputs, kernel, state)
     calls.check_no_grad(what, inputs, kernel, state)
-    return calls.step(_update, inputs, kernel, state, state_slots, cu_seqlens, activation)
+    return calls.step(_update, inputs, kernel, K, state, state_slots, cu_seqlens, activation)
 
 
-def _update(x, w, state, state_slots, cu_seqlens, activation):
+def _update(x, w, taps, state, state_slots, cu_seqlens, activation):
     what = "causal_conv1d_update"
     rows, channels = x.shape
     nseq, cu, slots = calls.packed(what, rows, cu_seqlens, state, state_slots)
@@ -124,7 +122,7 @@ def _update(x, w, state, state_slots, cu_seqlens, activation):
     w = calls.aligned(L.contig(w))
     y = x.new_empty((rows, channels))
     arg = L.ConvUpdate(x.data_ptr(), w.data_ptr(), state.data_ptr(), y.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, channels,
-                       w.shape[0], x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
+                       taps, x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
     calls.call("causal_conv1d_update", x.device, L.lib().lsurge_causal_conv1d_update, arg)
     torch.autograd.graph.increment_version(state)
     return y
