@@ -195,7 +195,8 @@ __global__ void causal_conv_dw_reduce_kernel(const float* __restrict__ part, int
 // Packed new rows through the states.  One thread owns 8 channels over a tile of `tile` rows, as above.  The thread that
 // meets a sequence's first row computes its first K - 1 rows, also where they pass the end of its tile (the next tile leaves
 // them out), and it alone reads the slot and afterwards writes it: no other thread's row needs what it replaces.  Bound by
-// memory: x and y once, K - 1 rows read again a tile, the states read and written.
+// memory: x and y once, K - 1 rows read again a tile, the states read and written.  26369 rows of 8192 channels: 158 us, 5.5 TB/s
+// (a copy reaches 5.1); 64 single rows of 2048: 3.7 us, a launch and a trip to memory.
 struct UpdateArgs {
   const bf16_t *x, *w;
   int64_t x_stride;
@@ -291,13 +292,16 @@ int check_conv(const void* x, const void* w, int64_t b, int64_t t, int64_t c, in
   return LSURGE_OK;
 }
 
-// Rows a thread of the update walks: one while that leaves threads for every SIMD, then more, which reads fewer rows twice.
-int update_tile(int64_t rows, int64_t groups) {
-  int tile = 1;
-  while (tile < 32 && rows * groups / (2 * tile) >= (1 << 18)) tile *= 2;
+// Rows a thread of the update walks.  One where every row is a sequence of its own; of packed runs at least 4, which share the
+// search for their sequence, and up to 16 while that leaves threads for every SIMD.  us for 1, 4, 8, 16, 32 rows: 64 single rows
+// of 2048 channels 3.7, 7.0, 12, 23, 53; 4 runs of 500 11.5, 8.3, 9.5, 12, 16, of 8192 channels 32, 20, 18, 20, 23; 24 runs of
+// 1083 rows of 8192 430, 201, 162, 158, 165.
+int update_tile(bool packed, int64_t rows, int64_t groups) {
+  if (!packed) return 1;
+  int tile = 4;
+  while (tile < 16 && rows * groups / (2 * tile) >= (3 << 16)) tile *= 2;
   return tile;
 }
-
 #define CONV_K_CASES(M) M(1) M(2) M(3) M(4) M(5) M(6) M(7) M(8)
 
 }  // namespace
@@ -385,7 +389,7 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
   a.state = (bf16_t*)u->state, a.slot_stride = u->slot_stride;
   a.slots = u->slots, a.cu = u->cu, a.y = (bf16_t*)u->y;
   a.rows = (int)rows, a.nseq = (int)u->nseq, a.num_slots = (int)u->num_slots, a.groups = (int)(c / 8);
-  a.tile = update_tile(rows, a.groups);
+  a.tile = update_tile(u->cu, rows, a.groups);
   const int64_t threads = (rows + a.tile - 1) / a.tile * a.groups;
   LSURGE_REQUIRE(threads < (1ll << 32), "causal_conv1d_update: %lld rows of %lld channels", (long long)rows, (long long)c);
   const unsigned grid = (unsigned)((threads + CT - 1) / CT);

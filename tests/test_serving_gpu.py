@@ -334,7 +334,7 @@ def test_conv_one_row_each(n, C, dev):
 
 @pytest.mark.parametrize("K", [2, 4, 8])
 def test_conv_tiles_of_every_size(K, dev):
-    """So many rows that a thread walks 2 to 32 of them: sequences that begin at and around the tiles' ends, and many of fewer
+    """So many rows that a thread walks 4 to 16 of them: sequences that begin at and around the tiles' ends, and many of fewer
     rows than taps."""
     rng = np.random.default_rng(K)
     for C, lens in ((8192, [31, 1, 33, 32, 2, 64, 7, 130, 600, 30, 1, 1, 2, 95]),
