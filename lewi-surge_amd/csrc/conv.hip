@@ -210,6 +210,9 @@ template <int K, int DT, bool SILU>
 __global__ __launch_bounds__(CT) void causal_conv_update_kernel(UpdateArgs a) {
   const int64_t id = (int64_t)blockIdx.x * CT + threadIdx.x;
   const int64_t t0 = id / a.groups * a.tile;
+  // the sequence of the wave's first row, by all of its lanes
+  int near = a.cu ? lsrows::find_seq(a.cu, a.nseq, __builtin_amdgcn_readfirstlane((int)min(t0, (int64_t)a.rows - 1)),
+                                     threadIdx.x & 63) : 0;
   if (t0 >= a.rows) return;
   const int cg = (int)(id % a.groups);
   const int64_t C = 8 * (int64_t)a.groups;
@@ -222,7 +225,8 @@ __global__ __launch_bounds__(CT) void causal_conv_update_kernel(UpdateArgs a) {
   auto x_row = [&](int64_t t) { return *reinterpret_cast<const u32x4*>(xb + t * a.x_stride); };
 
   for (int r = first; r < t1;) {
-    const lsrows::Seq s = lsrows::seq_of(a.cu, a.nseq, a.rows, r);
+    const lsrows::Seq s = lsrows::seq_from(a.cu, a.nseq, a.rows, r, near);
+    near = max(near, s.seq);
     const int slot = s.seq < 0 ? -1 : a.slots ? a.slots[s.seq] : s.seq;
     const bool owner = s.begin >= first;  // of the sequence's first rows
     int t = owner ? r : max(r, s.begin + K - 1);

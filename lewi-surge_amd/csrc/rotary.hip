@@ -50,23 +50,45 @@ __device__ __forceinline__ void cos_sin_turn(float u, float& c, float& s) {
   s = m & 2 ? -b : b;
 }
 
+// 6 waves a SIMD: the compiler's own choice leaves 3 to 5 and takes 10% longer, for 8 it spills.
 template <int DT, bool INTER, int HEADS>
-__global__ __launch_bounds__(RT) void rotary_kernel(RotaryArgs a, int row0) {
+__global__ __launch_bounds__(RT, 6) void rotary_kernel(RotaryArgs a, int row0) {
   using lsrows::pack8;
   using lsrows::unpack8;
   const uint32_t id = blockIdx.x * RT + threadIdx.x;
   const uint32_t per_row = (uint32_t)a.groups << a.log2_units;
   const int64_t row64 = (int64_t)row0 + id / per_row;
+  const int row = (int)min(row64, (int64_t)a.rows - 1);
+  // the sequence of the wave's first row, by all of its lanes
+  const int near = a.cu ? lsrows::find_seq(a.cu, a.nseq, __builtin_amdgcn_readfirstlane(row), threadIdx.x & 63) : 0;
   if (row64 >= a.rows) return;
-  const int row = (int)row64;
   const uint32_t in_row = id % per_row;
   const int unit = in_row & ((1 << a.log2_units) - 1), group = in_row >> a.log2_units;
   const int D = 16 << a.log2_units, heads = a.hq + a.hk + a.hv;
 
+  const bool turns = unit < a.turned;
+  // a unit's 16 values: two runs of 8, half of the turned values apart, or consecutive
+  const int at0 = turns && !INTER ? 8 * unit : 16 * unit;
+  const int at1 = at0 + (turns && !INTER ? 8 * a.turned : 8);
+
+  const int pos = a.pos ? a.pos[row] : 0;
+  // The row is read whatever it holds, while its token is looked up.
+  u32x4 x[HEADS][2];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    const int h = i * a.groups + group;
+    if (h >= heads) continue;
+    const uint16_t* p = h < a.hq          ? a.q + row * a.q_row + h * a.q_head
+                        : h < a.hq + a.hk ? a.k + row * a.k_row + (h - a.hq) * a.k_head
+                                          : a.v + row * a.v_row + (h - a.hq - a.hk) * a.v_head;
+    const bool moved = turns && h < a.hq + a.hk;
+    x[i][0] = *reinterpret_cast<const u32x4*>(p + (moved ? at0 : 16 * unit));
+    x[i][1] = *reinterpret_cast<const u32x4*>(p + (moved ? at1 : 16 * unit + 8));
+  }
   // the row's token: its position, and its place in the cache
   int seq = -1, tok = -1;
   if (a.lens || a.cu) {
-    const lsrows::Seq s = lsrows::seq_of(a.cu, a.nseq, a.rows, row);
+    const lsrows::Seq s = lsrows::seq_from(a.cu, a.nseq, a.rows, row, near);
     seq = s.seq;
     if (seq >= 0) tok = a.lens ? max(a.lens[seq], 0) - (s.end - row) : row - s.begin;
   } else {
@@ -79,26 +101,9 @@ __global__ __launch_bounds__(RT) void rotary_kernel(RotaryArgs a, int row0) {
     slot = tok & ((1 << a.c.page_log2) - 1);
   }
   const bool paged = (unsigned)page < (unsigned)a.c.num_pages;
-  const bool turns = unit < a.turned;
-  // a unit's 16 values: two runs of 8, half of the turned values apart, or consecutive
-  const int at0 = turns && !INTER ? 8 * unit : 16 * unit;
-  const int at1 = at0 + (turns && !INTER ? 8 * a.turned : 8);
-
-  u32x4 x[HEADS][2];
-#pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    const int h = i * a.groups + group;
-    if (h >= heads || !live) continue;
-    const uint16_t* p = h < a.hq          ? a.q + row * a.q_row + h * a.q_head
-                        : h < a.hq + a.hk ? a.k + row * a.k_row + (h - a.hq) * a.k_head
-                                          : a.v + row * a.v_row + (h - a.hq - a.hk) * a.v_head;
-    const bool moved = turns && h < a.hq + a.hk;
-    x[i][0] = *reinterpret_cast<const u32x4*>(p + (moved ? at0 : 16 * unit));
-    x[i][1] = *reinterpret_cast<const u32x4*>(p + (moved ? at1 : 16 * unit + 8));
-  }
   float c[8], s[8];
   if (turns && live) {
-    const double p = (double)(a.pos ? a.pos[row] : tok) * 0.15915494309189533577;  // 1 / 2 pi
+    const double p = (double)(a.pos ? pos : tok) * 0.15915494309189533577;  // 1 / 2 pi
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const double t = p * a.freq[8 * unit + i];

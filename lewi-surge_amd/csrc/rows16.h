@@ -38,17 +38,30 @@ struct Seq {
   int seq, begin, end;
 };
 __device__ __forceinline__ int end_at(const int32_t* cu, int i, int rows) { return min(max(cu[i], 0), rows); }
-__device__ __forceinline__ Seq seq_of(const int32_t* cu, int nseq, int rows, int row) {
+// The last sequence that starts at or before a row that all 64 lanes of the wave ask for: one trip to memory for up to 64
+// sequences, two for up to 4096.  0 where none does.
+__device__ __forceinline__ int find_seq(const int32_t* cu, int nseq, int row, int lane) {
+  int lo = 0, n = nseq;
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int c = __popcll(__ballot(lane * step < n && cu[lo + min(lane * step, n - 1)] <= row));
+    if (c == 0) return 0;
+    n = min(step, n - (c - 1) * step);
+    lo += (c - 1) * step;
+  }
+  return lo;
+}
+// The sequence of a row, looked for from sequence `s` on, which starts no later.
+__device__ __forceinline__ Seq seq_from(const int32_t* cu, int nseq, int rows, int row, int s) {
   if (!cu) return {row, row, row + 1};
   if (nseq < 1) return {-1, row, row + 1};
-  int lo = 0, hi = nseq;  // the last sequence that starts at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (cu[mid] <= row) lo = mid;
-    else hi = mid;
+  int begin = end_at(cu, s, rows), end = end_at(cu, s + 1, rows);
+  while (end <= row && s + 1 < nseq) {
+    ++s;
+    begin = end;
+    end = end_at(cu, s + 1, rows);
   }
-  const Seq s{lo, end_at(cu, lo, rows), end_at(cu, lo + 1, rows)};
-  return s.begin <= row && row < s.end ? s : Seq{-1, row, row + 1};
+  return begin <= row && row < end ? Seq{s, begin, end} : Seq{-1, row, row + 1};
 }
 
 }  // namespace lsrows
