@@ -264,7 +264,19 @@ __device__ __forceinline__ f32x4 mma_32(u32x4 p, u32x4 q, f32x4 c) {  // D[16 x 
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
 }
-// x as a sum of N terms of DT, four values each
+// c minus the lower (HIGH: the upper) value of a register of two
+template <int DT, bool HIGH>
+__device__ __forceinline__ float minus(uint32_t x, float c) {
+  if constexpr (DT == LSURGE_F16) {
+    const lsrows::f16x2_t one{(_Float16)(HIGH ? 0.f : -1.f), (_Float16)(HIGH ? -1.f : 0.f)};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(lsrows::f16x2_t, x), one, c, false);
+  } else {
+    uint32_t one = HIGH ? 0xbf800000u : 0xbf80u;
+    asm("" : "+s"(one));  // as a literal the compiler encodes (-1, 0) as (-1, -1)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, one), c, false);
+  }
+}
+// x as a sum of N terms of DT, four values each.  What a term leaves over is exact, and one instruction a value.
 template <int DT, int N>
 __device__ __forceinline__ void split(f32x4 x, u32x2* t) {
 #pragma unroll
@@ -273,10 +285,8 @@ __device__ __forceinline__ void split(f32x4 x, u32x2* t) {
     if (n + 1 < N) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float lo, hi;
-        unpack2<DT>(t[n][i], lo, hi);
-        x[2 * i] -= lo;
-        x[2 * i + 1] -= hi;
+        x[2 * i] = minus<DT, false>(t[n][i], x[2 * i]);
+        x[2 * i + 1] = minus<DT, true>(t[n][i], x[2 * i + 1]);
       }
     }
   }
