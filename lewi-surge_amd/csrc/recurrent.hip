@@ -710,12 +710,6 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
       if (st < 3) {
         split<DT, NT>(S[2 * st + 2], s[(st + 1) & 1][0]);
         split<DT, NT>(S[2 * st + 3], s[(st + 1) & 1][1]);
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);  // LDS reads, then a product and a part of the splits in turn
-#pragma unroll
-        for (int i = 0; i < 2 * (NT + 2); ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
-        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
