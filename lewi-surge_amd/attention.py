@@ -312,7 +312,11 @@ class _RotaryFn(torch.autograd.Function):
         ctx.save_for_backward(inv_freq, positions, cu)
         ctx.rest = interleaved, nseq, q.dtype
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq))
+        out = _rotate(q, k, inv_freq, positions, cu, interleaved, False, nseq)
+        want = ctx.needs_input_grad[:2]
+        if want[0] != want[1]:  # the other's result needs no gradient either, so that a cache takes it
+            ctx.mark_non_differentiable(out[want[0]])
+        return tuple(out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable

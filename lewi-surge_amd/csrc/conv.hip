@@ -382,8 +382,8 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
                  u->activation);
   if (rows == 0) return LSURGE_OK;
   LSURGE_REQUIRE(u->num_slots >= 0 && u->num_slots < (1ll << 31) && u->slot_stride >= 0 && u->slot_stride < (1ll << 40) &&
-                     u->slot_stride % 8 == 0 && u->x_stride >= 0 && u->x_stride < (1ll << 32) && u->x_stride % 8 == 0,
-                 "causal_conv1d_update: %lld slots, strides of a slot %lld and a row %lld (multiples of 8)",
+                     u->slot_stride % 8 == 0 && (u->num_slots < 2 || u->slot_stride >= (k - 1) * c) && u->x_stride >= 0 && u->x_stride < (1ll << 32) && u->x_stride % 8 == 0,
+                 "causal_conv1d_update: %lld slots, strides of a slot %lld and a row %lld (multiples of 8, slots apart)",
                  (long long)u->num_slots, (long long)u->slot_stride, (long long)u->x_stride);
   LSURGE_REQUIRE(u->x && u->w && u->y && (u->state || u->num_slots == 0), "causal_conv1d_update: null pointer");
   LSURGE_REQUIRE(((uintptr_t)u->x | (uintptr_t)u->w | (uintptr_t)u->y | (uintptr_t)u->state) % 16 == 0,
@@ -395,7 +395,7 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
   a.rows = (int)rows, a.nseq = (int)u->nseq, a.num_slots = (int)u->num_slots, a.groups = (int)(c / 8);
   a.tile = update_tile(u->cu, rows, a.groups);
   const int64_t threads = (rows + a.tile - 1) / a.tile * a.groups;
-  LSURGE_REQUIRE(threads < (1ll << 32), "causal_conv1d_update: %lld rows of %lld channels", (long long)rows, (long long)c);
+  LSURGE_REQUIRE(threads <= (1ll << 32) - CT, "causal_conv1d_update: %lld rows of %lld channels", (long long)rows, (long long)c);
   const unsigned grid = (unsigned)((threads + CT - 1) / CT);
   hipStream_t s = (hipStream_t)stream;
 #define CONV_UPDATE(KK, DT, SILU)                                                                          \

@@ -220,7 +220,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 //
 // Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
 // terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
-// the state is kept times a power of two there, its largest value between 2^8 and 2^15: what is lost is below 2^-33 of it).
+// the state is kept times a power of two there, its largest value between 2^8 and 2^15: what is lost is below 2^-33 of it; the
+// power ends at 2^60, so a column below 2^-52, nothing beside f16 inputs, loses 2^-85).
 // The 16 x 16 matrices R, X, A and the inverse of A's diagonal blocks are three bf16 terms, and two where they reach o alone,
 // which is rounded to 11 bits or fewer.  A wave's 16 columns of every matrix lie in its lanes (lane l: column l % 16), so that
 // each product's result is in place as the next one's operand: the state, R and X never leave their lane.  (I + A) is solved by
@@ -532,9 +533,10 @@ __device__ __forceinline__ float column_max(float x) {
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// S and its scale changed by a power of two that brings a column's `most` to 2^12 .. 2^13, where it is outside [least, 2^15)
-__device__ __forceinline__ void rescale(float most, float least, f32x4* S, float& scale, float& unscale) {
-  const bool out = most < least || most >= 0x1p15f;
+// S, its scale and a column's `most` changed by a power of two that brings `most` to 2^12 .. 2^13, where it is outside
+// [2^8, 2^15)
+__device__ __forceinline__ void rescale(float& most, f32x4* S, float& scale, float& unscale) {
+  const bool out = most < 0x1p8f || most >= 0x1p15f;
   if (__ballot(out) == 0) return;
   const int e = out && most > 0.f ? (int)(__float_as_uint(most) >> 23) - 127 : 12;  // 2^e <= most < 2^(e + 1)
   const int now = (int)(__float_as_uint(scale) >> 23) - 127;
@@ -542,7 +544,7 @@ __device__ __forceinline__ void rescale(float most, float least, f32x4* S, float
   const float up = __uint_as_float((uint32_t)(127 + n) << 23), down = __uint_as_float((uint32_t)(127 - n) << 23);
 #pragma unroll
   for (int m = 0; m < 8; ++m) S[m] *= up;
-  scale *= up, unscale *= down;
+  most *= up, scale *= up, unscale *= down;
 }
 
 template <int DT, bool BETA32>
@@ -666,13 +668,14 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
     store_tiles(tiles[ring == 0 ? 2 : ring - 1]);  // of chunk n + 2, zeros behind the last
     load_tiles();
     ring = ring == 2 ? 0 : ring + 1;
+    float most = 0.f;  // f16: the largest of the column's values
     if constexpr (DT == LSURGE_F16) {
-      float most = 0.f;
 #pragma unroll
       for (int m = 0; m < 8; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(S[m][r]));
-      rescale(column_max(most), 0x1p8f, S, scale, unscale);
+      most = column_max(most);
+      rescale(most, S, scale, unscale);
       split<DT, NT>(S[0], s[0][0]);
       split<DT, NT>(S[1], s[0][1]);
     }
@@ -746,13 +749,14 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
     O[1] = mma_pair(m1[0][0], x0[0], m1[1][0], x0[0], O[1]);
     // the state's update
     f32x4 E[2] = {X[0] * w[0], X[1] * w[1]};
-    if constexpr (DT == LSURGE_F16) {
-      float most = 0.f;
+    if constexpr (DT == LSURGE_F16) {  // the decayed state's size, or what is added to it
+      float added = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(E[i][r]));
-      rescale(column_max(most) * scale, 0.f, S, scale, unscale);
+        for (int r = 0; r < 4; ++r) added = fmaxf(added, fabsf(E[i][r]));
+      most = fmaxf(most * decay, column_max(added) * scale);
+      rescale(most, S, scale, unscale);
 #pragma unroll
       for (int i = 0; i < 2; ++i) E[i] *= scale;
     }
@@ -814,7 +818,7 @@ int check_tokens(const lsurge_gdn_tokens* t) {
   LSURGE_REQUIRE(((uintptr_t)t->state | (uintptr_t)t->o) % 16 == 0 && (uintptr_t)t->g % 4 == 0, "%s: misaligned pointer", what);
   LSURGE_REQUIRE(t->g_stride >= t->hv && t->g_stride < MOST_ROW && t->beta_stride >= t->hv && t->beta_stride < MOST_ROW &&
                      t->num_slots >= 0 && t->num_slots < (1ll << 31) && t->slot_stride >= 0 && t->slot_stride < (1ll << 40) &&
-                     t->slot_stride % 4 == 0,
+                     t->slot_stride % 4 == 0 && (t->num_slots < 2 || t->slot_stride >= t->hv * D * D),
                  "%s: strides of g, beta and a slot (%lld, %lld, %lld), %lld slots", what, (long long)t->g_stride,
                  (long long)t->beta_stride, (long long)t->slot_stride, (long long)t->num_slots);
   return LSURGE_OK;

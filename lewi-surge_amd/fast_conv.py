@@ -17,7 +17,6 @@ MaxText, third-party and not vendored):
 """
 from __future__ import annotations
 
-
 import torch
 
 import _calls as calls
@@ -77,7 +76,8 @@ def causal_conv1d(inputs, kernel):
 
 
 def alloc_conv_state(slots, taps, channels, dtype=torch.bfloat16, device="cuda"):
-    """The kept inputs of sequences that have no row yet, zeros [slots, taps - 1, channels]."""
+    """The kept inputs of sequences that have no row yet, zeros [slots, taps - 1, channels].  A slot that passes on to a new
+    sequence is cleared by the caller."""
     return torch.zeros((slots, taps - 1, channels), dtype=dtype, device=device)
 
 
@@ -121,8 +121,8 @@ def _update(x, w, taps, state, state_slots, cu_seqlens, activation):
         x = x.clone(memory_format=torch.contiguous_format)
     w = calls.aligned(L.contig(w))
     y = x.new_empty((rows, channels))
-    arg = L.ConvUpdate(x.data_ptr(), w.data_ptr(), state.data_ptr(), y.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq, channels,
-                       taps, x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
-    calls.call("causal_conv1d_update", x.device, L.lib().lsurge_causal_conv1d_update, arg)
+    arg = L.ConvUpdate(x.data_ptr(), w.data_ptr(), state.data_ptr(), y.data_ptr(), calls.ptr(slots), calls.ptr(cu), rows, nseq,
+                       channels, taps, x.stride(0), state.shape[0], stride, L.dt(x), _ACTIVATIONS[activation])
+    calls.call(what, x.device, L.lib().lsurge_causal_conv1d_update, arg)
     torch.autograd.graph.increment_version(state)
     return y

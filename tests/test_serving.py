@@ -292,9 +292,11 @@ def _tokens(**kw):
     (dict(rows=5), b"5 rows of 4"), (dict(rows=-1, cu=FAKE), b"-1 rows"), (dict(hv=3, hk=2), b"3 value heads over 2"),
     (dict(hk=0), b"value heads over 0"), (dict(dtype=L.F32), b"bf16 or f16"), (dict(beta_dtype=L.F16), b"beta alike"),
     (dict(q=_rows(stride=132)), b"multiples of 8"), (dict(k=_rows(stride=120)), b"multiples of 8"),
-    (dict(v=_rows(stride=1 << 22)), b"multiples of 8"), (dict(g_stride=1), b"strides"), (dict(beta_stride=1 << 22), b"strides"), (dict(k=_rows(data=264)), b"misaligned rows"), (dict(v=_rows(data=0)), b"null"),
+    (dict(v=_rows(stride=1 << 22)), b"multiples of 8"),
+    (dict(g_stride=1), b"strides"), (dict(beta_stride=1 << 22), b"strides"), (dict(k=_rows(data=264)), b"misaligned rows"), (dict(v=_rows(data=0)), b"null"),
     (dict(o=0), b"null pointer"), (dict(state=0), b"null pointer"), (dict(state=264), b"misaligned"),
-    (dict(slot_stride=32770), b"strides"), (dict(num_slots=-1), b"slots"), (dict(rows=1 << 30, nseq=1 << 30), b"rows of"),
+    (dict(slot_stride=32770), b"strides"), (dict(slot_stride=32764), b"strides"),
+    (dict(num_slots=-1), b"slots"), (dict(rows=1 << 30, nseq=1 << 30), b"rows of"),
 ])
 def test_recurrent_abi_refusals(kw, msg):
     lib, t = L.lib(), _tokens(**kw)
@@ -317,8 +319,8 @@ def _update(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(channels=12), b"12 channels"), (dict(taps=1), b"1 taps"), (dict(taps=9), b"9 taps"), (dict(rows=3), b"3 rows of 4"),
-    (dict(dtype=L.F32), b"bf16 or f16"), (dict(activation=2), b"activation 2"), (dict(slot_stride=44), b"strides"),
-    (dict(x_stride=17), b"strides"), (dict(x=0), b"null pointer"), (dict(state=0), b"null pointer"), (dict(y=264), b"aligned"),
+    (dict(dtype=L.F32), b"bf16 or f16"), (dict(activation=2), b"activation 2"),
+    (dict(slot_stride=44), b"strides"), (dict(slot_stride=40), b"strides"), (dict(x_stride=17), b"strides"), (dict(x=0), b"null pointer"), (dict(state=0), b"null pointer"), (dict(y=264), b"aligned"),
 ])
 def test_conv_update_abi_refusals(kw, msg):
     lib, u = L.lib(), _update(**kw)

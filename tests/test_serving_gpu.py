@@ -3,6 +3,7 @@ float64 oracle derives from the roundings (oracle/serving_oracle.py); what has t
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import attention as A
 import fast_conv as FC
@@ -264,6 +265,67 @@ def test_rule_values_that_are_not_finite_stay_in_their_sequence(dev):
             assert torch.equal(o[at[b]:at[b + 1]], want[at[b]:at[b + 1]]) and torch.equal(r.state[r.slots[b]], after[r.slots[b]])
 
 
+def test_rule_states_of_any_size(dev):
+    """Columns of sizes from 2^-50 to 2^60 side by side; the rule takes columns apart, so each group of one size is held to its
+    own bounds.  f16's range is short: a column's state is scaled there.  Without values and queries, the states alone.
+
+    The decays take some columns below what any type holds.  float32 loses up to 2^-126 a value there.  f16 scales by 2^60 at
+    most, and two terms leave up to 2^-25 of a scaled value over, so 2^-85: k, a unit vector of 128 values, sums that to
+    sqrt(128) 2^-85 a column, 4 sqrt(128) 2^-85 in the 2-norm over 16 columns, which d and, times k, the state take over, and
+    the update's own terms as much again, at each of the n tokens, with factors of at most 1 afterwards."""
+    scale = torch.tensor([2.0 ** e for e in (-50, -30, -14, 0, 10, 30, 50, 60)], device=dev).repeat_interleave(16)
+    for dt, decay in ((F16, 0.05), (F16, 2.0), (BF16, 0.05)):
+        r = Rule(dt, 1, 2, [70, 5, 2], dev, decay=decay)
+        r.q.zero_(), r.v.zero_(), r.state.mul_(scale)
+        before = r.state.clone()
+        assert not r.call().any()
+        at = _starts(r.lens)
+        for b, n in enumerate(r.lens):
+            rows = slice(at[b], at[b] + n)
+            for c in range(0, 128, 16):
+                _, want, _, bound = so.delta_rule(*(_np(t[rows]) for t in (r.q, r.k)), np.zeros((n, 2, 16)), _np(r.g[rows]),
+                                                  _np(r.beta[rows]), _np(before[r.slots[b]][..., c:c + 16]), True)
+                off = np.linalg.norm(_np(r.state[r.slots[b]][..., c:c + 16]) - want, axis=(1, 2))
+                least = 2 * n * 4 * 128 ** 0.5 * 2.0 ** (-85 if dt is F16 else -126)
+                assert (off <= bound + least).all(), (dt, decay, n, c, off, bound)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_rule_reads_what_was_erased(dt, dev):
+    """Queries equal to their keys, beta 1, no decay and no values: each token erases what it reads, and o is 0 but for what the
+    chunks' parts of o are held to.  These are q_i.S0 and (q_i.k_j) d_j, |d_j| <= |S0|, each with 2^-18 of either factor left
+    out and 2^-18 of both together, 2^-16 at most; the state's own bound besides."""
+    r = Rule(dt, 1, 2, [32], dev, norm=True, beta32=True)
+    r.q.copy_(r.k), r.v.zero_(), r.g.zero_(), r.beta.fill_(1)
+    before = r.state.clone()
+    o = _np(r.call())
+    k = _np(r.k)[:, 0]
+    k /= np.sqrt((k * k).sum(-1, keepdims=True) + 1e-6)
+    wo, wS, bo, bS = so.delta_rule(*(_np(t) for t in (r.q, r.k, r.v, r.g, r.beta)), _np(before[r.slots[0]]), True)
+    size = np.linalg.norm(_np(before[r.slots[0]]), axis=(1, 2))
+    parts = (1 + np.tril(np.abs(k @ k.T)).sum(1))[:, None] * size / 128 ** 0.5
+    assert (np.linalg.norm(o - wo, axis=-1) <= bo + 2.0 ** -16 * parts * (1 + so.HALF_STEP[NAME[dt]])).all()
+    assert (np.linalg.norm(_np(r.state[r.slots[0]]) - wS, axis=(1, 2)) <= bS).all()
+
+
+def test_rule_columns_of_any_size(dev):
+    """Values from f16's smallest to its largest in one head: each group of columns of one size within its own bounds."""
+    scale = torch.tensor([2.0 ** e for e in (-22, -14, -8, -2, 0, 4, 8, 12)], device=dev).repeat_interleave(16)
+    r = Rule(F16, 1, 2, [100, 6], dev)
+    r.v.copy_((r.v.float() * scale).half()), r.state.mul_(scale)
+    before = r.state.clone()
+    o, at = r.call(), _starts(r.lens)
+    for b, n in enumerate(r.lens):
+        rows = slice(at[b], at[b] + n)
+        for c in range(0, 128, 16):
+            wo, want, bo, bound = so.delta_rule(*(_np(t[rows]) for t in (r.q, r.k)), _np(r.v[rows][..., c:c + 16]), _np(r.g[rows]),
+                                                _np(r.beta[rows]), _np(before[r.slots[b]][..., c:c + 16]), True)
+            off = np.linalg.norm(_np(r.state[r.slots[b]][..., c:c + 16]) - want, axis=(1, 2))
+            assert (off <= bound).all(), (n, c, off, bound)
+            off = np.linalg.norm(_np(o[rows][..., c:c + 16]) - wo, axis=-1)
+            assert (off <= bo + so.HALF_STEP["f16"] * (np.linalg.norm(wo, axis=-1) + bo) + 4 * so.TINY["f16"]).all(), (n, c)
+
+
 def test_rule_far_slots(dev):
     """A pool of more than 2^31 elements."""
     hv = 8
@@ -340,6 +402,14 @@ def test_conv_tiles_of_every_size(K, dev):
     for C, lens in ((8192, [31, 1, 33, 32, 2, 64, 7, 130, 600, 30, 1, 1, 2, 95]),
                     (4096, [int(n) for n in rng.integers(0, 12, 700)]), (2048, [4000, 63, 1, 65, 31, 3, 2500])):
         run_conv(BF16, K, C, lens, dev, tail=70)
+
+
+def test_conv_thousands_of_sequences(dev):
+    """More than 64 and more than 64^2 ends to find a row's sequence among, many of them without rows."""
+    rng = np.random.default_rng(1)
+    for n, most in ((65, 4), (4097, 3), (9000, 2)):
+        run_conv(BF16, 4, 8, [int(i) for i in rng.integers(0, most, n)], dev, tail=3)
+    run_conv(BF16, 4, 16, [0] * 5000 + [7] + [0] * 5000, dev)
 
 
 def test_conv_places_without_a_slot(dev):
@@ -458,6 +528,16 @@ def test_rotary_heads_a_thread(rows, heads, dev):
     check_rotary(q, k, A.rotary_inv_freq(128, 1e6, dev), _pos([rows]), False, rows, cu_seqlens=_ends([rows], dev))
 
 
+def test_rotary_thousands_of_sequences(dev):
+    rng = np.random.default_rng(2)
+    gen = torch.Generator().manual_seed(2)
+    f = A.rotary_inv_freq(16, 1e4, dev)
+    for n, most in ((65, 40), (4097, 3), (9000, 2)):
+        lens = [int(i) for i in rng.integers(0, most, n)]
+        rows = _randn(gen, (sum(lens) + 4, 2, 64), F16, dev)
+        check_rotary(rows[:, :1], rows[:, 1:], f, _pos(lens), False, sum(lens), cu_seqlens=_ends(lens, dev))
+
+
 def test_rotary_far_positions(dev):
     """Positions up to 2^31 - 1 and negative ones, given by themselves."""
     pos = [0, 1, -1, 100003, 10 ** 6, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31]
@@ -504,6 +584,50 @@ def test_rotary_one_gradient_and_empty(dev):
     assert o.shape == (0, 2, 64) and p.shape == (0, 1, 64)
     o, p = A.rotary(q, k, f, cu_seqlens=_i32([0], dev))  # no sequence: every row is behind the last
     assert not o.any() and not p.any()
+
+
+def test_rotary_results_without_a_gradient(dev):
+    """What comes of a tensor that needs no gradient needs none: a turned k goes into a cache beside a q that trains."""
+    gen = torch.Generator().manual_seed(8)
+    q, k = _randn(gen, (9, 2, 64), BF16, dev).requires_grad_(), _randn(gen, (9, 1, 64), BF16, dev)
+    f, cu = A.rotary_inv_freq(64, 1e4, dev), _i32([0, 9], dev)
+    oq, ok = A.rotary(q, k, f, cu_seqlens=cu)
+    assert oq.requires_grad and not ok.requires_grad
+    c = Cache(BF16, 1, 64, 16, [9], dev)
+    A.append_kv(c.k, c.v, c.table, c.lens, ok, k, cu_seqlens=cu)
+    grad, = torch.autograd.grad(oq, q, q)
+    ok, oq = A.rotary(k, q[:, :1], f, cu_seqlens=cu)
+    assert oq.requires_grad and not ok.requires_grad
+    assert torch.equal(torch.autograd.grad(oq, q, q[:, :1])[0][:, :1], grad[:, :1])
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in A.rotary(q, k, f, cu_seqlens=cu))
+
+
+def test_rotary_refuses_what_its_gradient_cannot_give(dev):
+    gen = torch.Generator().manual_seed(9)
+    q, k = _randn(gen, (9, 2, 64), BF16, dev).requires_grad_(), _randn(gen, (9, 1, 64), BF16, dev)
+    f, cu, pos = A.rotary_inv_freq(64, 1e4, dev), _i32([0, 9], dev), _i32(range(9), dev)
+    for kw in (dict(positions=pos), dict(cu_seqlens=cu), dict(cu_seqlens=cu, positions=pos)):
+        for t in kw.values():
+            out = A.rotary(q, k, f, **kw)[0].sum()
+            t.add_(0)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.backward()
+    dq, = torch.autograd.grad(A.rotary(q, k, f, cu_seqlens=cu)[0].square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.sum().backward()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q.detach(), torch.ones_like(q))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            A.rotary(dual, k, f, cu_seqlens=cu)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            A.rotary(k, k, forward_ad.make_dual(f, torch.ones_like(f)), cu_seqlens=cu)
+        r, c = Rule(BF16, 1, 2, [1], dev), Conv(BF16, 4, 16, [1], dev)
+        r.v = forward_ad.make_dual(r.v, torch.ones_like(r.v))
+        c.x = forward_ad.make_dual(c.x, torch.ones_like(c.x))
+        for call in (r.call, c.call):
+            with pytest.raises(ValueError, match="of the forward mode neither"):
+                call()
 
 
 def test_rotary_then_attention_trains(dev):
@@ -599,6 +723,12 @@ def test_append_lengths_shorter_than_the_rows_and_pages_missing(dev):
 
 def test_append_positions(dev):
     check_append(F16, 2, 1, 128, 128, 16, [3, 5], [3, 40], dev, positions=[5, 6, 7, 10 ** 6, -4, 0, 2 ** 31 - 1, 12])
+
+
+def test_append_thousands_of_sequences(dev):
+    rng = np.random.default_rng(3)
+    new = [int(i) for i in rng.integers(0, 3, 4200)]
+    check_append(BF16, 2, 1, 64, 64, 8, new, [n + int(i) for n, i in zip(new, rng.integers(0, 9, 4200))], dev, tail=2)
 
 
 def test_append_no_sequence(dev):
@@ -790,3 +920,109 @@ def test_traces_hold_the_calls(dev):
     want = fn(*args, r.state.clone())
     traced = torch.jit.trace(fn, (*args, r.state.clone()), check_trace=False)
     assert torch.equal(traced(*args, r.state.clone()), want)
+
+    w, f = torch.ones((4, 16), dtype=BF16, device=dev), A.rotary_inv_freq(64, 1e4, dev)
+    gen = torch.Generator().manual_seed(14)
+    x, states = _randn(gen, (2, 16), BF16, dev), FC.alloc_conv_state(2, 4, 16, BF16, dev)
+
+    def conv(x, state):
+        return FC.causal_conv1d_update(x, w, state)
+
+    traced = torch.jit.trace(conv, (x, states.clone()), check_trace=False)
+    y, kept, kept2 = 2 * x, states.clone(), states.clone()
+    assert torch.equal(traced(y, kept), conv(y, kept2)) and torch.equal(kept, kept2)
+
+    rows = _randn(gen, (2, 4, 64), BF16, dev)
+    table, lens = _i32([[0], [1]], dev), _i32([3, 8], dev)
+
+    def append(rows, kc, vc):
+        return A.rotary_append_kv(rows[:, :2], rows[:, 2:3], rows[:, 3:], kc, vc, table, lens, f)
+
+    caches = [[torch.zeros_like(t) for t in A.alloc_kv_cache(2, 8, 1, 64, BF16, dev)] for _ in range(3)]
+    traced = torch.jit.trace(append, (rows, *caches[0]), check_trace=False)
+    rows = 2 * rows
+    assert torch.equal(traced(rows, *caches[1]), append(rows, *caches[2]))
+    assert torch.equal(caches[1][0], caches[2][0]) and torch.equal(caches[1][1], caches[2][1])
+    assert caches[1][0].any() and caches[1][1].any()
+
+    def turn(rows):
+        return A.rotary(rows[:, :3], rows[:, 3:], f, positions=lens)
+
+    traced = torch.jit.trace(turn, (rows,), check_trace=False)
+    assert all(torch.equal(a, b) for a, b in zip(traced(2 * rows), turn(2 * rows)))
+
+
+def test_captured_runs_replay(dev):
+    """Prompts and single tokens in a graph whose sequences' ends, slots and lengths change between replays, the last of them
+    without rows; padding rows of NaN behind them."""
+    gen = torch.Generator().manual_seed(15)
+    p = _layer(gen, dev)
+    n, rows, hv = 4, 90, p["hv"]
+    x, qkv = _randn(gen, (rows, p["C"]), BF16, dev), _randn(gen, (rows, p["hq"] + 2 * p["hkv"], p["D"]), BF16, dev)
+    g, beta = -0.1 * torch.rand((rows, hv), device=dev), torch.ones((rows, hv), dtype=BF16, device=dev)
+    slots, lens, cu = _i32([0, 1, 2, 3], dev), _i32([1, 40, 2, 5], dev), _i32([0, 1, 41, 43, 48], dev)
+    c = Cache(BF16, p["hkv"], p["D"], 8, [90] * n, dev)
+    states = FC.alloc_conv_state(6, 4, p["C"], BF16, dev), G.alloc_delta_state(6, hv, dev)
+    keep = [*states, c.k, c.v]
+
+    def step():
+        y = FC.causal_conv1d_update(x, p["conv"], states[0], slots, cu, activation="silu")
+        q, k, v = y.view(rows, -1, 128).split((p["hk"], p["hk"], hv), 1)
+        o = G.recurrent_gated_delta_rule(q, k, v, g, beta, states[1], slots, cu, use_qk_norm_in_gdn=True)
+        q, k, v = qkv.split((p["hq"], p["hkv"], p["hkv"]), 1)
+        return [y, o, *A.rotary_append_kv(q, k, v, c.k, c.v, c.table, lens, p["freq"], cu_seqlens=cu, return_k=True)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i, ends in enumerate(([1, 2, 3, 4], [33, 34, 34, 90], [0, 0, 0, 0], [70, 75, 77, 80], [1, 41, 43, 48])):
+        x.copy_(_randn(gen, x.shape, BF16, dev)), qkv.copy_(_randn(gen, qkv.shape, BF16, dev))
+        x[ends[-1]:], qkv[ends[-1]:] = float("nan"), float("nan")
+        cu.copy_(_i32([0] + ends, dev))
+        slots.copy_(_i32([5, -1, 0, 1] if i % 2 else [3, 2, 4, -1], dev))
+        lens.copy_(_i32([max(b - a, 0) + i for a, b in zip([0] + ends, ends)], dev))
+        before = [t.clone() for t in keep]
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in (*out, *keep)]
+        for t, b in zip(keep, before):
+            t.copy_(b)
+        eager = step()
+        torch.cuda.synchronize()
+        for a, b in zip(replayed, (*eager, *keep)):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(dev):
+    """Two streams' calls on slots of their own of the same pools, in flight together, give what they give in turn."""
+    calls, before, want = [], [], []
+    for seed in range(2):
+        r, c = Rule(BF16, 2, 8, [200, 1, 33, 5], dev, seed=seed), Conv(BF16, 4, 1024, [200, 1, 33, 5], dev, seed=seed)
+        if calls:  # one pool for both
+            pool, conv = calls[0][0].state, calls[0][1].state
+            pool[7:], conv[7:] = r.state, c.state
+            r.state, c.state = pool, conv
+            r.slots, c.slots = [s + 7 for s in r.slots], [s + 7 for s in c.slots]
+        else:
+            r.state, c.state = torch.cat([r.state, r.state]), torch.cat([c.state, c.state])
+        calls.append((r, c))
+    pools = calls[0][0].state, calls[0][1].state
+    before = [t.clone() for t in pools]
+    want = [(r.call(), c.call()) for r, c in calls]
+    after = [t.clone() for t in pools]
+    for t, b in zip(pools, before):
+        t.copy_(b)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], []
+    for s, (r, c) in zip(streams, calls):
+        with torch.cuda.stream(s):
+            got.append((r.call(), c.call()))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(pools[0], after[0]) and torch.equal(pools[1], after[1])
