@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 //   o_i = (e^{G_i} S0^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i.k_j) x_j) / sqrt(128),
 //   S = e^{G_C} S0 + sum_j e^{G_C - G_j} k_j x_j^T
 // (row i of X is the token's d).  A and the weights of o do not depend on the state: two waves form them for the next chunk
-// while four waves of 16 columns each take this one, with one barrier a chunk.
+// while two or four waves of 16 columns each take this one, with one barrier a chunk.
 //
 // Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
 // terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
@@ -232,7 +232,6 @@ constexpr int C = 32;
 // 5 35.3 and 31.3, 7 41.6 and 31.4.
 constexpr int CHUNKED = 4;
 constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
-constexpr int RUN_THREADS = 64 * 6;
 constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
 constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
 
@@ -547,8 +546,10 @@ __device__ __forceinline__ void rescale(float& most, f32x4* S, float& scale, flo
   most *= up, scale *= up, unscale *= down;
 }
 
-template <int DT, bool BETA32>
-__global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
+// NW waves take columns, two prepare.
+template <int DT, bool BETA32, int NW>
+__global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel(TokenArgs a) {
+  constexpr int PARTS = D / (16 * NW);  // workgroups a (sequence, head)
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
   __shared__ ChunkTiles tiles[3];
   __shared__ ChunkTerms terms[2];
@@ -556,63 +557,26 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
   __shared__ float blocks[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
-  const Unit u = unit_of(a, blockIdx.x >> 1);
-  const int col0 = (blockIdx.x & 1) * 64 + wave * 16;
+  // Workgroups go to the 8 XCDs in turn: all that read one key head's rows to one of them, for its L2 (1 to 3%).
+  const uint32_t group = PARTS * (a.hv / a.hk), in = blockIdx.x % (8 * group);
+  const uint32_t id = (blockIdx.x - in) + in % 8 * group + in / 8;
+  if ((int)id >= a.nseq * a.hv * PARTS) return;
+  const Unit u = unit_of(a, id / PARTS);
+  const int col0 = (id % PARTS * NW + wave) * 16;
   const int total = u.end - u.begin;
   if (total <= 0) return;
   if (total < CHUNKED || (unsigned)u.slot >= (unsigned)a.num_slots) {
-    if (wave < 4) walk_tokens<DT, 16, BETA32>(a, u, col0, lane);
+    if (wave < NW) walk_tokens<DT, 16, BETA32>(a, u, col0, lane);
     return;
   }
   const int chunks = (total + C - 1) / C;
   const int c = lane & 15, g = lane >> 4;
 
-  // While four waves take chunk n, two prepare chunk n + 1 from its tiles, which the four staged during chunk n - 1.
-  if (wave >= 4) {
-    const int g_off = (lane & 31) * (int)a.g_row * 4, b_size = BETA32 ? 4 : 2, b_off = (lane & 31) * (int)a.beta_row * b_size;
-    ChunkRows gs(u, a.g + u.h, a.g_row, 1, 4), bs(u, (const char*)a.beta + u.h * b_size, a.beta_row, 1, b_size);
-    auto load = [&](float& decay, float& beta) {
-      const auto gb = gs.next(), bb = bs.next();
-      decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gb, g_off, 0, 0));
-      if constexpr (BETA32) {
-        beta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bb, b_off, 0, 0));
-      } else {
-        const uint16_t x = __builtin_amdgcn_raw_buffer_load_b16(bb, b_off, 0, 0);
-        beta = DT == LSURGE_F16 ? f16_to_f32(x) : bf16_to_f32(x);
-      }
-    };
-    float decay, beta, decay1, beta1;
-    load(decay, beta);
-    stage_barrier();  // the first chunk is staged
-    for (int n = 0; n < chunks; ++n) {
-      load(decay1, beta1);
-      if (wave == 4) prepare_inverse<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch[0], blocks, terms[n & 1]);
-      else prepare_rest<DT>(tiles[n % 3], decay, beta, a.l2_eps, lane, scratch[1], terms[n & 1]);
-      decay = decay1, beta = beta1;
-      stage_barrier();  // chunk n is prepared
-    }
-    return;
-  }
-
-  // wave < 4: the columns col0 .. + 15 of the state: tile m, register r: row 16 m + 4 g + r, column c
-  float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + 4 * g * D + col0 + c;
-  f32x4 S[8];
-  float scale = 1.f, unscale = 1.f;  // f16: S holds the state times `scale`, a power of two of the column's own
-#pragma unroll
-  for (int m = 0; m < 8; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) S[m][r] = sp[(16 * m + r) * D];
-
-  const int kh = u.h / (a.hv / a.hk);
-  // this thread's part of the tiles: two pieces of 8 values of k and of q
-  const int srow = threadIdx.x >> 4, scol = (threadIdx.x & 15) * 8;
+  // The first four waves stage: a thread's part of the tiles is two pieces of 8 values of k and of q.
+  const int kh = u.h / (a.hv / a.hk), srow = threadIdx.x >> 4, scol = (threadIdx.x & 15) * 8;
   int k_off = (srow * (int)a.k_row + scol) * 2, q_off = (srow * (int)a.q_row + scol) * 2;
-  const int o_row = a.hv * D;
-  int v_off = (4 * g * (int)a.v_row + col0 + c) * 2, o_off = (4 * g * o_row + col0 + c) * 2;
   u32x4 kr[2], qr[2];
-  uint16_t vr[8];
   ChunkRows ks(u, a.k + kh * a.k_head, a.k_row, D, 2), qs(u, a.q + kh * a.q_head, a.q_row, D, 2);
-  ChunkRows vs(u, a.v + u.h * a.v_head, a.v_row, D, 2), os(u, a.o + (int64_t)u.h * D, o_row, D, 2);
   auto load_tiles = [&]() {
     const auto kb = ks.next(), qb = qs.next();
 #pragma unroll
@@ -628,6 +592,58 @@ __global__ __launch_bounds__(RUN_THREADS, 3) void gdn_run_kernel(TokenArgs a) {
       *reinterpret_cast<u32x4*>(&x.q[srow + 16 * i][scol]) = qr[i];
     }
   };
+
+  // While the others take chunk n - 1, two waves prepare chunk n from its tiles; chunk n + 1 is staged.
+  if (wave >= NW) {
+    constexpr bool stages = NW == 2;  // two of the first four waves
+    const int g_off = (lane & 31) * (int)a.g_row * 4, b_size = BETA32 ? 4 : 2, b_off = (lane & 31) * (int)a.beta_row * b_size;
+    ChunkRows gs(u, a.g + u.h, a.g_row, 1, 4), bs(u, (const char*)a.beta + u.h * b_size, a.beta_row, 1, b_size);
+    auto load = [&](float& decay, float& beta) {
+      const auto gb = gs.next(), bb = bs.next();
+      decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gb, g_off, 0, 0));
+      if constexpr (BETA32) {
+        beta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(bb, b_off, 0, 0));
+      } else {
+        const uint16_t x = __builtin_amdgcn_raw_buffer_load_b16(bb, b_off, 0, 0);
+        beta = DT == LSURGE_F16 ? f16_to_f32(x) : bf16_to_f32(x);
+      }
+    };
+    float decay, beta, decay1, beta1;
+    if (stages) load_tiles();
+    load(decay, beta);
+    if (stages) store_tiles(tiles[0]), load_tiles();
+    stage_barrier();  // the first chunk is staged
+    int ring = 0;  // n % 3
+    for (int n = 0; n < chunks; ++n) {
+      const ChunkTiles& tile = tiles[ring];
+      ring = ring == 2 ? 0 : ring + 1;
+      if (stages) {
+        asm volatile("" : "+v"(k_off), "+v"(q_off));
+        store_tiles(tiles[ring]);
+        load_tiles();
+      }
+      load(decay1, beta1);
+      if (wave == NW) prepare_inverse<DT>(tile, decay, beta, a.l2_eps, lane, scratch[0], blocks, terms[n & 1]);
+      else prepare_rest<DT>(tile, decay, beta, a.l2_eps, lane, scratch[1], terms[n & 1]);
+      decay = decay1, beta = beta1;
+      stage_barrier();  // chunk n is prepared
+    }
+    return;
+  }
+
+  // the columns col0 .. + 15 of the state: tile m, register r: row 16 m + 4 g + r, column c
+  float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + 4 * g * D + col0 + c;
+  f32x4 S[8];
+  float scale = 1.f, unscale = 1.f;  // f16: S holds the state times `scale`, a power of two of the column's own
+#pragma unroll
+  for (int m = 0; m < 8; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[m][r] = sp[(16 * m + r) * D];
+
+  const int o_row = a.hv * D;
+  int v_off = (4 * g * (int)a.v_row + col0 + c) * 2, o_off = (4 * g * o_row + col0 + c) * 2;
+  uint16_t vr[8];
+  ChunkRows vs(u, a.v + u.h * a.v_head, a.v_row, D, 2), os(u, a.o + (int64_t)u.h * D, o_row, D, 2);
   auto load_v = [&]() {
     const auto vb = vs.next();
 #pragma unroll
@@ -841,6 +857,10 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
 // which reads whole lines.  us for 8 and 32, states in the caches: 64 pairs 4.2 and 6.1, 128 5.6 and 6.7, 256 8.8 and 7.3; from
 // memory: 128 7.7 and 7.7, 256 12.1 and 10.1, 2048 70 and 55.6 (16 columns: 61), where a copy of the states takes 52.3.
 int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
+// Waves of a workgroup that take columns of runs: 2 as long as each of the 256 CUs then holds one workgroup at most, whose four
+// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 106 and
+// 135, 8 of up to 2000 74 and 92, 8 of 40 to 80 10.0 and 10.9, 16 of 1 to 2000 158 and 125, of 40 to 80 14 and 12.
+int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
 
 }  // namespace
 }  // namespace lsgdn
@@ -857,20 +877,26 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   hipStream_t s = (hipStream_t)stream;
   LSURGE_REQUIRE(sh < (1ll << 20), "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
   const bool b32 = t->beta_dtype == LSURGE_F32;
-  if (t->cu) {  // runs of any length, two workgroups a (sequence, head)
+  if (t->cu) {  // runs of any length
     const int64_t tail = std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17));
-    a.units = (int)(2 * sh);
-#define RUNS(DT, B32)                                                                                                   \
+    const int nw = takers(sh);
+    const int64_t group = 8 * (D / 16 / nw) * (t->hv / t->hk), grid = (sh * (D / 16 / nw) + group - 1) / group * group;
+    a.units = (int)grid;
+#define RUNS_NW(DT, B32, NW)                                                                                            \
   LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                                        \
-                hipLaunchKernelGGL((gdn_run_kernel<DT, B32>), dim3((unsigned)(a.units + tail)), dim3(RUN_THREADS), 0, s, a))
+                hipLaunchKernelGGL((gdn_run_kernel<DT, B32, NW>), dim3((unsigned)(grid + tail)), dim3(64 * (NW + 2)), 0, s, a))
+#define RUNS(DT, B32)                   \
+  if (nw == 2) { RUNS_NW(DT, B32, 2); } \
+  else { RUNS_NW(DT, B32, 4); }
     if (t->dtype == LSURGE_BF16) {
-      if (b32) { RUNS(LSURGE_BF16, true); }
-      else { RUNS(LSURGE_BF16, false); }
+      if (b32) { RUNS(LSURGE_BF16, true) }
+      else { RUNS(LSURGE_BF16, false) }
     } else {
-      if (b32) { RUNS(LSURGE_F16, true); }
-      else { RUNS(LSURGE_F16, false); }
+      if (b32) { RUNS(LSURGE_F16, true) }
+      else { RUNS(LSURGE_F16, false) }
     }
 #undef RUNS
+#undef RUNS_NW
     return LSURGE_OK;
   }
   const int cb = columns(sh);

@@ -120,6 +120,29 @@ def test_rule_long_runs(dt, norm, decay, dev):
     run_rule(dt, 1, 2, [63, 64, 65, 127, 128, 129, 1, 200, 333, 0, 32, 31, 33], dev, norm=norm, decay=decay, tail=5, seed=7)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("hk,hv", [(2, 8), (5, 5), (1, 13)])
+def test_rule_runs_of_many_heads(dt, hk, hv, dev):
+    """More (sequence, head) pairs than get two taking waves a workgroup."""
+    run_rule(dt, hk, hv, [1, 5, 0, 2, 31, 17, 0, 8, 3, 150, 4, 64, 33, 32], dev, beta32=hv == 8, tail=3, seed=hv)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_rule_has_the_same_bits_in_any_batch(dt, dev):
+    """One sequence alone, among few and among many."""
+    r = Rule(dt, 2, 4, [77], dev, seed=3, extra=2)
+    before = r.state.clone()
+    o, whole = r.call(), r.state.clone()
+    for n in (3, 40):
+        many = Rule(dt, 2, 4, [5] * n + [77, 1, 0, 200], dev, seed=n)
+        at = 5 * n
+        for t in "qkvg":
+            getattr(many, t)[at:at + 77] = getattr(r, t)
+        many.beta[at:at + 77] = r.beta
+        many.state[many.slots[n]] = before[r.slots[0]]
+        assert torch.equal(many.call()[at:at + 77], o) and torch.equal(many.state[many.slots[n]], whole[r.slots[0]])
+
+
 def test_rule_keys_without_a_norm(dev):
     """Keys twice as long as unit ones with beta near 1: a step's factor is larger than one, and the state grows."""
     r = Rule(BF16, 1, 2, [40, 9], dev, norm=False, unit=True, decay=0.5)
