@@ -9,8 +9,11 @@
 // so that one exchange between lanes serves both; the l2 norms of q and k are factors of these sums and cost no pass of their
 // own.  Everything is f32 but the inputs and o.
 //
-// Bound by memory for a token or a few (the state's 128 KiB a sequence and head), by the vector unit from about ten tokens on:
-// 4 x 128 x 128 multiply-adds a token and head, which have to follow each other.
+// Bound by memory for a token or a few (64 KiB of state a sequence and head, read and written): one token for 64 sequences of
+// 32 heads takes 42 us, 6.1 TB/s, with a part of the states in the caches, 55.6 us, 4.8 TB/s, with none (a copy reaches 5.1);
+// 100 runs of 1 to 8 tokens of 8 heads 28 us, 3.9 TB/s.  Longer runs go in chunks on the matrix cores and are a chain: 2000
+// tokens take 100 us, 1.6 us for 32 of them.  A chunk's products follow each other in one wave: its matrix instructions are 1250
+// of the 3600 cycles, its vector instructions 1650, the rest waits for the one before.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -228,8 +231,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
 // since differences of sums go into exponents.
 constexpr int C = 32;
-// us for 100 sequences of 8 heads, token by token and in a chunk: 2 tokens each 27.5 and 31.0, 3 30.5 and 31.0, 4 32.8 and 31.1,
-// 5 35.3 and 31.3, 7 41.6 and 31.4.
+// us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 31, 3 31 and 32 (f16: 31 and 30),
+// 4 33.8 and 32.2 (33.7 and 29.0), 5 36 and 32, 7 43 and 32; 4 sequences with 3 5.5 and 6.1, 4 6.1 and 6.1, 5 6.8 and 6.2.
 constexpr int CHUNKED = 4;
 constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
 constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
@@ -247,10 +250,10 @@ struct ChunkTiles {
 };
 struct ChunkTerms {
   // operands of products over 16 tokens, lane l's four values (row l % 16, columns 4 (l / 16) .. + 3) at [l]
-  u32x2 inv[2][3][64];  // the inverses of the diagonal blocks of I + A
+  u32x2 inv[2][3][64];  // the inverses of the diagonal blocks of I + A, by terms as `left` takes them
   u32x2 a10[3][64];     // -A, rows 16.., columns ..15
-  u32x2 m00[2][64];     // the weights of o
-  u32x2 m1[2][2][64];   // their rows 16.., columns by halves
+  u32x4 m00[64];        // the weights of o, both terms
+  u32x4 m1[2][64];      // their rows 16.., columns by halves
   // by token: R = beta v - c1 (S0^T k), o = c2 (S0^T q) + .., the factor of k in the state's update
   float beta[C], c1[C], c2[C], w[C];
   float decay;
@@ -276,7 +279,8 @@ __device__ __forceinline__ float minus(uint32_t x, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, one), c, false);
   }
 }
-// x as a sum of N terms of DT, four values each.  What a term leaves over is exact, and one instruction a value.
+// x as a sum of N terms of DT, four values each.  What a term leaves over is exact.  The dot product overwrites its c, and a
+// copy of x and it are no fewer instructions than a shift and a difference: bf16's first term takes these (2% of a long run).
 template <int DT, int N>
 __device__ __forceinline__ void split(f32x4 x, u32x2* t) {
 #pragma unroll
@@ -285,8 +289,13 @@ __device__ __forceinline__ void split(f32x4 x, u32x2* t) {
     if (n + 1 < N) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        x[2 * i] = minus<DT, false>(t[n][i], x[2 * i]);
-        x[2 * i + 1] = minus<DT, true>(t[n][i], x[2 * i + 1]);
+        if (DT == LSURGE_BF16 && n == 0) {
+          x[2 * i] -= __uint_as_float(t[n][i] << 16);
+          x[2 * i + 1] -= __uint_as_float(t[n][i] & 0xffff0000u);
+        } else {
+          x[2 * i] = minus<DT, false>(t[n][i], x[2 * i]);
+          x[2 * i + 1] = minus<DT, true>(t[n][i], x[2 * i + 1]);
+        }
       }
     }
   }
@@ -299,17 +308,30 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 __device__ __forceinline__ u32x4 join(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
-// P0 Q0 + P1 Q1 of 16 x 16 operands (lane l: row / column l % 16 at 4 (l / 16) .. + 3), added to c
-__device__ __forceinline__ f32x4 mma_pair(u32x2 p0, u32x2 q0, u32x2 p1, u32x2 q1, f32x4 c) {
-  return mma_32<LSURGE_BF16>(join(p0, p1), join(q0, q1), c);
+// 16 x 16 operands (lane l: row / column l % 16 at 4 (l / 16) .. + 3), whose terms are taken two at a time.  They lie so that
+// every pair is a range of registers: 1, 0, 2 of a left one, 2, 0, 1, 0 of a right one.
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ u32x8 left(const u32x2 (*t)[64], int lane) {
+  const u32x2 a = t[0][lane], b = t[1][lane], c = t[2][lane];
+  return u32x8{a[0], a[1], b[0], b[1], c[0], c[1], 0u, 0u};
 }
-// c + P Q of such operands of three terms: the six products of 2^-24 and more
-__device__ __forceinline__ f32x4 mma_f32(const u32x2* p, const u32x2* q, f32x4 c) {
-  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-  f32x4 less = mma_pair(p[2], q[0], p[0], q[2], zero);
-  c = mma_pair(p[1], q[1], p[0], q[0], c);
-  less = mma_pair(p[1], q[0], p[0], q[1], less);
+__device__ __forceinline__ u32x8 right(f32x4 x) {
+  u32x2 t[3];
+  split<3>(x, t);
+  return u32x8{t[2][0], t[2][1], t[0][0], t[0][1], t[1][0], t[1][1], t[0][0], t[0][1]};
+}
+template <int AT>
+__device__ __forceinline__ u32x4 pair(u32x8 x) { return __builtin_shufflevector(x, x, AT, AT + 1, AT + 2, AT + 3); }
+// c + P Q: the six products of 2^-24 and more
+__device__ __forceinline__ f32x4 mma_f32(u32x8 p, u32x8 q, f32x4 c) {
+  f32x4 less = mma_32<LSURGE_BF16>(pair<2>(p), pair<0>(q), f32x4{0.f, 0.f, 0.f, 0.f});
+  c = mma_32<LSURGE_BF16>(pair<0>(p), pair<4>(q), c);
+  less = mma_32<LSURGE_BF16>(pair<0>(p), pair<2>(q), less);
   return c + less;
+}
+// c + P Q of two terms each, p's as 0, 1
+__device__ __forceinline__ f32x4 mma_2(u32x4 p, u32x8 q, f32x4 c) {
+  return mma_32<LSURGE_BF16>(p, pair<2>(q), mma_32<LSURGE_BF16>(p, pair<4>(q), c));
 }
 
 // Two waves form a chunk's terms from its tiles.
@@ -442,7 +464,7 @@ __device__ __forceinline__ void prepare_inverse(const ChunkTiles& x, float decay
     for (int r = 0; r < 4; ++r) z[r] = g & 1 ? y[8 + 4 * h + r] : y[4 * h + r];
     split<3>(z, terms);
 #pragma unroll
-    for (int n = 0; n < 3; ++n) out.inv[blk][n][c + 16 * (2 * (g & 1) + h)] = terms[n];
+    for (int n = 0; n < 3; ++n) out.inv[blk][n < 2 ? 1 - n : 2][c + 16 * (2 * (g & 1) + h)] = terms[n];
   }
 }
 
@@ -498,12 +520,11 @@ __device__ __forceinline__ void prepare_rest(const ChunkTiles& x, float decay, f
     for (int r = 0; r < 4; ++r) m[r] = j0 + r <= i ? f * (e[r] * kq[b][r]) : 0.f;
     u32x2 terms[3];
     split<2>(m, terms);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) (b == 0 ? out.m00[n] : out.m1[n][b == 1])[lane] = terms[n];
+    (b == 0 ? out.m00 : out.m1[b == 1])[lane] = join(terms[0], terms[1]);
     if (b == 2) {
       split<3>(-s.beta[i] * s.rk[i] * (e * kk[2]), terms);
 #pragma unroll
-      for (int n = 0; n < 3; ++n) out.a10[n][lane] = terms[n];
+      for (int n = 0; n < 3; ++n) out.a10[n < 2 ? 1 - n : 2][lane] = terms[n];
     }
   }
 }
@@ -557,12 +578,8 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
   __shared__ float blocks[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
-  // Workgroups go to the 8 XCDs in turn: all that read one key head's rows to one of them, for its L2 (1 to 3%).
-  const uint32_t group = PARTS * (a.hv / a.hk), in = blockIdx.x % (8 * group);
-  const uint32_t id = (blockIdx.x - in) + in % 8 * group + in / 8;
-  if ((int)id >= a.nseq * a.hv * PARTS) return;
-  const Unit u = unit_of(a, id / PARTS);
-  const int col0 = (id % PARTS * NW + wave) * 16;
+  const Unit u = unit_of(a, blockIdx.x / PARTS);
+  const int col0 = (blockIdx.x % PARTS * NW + wave) * 16;
   const int total = u.end - u.begin;
   if (total <= 0) return;
   if (total < CHUNKED || (unsigned)u.slot >= (unsigned)a.num_slots) {
@@ -700,7 +717,8 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) P[i] = O[i] = zero;
-    u32x2 inv0[3], inv1[3], a10[3], m00[2], m1[2][2];
+    u32x8 inv0, inv1, a10;
+    u32x4 m00, m1[2];
     f32x4 beta[2], c1[2], c2[2], w[2];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -713,10 +731,8 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
           const int t = 16 * i + 4 * g;
           beta[i] = *reinterpret_cast<const f32x4*>(&x.beta[t]), c1[i] = *reinterpret_cast<const f32x4*>(&x.c1[t]);
         }
-#pragma unroll
-        for (int j = 0; j < 3; ++j) inv0[j] = x.inv[0][j][lane], a10[j] = x.a10[j][lane], inv1[j] = x.inv[1][j][lane];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) m00[j] = x.m00[j][lane], m1[j][0] = x.m1[j][0][lane], m1[j][1] = x.m1[j][1][lane];
+        inv0 = left(x.inv[0], lane), a10 = left(x.a10, lane), inv1 = left(x.inv[1], lane);
+        m00 = x.m00[lane], m1[0] = x.m1[0][lane], m1[1] = x.m1[1][lane];
       }
       const u32x2(*now)[NT] = s[st & 1];
 #pragma unroll
@@ -746,23 +762,18 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
     }
     const float decay = x.decay;
     load_v();
-    u32x2 r0[3], x0[3], r1[3], x1[3];
-    split<3>(R[0], r0);
-    X[0] = mma_f32(inv0, r0, zero);
+    X[0] = mma_f32(inv0, right(R[0]), zero);
 #pragma unroll
     for (int m = 0; m < 4; ++m) S[m] *= decay;  // beside the chain of products
-    split<3>(X[0], x0);
-    X[1] = mma_f32(a10, x0, R[1]);
+    const u32x8 x0 = right(X[0]);
+    X[1] = mma_f32(inv1, right(mma_f32(a10, x0, R[1])), zero);
 #pragma unroll
     for (int m = 4; m < 8; ++m) S[m] *= decay;
-    split<3>(X[1], r1);
-    X[1] = mma_f32(inv1, r1, zero);
     // o's products of two terms, 2^-16 of them
 #pragma unroll
     for (int i = 0; i < 2; ++i) O[i] *= c2[i] * unscale;
-    O[0] = mma_pair(m00[0], x0[1], m00[1], x0[0], O[0]);
-    O[0] = mma_pair(m00[0], x0[0], u32x2{0u, 0u}, x0[0], O[0]);
-    O[1] = mma_pair(m1[0][0], x0[0], m1[1][0], x0[0], O[1]);
+    O[0] = mma_2(m00, x0, O[0]);
+    O[1] = mma_2(m1[0], x0, O[1]);
     // the state's update
     f32x4 E[2] = {X[0] * w[0], X[1] * w[1]};
     if constexpr (DT == LSURGE_F16) {  // the decayed state's size, or what is added to it
@@ -787,7 +798,6 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
     u32x2 e0[NT], e1[NT];
     split<DT, NT>(E[0], e0);
     split<DT, NT>(E[1], e1);
-    split<2>(X[1], x1);
 #pragma unroll
     for (int m = 0; m < 8; m += 2)  // two tiles in turn: a product waits for the one before it
 #pragma unroll
@@ -796,8 +806,7 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
         S[m + 1] = mma_32<DT>(kt[m + 1], join(e0[j], e1[j]), S[m + 1]);
       }
     if constexpr (DT == LSURGE_BF16) split<DT, NT>(S[0], s[0][0]), split<DT, NT>(S[1], s[0][1]);
-    O[1] = mma_pair(m1[0][0], x0[1], m1[0][1], x1[1], O[1]);
-    O[1] = mma_pair(m1[0][1], x1[0], m1[1][1], x1[0], O[1]);
+    O[1] = mma_2(m1[1], right(X[1]), O[1]);
     const auto ob = os.next();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -807,10 +816,11 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
     }
   }
   asm volatile("" : "+v"(sp));  // its 32 addresses are formed again, not kept in 64 registers through the loop
+  auto* to = (__attribute__((address_space(1))) float*)sp;
 #pragma unroll
   for (int m = 0; m < 8; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sp[(16 * m + r) * D] = S[m][r] * unscale;
+    for (int r = 0; r < 4; ++r) to[(16 * m + r) * D] = S[m][r] * unscale;
 }
 
 int check_tokens(const lsurge_gdn_tokens* t) {
@@ -858,8 +868,8 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
 // memory: 128 7.7 and 7.7, 256 12.1 and 10.1, 2048 70 and 55.6 (16 columns: 61), where a copy of the states takes 52.3.
 int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 // Waves of a workgroup that take columns of runs: 2 as long as each of the 256 CUs then holds one workgroup at most, whose four
-// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 106 and
-// 135, 8 of up to 2000 74 and 92, 8 of 40 to 80 10.0 and 10.9, 16 of 1 to 2000 158 and 125, of 40 to 80 14 and 12.
+// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 100 and
+// 128, 8 of up to 2000 70 and 88, 8 of 40 to 80 9.7 and 11.0, 16 of up to 2000 143 and 121, of 40 to 80 13.8 and 11.8.
 int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
 
 }  // namespace
@@ -880,11 +890,10 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   if (t->cu) {  // runs of any length
     const int64_t tail = std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17));
     const int nw = takers(sh);
-    const int64_t group = 8 * (D / 16 / nw) * (t->hv / t->hk), grid = (sh * (D / 16 / nw) + group - 1) / group * group;
-    a.units = (int)grid;
+    a.units = (int)(sh * (D / 16 / nw));
 #define RUNS_NW(DT, B32, NW)                                                                                            \
   LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                                        \
-                hipLaunchKernelGGL((gdn_run_kernel<DT, B32, NW>), dim3((unsigned)(grid + tail)), dim3(64 * (NW + 2)), 0, s, a))
+                hipLaunchKernelGGL((gdn_run_kernel<DT, B32, NW>), dim3((unsigned)(a.units + tail)), dim3(64 * (NW + 2)), 0, s, a))
 #define RUNS(DT, B32)                   \
   if (nw == 2) { RUNS_NW(DT, B32, 2); } \
   else { RUNS_NW(DT, B32, 4); }
