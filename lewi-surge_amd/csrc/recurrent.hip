@@ -218,8 +218,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 //   (I + A) X = R,  R_i = beta_i (v_i - e^{G_i} S0^T k_i),  A_ij = beta_i e^{G_i - G_j} k_i.k_j (j < i),
 //   o_i = (e^{G_i} S0^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i.k_j) x_j) / sqrt(128),
 //   S = e^{G_C} S0 + sum_j e^{G_C - G_j} k_j x_j^T
-// (row i of X is the token's d).  A and the weights of o do not depend on the state: two waves form them for the next chunk
-// while two or four waves of 16 columns each take this one, with one barrier a chunk.
+// (row i of X is the token's d).  A and the weights of o do not depend on the state: a pair of waves forms them a chunk
+// ahead, or two pairs in turn two chunks ahead, while two or four waves of 16 columns each take this one; one barrier a chunk.
 //
 // Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
 // terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
@@ -334,7 +334,7 @@ __device__ __forceinline__ f32x4 mma_2(u32x4 p, u32x8 q, f32x4 c) {
   return mma_32<LSURGE_BF16>(p, pair<2>(q), mma_32<LSURGE_BF16>(p, pair<4>(q), c));
 }
 
-// Two waves form a chunk's terms from its tiles.
+// A pair of waves forms a chunk's terms from its tiles.
 struct Scratch {
   double G[C];  // sums of the log2 decays
   float rk[C], rq[C], beta[C];
@@ -410,9 +410,10 @@ __device__ __forceinline__ void subtract_rows(float* y, const float* A, std::int
 }
 
 // The inverses of A's diagonal blocks; the log decay and beta are those of token lane % 32 (0 behind the end).
-template <int DT>
+// half: called half way.
+template <int DT, class F>
 __device__ __forceinline__ void prepare_inverse(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, Scratch& s,
-                                                float (*blocks)[16][20], ChunkTerms& out) {
+                                                float (*blocks)[16][20], ChunkTerms& out, F half) {
   asm volatile("" : "+v"(lane));  // LDS addresses are formed again in every chunk, not kept in registers that spill
   const int c = lane & 15, g = lane >> 4, t = lane & 31;
   u32x4 k[2][4];
@@ -444,6 +445,7 @@ __device__ __forceinline__ void prepare_inverse(const ChunkTiles& x, float decay
     *reinterpret_cast<f32x4*>(&blocks[b][c][4 * g]) = A;
   }
   wave_sync();
+  half();
   // Row c of a block's inverse, y (I + A) = e_c, from its last value on; lanes below 32 the first block, the others the second.
   // Lane k of a row of 16 holds row k of -A, which the others read from its register as they go: 120 multiply-adds, no LDS.
   const int blk = lane >> 5;
@@ -469,9 +471,9 @@ __device__ __forceinline__ void prepare_inverse(const ChunkTiles& x, float decay
 }
 
 // Everything else: A's block (1, 0), the weights of o, the factors by token.
-template <int DT>
+template <int DT, class F>
 __device__ __forceinline__ void prepare_rest(const ChunkTiles& x, float decay, float beta, float l2_eps, int lane, Scratch& s,
-                                             ChunkTerms& out) {
+                                             ChunkTerms& out, F half) {
   asm volatile("" : "+v"(lane));
   const int c = lane & 15, g = lane >> 4, t = lane & 31;
   double last;
@@ -502,6 +504,7 @@ __device__ __forceinline__ void prepare_rest(const ChunkTiles& x, float decay, f
     }
   }
   wave_sync();
+  half();
   if (lane < C) {
     const float rk = s.rk[t], e = __builtin_amdgcn_exp2f((float)G);
     out.beta[t] = beta;
@@ -567,15 +570,16 @@ __device__ __forceinline__ void rescale(float& most, f32x4* S, float& scale, flo
   most *= up, scale *= up, unscale *= down;
 }
 
-// NW waves take columns, two prepare.
-template <int DT, bool BETA32, int NW>
-__global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel(TokenArgs a) {
+// NW waves take columns, PAIRS pairs of waves prepare: one pair during the chunk before, two in turn during two.
+template <int DT, bool BETA32, int NW, int PAIRS>
+__global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 2) void gdn_run_kernel(TokenArgs a) {
   constexpr int PARTS = D / (16 * NW);  // workgroups a (sequence, head)
+  constexpr int RING = PAIRS + 2;
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
-  __shared__ ChunkTiles tiles[3];
+  __shared__ ChunkTiles tiles[RING];
   __shared__ ChunkTerms terms[2];
-  __shared__ Scratch scratch[2];
-  __shared__ float blocks[2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
+  __shared__ Scratch scratch[2 * PAIRS];
+  __shared__ float blocks[PAIRS][2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
   const Unit u = unit_of(a, blockIdx.x / PARTS);
@@ -610,9 +614,11 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
     }
   };
 
-  // While the others take chunk n - 1, two waves prepare chunk n from its tiles; chunk n + 1 is staged.
+  // Between barriers n and n + 1 the takers take chunk n - PAIRS, the pair of chunk n begins to prepare it, and chunk n + 1 is
+  // staged; a chunk is prepared PAIRS barriers after its begin.
   if (wave >= NW) {
     constexpr bool stages = NW == 2;  // two of the first four waves
+    const int mine = __builtin_amdgcn_readfirstlane(wave) - NW, pair = mine >> 1;  // scalar: barriers depend on them
     const int g_off = (lane & 31) * (int)a.g_row * 4, b_size = BETA32 ? 4 : 2, b_off = (lane & 31) * (int)a.beta_row * b_size;
     ChunkRows gs(u, a.g + u.h, a.g_row, 1, 4), bs(u, (const char*)a.beta + u.h * b_size, a.beta_row, 1, b_size);
     auto load = [&](float& decay, float& beta) {
@@ -625,28 +631,41 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
         beta = DT == LSURGE_F16 ? f16_to_f32(x) : bf16_to_f32(x);
       }
     };
+    auto skip = [&]() {
+      gs.next();
+      bs.next();
+    };
     float decay, beta, decay1, beta1;
     if (stages) load_tiles();
+    if (pair) skip();
     load(decay, beta);
     if (stages) store_tiles(tiles[0]), load_tiles();
     stage_barrier();  // the first chunk is staged
-    int ring = 0;  // n % 3
-    for (int n = 0; n < chunks; ++n) {
+    if (pair) stage_barrier();
+    int barriers = 1 + pair;
+    for (int n = pair, ring = pair; n < chunks; n += PAIRS) {
       const ChunkTiles& tile = tiles[ring];
-      ring = ring == 2 ? 0 : ring + 1;
+      ring = ring + PAIRS < RING ? ring + PAIRS : ring + PAIRS - RING;  // n % RING
       if (stages) {
         asm volatile("" : "+v"(k_off), "+v"(q_off));
         store_tiles(tiles[ring]);
         load_tiles();
       }
+      if (PAIRS == 2) skip();
       load(decay1, beta1);
-      if (wave == NW) prepare_inverse<DT>(tile, decay, beta, a.l2_eps, lane, scratch[0], blocks, terms[n & 1]);
-      else prepare_rest<DT>(tile, decay, beta, a.l2_eps, lane, scratch[1], terms[n & 1]);
+      auto half = [&]() {
+        if (PAIRS == 2) stage_barrier();
+      };
+      if (mine & 1) prepare_rest<DT>(tile, decay, beta, a.l2_eps, lane, scratch[mine], terms[n & 1], half);
+      else prepare_inverse<DT>(tile, decay, beta, a.l2_eps, lane, scratch[mine], blocks[pair], terms[n & 1], half);
       decay = decay1, beta = beta1;
       stage_barrier();  // chunk n is prepared
+      barriers += PAIRS;
     }
+    for (; barriers < chunks + PAIRS; ++barriers) stage_barrier();  // as many as the takers'
     return;
   }
+  static_assert(NW == 4 || PAIRS == 1, "a preparing wave that stages does so once a barrier");
 
   // the columns col0 .. + 15 of the state: tile m, register r: row 16 m + 4 g + r, column c
   float* sp = a.state + u.slot * a.slot_stride + (int64_t)u.h * D * D + 4 * g * D + col0 + c;
@@ -673,14 +692,19 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
   stage_barrier();  // the first chunk is staged
   store_tiles(tiles[1]);
   load_tiles();
+  if (PAIRS == 2) {
+    stage_barrier();
+    store_tiles(tiles[2]);
+    load_tiles();
+  }
   __builtin_amdgcn_sched_barrier(0);  // in the loop's order, or its first wait is for all of them in every turn
   load_v();
   u32x2 s[2][2][NT];  // two tiles of the state by terms, and the next two
   if constexpr (DT == LSURGE_BF16) split<DT, NT>(S[0], s[0][0]), split<DT, NT>(S[1], s[0][1]);
 
-  int ring = 0;  // n % 3
+  int ring = 0;  // n % RING
   for (int n = 0; n < chunks; ++n) {
-    stage_barrier();  // chunk n is prepared, chunk n + 1 staged, chunk n - 1 no longer read
+    stage_barrier();  // chunk n is prepared, chunk n + PAIRS staged, chunk n - 1 no longer read
     const ChunkTiles& tile = tiles[ring];
     const ChunkTerms& x = terms[n & 1];
     // the addresses' multiples of the rows are added again in every chunk: kept, they spill, and a spill's reload waits for
@@ -698,9 +722,9 @@ __global__ __launch_bounds__(64 * (NW + 2), NW == 4 ? 3 : 2) void gdn_run_kernel
       }
     };
     frags(0);
-    store_tiles(tiles[ring == 0 ? 2 : ring - 1]);  // of chunk n + 2, zeros behind the last
+    store_tiles(tiles[ring == 0 ? RING - 1 : ring - 1]);  // of chunk n + RING - 1, zeros behind the last
     load_tiles();
-    ring = ring == 2 ? 0 : ring + 1;
+    ring = ring == RING - 1 ? 0 : ring + 1;
     float most = 0.f;  // f16: the largest of the column's values
     if constexpr (DT == LSURGE_F16) {
 #pragma unroll
@@ -871,6 +895,13 @@ int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 // waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 100 and
 // 128, 8 of up to 2000 70 and 88, 8 of 40 to 80 9.7 and 11.0, 16 of up to 2000 143 and 121, of 40 to 80 13.8 and 11.8.
 int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
+// Pairs of waves that prepare beside four takers: two share the work of a chunk out to all SIMDs, for a longer start, and leave
+// one workgroup a CU where else there may be two.  So it takes long sequences, on average, which is all the host knows.  us for
+// one pair and two: 12 sequences of 8 heads of 32 tokens 7.2 and 7.4, of 128 14.2 and 13.5, of 1000 73 and 65; 32 of 32 12.3 and
+// 13.9, of 256 46.7 and 48.7, of 512 80 and 78, of 1000 148 and 135, of up to 2000 192 and 175.
+int preparing_pairs(int64_t seq_heads, int64_t rows, int64_t nseq) {
+  return rows >= nseq * (seq_heads <= 128 ? 64 : 300) ? 2 : 1;
+}
 
 }  // namespace
 }  // namespace lsgdn
@@ -889,14 +920,16 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   const bool b32 = t->beta_dtype == LSURGE_F32;
   if (t->cu) {  // runs of any length
     const int64_t tail = std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17));
-    const int nw = takers(sh);
+    const int nw = takers(sh), pairs = preparing_pairs(sh, t->rows, t->nseq);
     a.units = (int)(sh * (D / 16 / nw));
-#define RUNS_NW(DT, B32, NW)                                                                                            \
-  LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                                        \
-                hipLaunchKernelGGL((gdn_run_kernel<DT, B32, NW>), dim3((unsigned)(a.units + tail)), dim3(64 * (NW + 2)), 0, s, a))
-#define RUNS(DT, B32)                   \
-  if (nw == 2) { RUNS_NW(DT, B32, 2); } \
-  else { RUNS_NW(DT, B32, 4); }
+#define RUNS_AS(DT, B32, NW, PAIRS)                                                                      \
+  LSURGE_LAUNCH(KID_GDN_SCAN, s,                                                                         \
+                hipLaunchKernelGGL((gdn_run_kernel<DT, B32, NW, PAIRS>), dim3((unsigned)(a.units + tail)), \
+                                   dim3(64 * (NW + 2 * PAIRS)), 0, s, a))
+#define RUNS(DT, B32)                             \
+  if (nw == 2) { RUNS_AS(DT, B32, 2, 1); }        \
+  else if (pairs == 2) { RUNS_AS(DT, B32, 4, 2); } \
+  else { RUNS_AS(DT, B32, 4, 1); }
     if (t->dtype == LSURGE_BF16) {
       if (b32) { RUNS(LSURGE_BF16, true) }
       else { RUNS(LSURGE_BF16, false) }
@@ -905,7 +938,7 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
       else { RUNS(LSURGE_F16, false) }
     }
 #undef RUNS
-#undef RUNS_NW
+#undef RUNS_AS
     return LSURGE_OK;
   }
   const int cb = columns(sh);

@@ -128,14 +128,22 @@ def test_rule_runs_of_many_heads(dt, hk, hv, dev):
 
 
 @pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("hv,lens", [(6, [63, 64, 65, 127, 128, 129, 1, 200, 333, 0, 32, 31, 33]), (7, [1000, 2, 96, 4, 0, 160, 161, 3, 7, 5]),
+                                     (32, [700, 1, 40, 500, 290])])
+def test_rule_long_runs_of_many_heads(dt, hv, lens, dev):
+    """So long on average that two pairs of waves prepare: odd and even numbers of chunks, and sequences of one."""
+    run_rule(dt, 1, hv, lens, dev, beta32=hv == 7, seed=hv, tail=2)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
 def test_rule_has_the_same_bits_in_any_batch(dt, dev):
     """One sequence alone, among few and among many."""
     r = Rule(dt, 2, 4, [77], dev, seed=3, extra=2)
     before = r.state.clone()
     o, whole = r.call(), r.state.clone()
-    for n in (3, 40):
-        many = Rule(dt, 2, 4, [5] * n + [77, 1, 0, 200], dev, seed=n)
-        at = 5 * n
+    for n, size in ((3, 5), (40, 5), (20, 100)):
+        many = Rule(dt, 2, 4, [size] * n + [77, 1, 0, 200], dev, seed=n)
+        at = size * n
         for t in "qkvg":
             getattr(many, t)[at:at + 77] = getattr(r, t)
         many.beta[at:at + 77] = r.beta
