@@ -234,7 +234,6 @@ constexpr int C = 32;
 // us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 31, 3 31 and 32 (f16: 31 and 30),
 // 4 33.8 and 32.2 (33.7 and 29.0), 5 36 and 32, 7 43 and 32; 4 sequences with 3 5.5 and 6.1, 4 6.1 and 6.1, 5 6.8 and 6.2.
 constexpr int CHUNKED = 4;
-constexpr int PITCH = D + 8;  // of a tile's row in LDS: rows start 16 bytes apart in the banks
 constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
 constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
 
@@ -245,6 +244,9 @@ __device__ __forceinline__ void stage_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// A row's 16 bytes 4 b + g hold the values 32 b + 4 g .. + 3 and 32 b + 16 + 4 g .. + 3, as the products with the state take them.
+// Rows 32 bytes apart in the banks: reads of a row's 16 bytes by 16 rows, which is most of them, meet no bank twice.
+constexpr int PITCH = D + 16;
 struct ChunkTiles {
   uint16_t k[C][PITCH], q[C][PITCH];
 };
@@ -595,6 +597,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
 
   // The first four waves stage: a thread's part of the tiles is two pieces of 8 values of k and of q.
   const int kh = u.h / (a.hv / a.hk), srow = threadIdx.x >> 4, scol = (threadIdx.x & 15) * 8;
+  const int place = scol / 32 * 32 + scol % 16 * 2 + scol % 32 / 16 * 4;  // its first four values' place, its others' 8 further
   int k_off = (srow * (int)a.k_row + scol) * 2, q_off = (srow * (int)a.q_row + scol) * 2;
   u32x4 kr[2], qr[2];
   ChunkRows ks(u, a.k + kh * a.k_head, a.k_row, D, 2), qs(u, a.q + kh * a.q_head, a.q_row, D, 2);
@@ -609,8 +612,10 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
   auto store_tiles = [&](ChunkTiles& x) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      *reinterpret_cast<u32x4*>(&x.k[srow + 16 * i][scol]) = kr[i];
-      *reinterpret_cast<u32x4*>(&x.q[srow + 16 * i][scol]) = qr[i];
+      *reinterpret_cast<u32x2*>(&x.k[srow + 16 * i][place]) = u32x2{kr[i][0], kr[i][1]};
+      *reinterpret_cast<u32x2*>(&x.k[srow + 16 * i][place + 8]) = u32x2{kr[i][2], kr[i][3]};
+      *reinterpret_cast<u32x2*>(&x.q[srow + 16 * i][place]) = u32x2{qr[i][0], qr[i][1]};
+      *reinterpret_cast<u32x2*>(&x.q[srow + 16 * i][place + 8]) = u32x2{qr[i][2], qr[i][3]};
     }
   };
 
@@ -716,9 +721,8 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     auto frags = [&](int st) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint16_t *k = &tile.k[16 * i + c][32 * st + 4 * g], *q = &tile.q[16 * i + c][32 * st + 4 * g];
-        kf[st & 1][i] = join(*reinterpret_cast<const u32x2*>(k), *reinterpret_cast<const u32x2*>(k + 16));
-        qf[st & 1][i] = join(*reinterpret_cast<const u32x2*>(q), *reinterpret_cast<const u32x2*>(q + 16));
+        kf[st & 1][i] = token_frag(tile.k, i, st, lane);
+        qf[st & 1][i] = token_frag(tile.q, i, st, lane);
       }
     };
     frags(0);
@@ -814,7 +818,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     u32x4 kt[8];  // k's values 16 m + c of the tokens 4 g .. + 3 and 16 + 4 g .. + 3
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      const uint16_t* p = &tile.k[4 * g + (c >> 2)][16 * m + 4 * (c & 3)];
+      const uint16_t* p = &tile.k[4 * g + (c >> 2)][32 * (m >> 1) + 8 * (c & 3) + 4 * (m & 1)];
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p + 16 * PITCH));
       kt[m] = join(__builtin_bit_cast(u32x2, lo), __builtin_bit_cast(u32x2, hi));
