@@ -231,8 +231,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
 // since differences of sums go into exponents.
 constexpr int C = 32;
-// us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 31, 3 31 and 32 (f16: 31 and 30),
-// 4 33.8 and 32.2 (33.7 and 29.0), 5 36 and 32, 7 43 and 32; 4 sequences with 3 5.5 and 6.1, 4 6.1 and 6.1, 5 6.8 and 6.2.
+// us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 33, 3 30.5 and 32 (f16: 30.5 and 30),
+// 4 32.8 and 32.1 (32.8 and 29.7), 5 36 and 32, 7 42 and 32; 4 sequences with 3 5.4 and 6.0, 4 6.0 and 6.0, 5 6.7 and 6.0.
 constexpr int CHUNKED = 4;
 constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
 constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
@@ -897,12 +897,12 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
 int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 // Waves of a workgroup that take columns of runs: 2 as long as each of the 256 CUs then holds one workgroup at most, whose four
 // waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 100 and
-// 128, 8 of up to 2000 70 and 88, 8 of 40 to 80 9.7 and 11.0, 16 of up to 2000 143 and 121, of 40 to 80 13.8 and 11.8.
+// 112, 8 of up to 2000 69 and 76, 8 of 60 8.4 and 8.9, 16 of up to 2000 146 and 105, of 40 to 80 14.6 and 11.4.
 int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
 // Pairs of waves that prepare beside four takers: two share the work of a chunk out to all SIMDs, for a longer start, and leave
 // one workgroup a CU where else there may be two.  So it takes long sequences, on average, which is all the host knows.  us for
-// one pair and two: 12 sequences of 8 heads of 32 tokens 7.2 and 7.4, of 128 14.2 and 13.5, of 1000 73 and 65; 32 of 32 12.3 and
-// 13.9, of 256 46.7 and 48.7, of 512 80 and 78, of 1000 148 and 135, of up to 2000 192 and 175.
+// one pair and two: 12 sequences of 8 heads of 32 tokens 7.3 and 7.5, of 128 13.8 and 13.2, of 1000 69 and 62; 32 of 32 12.0 and
+// 13.8, of 256 48.2 and 48.5, of 512 78 and 77, of 1000 138 and 131, of up to 2000 187 and 168.
 int preparing_pairs(int64_t seq_heads, int64_t rows, int64_t nseq) {
   return rows >= nseq * (seq_heads <= 128 ? 64 : 300) ? 2 : 1;
 }
