@@ -920,7 +920,8 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   TokenArgs a = token_args(t);
   const int64_t sh = t->nseq * t->hv;
   hipStream_t s = (hipStream_t)stream;
-  LSURGE_REQUIRE(sh < (1ll << 20), "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
+  // a launch holds less than 2^32 threads: two workgroups of up to 512 a pair, and 256 for the rows behind
+  LSURGE_REQUIRE(sh <= (1ll << 22) - 256, "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
   const bool b32 = t->beta_dtype == LSURGE_F32;
   if (t->cu) {  // runs of any length
     const int64_t tail = std::min<int64_t>(256, 1 + t->rows * t->hv * D * 2 / (1 << 17));

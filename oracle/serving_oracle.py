@@ -1,7 +1,7 @@
 """CPU oracle of the operators that carry a hybrid model's sequences from token to token, in float64: the gated delta rule and
 the causal convolution from kept states, and the rotation of heads by their positions.
 
-TEST INFRASTRUCTURE ONLY: only `tests/` may import this module, as the checker.  No product code calls it.
+TEST INFRASTRUCTURE ONLY: only `tests/` may import this module.  No product code calls it.
 
 The rule and the convolution are those of modal/gdn_fast.py and modal/fast_conv.py token by token; carrying their state between
 calls and the rotation have no counterpart in the reference.  Each function also returns how far a float32 computation with one

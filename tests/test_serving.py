@@ -297,6 +297,7 @@ def _tokens(**kw):
     (dict(o=0), b"null pointer"), (dict(state=0), b"null pointer"), (dict(state=264), b"misaligned"),
     (dict(slot_stride=32770), b"strides"), (dict(slot_stride=32764), b"strides"),
     (dict(num_slots=-1), b"slots"), (dict(rows=1 << 30, nseq=1 << 30), b"rows of"),
+    (dict(rows=1 << 21, nseq=1 << 21), b"sequences of 2 heads"),
 ])
 def test_recurrent_abi_refusals(kw, msg):
     lib, t = L.lib(), _tokens(**kw)

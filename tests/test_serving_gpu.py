@@ -443,6 +443,21 @@ def test_conv_thousands_of_sequences(dev):
     run_conv(BF16, 4, 16, [0] * 5000 + [7] + [0] * 5000, dev)
 
 
+def test_conv_far_rows(dev):
+    """Inputs and outputs of more than 2^31 values: the last rows against a call of their own after the rows before them."""
+    rows, C = 270000, 8192
+    x = torch.zeros((rows, C), dtype=BF16, device=dev)
+    gen = torch.Generator().manual_seed(21)
+    x[-40:] = _randn(gen, (40, C), BF16, dev)
+    w = _randn(gen, (4, C), BF16, dev)
+    state = FC.alloc_conv_state(2, 4, C, BF16, dev)
+    y = FC.causal_conv1d_update(x, w, state, cu_seqlens=_i32([0, 100000, rows], dev), activation="silu")
+    own = FC.alloc_conv_state(1, 4, C, BF16, dev)
+    want = FC.causal_conv1d_update(x[-40:], w, own, cu_seqlens=_i32([0, 40], dev), activation="silu")
+    assert torch.equal(y[-40:], want) and torch.equal(state[1], own[0])
+    assert not y[:-40].any() and not state[0].any()
+
+
 def test_conv_places_without_a_slot(dev):
     c = Conv(BF16, 4, 64, [1, 6, 2, 70, 0, 4], dev)
     before = c.state.clone()
@@ -760,6 +775,20 @@ def test_append_thousands_of_sequences(dev):
     rng = np.random.default_rng(3)
     new = [int(i) for i in rng.integers(0, 3, 4200)]
     check_append(BF16, 2, 1, 64, 64, 8, new, [n + int(i) for n, i in zip(new, rng.integers(0, 9, 4200))], dev, tail=2)
+
+
+def test_append_far_pages(dev):
+    """Caches of more than 2^31 values, pages at both ends."""
+    pages, D = 140000, 256
+    gen = torch.Generator().manual_seed(22)
+    kc, vc = (torch.zeros((pages, 64, 1, D), dtype=BF16, device=dev) for _ in range(2))
+    q, k, v = _randn(gen, (70, 2, D), BF16, dev), _randn(gen, (70, 1, D), BF16, dev), _randn(gen, (70, 1, D), BF16, dev)
+    table, f = _i32([[pages - 1, 0]], dev), A.rotary_inv_freq(64, 1e4, dev)
+    _, kt = A.rotary_append_kv(q, k, v, kc, vc, table, _i32([70], dev), f, cu_seqlens=_i32([0, 70], dev), return_k=True)
+    _within(kt, *so.rotate(_np(k), np.arange(70), _np(f), False, so.HALF_STEP["bf16"], so.TINY["bf16"]))
+    for c, t in ((kc, kt), (vc, v)):
+        assert torch.equal(c[pages - 1], t[:64]) and torch.equal(c[0, :6], t[64:])
+        assert not c[1:pages - 1].any() and not c[0, 6:].any()
 
 
 def test_append_no_sequence(dev):
