@@ -577,6 +577,9 @@ template <int DT, bool BETA32, int NW, int PAIRS>
 __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 2) void gdn_run_kernel(TokenArgs a) {
   constexpr int PARTS = D / (16 * NW);  // workgroups a (sequence, head)
   constexpr int RING = PAIRS + 2;
+  // The state's products with q go beside the chain that solves for X where registers are left to keep its terms until then
+  // (us before and with it: one sequence of 2000 tokens 98.6 and 97.4, 16 of up to 2000 105 and 102, 64 330 and 311).
+  constexpr bool LATE = NW == 2 || PAIRS == 2;
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
   __shared__ ChunkTiles tiles[RING];
   __shared__ ChunkTerms terms[2];
@@ -722,7 +725,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         kf[st & 1][i] = token_frag(tile.k, i, st, lane);
-        qf[st & 1][i] = token_frag(tile.q, i, st, lane);
+        if constexpr (!LATE) qf[st & 1][i] = token_frag(tile.q, i, st, lane);
       }
     };
     frags(0);
@@ -745,6 +748,17 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) P[i] = O[i] = zero;
+    u32x4 kept[4][2];  // LATE: the first two terms by step
+    auto late = [&](int st) {
+      if constexpr (LATE) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 f = token_frag(tile.q, i, st, lane);
+          O[i] = mma_32<DT>(f, kept[st][1], O[i]);
+          O[i] = mma_32<DT>(f, kept[st][0], O[i]);
+        }
+      }
+    };
     u32x8 inv0, inv1, a10;
     u32x4 m00, m1[2];
     f32x4 beta[2], c1[2], c2[2], w[2];
@@ -763,12 +777,13 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
         m00 = x.m00[lane], m1[0] = x.m1[0][lane], m1[1] = x.m1[1][lane];
       }
       const u32x2(*now)[NT] = s[st & 1];
+      if constexpr (LATE) kept[st][0] = join(now[0][0], now[1][0]), kept[st][1] = join(now[0][1], now[1][1]);
 #pragma unroll
       for (int j = NT - 1; j >= 0; --j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           P[i] = mma_32<DT>(kf[st & 1][i], join(now[0][j], now[1][j]), P[i]);
-          if (j < 2) O[i] = mma_32<DT>(qf[st & 1][i], join(now[0][j], now[1][j]), O[i]);
+          if (!LATE && j < 2) O[i] = mma_32<DT>(qf[st & 1][i], join(now[0][j], now[1][j]), O[i]);
         }
       if (st < 3) {
         split<DT, NT>(S[2 * st + 2], s[(st + 1) & 1][0]);
@@ -793,10 +808,14 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     X[0] = mma_f32(inv0, right(R[0]), zero);
 #pragma unroll
     for (int m = 0; m < 4; ++m) S[m] *= decay;  // beside the chain of products
+    late(0);
+    late(1);
     const u32x8 x0 = right(X[0]);
     X[1] = mma_f32(inv1, right(mma_f32(a10, x0, R[1])), zero);
 #pragma unroll
     for (int m = 4; m < 8; ++m) S[m] *= decay;
+    late(2);
+    late(3);
     // o's products of two terms, 2^-16 of them
 #pragma unroll
     for (int i = 0; i < 2; ++i) O[i] *= c2[i] * unscale;
