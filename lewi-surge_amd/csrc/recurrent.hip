@@ -12,8 +12,8 @@
 // Bound by memory for a token or a few (64 KiB of state a sequence and head, read and written): one token for 64 sequences of
 // 32 heads takes 42 us, 6.1 TB/s, with a part of the states in the caches, 55.6 us, 4.8 TB/s, with none (a copy reaches 5.1);
 // 100 runs of 1 to 8 tokens of 8 heads 28 us, 3.9 TB/s.  Longer runs go in chunks on the matrix cores and are a chain: 2000
-// tokens take 100 us, 1.6 us for 32 of them.  A chunk's products follow each other in one wave: its matrix instructions are 1250
-// of the 3600 cycles, its vector instructions 1650, the rest waits for the one before.
+// tokens take 98 us, 1.55 us for 32 of them.  A chunk's products follow each other in one wave: its matrix instructions are 1250
+// of the 3500 cycles, its vector instructions 1650, the rest waits for the one before.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -915,13 +915,13 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
 // memory: 128 7.7 and 7.7, 256 12.1 and 10.1, 2048 70 and 55.6 (16 columns: 61), where a copy of the states takes 52.3.
 int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 // Waves of a workgroup that take columns of runs: 2 as long as each of the 256 CUs then holds one workgroup at most, whose four
-// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 100 and
-// 112, 8 of up to 2000 69 and 76, 8 of 60 8.4 and 8.9, 16 of up to 2000 146 and 105, of 40 to 80 14.6 and 11.4.
+// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 98 and
+// 109, 8 of up to 2000 68 and 75, 8 of 60 8.5 and 9.0, 16 of up to 2000 142 and 103, of 40 to 80 14.4 and 11.4.
 int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
 // Pairs of waves that prepare beside four takers: two share the work of a chunk out to all SIMDs, for a longer start, and leave
 // one workgroup a CU where else there may be two.  So it takes long sequences, on average, which is all the host knows.  us for
-// one pair and two: 12 sequences of 8 heads of 32 tokens 7.3 and 7.5, of 128 13.8 and 13.2, of 1000 69 and 62; 32 of 32 12.0 and
-// 13.8, of 256 48.2 and 48.5, of 512 78 and 77, of 1000 138 and 131, of up to 2000 187 and 168.
+// one pair and two: 12 sequences of 8 heads of 32 tokens 7.4 and 7.5, of 128 13.7 and 13.1, of 1000 69 and 61; 32 of 32 12.2 and
+// 13.9, of 256 45.9 and 47.2, of 512 77 and 75.5, of 1000 139 and 130, of up to 2000 187 and 164.
 int preparing_pairs(int64_t seq_heads, int64_t rows, int64_t nseq) {
   return rows >= nseq * (seq_heads <= 128 ? 64 : 300) ? 2 : 1;
 }
