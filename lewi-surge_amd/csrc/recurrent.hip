@@ -225,8 +225,9 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
 // the state is kept times a power of two there, its largest value between 2^8 and 2^15: what is lost is below 2^-33 of it; the
 // power ends at 2^60, so a column below 2^-52, nothing beside f16 inputs, loses 2^-85).
-// The 16 x 16 matrices R, X, A and the inverse of A's diagonal blocks are three bf16 terms, and two where they reach o alone,
-// which is rounded to 11 bits or fewer.  A wave's 16 columns of every matrix lie in its lanes (lane l: column l % 16), so that
+// The 16 x 16 matrices R, X, A, the inverse of A's diagonal blocks and the weights of o are three bf16 terms: o is held to f32
+// before its own rounding too, since a token that reads what it erases is a small difference of large parts (with two terms for
+// o's parts 12 prompts took 103 us instead of 113).  A wave's 16 columns of every matrix lie in its lanes (lane l: column l % 16), so that
 // each product's result is in place as the next one's operand: the state, R and X never leave their lane.  (I + A) is solved by
 // blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
 // since differences of sums go into exponents.
@@ -254,8 +255,8 @@ struct ChunkTerms {
   // operands of products over 16 tokens, lane l's four values (row l % 16, columns 4 (l / 16) .. + 3) at [l]
   u32x2 inv[2][3][64];  // the inverses of the diagonal blocks of I + A, by terms as `left` takes them
   u32x2 a10[3][64];     // -A, rows 16.., columns ..15
-  u32x4 m00[64];        // the weights of o, both terms
-  u32x4 m1[2][64];      // their rows 16.., columns by halves
+  u32x2 m00[3][64];     // the weights of o
+  u32x2 m1[2][3][64];   // their rows 16.., columns by halves
   // by token: R = beta v - c1 (S0^T k), o = c2 (S0^T q) + .., the factor of k in the state's update
   float beta[C], c1[C], c2[C], w[C];
   float decay;
@@ -331,9 +332,11 @@ __device__ __forceinline__ f32x4 mma_f32(u32x8 p, u32x8 q, f32x4 c) {
   less = mma_32<LSURGE_BF16>(pair<0>(p), pair<2>(q), less);
   return c + less;
 }
-// c + P Q of two terms each, p's as 0, 1
-__device__ __forceinline__ f32x4 mma_2(u32x4 p, u32x8 q, f32x4 c) {
-  return mma_32<LSURGE_BF16>(p, pair<2>(q), mma_32<LSURGE_BF16>(p, pair<4>(q), c));
+// the same six, one after the other
+__device__ __forceinline__ f32x4 mma_f32_on(u32x8 p, u32x8 q, f32x4 c) {
+  c = mma_32<LSURGE_BF16>(pair<2>(p), pair<0>(q), c);
+  c = mma_32<LSURGE_BF16>(pair<0>(p), pair<2>(q), c);
+  return mma_32<LSURGE_BF16>(pair<0>(p), pair<4>(q), c);
 }
 
 // A pair of waves forms a chunk's terms from its tiles.
@@ -524,8 +527,9 @@ __device__ __forceinline__ void prepare_rest(const ChunkTiles& x, float decay, f
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = j0 + r <= i ? f * (e[r] * kq[b][r]) : 0.f;
     u32x2 terms[3];
-    split<2>(m, terms);
-    (b == 0 ? out.m00 : out.m1[b == 1])[lane] = join(terms[0], terms[1]);
+    split<3>(m, terms);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) (b == 0 ? out.m00 : out.m1[b == 1])[n < 2 ? 1 - n : 2][lane] = terms[n];
     if (b == 2) {
       split<3>(-s.beta[i] * s.rk[i] * (e * kk[2]), terms);
 #pragma unroll
@@ -577,9 +581,6 @@ template <int DT, bool BETA32, int NW, int PAIRS>
 __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 2) void gdn_run_kernel(TokenArgs a) {
   constexpr int PARTS = D / (16 * NW);  // workgroups a (sequence, head)
   constexpr int RING = PAIRS + 2;
-  // The state's products with q go beside the chain that solves for X where registers are left to keep its terms until then
-  // (us before and with it: one sequence of 2000 tokens 98.6 and 97.4, 16 of up to 2000 105 and 102, 64 330 and 311).
-  constexpr bool LATE = NW == 2 || PAIRS == 2;
   constexpr int NT = DT == LSURGE_F16 ? 2 : 3;  // terms of f32 operands against k and q
   __shared__ ChunkTiles tiles[RING];
   __shared__ ChunkTerms terms[2];
@@ -725,7 +726,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         kf[st & 1][i] = token_frag(tile.k, i, st, lane);
-        if constexpr (!LATE) qf[st & 1][i] = token_frag(tile.q, i, st, lane);
+        qf[st & 1][i] = token_frag(tile.q, i, st, lane);
       }
     };
     frags(0);
@@ -748,19 +749,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) P[i] = O[i] = zero;
-    u32x4 kept[4][2];  // LATE: the first two terms by step
-    auto late = [&](int st) {
-      if constexpr (LATE) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const u32x4 f = token_frag(tile.q, i, st, lane);
-          O[i] = mma_32<DT>(f, kept[st][1], O[i]);
-          O[i] = mma_32<DT>(f, kept[st][0], O[i]);
-        }
-      }
-    };
-    u32x8 inv0, inv1, a10;
-    u32x4 m00, m1[2];
+    u32x8 inv0, inv1, a10, m00, m1[2];
     f32x4 beta[2], c1[2], c2[2], w[2];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -774,16 +763,15 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
           beta[i] = *reinterpret_cast<const f32x4*>(&x.beta[t]), c1[i] = *reinterpret_cast<const f32x4*>(&x.c1[t]);
         }
         inv0 = left(x.inv[0], lane), a10 = left(x.a10, lane), inv1 = left(x.inv[1], lane);
-        m00 = x.m00[lane], m1[0] = x.m1[0][lane], m1[1] = x.m1[1][lane];
+        m00 = left(x.m00, lane), m1[0] = left(x.m1[0], lane), m1[1] = left(x.m1[1], lane);
       }
       const u32x2(*now)[NT] = s[st & 1];
-      if constexpr (LATE) kept[st][0] = join(now[0][0], now[1][0]), kept[st][1] = join(now[0][1], now[1][1]);
 #pragma unroll
       for (int j = NT - 1; j >= 0; --j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           P[i] = mma_32<DT>(kf[st & 1][i], join(now[0][j], now[1][j]), P[i]);
-          if (!LATE && j < 2) O[i] = mma_32<DT>(qf[st & 1][i], join(now[0][j], now[1][j]), O[i]);
+          O[i] = mma_32<DT>(qf[st & 1][i], join(now[0][j], now[1][j]), O[i]);
         }
       if (st < 3) {
         split<DT, NT>(S[2 * st + 2], s[(st + 1) & 1][0]);
@@ -808,19 +796,14 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
     X[0] = mma_f32(inv0, right(R[0]), zero);
 #pragma unroll
     for (int m = 0; m < 4; ++m) S[m] *= decay;  // beside the chain of products
-    late(0);
-    late(1);
     const u32x8 x0 = right(X[0]);
     X[1] = mma_f32(inv1, right(mma_f32(a10, x0, R[1])), zero);
 #pragma unroll
     for (int m = 4; m < 8; ++m) S[m] *= decay;
-    late(2);
-    late(3);
-    // o's products of two terms, 2^-16 of them
 #pragma unroll
     for (int i = 0; i < 2; ++i) O[i] *= c2[i] * unscale;
-    O[0] = mma_2(m00, x0, O[0]);
-    O[1] = mma_2(m1[0], x0, O[1]);
+    O[0] = mma_f32_on(m00, x0, O[0]);
+    O[1] = mma_f32_on(m1[0], x0, O[1]);
     // the state's update
     f32x4 E[2] = {X[0] * w[0], X[1] * w[1]};
     if constexpr (DT == LSURGE_F16) {  // the decayed state's size, or what is added to it
@@ -853,7 +836,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
         S[m + 1] = mma_32<DT>(kt[m + 1], join(e0[j], e1[j]), S[m + 1]);
       }
     if constexpr (DT == LSURGE_BF16) split<DT, NT>(S[0], s[0][0]), split<DT, NT>(S[1], s[0][1]);
-    O[1] = mma_2(m1[1], right(X[1]), O[1]);
+    O[1] = mma_f32_on(m1[1], right(X[1]), O[1]);
     const auto ob = os.next();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

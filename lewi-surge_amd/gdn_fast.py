@@ -163,11 +163,10 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=No
     A sequence without rows keeps its state.  One whose slot is outside [0, slots), such as -1 for a place of the batch that
     is not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one
     slot.  use_qk_norm_in_gdn: query and key heads are l2-normalised first (eps 1e-6), without the rounding of the normalised
-    heads that fast_chunk_gated_delta_rule makes.  What the states are formed of is held to float32 or more, so a prompt's state
-    comes out exact to float32, where the chunked form rounds as the reference does; its last bits depend on how a sequence is
-    cut into calls, not on what else is in a call with cu_seqlens.  From four rows on a sequence goes in chunks of 32: o's parts
-    are held to 2^-16 there, before its own rounding, and a value that is not finite, or a head whose squares' sum is not,
-    reaches all rows of its chunk.  Strides are free: views of one projection are read in place.  No gradient."""
+    heads that fast_chunk_gated_delta_rule makes.  States and o are held to float32 until o's one rounding, where the chunked form
+    rounds as the reference does; their last bits depend on how a sequence is cut into calls, not on what else is in a call with
+    cu_seqlens.  From four rows on a sequence goes in chunks of 32: a value that is not finite, or a head whose squares' sum is
+    not, reaches all rows of its chunk.  Strides are free: views of one projection are read in place.  No gradient."""
     what = "recurrent_gated_delta_rule"
     shape, vshape = query.shape, value.shape
     if len(shape) != 3 or key.shape != shape or len(vshape) != 3 or vshape[0] != shape[0] or shape[2] != D or vshape[2] != D:

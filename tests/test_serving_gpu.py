@@ -339,6 +339,51 @@ def test_rule_reads_what_was_erased(dt, dev):
     assert (np.linalg.norm(_np(r.state[r.slots[0]]) - wS, axis=(1, 2)) <= bS).all()
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("n,length", [(1, 32), (2, 150), (40, 32), (33, 64)])
+def test_rule_reads_what_was_erased_by_every_kernel(dt, n, length, dev):
+    """Queries equal to their keys, beta 1 and no decay in workgroups of two and of four taking waves, with one and two pairs
+    that prepare; o within the bound of any other input, without values and beside states a thousand times as large."""
+    for size in (0.0, 1.0):
+        r = Rule(dt, 1, 2, [length] * n, dev, norm=True, beta32=True, seed=n)
+        r.q.copy_(r.k), r.g.zero_(), r.beta.fill_(1), r.v.mul_(size), r.state.mul_(1000)
+        before = r.state.clone()
+        r.check(r.call(), before, r.state)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("lag", [0, 1, 5, 17])
+@pytest.mark.parametrize("lens", [[4, 5, 31, 1, 3, 128, 2], [32] * 40, [64] * 33 + [127], [20, 1, 8, 4] * 20])
+def test_rule_o_is_float32_beside_large_states(dt, lens, lag, dev):
+    """Every token has an axis of its own as its key, beta 1, and reads that axis or the one of `lag` tokens before: o is that
+    token's value / sqrt(128), whatever the state held there, 2^13 times as large here.  With one value that is not 0 to a
+    product, what remains are single roundings of EPS times p, the state's decayed value: of the right side, of the sums of
+    three terms (the state against k 2 and q 2, two solutions 6, the weight times what was solved for 6 and the terms left out 1)
+    and of the factors of o (2): 20.  A value read from a state was rounded on the way in instead, 12 times.  Without decays
+    where another token is read, since the exponentials of two tokens are rounded apart."""
+    r = Rule(dt, 1, 2, lens, dev, norm=False, beta32=True, seed=len(lens), decay=0.01)
+    gen = torch.Generator().manual_seed(lag)
+    at = _starts(lens)
+    axis = torch.cat([torch.randperm(128, generator=gen)[:n] for n in lens])
+    read = torch.cat([torch.arange(a, a + n).sub(lag).clamp(min=a) if lag else torch.arange(a, a + n) for a, n in zip(at, lens)])
+    if lag:  # the first ones read themselves
+        first = torch.cat([torch.arange(n) < lag for n in lens])
+        read[first] = torch.arange(len(read))[first]
+        r.g.zero_()
+    eye = torch.eye(128, dtype=dt)
+    r.k.copy_(eye[axis][:, None]), r.q.copy_(eye[axis[read]][:, None]), r.beta.fill_(1), r.state.mul_(10 * 2.0 ** 13)
+    held = _np(r.state[r.slots])
+    o, v = _np(r.call()), _np(r.v)
+    u, tiny = so.HALF_STEP[NAME[dt]], so.TINY[NAME[dt]]
+    for b, (a, n) in enumerate(zip(at, lens)):
+        rows = read[a:a + n].numpy()
+        want = v[rows] / 128 ** 0.5
+        p = np.abs(held[b][:, axis[rows].numpy()]).transpose(1, 0, 2) / 128 ** 0.5  # decays are at most 1
+        off = 20 * so.EPS * p
+        err = np.abs(o[a:a + n] - want) - (off + u * (np.abs(want) + off) + tiny)
+        assert (err <= 0).all(), f"sequence {b} ({n} rows): {err.max():.2e} over"
+
+
 def test_rule_columns_of_any_size(dev):
     """Values from f16's smallest to its largest in one head: each group of columns of one size within its own bounds."""
     scale = torch.tensor([2.0 ** e for e in (-22, -14, -8, -2, 0, 4, 8, 12)], device=dev).repeat_interleave(16)
