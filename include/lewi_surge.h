@@ -523,10 +523,10 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
  * q and k of head h / (hv / hk).  q, k [rows, hk, 128] and v [rows, hv, 128] by strides (multiples of 8, rows 128 to 2^22 apart),
  * dtype LSURGE_BF16 or LSURGE_F16; g [rows, hv] f32 (log decay) and beta [rows, hv] of dtype or LSURGE_F32 (beta_dtype), rows g_stride and
  * beta_stride elements apart; o [rows, hv, 128] of dtype.  l2_eps >= 0: q and k are first multiplied by rsqrt(sum x^2 + l2_eps)
- * (not rounded in between); negative: taken as they are.  Packed rows, slots and rows without one as for
- * lsurge_causal_conv1d_update; state: [num_slots] of [hv, 128, 128] f32, slot_stride elements apart (a multiple of 4),
- * 16-byte aligned.  States and o are held to f32 until o's one rounding, also in runs of four rows and more, which go in chunks
- * of 32.  Results repeat bit for bit for the same batch; the last bits depend on how a sequence is cut into calls, a single
+ * (not rounded in between; without an eps heads of zeros stay zeros); negative: taken as they are.  Packed rows, slots and rows
+ * without one as for lsurge_causal_conv1d_update; state: [num_slots] of [hv, 128, 128] f32, slot_stride elements apart (a
+ * multiple of 4), 16-byte aligned.  States and o are held to f32 until o's one rounding, also in runs of four rows and more,
+ * which go in chunks of 32.  Results repeat bit for bit for the same batch; the last bits depend on how a sequence is cut into calls, a single
  * token's (cu = NULL) on the batch's size. */
 typedef struct {
   lsurge_attn_rows q, k, v;

@@ -60,6 +60,12 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
+// what the l2 norm multiplies a head by; without an eps zeros stay zeros (a chunk's rows behind the end are such)
+__device__ __forceinline__ float norm_factor(float square, float eps) {
+  const float x = square + eps;
+  return eps < 0.f || x == 0.f ? 1.f : rsqrtf(x);
+}
+
 template <int DT>
 __device__ __forceinline__ float scalar_at(const void* p, int64_t i, int f32) {
   if (f32) return ((const float*)p)[i];
@@ -171,8 +177,8 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
     kq = group_sum<RG>(kq);
     float rk = 1.f, rq = 0.08838834764831845f;  // 1 / sqrt(128)
     if (a.l2_eps >= 0.f) {
-      rk = rsqrtf(group_sum<RG>(kk) + a.l2_eps);
-      rq *= rsqrtf(group_sum<RG>(qq) + a.l2_eps);
+      rk = norm_factor(group_sum<RG>(kk), a.l2_eps);
+      rq *= norm_factor(group_sum<RG>(qq), a.l2_eps);
     }
     // The decay goes to the factor c, one multiplication for the whole state, until c is far from 1.
     c *= expf(cur.g);
@@ -379,7 +385,6 @@ __device__ __forceinline__ float diagonal(f32x4 x, int lane) {
     if ((lane & 3) == r) d = x[r];
   return d;
 }
-__device__ __forceinline__ float norm_factor(float square, float eps) { return eps >= 0.f ? rsqrtf(square + eps) : 1.f; }
 
 // e^{G_i - G_j} times k's factor, j = j0 .. + 3; without branches, whose loads would wait one after the other
 __device__ __forceinline__ f32x4 decays(const Scratch& s, int i, int j0) {

@@ -1,10 +1,13 @@
 """The operators that carry a hybrid model's sequences from token to token, on the GPU: every output within the bounds that the
 float64 oracle derives from the roundings (oracle/serving_oracle.py); what has to stay as it was compared bit for bit."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+import _lib as L
 import attention as A
 import fast_conv as FC
 import gdn_fast as G
@@ -149,6 +152,48 @@ def test_rule_has_the_same_bits_in_any_batch(dt, dev):
         many.beta[at:at + 77] = r.beta
         many.state[many.slots[n]] = before[r.slots[0]]
         assert torch.equal(many.call()[at:at + 77], o) and torch.equal(many.state[many.slots[n]], whole[r.slots[0]])
+
+
+def _rule_by_abi(r, cu, l2_eps):
+    o = torch.full(r.v.shape, 7.0, dtype=r.dt, device=r.dev)
+    slots, cu = _i32(r.slots, r.dev), _ends(r.lens, r.dev) if cu else None
+    arg = L.GdnTokens(*(x for t in (r.q, r.k, r.v) for x in (t.data_ptr(), *t.stride()[:2])), r.g.data_ptr(), r.beta.data_ptr(),
+                      r.state.data_ptr(), o.data_ptr(), slots.data_ptr(), None if cu is None else cu.data_ptr(), r.v.shape[0],
+                      len(r.lens), r.k.shape[1], r.v.shape[1], r.g.stride(0), r.beta.stride(0), r.state.shape[0],
+                      r.state.stride(0), l2_eps, L.dt(o), L.dt(r.beta))
+    L.check(L.lib().lsurge_gdn_recurrent(ctypes.byref(arg), torch.cuda.current_stream().cuda_stream), "gdn_recurrent")
+    torch.cuda.synchronize()
+    return o
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("lens,cu", [([1, 1, 1], False), ([3, 5, 31, 32, 33, 0, 71, 2], True), ([5, 31, 33] * 14, True),
+                                     ([71, 95] * 17, True)])
+def test_rule_norm_without_an_eps(dt, lens, cu, dev):
+    """l2_eps 0 of the C entry at lengths that end inside a chunk, in every kernel: rows behind a sequence's end count for
+    nothing, and heads of zeros and of values whose squares are below float32's smallest normal number are as good as any."""
+    r = Rule(dt, 1, 2, lens, dev, norm=False, unit=False, seed=len(lens), tail=2 if cu else 0)
+    at = _starts(lens)
+    r.k[at[1]], r.q[at[1]] = 0, 0
+    if cu:
+        r.k[at[1] + 1], r.q[at[2] + 1] = 0, 0
+        if dt is BF16:
+            r.k[at[3] + 3] *= 2.0 ** -70
+    before = r.state.clone()
+    o = _rule_by_abi(r, cu, 0.0)
+    unit = [_np(x) / np.maximum(np.linalg.norm(_np(x), axis=-1, keepdims=True), 1e-300) for x in (r.q, r.k)]
+    v, g, beta = (_np(x) for x in (r.v, r.g, r.beta))
+    u, tiny = so.HALF_STEP[NAME[dt]], so.TINY[NAME[dt]]
+    for b, (a, n) in enumerate(zip(at, lens)):
+        rows = slice(a, a + n)
+        wo, wS, bo, bS = so.delta_rule(unit[0][rows], unit[1][rows], v[rows], g[rows], beta[rows], _np(before[r.slots[b]]), False)
+        if n == 0:
+            continue
+        off = np.linalg.norm(_np(r.state[r.slots[b]]) - wS, axis=(1, 2))
+        assert (off <= bS).all(), (b, n, off, bS)
+        off = np.linalg.norm(_np(o[rows]) - wo, axis=-1)
+        assert (off <= bo + u * (np.linalg.norm(wo, axis=-1) + bo) + 128 ** 0.5 * tiny).all(), (b, n)
+    assert not o[at[-1]:].any()
 
 
 def test_rule_keys_without_a_norm(dev):
