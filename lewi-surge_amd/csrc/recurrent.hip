@@ -39,7 +39,7 @@ struct TokenArgs {
   const int32_t *slots, *cu;
   int rows, nseq, hk, hv, num_slots;
   float l2_eps;
-  int units;  // workgroups of the sequences; those behind them clear the rows behind the last sequence
+  int units;  // workgroups of the sequences; those behind them clear the rows of none
 };
 
 // the sum over the RG lanes of a group (RG consecutive lanes), in all of them
@@ -98,12 +98,15 @@ __device__ __forceinline__ Unit unit_of(const TokenArgs& a, int sh) {
   u.slot = a.slots ? a.slots[u.b] : u.b;
   return u;
 }
-// workgroup i of n: the rows behind the last sequence give zeros
-__device__ __forceinline__ void clear_tail(const TokenArgs& a, int i, int n) {
-  const int64_t first = a.nseq ? lsrows::end_at(a.cu, a.nseq, a.rows) : 0;
-  const int64_t count = (a.rows - first) * a.hv * (D / 8);
-  u32x4* o = reinterpret_cast<u32x4*>(a.o + first * a.hv * D);
-  for (int64_t j = (int64_t)i * blockDim.x + threadIdx.x; j < count; j += (int64_t)n * blockDim.x) o[j] = u32x4{0u, 0u, 0u, 0u};
+// workgroup i of n: the rows before the first sequence and behind the last give zeros
+__device__ __forceinline__ void clear_others(const TokenArgs& a, int i, int n) {
+  const int64_t row = (int64_t)a.hv * (D / 8);  // 16-byte pieces
+  const int64_t before = a.nseq ? lsrows::end_at(a.cu, 0, a.rows) * row : 0;
+  const int64_t behind = a.nseq ? lsrows::end_at(a.cu, a.nseq, a.rows) * row : 0;
+  u32x4* o = reinterpret_cast<u32x4*>(a.o);
+  const int64_t j0 = (int64_t)i * blockDim.x + threadIdx.x, step = (int64_t)n * blockDim.x;
+  for (int64_t j = j0; j < before; j += step) o[j] = u32x4{0u, 0u, 0u, 0u};
+  for (int64_t j = behind + j0; j < a.rows * row; j += step) o[j] = u32x4{0u, 0u, 0u, 0u};
 }
 
 // Columns `col0` .. + CB - 1 through a unit's tokens by one wave, token by token: lane l holds the rows R (l % RG) .. + R - 1 of
@@ -592,7 +595,7 @@ __global__ __launch_bounds__(64 * (NW + 2 * PAIRS), NW == 4 && PAIRS == 1 ? 3 : 
   __shared__ Scratch scratch[2 * PAIRS];
   __shared__ float blocks[PAIRS][2][16][20];  // the diagonal blocks of -A, rows 16 bytes apart
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x >= a.units) return clear_tail(a, blockIdx.x - a.units, gridDim.x - a.units);
+  if ((int)blockIdx.x >= a.units) return clear_others(a, blockIdx.x - a.units, gridDim.x - a.units);
   const Unit u = unit_of(a, blockIdx.x / PARTS);
   const int col0 = (blockIdx.x % PARTS * NW + wave) * 16;
   const int total = u.end - u.begin;
@@ -927,7 +930,7 @@ int lsurge_gdn_recurrent(const lsurge_gdn_tokens* t, lsurge_stream_t stream) {
   TokenArgs a = token_args(t);
   const int64_t sh = t->nseq * t->hv;
   hipStream_t s = (hipStream_t)stream;
-  // a launch holds less than 2^32 threads: two workgroups of up to 512 a pair, and 256 for the rows behind
+  // a launch holds less than 2^32 threads: two workgroups of up to 512 a pair, and 256 for the rows of none
   LSURGE_REQUIRE(sh <= (1ll << 22) - 256, "gdn_recurrent: %lld sequences of %lld heads", (long long)t->nseq, (long long)t->hv);
   const bool b32 = t->beta_dtype == LSURGE_F32;
   if (t->cu) {  // runs of any length

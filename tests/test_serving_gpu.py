@@ -271,6 +271,32 @@ def test_rule_ends_out_of_range_stay_inside(cu, dev):
     assert torch.equal(before[kept], r.state[kept]) and o.shape == r.v.shape
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("lens", [[2, 1, 3], [5, 40, 1], [33] * 40, [70, 100] * 17])
+def test_rows_before_the_first_sequence_give_zeros(dt, lens, dev):
+    """Ends that start behind 0: the rows before are rows of no sequence, in all operators of packed rows, and the others have
+    the bits of a call without them."""
+    skip = 3
+    r, c = Rule(dt, 1, 2, lens, dev, tail=2), Conv(dt, 4, 64, lens, dev, tail=2)
+    before, kept = r.state.clone(), c.state.clone()
+    want, after = (r.call(), c.call()), (r.state.clone(), c.state.clone())
+    f = A.rotary_inv_freq(64, 1e4, dev)
+    turned = A.rotary(r.q, r.k, f, cu_seqlens=_ends(lens, dev))
+    nan = lambda t: torch.cat([torch.full_like(t[:skip], float("nan")), t])  # noqa: E731
+    r.q, r.k, r.v, r.g, r.beta, c.x = (nan(t) for t in (r.q, r.k, r.v, r.g, r.beta, c.x))
+    r.state.copy_(before), c.state.copy_(kept)
+    cu = _ends(lens, dev) + skip
+    for shape, call in ((r.v.shape, lambda: G.recurrent_gated_delta_rule(r.q, r.k, r.v, r.g, r.beta, r.state, _i32(r.slots, dev),
+                                                                         cu, use_qk_norm_in_gdn=True)),
+                        (c.x.shape, lambda: FC.causal_conv1d_update(c.x, c.w, c.state, _i32(c.slots, dev), cu, "silu"))):
+        torch.full(shape, 7.0, dtype=dt, device=dev)  # freed: where an output of its size goes
+        got, w = call(), want[len(shape) == 2]
+        assert not got[:skip].any() and torch.equal(got[skip:], w)
+    assert torch.equal(r.state, after[0]) and torch.equal(c.state, after[1])
+    for got, w in zip(A.rotary(r.q, r.k, f, cu_seqlens=cu), turned):
+        assert not got[:skip].any() and torch.equal(got[skip:], w)
+
+
 def test_rule_split_into_calls(dev):
     """A sequence taken in calls of any size ends in the state of one call; alone or among others it has the same bits."""
     r = Rule(BF16, 2, 4, [77], dev, seed=3, extra=2)
