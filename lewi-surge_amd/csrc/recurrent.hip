@@ -4,8 +4,8 @@
 // Per sequence and value head, S [128, 128] f32:  S <- e^g S,  d = beta (v - S^T k),  S <- S + k d^T,  o = S^T q / sqrt(128).
 // The columns of S evolve independently of each other, so a wave takes a block of them through all tokens of its sequence:
 // its part of S stays in registers, is read once and written once, and no wave waits for another.  A token's two products run
-// on the S before it, S^T k and S^T q in one walk over the registers, with
-//   o = (e^g S^T q + (k . q) d) / sqrt(128),
+// on the decayed S before it, S^T k and S^T q in one walk over the registers, with
+//   o = (S^T q + (k . q) d) / sqrt(128),
 // so that one exchange between lanes serves both; the l2 norms of q and k are factors of these sums and cost no pass of their
 // own.  Everything is f32 but the inputs and o.
 //
@@ -123,10 +123,9 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
     return;
   }
   float* sp = a.state + u.slot * a.slot_stride + (int64_t)h * D * D + (int64_t)rg * R * D + col;
-  f32x4 S[R];  // the state divided by `c`
+  f32x4 S[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) S[i] = *reinterpret_cast<const f32x4*>(sp + i * D);
-  float c = 1.f;
 
   const int kh = h / (a.hv / a.hk);
   const uint16_t* qp = a.q + kh * a.q_head + rg * R;
@@ -164,6 +163,7 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
       lsrows::unpack8<DT>(cur.q[i], q + 8 * i);
       lsrows::unpack8<DT>(cur.k[i], k + 8 * i);
     }
+    const float decay = expf(cur.g);
     float kk = 0.f, qq = 0.f, kq = 0.f;
     f32x4 kS{0.f, 0.f, 0.f, 0.f}, qS{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -171,6 +171,7 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
       kk = fmaf(k[i], k[i], kk);
       qq = fmaf(q[i], q[i], qq);
       kq = fmaf(k[i], q[i], kq);
+      S[i] *= decay;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         kS[j] = fmaf(k[i], S[i][j], kS[j]);
@@ -183,23 +184,13 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
       rk = norm_factor(group_sum<RG>(kk), a.l2_eps);
       rq *= norm_factor(group_sum<RG>(qq), a.l2_eps);
     }
-    // The decay goes to the factor c, one multiplication for the whole state, until c is far from 1.
-    c *= expf(cur.g);
-    if (!(c > 0x1p-40f && c < 0x1p40f)) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) S[i] *= c;
-      kS *= c, qS *= c;
-      c = 1.f;
-    }
     float v[4], out[4], kd[4];
     unpack2<DT>(cur.v[0], v[0], v[1]);
     unpack2<DT>(cur.v[1], v[2], v[3]);
-    const float ic = 1.f / c;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      kd[j] = rk * (cur.beta * fmaf(-c * rk, group_sum<RG>(kS[j]), v[j]));  // rk d
-      out[j] = rq * fmaf(c, group_sum<RG>(qS[j]), kq * kd[j]);
-      kd[j] *= ic;
+      kd[j] = rk * (cur.beta * fmaf(-rk, group_sum<RG>(kS[j]), v[j]));  // rk d
+      out[j] = rq * fmaf(kq, kd[j], group_sum<RG>(qS[j]));
     }
     if (rg == 0)
       *reinterpret_cast<u32x2*>(o + t * o_row) = u32x2{lsrows::pack2<DT>(out[0], out[1]), lsrows::pack2<DT>(out[2], out[3])};
@@ -209,7 +200,7 @@ __device__ __forceinline__ void walk_tokens(const TokenArgs& a, const Unit& u, i
       for (int j = 0; j < 4; ++j) S[i][j] = fmaf(k[i], kd[j], S[i][j]);
   }
 #pragma unroll
-  for (int i = 0; i < R; ++i) *reinterpret_cast<f32x4*>(sp + i * D) = S[i] * c;
+  for (int i = 0; i < R; ++i) *reinterpret_cast<f32x4*>(sp + i * D) = S[i];
 }
 
 // One token for each sequence.

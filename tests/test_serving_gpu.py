@@ -228,6 +228,25 @@ def test_rule_decay_of_nothing_and_of_everything(dev):
     r.check(o, before, r.state)
 
 
+@pytest.mark.parametrize("lens,cu", [([1] * 5, False), ([1] * 140, False), ([1, 2, 3, 4, 40], True)])
+def test_rule_values_far_from_what_the_decay_leaves(lens, cu, dev):
+    """Values of 10^27 after decays of e^-27 and more, and small ones beside a state that grows: both the values and what is left
+    are float32 numbers, their quotients are not."""
+    for size, g in ((1e27, -27.0), (1e27, -60.0), (1e-30, 26.0), (1e30, -0.5)):
+        r = Rule(BF16, 1, 2, lens, dev, norm=True, seed=3)
+        if g > 0:
+            r.state.zero_()  # three steps of it at most
+            r.lens = [min(n, 3) for n in lens]
+            for t in (r.q, r.k, r.v, r.g, r.beta):
+                t[sum(r.lens):] = float("nan")
+        r.v.mul_(size), r.g.fill_(g)
+        before = r.state.clone()
+        o = r.call(cu)
+        torch.cuda.synchronize()
+        assert torch.isfinite(r.state).all()
+        r.check(o, before, r.state)
+
+
 def test_rule_places_without_a_slot(dev):
     """-1 and slots behind the pool give zeros, change nothing, and leave the other sequences' bits alone."""
     r = Rule(BF16, 2, 4, [1] * 9, dev)
