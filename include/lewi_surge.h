@@ -526,8 +526,9 @@ int lsurge_causal_conv1d_update(const lsurge_conv_update* u, lsurge_stream_t str
  * (not rounded in between; without an eps heads of zeros stay zeros); negative: taken as they are.  Packed rows, slots and rows
  * without one as for lsurge_causal_conv1d_update; state: [num_slots] of [hv, 128, 128] f32, slot_stride elements apart (a
  * multiple of 4), 16-byte aligned.  States and o are held to f32 until o's one rounding, also in runs of four rows and more,
- * which go in chunks of 32.  Results repeat bit for bit for the same batch; the last bits depend on how a sequence is cut into calls, a single
- * token's (cu = NULL) on the batch's size. */
+ * which go in chunks of 32 (beside f16 rows the state and what is added to it enter products with 23 bits there).  Results
+ * repeat bit for bit for the same batch; the last bits depend on how a sequence is cut into calls, a single token's (cu = NULL)
+ * on the batch's size. */
 typedef struct {
   lsurge_attn_rows q, k, v;
   const float* g;

@@ -222,15 +222,17 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // ahead, or two pairs in turn two chunks ahead, while two or four waves of 16 columns each take this one; one barrier a chunk.
 //
 // Every product runs on the matrix cores of 16-bit operands with f32 sums.  The inputs are exact operands; f32 ones are sums of
-// terms of 16 bits.  Against inputs, three bf16 terms or two f16 ones hold all 24 bits (f16's range is short, so a column of
-// the state is kept times a power of two there, its largest value between 2^8 and 2^15: what is lost is below 2^-33 of it; the
-// power ends at 2^60, so a column below 2^-52, nothing beside f16 inputs, loses 2^-85).
+// terms of 16 bits.  Against inputs, three bf16 terms hold all 24 bits; two f16 ones leave up to 2^-23 of a value over, two
+// roundings of f32 (the first leaves 12 bits and a sign, the second holds 11), since a third would take a prompt of 2000 tokens
+// from 109 to 128 us.  f16's range is short, so a column of the state is kept times a power of two there, its largest value
+// between 2^8 and 2^15: what is lost of small values is below 2^-33 of it; the power ends at 2^60, so a column below 2^-52,
+// nothing beside f16 inputs, loses 2^-85.
 // The 16 x 16 matrices R, X, A, the inverse of A's diagonal blocks and the weights of o are three bf16 terms: o is held to f32
 // before its own rounding too, since a token that reads what it erases is a small difference of large parts (with two terms for
-// o's parts 12 prompts took 103 us instead of 113).  A wave's 16 columns of every matrix lie in its lanes (lane l: column l % 16), so that
-// each product's result is in place as the next one's operand: the state, R and X never leave their lane.  (I + A) is solved by
-// blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are summed in 64 bits,
-// since differences of sums go into exponents.
+// o's parts 12 prompts took 103 us instead of 113).  A wave's 16 columns of every matrix lie in its lanes (lane l: column
+// l % 16), so that each product's result is in place as the next one's operand: the state, R and X never leave their lane.
+// (I + A) is solved by blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are
+// summed in 64 bits, since differences of sums go into exponents.
 constexpr int C = 32;
 // us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 33, 3 30.5 and 32 (f16: 30.5 and 30),
 // 4 32.8 and 32.1 (32.8 and 29.7), 5 36 and 32, 7 42 and 32; 4 sequences with 3 5.4 and 6.0, 4 6.0 and 6.0, 5 6.7 and 6.0.

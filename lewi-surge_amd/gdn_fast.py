@@ -165,7 +165,8 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=No
     slot.  use_qk_norm_in_gdn: query and key heads are l2-normalised first (eps 1e-6), without the rounding of the normalised
     heads that fast_chunk_gated_delta_rule makes.  States and o are held to float32 until o's one rounding, where the chunked form
     rounds as the reference does; their last bits depend on how a sequence is cut into calls, not on what else is in a call with
-    cu_seqlens.  From four rows on a sequence goes in chunks of 32: a value that is not finite, or a head whose squares' sum is
+    cu_seqlens.  From four rows on a sequence goes in chunks of 32: beside float16 rows the state and what is added to it enter
+    products with 23 bits, one less than float32's, and a value that is not finite, or a head whose squares' sum is
     not, reaches all rows of its chunk.  Strides are free: views of one projection are read in place.  No gradient."""
     what = "recurrent_gated_delta_rule"
     shape, vshape = query.shape, value.shape

@@ -28,7 +28,8 @@ def delta_rule(q, k, v, g, beta, S, norm, terms=32):
     [H].  One step is S' = a (I - beta k k^T) S + beta k v^T, and its factor has a 2-norm of a max(1, |1 - beta k.k|), so what
     the state was off goes on no larger than that.  A step adds: its sums of D products, formed in at most `terms` additions
     one after the other (each product and addition rounded), hold to (terms + 2) EPS |k| |S|; the factors of decay, norms and
-    beta round a few times each (8 EPS of what they multiply); the update rounds twice each of its parts.  Steps taken together
+    beta round a few times each (8 EPS of what they multiply, 2 of them for what two f16 terms leave over of a float32 operand);
+    the update rounds twice each of its parts.  Steps taken together
     in chunks round no more of each part, in another order, and are held to the same."""
     q, k, v, g, beta, S = (np.array(x, np.float64) for x in (q, k, v, g, beta, S))
     T, H, D = v.shape[0], v.shape[1], k.shape[2]

@@ -76,6 +76,22 @@ def test_delta_rule_bounds_hold_for_float32_and_show_errors():
     assert np.linalg.norm(kept[0][150:] - o[150:]) > np.linalg.norm(bo[150:])
 
 
+def test_terms_of_a_float32_operand():
+    """Three bf16 terms hold a float32 value; two f16 ones leave up to 2^-23 of it over, in a quarter of all values."""
+    x = torch.from_numpy(np.random.default_rng(7).uniform(256, 32768, 1 << 16).astype(np.float32))
+    x = torch.cat([x, -x, 4096 + 2049 * 2.0 ** -11 * torch.ones(1)])
+
+    def left(t, dt, n):
+        for _ in range(n):
+            t = t - t.to(dt).float()  # exact
+        return t
+
+    assert not left(x, BF16, 3).any()
+    rest = (left(x, F16, 2) / x).abs()
+    assert rest.max() <= 2.0 ** -23 and rest.max() > 2.0 ** -23 * 0.99 and 0.2 < (rest > 0).float().mean() < 0.3
+    assert (left(x, F16, 3) / x).abs().max() < 2.0 ** -33
+
+
 @pytest.mark.parametrize("K", [2, 4, 8])
 def test_oracle_conv(K):
     rng = np.random.default_rng(K)
