@@ -112,6 +112,14 @@ def test_rule_batches_of_every_column_rule(hv, dev):
 
 
 @pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("beta32", [False, True])
+@pytest.mark.parametrize("hv,n", [(1, 255), (1, 256), (1, 257), (5, 51), (5, 52), (8, 31), (8, 32), (8, 33)])
+def test_rule_one_token_each_around_the_column_rule(dt, beta32, hv, n, dev):
+    """255 to 264 (sequence, head) pairs: the last with 8 columns a wave and the first with 32, in both types of beta."""
+    run_rule(dt, hv, hv, [1] * n, dev, seed=n, cu=False, norm=n % 2 == 0, beta32=beta32)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
 @pytest.mark.parametrize("norm", [False, True])
 def test_rule_runs_of_any_length(dt, norm, dev):
     run_rule(dt, 2, 4, [1, 5, 0, 2, 31, 17, 0, 8, 3], dev, norm=norm, beta32=norm, tail=11)
