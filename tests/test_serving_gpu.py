@@ -1019,6 +1019,30 @@ def test_a_models_life(dev):
         assert torch.equal(a[place], b[place])
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_drafts_taken_back(dt, dev):
+    """Drafted tokens of several sequences, of which some are accepted: with the slots' copies written back and the accepted
+    rows run again, outputs and states are those of a program that never saw the others."""
+    drafts, accepted = [5, 4, 1, 7], [2, 4, 1, 5]
+    r, c = Rule(dt, 1, 2, drafts, dev, seed=4), Conv(dt, 4, 64, drafts, dev, seed=4)
+    states = r.state, c.state
+    slots = [torch.tensor(x.slots, device=dev) for x in (r, c)]
+    fresh = [t.clone() for t in states]
+    keep = [t[s] for t, s in zip(states, slots)]
+    r.call(), c.call()
+    for t, s, k in zip(states, slots, keep):
+        t[s] = k
+    rows = torch.cat([torch.arange(a, a + n) for a, n in zip(_starts(drafts), accepted)]).to(dev)
+    r.q, r.k, r.v, r.g, r.beta, c.x = (t[rows] for t in (r.q, r.k, r.v, r.g, r.beta, c.x))
+    r.lens = c.lens = accepted
+    o, y = r.call(), c.call()
+    ends = [t.clone() for t in states]
+    r.state, c.state = fresh
+    assert torch.equal(r.call(), o) and torch.equal(c.call(), y)
+    assert torch.equal(r.state, ends[0]) and torch.equal(c.state, ends[1])
+    r.check(o, states[0].index_copy(0, slots[0], keep[0]), ends[0])
+
+
 def test_captured_step_replays(dev):
     """A decode step in a graph, replayed with other inputs, lengths and slots between eager calls, bit for bit."""
     gen = torch.Generator().manual_seed(12)
