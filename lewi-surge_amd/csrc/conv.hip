@@ -195,7 +195,7 @@ __global__ void causal_conv_dw_reduce_kernel(const float* __restrict__ part, int
 // Packed new rows through the states.  One thread owns 8 channels over a tile of `tile` rows, as above.  The thread that
 // meets a sequence's first row computes its first K - 1 rows, also where they pass the end of its tile (the next tile leaves
 // them out), and it alone reads the slot and afterwards writes it: no other thread's row needs what it replaces.  Bound by
-// memory: x and y once, K - 1 rows read again a tile, the states read and written.  26369 rows of 8192 channels: 158 us, 5.5 TB/s
+// memory: x and y once, K - 1 rows read again a tile, the states read and written.  26369 rows of 8192 channels: 160 us, 5.4 TB/s
 // (a copy reaches 5.1); 64 single rows of 2048: 3.7 us, a launch and a trip to memory.
 struct UpdateArgs {
   const bf16_t *x, *w;

@@ -10,10 +10,10 @@
 // own.  Everything is f32 but the inputs and o.
 //
 // Bound by memory for a token or a few (64 KiB of state a sequence and head, read and written): one token for 64 sequences of
-// 32 heads takes 42 us, 6.1 TB/s, with a part of the states in the caches, 55.6 us, 4.8 TB/s, with none (a copy reaches 5.1);
-// 100 runs of 1 to 8 tokens of 8 heads 28 us, 3.9 TB/s.  Longer runs go in chunks on the matrix cores and are a chain: 2000
-// tokens take 98 us, 1.55 us for 32 of them.  A chunk's products follow each other in one wave: its matrix instructions are 1250
-// of the 3500 cycles, its vector instructions 1650, the rest waits for the one before.
+// 32 heads takes 42.5 us, 6.0 TB/s, with a part of the states in the caches, 54 us, 5.0 TB/s, with none (a copy reaches 5.1);
+// 100 runs of 1 to 8 tokens of 8 heads 28.5 us, 3.8 TB/s.  Longer runs go in chunks on the matrix cores and are a chain: 2000
+// tokens take 107 us, 1.7 us for 32 of them.  A chunk's products follow each other in one wave: its 90 matrix instructions are
+// 1440 of the 3800 cycles, its 440 vector instructions 1750, the rest waits for the one before.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -229,13 +229,13 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_token_kernel(TokenArgs a) {
 // nothing beside f16 inputs, loses 2^-85.
 // The 16 x 16 matrices R, X, A, the inverse of A's diagonal blocks and the weights of o are three bf16 terms: o is held to f32
 // before its own rounding too, since a token that reads what it erases is a small difference of large parts (with two terms for
-// o's parts 12 prompts took 103 us instead of 113).  A wave's 16 columns of every matrix lie in its lanes (lane l: column
+// o's parts 12 prompts took 103 us instead of 112).  A wave's 16 columns of every matrix lie in its lanes (lane l: column
 // l % 16), so that each product's result is in place as the next one's operand: the state, R and X never leave their lane.
 // (I + A) is solved by blocks of 16: X0 = B0 R0, X1 = B1 (R1 - A10 X0), B the inverses of the diagonal blocks.  Log decays are
 // summed in 64 bits, since differences of sums go into exponents.
 constexpr int C = 32;
-// us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 28 and 33, 3 30.5 and 32 (f16: 30.5 and 30),
-// 4 32.8 and 32.1 (32.8 and 29.7), 5 36 and 32, 7 42 and 32; 4 sequences with 3 5.4 and 6.0, 4 6.0 and 6.0, 5 6.7 and 6.0.
+// us token by token and in a chunk: 100 sequences of 8 heads with 2 tokens each 27 and 30 (f16: 27 and 28), 3 30 and 30 (30 and
+// 28), 4 33 and 30 (33 and 28), 5 37 and 30, 7 43 and 31; 4 sequences with 3 5.4 and 6.2, 4 6.2 and 6.3, 5 7.0 and 6.2.
 constexpr int CHUNKED = 4;
 constexpr int64_t MOST_ROW = 1ll << 22;  // elements between rows: a chunk's are within 32 bits of bytes
 constexpr float QSCALE = 0.08838834764831845f;  // 1 / sqrt(128)
@@ -895,17 +895,17 @@ TokenArgs token_args(const lsurge_gdn_tokens* t) {
 }
 
 // Columns a wave takes: 8 where there are few (sequence, head) pairs, whose one walk over a state is then shorter, else 32,
-// which reads whole lines.  us for 8 and 32, states in the caches: 64 pairs 4.2 and 6.1, 128 5.6 and 6.7, 256 8.8 and 7.3; from
-// memory: 128 7.7 and 7.7, 256 12.1 and 10.1, 2048 70 and 55.6 (16 columns: 61), where a copy of the states takes 52.3.
+// which reads whole lines.  us for 8 and 32, states in the caches: 64 pairs 4.3 and 6.1, 128 5.5 and 6.7, 256 8.7 and 7.6; from
+// memory: 128 7.5 and 7.7, 256 12.0 and 9.6, 2048 70 and 54, where a copy of the states takes 52.3.
 int columns(int64_t seq_heads) { return seq_heads < 256 ? 8 : 32; }
 // Waves of a workgroup that take columns of runs: 2 as long as each of the 256 CUs then holds one workgroup at most, whose four
-// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 98 and
-// 109, 8 of up to 2000 68 and 75, 8 of 60 8.5 and 9.0, 16 of up to 2000 142 and 103, of 40 to 80 14.4 and 11.4.
+// waves have a SIMD each; else 4, which prepare half as often.  us for 2 and 4: one sequence of 2000 tokens and 8 heads 107 and
+// 119, 8 of up to 2000 105 and 117, 8 of 60 9.5 and 9.2, 16 of up to 2000 159 and 118, of 40 to 80 15.5 and 13.3.
 int takers(int64_t seq_heads) { return seq_heads <= 64 ? 2 : 4; }
 // Pairs of waves that prepare beside four takers: two share the work of a chunk out to all SIMDs, for a longer start, and leave
 // one workgroup a CU where else there may be two.  So it takes long sequences, on average, which is all the host knows.  us for
-// one pair and two: 12 sequences of 8 heads of 32 tokens 7.4 and 7.5, of 128 13.7 and 13.1, of 1000 69 and 61; 32 of 32 12.2 and
-// 13.9, of 256 45.9 and 47.2, of 512 77 and 75.5, of 1000 139 and 130, of up to 2000 187 and 164.
+// one pair and two: 12 sequences of 8 heads of 32 tokens 7.6 and 7.6, of 128 16.0 and 15.8, of 1000 75 and 66; 32 of 32 14.0 and
+// 15.8, of 256 48 and 49, of 512 83 and 81, of 1000 154 and 147, of up to 2000 259 and 229.
 int preparing_pairs(int64_t seq_heads, int64_t rows, int64_t nseq) {
   return rows >= nseq * (seq_heads <= 128 ? 64 : 300) ? 2 : 1;
 }

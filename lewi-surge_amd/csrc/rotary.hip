@@ -4,13 +4,13 @@
 // Pair i of a head's first `rot` values turns by the angle p f_i of the token's position p:
 //   (a, b) -> (a cos - b sin, b cos + a sin),   a, b = values i and i + rot / 2, or (interleaved) 2 i and 2 i + 1;
 // the values behind them pass through.  p f_i / 2 pi is formed in 64 bits and only its fraction goes on in f32: a position of
-// 10^6 is 10^5 turns, of which f32 would lose all but a few bits.  Sine and cosine are the Taylor series of the angle within
+// 10^6 is 1.6 10^5 turns, of whose fraction f32 would keep 6 bits.  Sine and cosine are the Taylor series of the angle within
 // an eighth of a turn (the rest is below 2^-24), the rotation is f32, each output rounded once.
 //
 // Bound by memory: every value read and written once.  A thread turns 16 values (two 16-byte loads and stores) of up to
 // HEADS heads of one row, so that angles, frequencies and the row's sequence are found once for all of them; a wave's lanes
 // cover whole heads in a row.  20652 tokens, 16 query and 2 key heads of 256, into their pages: 89 us, 5.0 TB/s (a copy reaches
-// 5.1); 32768 tokens of 10 heads of 128 by themselves: 32 us, 5.2 TB/s; 64 tokens: 4 us, a launch and three trips to memory.
+// 5.1); 32768 tokens of 10 heads of 128 by themselves: 34 us, 4.9 TB/s; 64 tokens: 4 us, a launch and three trips to memory.
 #include <algorithm>
 
 #include "kv_cache.h"

@@ -89,8 +89,9 @@ def causal_conv1d_update(inputs, kernel, state, state_slots=None, cu_seqlens=Non
     2 <= K <= 8, all bfloat16 or all float16, C a multiple of 8.  Row b is the one new row of sequence b, or with cu_seqlens
     (int32 [sequences + 1] on the device, ascending from 0) sequence b has the rows cu_seqlens[b] .. cu_seqlens[b + 1].  state
     [slots, K - 1, C] (alloc_conv_state), oldest first, of the same dtype: sequence b's last K - 1 inputs before its new rows are
-    in slot state_slots[b] (int32 on the device; None: b), and its last K - 1 with them replace them, in place.  activation:
-    None, or "silu", y = s / (1 + exp(-s)) of the float32 sum s.  Returns y [rows, C].
+    in slot state_slots[b] (int32 on the device; None: b), and its last K - 1 with all of them replace them, in place (who may
+    take drafted rows back keeps a copy of the slots).  activation: None, or "silu", y = s / (1 + exp(-s)) of the float32 sum s.
+    Returns y [rows, C].
 
     A sequence without rows keeps its state.  One whose slot is outside [0, slots), such as -1 for a place of the batch that is
     not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one slot.

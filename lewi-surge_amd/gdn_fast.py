@@ -156,9 +156,10 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, state, state_slots=No
     query, key [rows, Hk, 128] and value [rows, H, 128], bfloat16 or float16, head h reading query and key head
     h // (H // Hk); g [rows, H] float32, the log decay; beta [rows, H] float32 or the others' dtype.  Row b is the one new
     token of sequence b, or with cu_seqlens (int32 [sequences + 1] on the device, ascending from 0) sequence b has the rows
-    cu_seqlens[b] .. cu_seqlens[b + 1].  state [slots, H, 128, 128] float32 (alloc_delta_state, or the final states of
-    fast_chunk_gated_delta_rule) is updated in place: sequence b's in slot state_slots[b] (int32 on the device; None: b).
-    Returns o [rows, H, 128] in value's dtype.
+    cu_seqlens[b] .. cu_seqlens[b + 1].  state [slots, H, 128, 128] float32 (alloc_delta_state, or what
+    fast_chunk_gated_delta_rule ends with, as float32) is updated in place: sequence b's in slot state_slots[b] (int32 on the
+    device; None: b), by all of its rows: who may take drafted tokens back keeps a copy of the slots.  Returns o [rows, H, 128]
+    in value's dtype.
 
     A sequence without rows keeps its state.  One whose slot is outside [0, slots), such as -1 for a place of the batch that
     is not in use, and rows behind the last sequence give zeros and change no state.  No two sequences with rows may name one
